@@ -21,3 +21,8 @@ from .flashffn import (  # noqa: F401
     FlashFFNv3AdapterFunction, make_v3_adapter_forward, _v3_extract_proj_adapter,
     _v3_dora_col_norm, FlashFFNFunction, FlashFFN, StandardFFN,
 )
+from .lm import (  # noqa: F401
+    embedding, embedding_backward, EmbeddingFunction, ScaledEmbedding,
+    residual_norm, residual_norm_backward, ResidualNormFunction, ResidualNorm,
+    distill_topk, DistillTopKFunction, distill_loss,
+)

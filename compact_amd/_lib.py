@@ -93,6 +93,18 @@ SIGNATURES = {
     "cpt_transpose_bf16": [_P, _L, _L, _L, _P, _L, _P],
     "cpt_gemm_bf16_skinny_dual": [_P, _L, _P, _L, _I, _P, _L, _P, _L, ctypes.c_float, _P, _L, _I,
                                   ctypes.c_float, _L, _L, _L, _I, _P, _P],
+    "cpt_embedding": [_I, _P, _L, _L, _P, _I, _L, ctypes.c_float, _P, _P],
+    "cpt_embedding_backward": [_I, _I, _P, _L, _P, _I, _L, _L, _L, _L, ctypes.c_float, _I, _P, _P,
+                               _P],
+    "cpt_residual_norm": [_I, _I, _P, _L, _P, _L, _P, _P, _P, _I, _L, _L, _L, ctypes.c_float,
+                          ctypes.c_float, ctypes.c_float, _P, _P, _P, _P],
+    "cpt_residual_norm_backward": [_I, _I, _P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _P, _P, _I, _L,
+                                   _L, _L, ctypes.c_float, ctypes.c_float, _P, _P, _P, _P, _P, _P,
+                                   _P],
+    "cpt_distill_topk": [_I, _P, _L, _L, _L, _L, _L, _I, _P, _I, _P, _L, _P, _I, _P, _L,
+                         ctypes.c_float, ctypes.c_float, _I, ctypes.c_float, _P, _P, _P, _P, _L,
+                         _L, _P],
+    "cpt_scale_rows": [_I, _P, _L, _L, _P, _I, _P],
 }
 
 # size queries: name -> argument types (restype int64)
@@ -102,6 +114,8 @@ SIZE_QUERIES = {
     "cpt_dora_col_norm16_workspace_bytes": [_L, _L, _L],
     "cpt_gemm_stream_k_bytes": [],
     "cpt_gemm_bf16_skinny_dual_workspace_bytes": [_L, _L, _L, _I],
+    "cpt_embedding_backward_workspace_bytes": [_L, _L, _L],
+    "cpt_residual_norm_backward_workspace_bytes": [_L, _L, _L, _I],
 }
 
 CACHE_NONE, CACHE_BF16, CACHE_INT4, CACHE_INT8 = 0, 1, 4, 8

@@ -93,6 +93,14 @@ PyMethodDef methods[] = {
     CPT_ENTRY(cpt_dora_col_norm16_workspace_bytes),
     CPT_ENTRY(cpt_topk_abs),
     CPT_ENTRY(cpt_topk_scatter),
+    CPT_ENTRY(cpt_embedding),
+    CPT_ENTRY(cpt_embedding_backward),
+    CPT_ENTRY(cpt_embedding_backward_workspace_bytes),
+    CPT_ENTRY(cpt_residual_norm),
+    CPT_ENTRY(cpt_residual_norm_backward),
+    CPT_ENTRY(cpt_residual_norm_backward_workspace_bytes),
+    CPT_ENTRY(cpt_distill_topk),
+    CPT_ENTRY(cpt_scale_rows),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_capi", "compact_amd's C ABI", -1, methods,

@@ -1,0 +1,472 @@
+// What lies between two blocks of a language model, forward and backward: the
+// norm of a block's output, its gate and scale, the residual add, and the norm
+// that feeds the next block.
+//
+//   n1 = y rho1, rho1 = (mean y^2 + eps)^-1/2, u = n1 w_post    (no w_post: u = y)
+//   r' = beta r + alpha g u
+//   n2 = r' rho2, rho2 = (mean r'^2 + eps)^-1/2, x = n2 w_pre
+// The gate g is absent, a value per channel, per (sequence, channel) or per
+// token.  Backward, with dx and dr' given and mu(.) a row's mean:
+//   t = dr' + rho2 (dn2 - n2 mu(dn2 n2)), dn2 = dx w_pre;   dr = beta t
+//   dn1 = alpha g t w_post,  dy = rho1 (dn1 - n1 mu(dn1 n1))   (no w_post: dy = alpha g t)
+//   dw_pre = sum dx n2;  G = sum t n1 over tokens:  dw_post = alpha g G,
+//   dg = alpha w_post G;  a token's gate: dg = alpha sum_j t u.
+// Every sum, statistic and product is fp32; each output is rounded once.  x is
+// the norm of the unrounded r', which is still in registers.
+//
+// HBM-bound: the forward reads two and writes two row tensors, the backward
+// reads four and writes two.  A group of `tr` threads holds a row in registers,
+// eight columns per thread and vector; a block has `groups` of them side by
+// side and goes over its rows with the weights (and the backward's sums over
+// tokens) kept in registers.
+
+#include "compact_amd.h"
+#include "row_ops.h"
+
+namespace cpt {
+namespace resnorm {
+
+constexpr int kMaxThreads = 1024;
+constexpr int kMaxWaves = kMaxThreads / 64;
+enum Gate : int { kNone = 0, kChannel = 1, kSequence = 2, kToken = 3 };
+
+struct Shape {
+  int64_t rows;        // all tokens
+  int64_t seq;         // tokens per sequence (rows without a sequence gate)
+  int64_t d;
+  int tr, groups;      // threads per row, rows side by side in a block
+  int gate, wdt;       // Gate, weights' type
+  float alpha, beta, eps;
+};
+
+// Eight weights of a type known at run time, `none` where there is no tensor.
+__device__ __forceinline__ void ld_weights(const void* w, int wdt, int64_t base, int64_t j,
+                                           int64_t d, float none, float v[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    v[e] = !w ? none : j + e < d ? ld_any(w, wdt, base + j + e) : 0.f;
+}
+
+// Sums of N values over the threads of each row group, in every thread.  One
+// barrier; `red` alternates between two buffers from call to call.
+template <int N>
+__device__ __forceinline__ void group_sum(float (&v)[N], float (*red)[kMaxWaves], int tr) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+  const int wave = threadIdx.x >> 6, per = tr >> 6;
+  if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) red[i][wave] = v[i];
+  }
+  __syncthreads();
+  const int w0 = wave / per * per;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float s = 0.f;
+    for (int w = 0; w < per; ++w) s += red[i][w0 + w];
+    v[i] = s;
+  }
+}
+
+template <int DT, int NV>
+__global__ __launch_bounds__(kMaxThreads) void forward_kernel(
+    Shape s, const void* __restrict__ residual, int64_t ld_res, const void* __restrict__ y,
+    int64_t ld_y, const void* __restrict__ w_post, const void* __restrict__ w_pre,
+    const void* __restrict__ gate, void* residual_out, void* x, float* stats) {
+  using R = Row8<DT>;
+  using T = typename R::T;
+  __shared__ float red[2][2][kMaxWaves];
+  const int group = threadIdx.x / s.tr, tid = threadIdx.x - group * s.tr;
+  float a[NV][8], wp[NV][8];
+#pragma unroll
+  for (int c = 0; c < NV; ++c) {
+    const int64_t j = 8 * ((int64_t)c * s.tr + tid);
+    float g[8];
+    ld_weights(w_post, s.wdt, 0, j, s.d, 1.f, a[c]);
+    ld_weights(s.gate == kChannel ? gate : nullptr, s.wdt, 0, j, s.d, 1.f, g);
+    ld_weights(w_pre, s.wdt, 0, j, s.d, 1.f, wp[c]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[c][e] *= s.alpha * g[e];
+  }
+  const float inv_d = 1.f / (float)s.d;
+  int turn = 0;
+  const int64_t step = (int64_t)gridDim.x * s.groups;
+  for (int64_t row0 = (int64_t)blockIdx.x * s.groups; row0 < s.rows; row0 += step, turn ^= 1) {
+    const int64_t row = row0 + group;
+    const bool in = row < s.rows;
+    const int64_t d = in ? s.d : 0;   // a group past the last row reads and writes nothing
+    typename R::Raw ry[NV], rr[NV];
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      const int64_t j = 8 * ((int64_t)c * s.tr + tid);
+      rr[c] = row_ld<DT>((const T*)residual + row * ld_res, j, d, 0);
+      if (y) ry[c] = row_ld<DT>((const T*)y + row * ld_y, j, d, 0);
+    }
+    float r[NV][8];
+    float rho1 = 1.f;
+    if (y) {
+      if (w_post) {
+        float sum[1] = {0.f};
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+          float v[8];
+          R::unpack(ry[c], v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum[0] += v[e] * v[e];
+        }
+        group_sum<1>(sum, red[turn], s.tr);
+        rho1 = 1.f / sqrtf(sum[0] * inv_d + s.eps);
+      }
+      float k = rho1;
+      if (s.gate == kToken && in) k *= ld_any(gate, s.wdt, row);
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
+        const int64_t j = 8 * ((int64_t)c * s.tr + tid);
+        float v[8], g[8];
+        R::unpack(rr[c], r[c]);
+        R::unpack(ry[c], v);
+        if (s.gate == kSequence && in) {
+          ld_weights(gate, s.wdt, row / s.seq * s.d, j, s.d, 1.f, g);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= g[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[c][e] = s.beta * r[c][e] + a[c][e] * (v[e] * k);
+        row_st<DT>((T*)residual_out + row * s.d, j, d, R::pack(r[c]));
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < NV; ++c) R::unpack(rr[c], r[c]);
+    }
+    float rho2 = 1.f;
+    if (x) {
+      float sum[1] = {0.f};
+#pragma unroll
+      for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[0] += r[c][e] * r[c][e];
+      group_sum<1>(sum, red[turn] + 1, s.tr);
+      rho2 = 1.f / sqrtf(sum[0] * inv_d + s.eps);
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
+        const int64_t j = 8 * ((int64_t)c * s.tr + tid);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = r[c][e] * rho2 * wp[c][e];
+        row_st<DT>((T*)x + row * s.d, j, d, R::pack(v));
+      }
+    }
+    if (tid == 0 && in) {
+      stats[row] = rho1;
+      stats[s.rows + row] = rho2;
+    }
+  }
+}
+
+// grid (chunks of a sequence's rows, sequences).  Block (c, b) takes the row
+// groups c, c + chunks, ... of sequence b and leaves its sums over them in
+// partial[b * chunks + c]: dw_pre's columns, then G's.
+template <int DT, int NV>
+__global__ __launch_bounds__(kMaxThreads) void backward_kernel(
+    Shape s, const void* __restrict__ d_res_out, int64_t ld_dro, const void* __restrict__ d_x,
+    int64_t ld_dx, const void* __restrict__ res_out, int64_t ld_ro, const void* __restrict__ y,
+    int64_t ld_y, const float* __restrict__ stats, const void* __restrict__ w_post,
+    const void* __restrict__ w_pre, const void* __restrict__ gate, void* d_res, void* d_y,
+    void* d_gate, float* partial) {
+  using R = Row8<DT>;
+  using T = typename R::T;
+  extern __shared__ __align__(16) float combine[];
+  __shared__ float red[2][3][kMaxWaves];
+  const int group = threadIdx.x / s.tr, tid = threadIdx.x - group * s.tr;
+  const int64_t b = blockIdx.y;
+  float a[NV][8], wp[NV][8], acc_pre[NV][8], acc_g[NV][8];
+#pragma unroll
+  for (int c = 0; c < NV; ++c) {
+    const int64_t j = 8 * ((int64_t)c * s.tr + tid);
+    float g[8];
+    ld_weights(w_post, s.wdt, 0, j, s.d, 1.f, a[c]);
+    ld_weights(s.gate == kChannel || s.gate == kSequence ? gate : nullptr, s.wdt,
+               s.gate == kSequence ? b * s.d : 0, j, s.d, 1.f, g);
+    ld_weights(w_pre, s.wdt, 0, j, s.d, 1.f, wp[c]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      a[c][e] *= s.alpha * g[e];
+      acc_pre[c][e] = acc_g[c][e] = 0.f;
+    }
+  }
+  const float inv_d = 1.f / (float)s.d;
+  const int64_t step = (int64_t)gridDim.x * s.groups;
+  int turn = 0;
+  for (int64_t row0 = (int64_t)blockIdx.x * s.groups; row0 < s.seq; row0 += step, turn ^= 1) {
+    const bool in = row0 + group < s.seq;
+    const int64_t row = b * s.seq + row0 + group;
+    const int64_t d = in ? s.d : 0;
+    typename R::Raw q_dr[NV], q_dx[NV], q_r[NV], q_y[NV];
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      const int64_t j = 8 * ((int64_t)c * s.tr + tid);
+      q_dr[c] = q_dx[c] = q_r[c] = q_y[c] = R::zero();
+      if (d_res_out) q_dr[c] = row_ld<DT>((const T*)d_res_out + row * ld_dro, j, d, 0);
+      if (d_x) {
+        q_dx[c] = row_ld<DT>((const T*)d_x + row * ld_dx, j, d, 0);
+        q_r[c] = row_ld<DT>((const T*)res_out + row * ld_ro, j, d, 0);
+      }
+      if (y) q_y[c] = row_ld<DT>((const T*)y + row * ld_y, j, d, 0);
+    }
+    const float rho1 = in ? stats[row] : 0.f, rho2 = in ? stats[s.rows + row] : 0.f;
+    const float gt = s.gate == kToken && in ? ld_any(gate, s.wdt, row) : 1.f;
+    // one reduction for both norms: with t = dr' + rho2 (dn2 - n2 m2) left open in m2,
+    // sum a n1 t = sum a n1 (dr' + rho2 dn2) - rho2 m2 sum a n1 n2
+    float sum[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      float dr[8], dx[8], r[8], v[8];
+      R::unpack(q_dr[c], dr);
+      R::unpack(q_dx[c], dx);
+      R::unpack(q_r[c], r);
+      R::unpack(q_y[c], v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float n2 = r[e] * rho2, dn2 = dx[e] * wp[c][e], an1 = a[c][e] * (v[e] * rho1);
+        sum[0] += dn2 * n2;
+        sum[1] += an1 * (dr[e] + rho2 * dn2);
+        sum[2] += an1 * n2;
+      }
+    }
+    group_sum<3>(sum, red[turn], s.tr);
+    const float m2 = sum[0] * inv_d;
+    const float dgt = sum[1] - rho2 * m2 * sum[2];
+    const float m1 = w_post ? gt * dgt * inv_d : 0.f;
+    if (s.gate == kToken && in && tid == 0) st_any(d_gate, s.wdt, row, dgt);
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      const int64_t j = 8 * ((int64_t)c * s.tr + tid);
+      float dr[8], dx[8], r[8], v[8];
+      R::unpack(q_dr[c], dr);
+      R::unpack(q_dx[c], dx);
+      R::unpack(q_r[c], r);
+      R::unpack(q_y[c], v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float n2 = r[e] * rho2, n1 = v[e] * rho1;
+        const float t = dr[e] + rho2 * (dx[e] * wp[c][e] - n2 * m2);
+        acc_pre[c][e] += dx[e] * n2;
+        acc_g[c][e] += gt * t * n1;
+        dr[e] = s.beta * t;
+        v[e] = rho1 * (gt * a[c][e] * t - n1 * m1);
+      }
+      row_st<DT>((T*)d_res + row * s.d, j, d, R::pack(dr));
+      if (y) row_st<DT>((T*)d_y + row * s.d, j, d, R::pack(v));
+    }
+  }
+  // the groups' sums, in group order
+  float* out = partial + (b * gridDim.x + blockIdx.x) * 2 * s.d;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    auto& acc = which ? acc_g : acc_pre;
+    __syncthreads();
+    if (group > 0) {
+#pragma unroll
+      for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          combine[((group - 1) * NV + c) * 8 * s.tr + e * s.tr + tid] = acc[c][e];
+    }
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
+        const int64_t j = 8 * ((int64_t)c * s.tr + tid);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float v = acc[c][e];
+          for (int g = 1; g < s.groups; ++g)
+            v += combine[((g - 1) * NV + c) * 8 * s.tr + e * s.tr + tid];
+          if (j + e < s.d) out[which * s.d + j + e] = v;
+        }
+      }
+    }
+  }
+}
+
+constexpr int kFinCols = 64, kFinSlices = 16;
+
+// grid (columns / 64, 2 + sequences with a gate of their own): the chunks'
+// sums of 64 columns, sixteen slices of them added side by side and then in
+// order.  y = 0: dw_pre; y = 1: dw_post, and dg of a channel gate from the same
+// sum; y = 2 + b: dg of sequence b.
+__global__ __launch_bounds__(kFinCols* kFinSlices) void finish_kernel(
+    Shape s, const float* __restrict__ partial, int64_t chunks, int64_t seqs,
+    const void* __restrict__ w_post, const void* __restrict__ gate, void* d_w_pre, void* d_w_post,
+    void* d_gate) {
+  __shared__ float part[kFinSlices][kFinCols];
+  const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
+  const int64_t j = (int64_t)blockIdx.x * kFinCols + lane;
+  const int what = blockIdx.y;
+  const bool in = j < s.d;
+  const int64_t first = what >= 2 ? (what - 2) * chunks : 0;
+  const int64_t n = what >= 2 ? chunks : chunks * seqs;
+  const int64_t per = (n + kFinSlices - 1) / kFinSlices;
+  const int64_t c0 = min(n, slice * per), c1 = min(n, c0 + per);
+  const float* p = partial + (what ? s.d : 0) + (in ? j : 0);
+  float v = 0.f;
+  if (what == 1 && s.gate == kSequence) {
+    for (int64_t c = c0; c < c1; ++c)
+      v += p[(first + c) * 2 * s.d] * (in ? ld_any(gate, s.wdt, c / chunks * s.d + j) : 0.f);
+  } else {
+#pragma unroll 8
+    for (int64_t c = c0; c < c1; ++c) v += p[(first + c) * 2 * s.d];
+  }
+  part[slice][lane] = v;
+  __syncthreads();
+  if (slice > 0 || !in) return;
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < kFinSlices; ++k) sum += part[k][lane];
+  if (what == 0) {
+    if (d_w_pre) st_any(d_w_pre, s.wdt, j, sum);
+    return;
+  }
+  const float wq = w_post ? ld_any(w_post, s.wdt, j) : 1.f;
+  if (what >= 2) {
+    st_any(d_gate, s.wdt, (int64_t)(what - 2) * s.d + j, s.alpha * wq * sum);
+    return;
+  }
+  if (s.gate == kChannel) {
+    if (d_w_post) st_any(d_w_post, s.wdt, j, s.alpha * ld_any(gate, s.wdt, j) * sum);
+    st_any(d_gate, s.wdt, j, s.alpha * wq * sum);
+  } else if (d_w_post) {
+    st_any(d_w_post, s.wdt, j, s.alpha * sum);
+  }
+}
+
+inline int launched() { return hipGetLastError() == hipSuccess ? kOk : kErrLaunch; }
+
+constexpr int64_t kMaxD = 8 * kMaxThreads * 2;
+
+// Vectors per thread, and the threads and row groups of a block.
+int plan(Shape& s) {
+  const int64_t vecs = (s.d + 7) / 8;
+  const int nv = vecs <= kMaxThreads ? 1 : 2;
+  const int64_t t = (vecs + nv - 1) / nv;
+  s.tr = (int)((t + 63) / 64 * 64);
+  s.groups = kMaxThreads / s.tr;
+  if (s.groups > s.seq) s.groups = s.seq > 0 ? (int)s.seq : 1;
+  return nv;
+}
+
+// Chunks of a sequence's rows in the backward: one block of 16 wavefronts per CU
+// over all sequences, as far as there are rows.
+int64_t backward_chunks(const Shape& s, int64_t seqs) {
+  int64_t c = (256 + seqs - 1) / seqs;
+  const int64_t most = (s.seq + s.groups - 1) / s.groups;
+  if (c > most) c = most;
+  return c < 1 ? 1 : c;
+}
+
+bool shape_ok(int64_t rows, int64_t seq, int64_t d, int gate) {
+  return rows >= 0 && seq >= 0 && d >= 1 && gate >= kNone && gate <= kToken &&
+         (rows == 0 || (seq > 0 && rows % seq == 0)) && (gate == kSequence || seq == rows);
+}
+
+}  // namespace resnorm
+}  // namespace cpt
+
+using namespace cpt;
+using namespace cpt::resnorm;
+
+extern "C" {
+
+int cpt_residual_norm(int dtype, int weight_dtype, const void* residual, int64_t ld_residual,
+                      const void* y, int64_t ld_y, const void* w_post, const void* w_pre,
+                      const void* gate, int gate_kind, int64_t rows, int64_t seq, int64_t d,
+                      float scale, float residual_scale, float eps, void* residual_out, void* x,
+                      void* stats, void* stream) {
+  if (dtype < kF32 || dtype > kBF16 || (weight_dtype != kF32 && weight_dtype != dtype))
+    return kErrDType;
+  if (!shape_ok(rows, seq, d, gate_kind)) return kErrShape;
+  if (d > kMaxD) return kErrTooLarge;
+  if ((gate_kind != kNone) != (gate != nullptr)) return kErrShape;
+  if (!y && (w_post || gate || residual_scale != 1.f)) return kErrShape;
+  if ((y != nullptr) != (residual_out != nullptr) || (w_pre != nullptr) != (x != nullptr) ||
+      (!y && !x))
+    return kErrShape;
+  if (rows == 0) return kOk;
+  if (!residual || !stats || ld_residual < 0 || ld_y < 0) return kErrShape;
+  Shape s{rows, seq, d, 0, 0, gate_kind, weight_dtype, scale, residual_scale, eps};
+  s.seq = rows;   // blocks take rows of any sequence
+  const int nv = plan(s);
+  s.seq = seq;
+  const int threads = s.tr * s.groups;
+  const int64_t blocks = (rows + s.groups - 1) / s.groups;
+  const int64_t most = 256 * (2048 / threads);   // as many as can run at a time
+  const dim3 grid((unsigned)(blocks < most ? blocks : most));
+#define CPT_FWD(DT, NV)                                                                         \
+  forward_kernel<DT, NV><<<grid, threads, 0, (hipStream_t)stream>>>(                             \
+      s, residual, ld_residual, y, ld_y, w_post, w_pre, gate, residual_out, x, (float*)stats)
+#define CPT_FWD_NV(DT) (nv == 1 ? CPT_FWD(DT, 1) : CPT_FWD(DT, 2))
+  dtype == kF32 ? CPT_FWD_NV(kF32) : dtype == kF16 ? CPT_FWD_NV(kF16) : CPT_FWD_NV(kBF16);
+  return launched();
+}
+
+int64_t cpt_residual_norm_backward_workspace_bytes(int64_t rows, int64_t seq, int64_t d,
+                                                   int gate_kind) {
+  if (!shape_ok(rows, seq, d, gate_kind) || d > kMaxD) return -1;
+  if (rows == 0) return 0;
+  Shape s{rows, seq, d, 0, 0, gate_kind, kF32, 1.f, 1.f, 0.f};
+  plan(s);
+  const int64_t seqs = rows / seq;
+  return seqs * backward_chunks(s, seqs) * 2 * d * 4;
+}
+
+int cpt_residual_norm_backward(int dtype, int weight_dtype, const void* d_residual_out,
+                               int64_t ld_dro, const void* d_x, int64_t ld_dx,
+                               const void* residual_out, int64_t ld_ro, const void* y,
+                               int64_t ld_y, const void* stats, const void* w_post,
+                               const void* w_pre, const void* gate, int gate_kind, int64_t rows,
+                               int64_t seq, int64_t d, float scale, float residual_scale,
+                               void* d_residual, void* d_y, void* d_w_pre, void* d_w_post,
+                               void* d_gate, void* workspace, void* stream) {
+  if (dtype < kF32 || dtype > kBF16 || (weight_dtype != kF32 && weight_dtype != dtype))
+    return kErrDType;
+  if (!shape_ok(rows, seq, d, gate_kind)) return kErrShape;
+  if (d > kMaxD) return kErrTooLarge;
+  if ((gate_kind != kNone) != (gate != nullptr) || (gate != nullptr) != (d_gate != nullptr) ||
+      (w_post != nullptr) != (d_w_post != nullptr) || (w_pre != nullptr) != (d_w_pre != nullptr) ||
+      (w_pre != nullptr) != (d_x != nullptr) || (y != nullptr) != (d_y != nullptr))
+    return kErrShape;
+  if (!y && (w_post || gate || residual_scale != 1.f)) return kErrShape;
+  if (!y && !d_x) return kErrShape;
+  const int64_t seqs = rows == 0 ? 0 : rows / seq;
+  if (seqs > 65533) return kErrTooLarge;   // a grid's second extent
+  if (rows > 0 && (!stats || !d_residual || !workspace || (d_x && !residual_out) || ld_dro < 0 ||
+                   ld_dx < 0 || ld_ro < 0 || ld_y < 0))
+    return kErrShape;
+  Shape s{rows, seq, d, 0, 0, gate_kind, weight_dtype, scale, residual_scale, 0.f};
+  const int nv = plan(s);
+  const int64_t chunks = seqs == 0 ? 0 : backward_chunks(s, seqs);
+  const hipStream_t st = (hipStream_t)stream;
+  if (rows > 0) {
+    const int threads = s.tr * s.groups;
+    const dim3 grid((unsigned)chunks, (unsigned)seqs);
+    const size_t lds = (size_t)(s.groups - 1) * s.tr * 8 * nv * 4;
+#define CPT_BWD(DT, NV)                                                                         \
+  backward_kernel<DT, NV><<<grid, threads, lds, st>>>(                                           \
+      s, d_residual_out, ld_dro, d_x, ld_dx, residual_out, ld_ro, y, ld_y, (const float*)stats,  \
+      w_post, w_pre, gate, d_residual, d_y, d_gate, (float*)workspace)
+#define CPT_BWD_NV(DT) (nv == 1 ? CPT_BWD(DT, 1) : CPT_BWD(DT, 2))
+    dtype == kF32 ? CPT_BWD_NV(kF32) : dtype == kF16 ? CPT_BWD_NV(kF16) : CPT_BWD_NV(kBF16);
+    const int rc = launched();
+    if (rc != kOk) return rc;
+  }
+  if (d_w_pre || d_w_post || gate_kind == kChannel || gate_kind == kSequence) {
+    const dim3 grid((unsigned)((d + kFinCols - 1) / kFinCols),
+                    (unsigned)(gate_kind == kSequence ? 2 + seqs : 2));
+    finish_kernel<<<grid, kFinCols * kFinSlices, 0, st>>>(s, (const float*)workspace, chunks, seqs,
+                                                          w_post, gate, d_w_pre, d_w_post, d_gate);
+    return launched();
+  }
+  return kOk;
+}
+
+}  // extern "C"

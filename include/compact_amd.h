@@ -1,6 +1,7 @@
 /*
  * compact_amd.h -- C ABI of libcompact_amd.so, the gfx950 (MI355X) kernels of
- * the FlashFFN v3 hot path (SwiGLU FFN with a compressed GLU cache).
+ * the FlashFFN v3 hot path (SwiGLU FFN with a compressed GLU cache) and of the
+ * training step around it.
  *
  * Every entry point takes device pointers, sizes and a HIP stream (passed as
  * void*; NULL is the legacy default stream), launches asynchronously on that
@@ -557,6 +558,87 @@ int cpt_topk_scatter(const void* values, const void* indices, int dtype, int64_t
  * partial sum per wavefront.  FLOPs per launch = blocks * iters * 64 *
  * (FLOPs per MFMA). */
 int cpt_probe_mfma_rate(int shape, int blocks, int iters, float seed, void* out, void* stream);
+
+/* ---------------- around the FFN: embedding, residual norm, distillation ---------------- */
+/* Operators of the training step around the FFN.  The reference leaves them to
+ * torch (nn.Embedding, the norms and adds of a decoder layer, the loss). */
+
+/* out[n, d] = scale * weight[ids[n], :] (weight [vocab, d], out of one dtype); an
+ * id outside [0, vocab) gives a row of zeros.  ids: int64 (ids_wide = 1) or
+ * int32.  Any alignment of the element's size. */
+int cpt_embedding(int dtype, const void* weight, int64_t vocab, int64_t d, const void* ids,
+                  int ids_wide, int64_t n, float scale, void* out, void* stream);
+
+/* Its gradient: out[v, :] = scale * sum of grad[n, :] (rows ld_grad elements
+ * apart) over the tokens n with ids[n] = v, fp32 sums in the tokens' order (the
+ * same bits on every run); padding_idx and ids outside the table add nothing (-1:
+ * no padding).  out [vocab, d] of `dtype` or fp32 is written whole, or with
+ * `accumulate` added to, only rows with tokens being touched.  workspace:
+ * cpt_embedding_backward_workspace_bytes(n, vocab, d) bytes, 16-byte aligned
+ * (-1: sizes out of range). */
+int64_t cpt_embedding_backward_workspace_bytes(int64_t n, int64_t vocab, int64_t d);
+int cpt_embedding_backward(int dtype, int out_dtype, const void* grad, int64_t ld_grad,
+                           const void* ids, int ids_wide, int64_t n, int64_t vocab, int64_t d,
+                           int64_t padding_idx, float scale, int accumulate, void* out,
+                           void* workspace, void* stream);
+
+/* Between two blocks, per row of d columns (d <= 16384):
+ *   n1 = y / sqrt(mean y^2 + eps), u = n1 * w_post      (w_post NULL: u = y)
+ *   residual_out = residual_scale * residual + scale * gate * u
+ *   x = residual_out / sqrt(mean residual_out^2 + eps) * w_pre
+ * y NULL: only x, of the residual itself (residual_out NULL, residual_scale 1).
+ * w_pre and x NULL: no second norm.  gate_kind: 0 none, 1 [d], 2 [rows / seq, d]
+ * (one row for `seq` consecutive rows), 3 [rows]; seq = rows for all but 2.
+ * Weights and gate are of weight_dtype: dtype or fp32.  Inputs' rows lie ld_*
+ * elements apart, outputs are contiguous and alias no input.  stats: fp32
+ * [2, rows], the two norms' reciprocal roots (1 where there is no norm). */
+int cpt_residual_norm(int dtype, int weight_dtype, const void* residual, int64_t ld_residual,
+                      const void* y, int64_t ld_y, const void* w_post, const void* w_pre,
+                      const void* gate, int gate_kind, int64_t rows, int64_t seq, int64_t d,
+                      float scale, float residual_scale, float eps, void* residual_out, void* x,
+                      void* stats, void* stream);
+
+/* Its gradient from d_residual_out (NULL: zeros) and d_x, given what the forward
+ * left in residual_out and stats.  d_residual, d_y [rows, d] contiguous; d_w_pre,
+ * d_w_post, d_gate of the weights' type, present with their weights.  workspace:
+ * cpt_residual_norm_backward_workspace_bytes(...) bytes of fp32 partial sums. */
+int64_t cpt_residual_norm_backward_workspace_bytes(int64_t rows, int64_t seq, int64_t d,
+                                                   int gate_kind);
+int cpt_residual_norm_backward(int dtype, int weight_dtype, const void* d_residual_out,
+                               int64_t ld_dro, const void* d_x, int64_t ld_dx,
+                               const void* residual_out, int64_t ld_ro, const void* y,
+                               int64_t ld_y, const void* stats, const void* w_post,
+                               const void* w_pre, const void* gate, int gate_kind, int64_t rows,
+                               int64_t seq, int64_t d, float scale, float residual_scale,
+                               void* d_residual, void* d_y, void* d_w_pre, void* d_w_post,
+                               void* d_gate, void* workspace, void* stream);
+
+/* Distillation from a teacher's top k <= 2048 logits, over student logits of
+ * vocab <= 524288 columns (distill.hip has the formulas).  Row i's logits start
+ * at (i / seq) * ld_batch + (i % seq) * ld_row elements, its gradient in `grad`
+ * (NULL: none wanted; may be the logits themselves) likewise by gld_*.
+ * top_logits [rows, k] of top_dtype, top_indices [rows, k] int64 (idx_wide = 1)
+ * or int32; an index outside [0, vocab) is no entry.  top_lse fp32 [rows]: the
+ * teacher's log-sum-exp over its whole vocabulary at this temperature, or NULL
+ * (its entries are all).  labels [rows] int64 / int32 or NULL; rows labelled
+ * ignore_index or outside [0, vocab) are left out.  loss = alpha * soft +
+ * (1 - alpha) * hard; alpha < 1 needs labels.  row_loss fp32 [rows]; reduction
+ * 0: mean over the rows left in (0 where there are none), 1: sum, 2: none (loss
+ * may be NULL); loss fp32 [1].  The gradient is that of the reduced loss times
+ * grad_scale times grad_out (device fp32: [1], [rows] for reduction 2, or
+ * NULL). */
+int cpt_distill_topk(int dtype, const void* logits, int64_t rows, int64_t vocab, int64_t seq,
+                     int64_t ld_batch, int64_t ld_row, int top_dtype, const void* top_logits,
+                     int idx_wide, const void* top_indices, int64_t k, const void* top_lse,
+                     int label_wide, const void* labels, int64_t ignore_index, float temperature,
+                     float alpha, int reduction, float grad_scale, const void* grad_out,
+                     void* row_loss, void* loss, void* grad, int64_t gld_batch, int64_t gld_row,
+                     void* stream);
+
+/* x[rows, cols] *= factor (device fp32: one value, or with per_row one a row);
+ * rows whose factor is 1 are not touched. */
+int cpt_scale_rows(int dtype, void* x, int64_t rows, int64_t cols, const void* factor,
+                   int per_row, void* stream);
 
 #ifdef __cplusplus
 }
