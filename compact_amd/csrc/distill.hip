@@ -36,7 +36,6 @@ constexpr float kLn2 = 0.69314718055994530942f;
 constexpr int kMaxWaves = 16;
 constexpr int kMaxEntries = 2048;
 constexpr int64_t kMaxVocab = 1 << 19;
-constexpr int kStream = 0;   // NV of the kernel that reads a row twice
 
 struct Args {
   int64_t rows, vocab;
@@ -56,25 +55,41 @@ struct Args {
   const float* grad_out;          // null, one value or one per row
   int grad_out_rows, mean;
   float* row_loss;
+  float* loss;
 };
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// -inf stands for "no element": its differences with itself would be NaN.
-__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+// The exponentials are taken in powers of two about a whole number near the
+// maximum: 2^(k z - C), C = rint(k max).  The product and difference are one
+// fused operation, rounded once, and two bases differ by an exact power of two.
+// C stops at 2^28, beyond which its own spacing would count: rows that lie
+// there are moved to 0 first.
+constexpr float kFar = 268435456.f;
+__device__ __forceinline__ float base_of(float m, float k) {
+  return rintf(fminf(fmaxf(m * k, -kFar), kFar));
+}
 
-__device__ __forceinline__ bool row_live(const Args& a, int64_t row) {
-  if (!a.labels) return true;
-  const int64_t y = ld_index(a.labels, a.label_wide, row);
+__device__ __forceinline__ bool live_label(const Args& a, int64_t y) {
   return y != a.ignore && y >= 0 && y < a.vocab;
 }
 
 // Rows that count, over the whole batch (each block for itself: the labels are
 // read from cache once per block, which saves a launch).
-__device__ int64_t count_live(const Args& a, float* tmp) {
+__device__ __forceinline__ int64_t count_live(const Args& a, float* tmp) {
   if (!a.labels) return a.rows;
   int n = 0;
-  for (int64_t r = threadIdx.x; r < a.rows; r += blockDim.x) n += row_live(a, r);
+  constexpr int kAhead = 8;
+  for (int64_t r = threadIdx.x; r < a.rows; r += kAhead * (int64_t)blockDim.x) {
+    int64_t y[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t at = r + i * (int64_t)blockDim.x;
+      y[i] = at < a.rows ? ld_index(a.labels, a.label_wide, at) : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) n += live_label(a, y[i]);
+  }
   int* const t = reinterpret_cast<int*>(tmp);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off);
@@ -110,11 +125,30 @@ __device__ __forceinline__ bool first_of(const int* idx, int k) {
   return true;
 }
 
-template <int DT, int NV>
-__global__ __launch_bounds__(1024) void distill_kernel(Args a) {
+// Sum and maximum over 16 lanes (one value a wavefront of the block), in all.
+__device__ __forceinline__ float row16_sum(float x) {
+  x += dpp<0x111, 0xF>(0.f, x);
+  x += dpp<0x112, 0xF>(0.f, x);
+  x += dpp<0x114, 0xF>(0.f, x);
+  x += dpp<0x118, 0xF>(0.f, x);
+  return lane63(x);
+}
+__device__ __forceinline__ float row16_max(float x) {
+  x = fmaxf(x, dpp<0x111, 0xF>(x, x));
+  x = fmaxf(x, dpp<0x112, 0xF>(x, x));
+  x = fmaxf(x, dpp<0x114, 0xF>(x, x));
+  x = fmaxf(x, dpp<0x118, 0xF>(x, x));
+  return lane63(x);
+}
+
+// POW: the softmax at temperature 1 from the one at tau.  0: not wanted, or the
+// same (tau = 1); 1: exponentials of its own; 2: tau = 2, their squares.
+template <int DT, int NV, int POW, bool GRAD, int THREADS, int WAVES>
+__global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
   using R = Row8<DT>;
   using T = typename R::T;
-  constexpr int kN = NV == kStream ? 1 : NV;
+  using Raw = typename R::Raw;
+  constexpr uint32_t kBytes = 8 * sizeof(T);
   extern __shared__ __align__(16) uint32_t smem[];
   __shared__ float red_m[2][kMaxWaves], red_t[2][kMaxWaves], red_1[2][kMaxWaves];
   __shared__ Teacher teach;
@@ -125,67 +159,89 @@ __global__ __launch_bounds__(1024) void distill_kernel(Args a) {
   float* const s_p = reinterpret_cast<float*>(smem + 2 * a.k);
   float* const s_lp = reinterpret_cast<float*>(smem + 3 * a.k);
   uint32_t* const bits = smem + 4 * a.k;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
-  const int64_t v = a.vocab, vecs = (v + 7) / 8;
+  const uint32_t tid = threadIdx.x;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // whole vectors; the ragged end, one column a thread
+  const uint32_t v = (uint32_t)a.vocab, vecs = v / 8, ragged = v & 7;
   const bool tail = a.lse != nullptr;
   const bool hard = a.alpha != 1.f;
-  const bool two = hard && a.tau != 1.f;   // a second softmax, at temperature 1
   const float kt = kLog2e / a.tau, k1 = kLog2e;
-  for (int64_t w = tid; w < (v + 31) / 32; w += blockDim.x) bits[w] = 0;
+  for (uint32_t w = tid; w < (v + 31) / 32; w += THREADS) bits[w] = 0;
+  if (tid < 2 * kMaxWaves && tid % kMaxWaves >= THREADS / 64) {   // wavefronts there are not
+    red_m[tid / kMaxWaves][tid % kMaxWaves] = -INFINITY;
+    red_t[tid / kMaxWaves][tid % kMaxWaves] = red_1[tid / kMaxWaves][tid % kMaxWaves] = 0.f;
+  }
   float norm = a.grad_scale;
   if (a.mean) {
     const int64_t live = count_live(a, tmp);
     norm /= (float)(live > 0 ? live : 1);
+    if (blockIdx.x == 0 && tid == 0) *a.loss = (float)(live > 0 ? live : 1);   // for the total
   }
   __syncthreads();
 
-  // with a tail, the entries' columns leave the row: the first wavefront has them,
-  // and what the block sums is the rest, about a maximum of its own
-  auto mask = [&](float x[8], int64_t j) {
-    if (tail && j < v) {
-      const uint32_t top = bits[j >> 5] >> (j & 31);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = top >> e & 1 ? -INFINITY : x[e];
-    }
+  const auto offset = [&](int64_t r, int64_t ld_b, int64_t ld_s) {
+    const uint32_t rb = (uint32_t)r / (uint32_t)a.seq, rs = (uint32_t)r - rb * (uint32_t)a.seq;
+    return (rb * ld_b + rs * ld_s) * (int64_t)sizeof(T);
+  };
+  const auto label_of = [&](int64_t r) {
+    return a.labels && r < a.rows ? ld_index(a.labels, a.label_wide, r) : -1;
   };
 
   int turn = 0;
+  int64_t next_label = label_of(blockIdx.x);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const T* const z = (const T*)a.logits + row / a.seq * a.ld_b + row % a.seq * a.ld_s;
-    T* const g = a.grad ? (T*)a.grad + row / a.seq * a.gld_b + row % a.seq * a.gld_s : nullptr;
-    const int64_t label = a.labels ? ld_index(a.labels, a.label_wide, row) : -1;
-    if (!row_live(a, row)) {
+    const char* const z = (const char*)a.logits + offset(row, a.ld_b, a.ld_s);
+    char* const g = GRAD ? (char*)a.grad + offset(row, a.gld_b, a.gld_s) : nullptr;
+    const auto elem = [&](int64_t j) { return Elem<DT>::ld((const T*)z + j); };
+    const auto vec8 = [&](uint32_t vec) { return R::ld((const T*)(z + vec * kBytes)); };
+    const int64_t label = next_label;
+    if (a.labels && !live_label(a, label)) {
+      next_label = label_of(row + gridDim.x);
       if (tid == 0) a.row_loss[row] = 0.f;
-      if (g)
-        for (int64_t c = tid; c < vecs; c += blockDim.x) row_st<DT>(g, 8 * c, v, R::zero());
+      if (GRAD) {
+        for (uint32_t c = tid; c < vecs; c += THREADS) R::st((T*)(g + c * kBytes), R::zero());
+        if (tid < ragged) Elem<DT>::st((T*)g + vecs * 8 + tid, 0.f);
+      }
       continue;
     }
-    typename R::Raw q[kN];
-    if constexpr (NV != kStream) {
+    // loads come back in order: the first entries', needed first, lead
+    const auto entry = [&](int k, int* id, float* t) {
+      const int64_t i = ld_index(a.idx, a.idx_wide, row * a.k + k);
+      *t = ld_any(a.top, a.top_dtype, row * a.k + k);
+      *id = i >= 0 && i < v ? (int)i : -1;
+    };
+    int e_id = -1;
+    float e_t = 0.f;
+    if (wave == 0 && lane < a.k) entry(lane, &e_id, &e_t);
+    Raw q[NV > 0 ? NV : 1];
 #pragma unroll
-      for (int c = 0; c < kN; ++c)
-        q[c] = row_ld<DT>(z, 8 * ((int64_t)c * blockDim.x + tid), v, R::kNegInf);
+    for (int c = 0; c < NV; ++c) {
+      q[c] = R::fill(R::kNegInf);
+      if (c * THREADS + tid < vecs) q[c] = vec8(c * THREADS + tid);
     }
+    float xr = tid < ragged ? elem(vecs * 8 + tid) : -INFINITY;
+    next_label = label_of(row + gridDim.x);
     if (wave == 0) {
       // the teacher: entries, their probabilities, the student's logits there
       float m = -INFINITY;
       int again = 0;
       for (int k = lane; k < a.k; k += 64) {
-        const int64_t id = ld_index(a.idx, a.idx_wide, row * a.k + k);
-        const bool ok = id >= 0 && id < v;
-        const float t = ok ? ld_any(a.top, a.top_dtype, row * a.k + k) / a.tau : -INFINITY;
-        s_idx[k] = ok ? (int)id : -1;
-        s_z[k] = ok ? Elem<DT>::ld(z + id) : 0.f;
+        if (k >= 64) entry(k, &e_id, &e_t);
+        const float t = e_id >= 0 ? e_t / a.tau : -INFINITY;
+        s_idx[k] = e_id;
+        s_z[k] = e_id >= 0 ? elem(e_id) : 0.f;
         s_lp[k] = t;
         m = fmaxf(m, t);
-        if (ok) again |= atomicOr(&bits[id >> 5], 1u << (id & 31)) >> (id & 31) & 1;
+        if (e_id >= 0)
+          again |= atomicOr(&bits[e_id >> 5], 1u << (e_id & 31)) >> (e_id & 31) & 1;
       }
       again = __ballot(again) != 0;
       float base, sum = 0.f;
       if (tail) {
         base = a.lse[row];
       } else {
-        m = base_of(wave_max(m));
+        m = wave_max(m);
+        m = m == -INFINITY ? 0.f : m;
         for (int k = lane; k < a.k; k += 64) sum += exp2_fast((s_lp[k] - m) * kLog2e);
         sum = wave_sum(sum);
         base = m + __log2f(sum) * kLn2;
@@ -199,168 +255,205 @@ __global__ __launch_bounds__(1024) void distill_kernel(Args a) {
         mass += p;
       }
       mass = wave_sum(mass);
-      float mz = -INFINITY, st = 0.f, s1 = 0.f;
-      if (tail) {
-        for (int k = lane; k < a.k; k += 64)
-          if (s_idx[k] >= 0) mz = fmaxf(mz, s_z[k]);
-        mz = wave_max(mz);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        for (int k = lane; k < a.k; k += 64) {
-          if (s_idx[k] < 0 || (again && !first_of(s_idx, k))) continue;
-          const float y = s_z[k] - base_of(mz);
-          st += exp2_fast(y * kt);
-          if (two) s1 += exp2_fast(y * k1);
-        }
-        st = wave_sum(st);
-        s1 = wave_sum(s1);
-      }
       if (lane == 0) {
         teach.rest = tail ? fmaxf(0.f, 1.f - mass) : 0.f;
         teach.mass = mass;
-        teach.z_label = hard ? Elem<DT>::ld(z + label) : 0.f;
+        teach.z_label = hard ? elem(label) : 0.f;
         teach.repeated = again;
-        teach.m = mz, teach.st = st, teach.s1 = s1;
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    if (tail) __syncthreads();   // the bits are read below
-
-    // maximum and sums over the thread's columns
-    float m = -INFINITY, st = 0.f, s1 = 0.f;
-    if constexpr (NV != kStream) {
+    if (tail) {
+      // the entries' columns leave the row: the first wavefront has them, and what
+      // the block sums is the rest, about a maximum of its own
+      __syncthreads();
 #pragma unroll
-      for (int c = 0; c < kN; ++c) {
+      for (int c = 0; c < NV; ++c) {
+        const uint32_t vec = c * THREADS + tid;
+        const uint32_t top = vec < vecs ? bits[vec >> 2] >> (8 * (vec & 3)) & 255 : 0;
+        if (top) R::mask(q[c], top, R::kNegInf);
+      }
+      if (tid < ragged && bits[vecs >> 2] >> (8 * (vecs & 3) + tid) & 1) xr = -INFINITY;
+    }
+    // columns past the registers are read again: with a tail, without the entries'
+    float shift = 0.f;
+    const auto again8 = [&](uint32_t vec, float x[8]) {
+      Raw r = vec8(vec);
+      if (tail) {
+        const uint32_t top = bits[vec >> 2] >> (8 * (vec & 3)) & 255;
+        if (top) R::mask(r, top, R::kNegInf);
+      }
+      R::unpack(r, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] -= shift;
+    };
+
+    float m, st, s1, c_t, c_1, sr, m_row;
+    for (;;) {
+      // maximum and sums over the thread's columns
+      m = xr;
+      st = s1 = 0.f;
+      float ct = 0.f, c1 = 0.f;
+      const auto add = [&](float x) {
+        const float et = exp2_fast(fmaf(x, kt, -ct));
+        st += et;
+        if (POW == 1) s1 += exp2_fast(fmaf(x, k1, -c1));
+        if (POW == 2) s1 = fmaf(et, et, s1);
+      };
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
         float x[8];
         R::unpack(q[c], x);
-        if (tail) {
-          mask(x, 8 * ((int64_t)c * blockDim.x + tid));
-          q[c] = R::pack(x);
-        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) m = fmaxf(m, x[e]);
         repack<DT>(q[c]);
       }
-      const float mb = base_of(m);
+      ct = base_of(m, kt), c1 = base_of(m, k1);
 #pragma unroll
-      for (int c = 0; c < kN; ++c) {
+      for (int c = 0; c < NV; ++c) {
         float x[8];
         R::unpack(q[c], x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float y = x[e] - mb;
-          st += exp2_fast(y * kt);
-          if (two) s1 += exp2_fast(y * k1);
-        }
+        for (int e = 0; e < 8; ++e) add(x[e]);
         repack<DT>(q[c]);
       }
-    } else {
-      for (int64_t c = tid; c < vecs; c += blockDim.x) {
+      for (uint32_t vec = NV * THREADS + tid; vec < vecs; vec += THREADS) {
         float x[8], mc = m;
-        R::unpack(row_ld<DT>(z, 8 * c, v, R::kNegInf), x);
-        mask(x, 8 * c);
+        again8(vec, x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) mc = fmaxf(mc, x[e]);
-        const float mb = base_of(mc);
-        const float back = m == -INFINITY ? 0.f : m - mb;
-        st *= exp2_fast(back * kt);
-        if (two) s1 *= exp2_fast(back * k1);
-        m = mc;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float y = x[e] - mb;
-          st += exp2_fast(y * kt);
-          if (two) s1 += exp2_fast(y * k1);
+        if (mc > m) {
+          const float nt = base_of(mc, kt), n1 = base_of(mc, k1);
+          st *= exp2_fast(ct - nt);
+          if (POW == 1) s1 *= exp2_fast(c1 - n1);
+          if (POW == 2) s1 *= exp2_fast(2.f * (ct - nt));
+          m = mc, ct = nt, c1 = n1;
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) add(x[e]);
       }
-    }
-    // over the wavefront, then the block: sums are brought to the common maximum.  A
-    // maximum of -inf comes with sums of 0, or of NaN where every logit is NaN: both
-    // stay as they are
-    {
-      const float mw = wave_max(m), back = base_of(m) - base_of(mw);
-      st = wave_sum(m == -INFINITY ? st : st * exp2_fast(back * kt));
-      if (two) s1 = wave_sum(m == -INFINITY ? s1 : s1 * exp2_fast(back * k1));
+      add(xr);
+      // over the wavefront, then the block: sums are brought to the common base
+      const float mw = wave_max(m), cw = base_of(mw, kt);
+      st = wave_sum(st * exp2_fast(ct - cw));
+      if (POW == 1) s1 = wave_sum(s1 * exp2_fast(c1 - base_of(mw, k1)));
+      if (POW == 2) s1 = wave_sum(s1 * exp2_fast(2.f * (ct - cw)));
       if (lane == 0) {
         red_m[turn][wave] = mw;
         red_t[turn][wave] = st;
-        red_1[turn][wave] = s1;
+        if (POW) red_1[turn][wave] = s1;
       }
+      if (tail && wave == 0) {
+        // the same over the entries' columns, each once
+        float me = -INFINITY, te = 0.f, e1 = 0.f;
+        for (int k = lane; k < a.k; k += 64)
+          if (s_idx[k] >= 0) me = fmaxf(me, s_z[k] - shift);
+        me = wave_max(me);
+        for (int k = lane; k < a.k; k += 64) {
+          if (s_idx[k] < 0 || (teach.repeated && !first_of(s_idx, k))) continue;
+          const float et = exp2_fast(fmaf(s_z[k] - shift, kt, -base_of(me, kt)));
+          te += et;
+          if (POW == 1) e1 += exp2_fast(fmaf(s_z[k] - shift, k1, -base_of(me, k1)));
+          if (POW == 2) e1 = fmaf(et, et, e1);
+        }
+        te = wave_sum(te);
+        e1 = wave_sum(e1);
+        if (lane == 0) teach.m = me, teach.st = te, teach.s1 = e1;
+      }
+      __syncthreads();
+      {
+        const int w = lane & (kMaxWaves - 1);
+        const float mw = red_m[turn][w];
+        m = row16_max(mw);
+        c_t = base_of(m, kt), c_1 = POW == 2 ? 2.f * c_t : base_of(m, k1);
+        st = row16_sum(red_t[turn][w] * exp2_fast(base_of(mw, kt) - c_t));
+        if (POW == 1) s1 = row16_sum(red_1[turn][w] * exp2_fast(base_of(mw, k1) - c_1));
+        if (POW == 2) s1 = row16_sum(red_1[turn][w] * exp2_fast(2.f * (base_of(mw, kt) - c_t)));
+      }
+      turn ^= 1;
+      m_row = tail ? fmaxf(m, teach.m) : m;
+      if (shift != 0.f || fabsf(base_of(m_row, kt)) < kFar || fabsf(m_row) == INFINITY) break;
+      // a row of nothing but far values (masked by the type's lowest): move it to 0
+      shift = m_row;
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
+        float x[8];
+        R::unpack(q[c], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] -= shift;
+        q[c] = R::pack(x);
+      }
+      xr -= shift;
+      __syncthreads();   // `teach` is written again
     }
-    __syncthreads();
-    m = -INFINITY;
-    for (int w = 0; w < waves; ++w) m = fmaxf(m, red_m[turn][w]);
-    const float mb = base_of(m);
-    st = s1 = 0.f;
-    for (int w = 0; w < waves; ++w) {
-      const float mw = red_m[turn][w], back = base_of(mw) - mb;
-      const float t = red_t[turn][w], u = red_1[turn][w];
-      st += mw == -INFINITY ? t : t * exp2_fast(back * kt);
-      if (two) s1 += mw == -INFINITY ? u : u * exp2_fast(back * k1);
-    }
-    turn ^= 1;
-    // the block's maximum and sum (the rest's, with a tail) and the whole row's
-    const float sr = st;
-    float mz = mb, c_t = 1.f, c_1 = 1.f;
+    // c_t, c_1: the base of the block's sums.  sr: its sum (the rest's, with a tail);
+    // st, s1: the whole row's, about b_t and b_1, u_t and u_1 apart
+    sr = st;
+    float b_t = c_t, b_1 = c_1, u_t = 1.f, u_1 = 1.f;
     if (tail) {
-      const float mt = teach.m;
-      mz = base_of(fmaxf(m, mt));
-      c_t = exp2_fast((mb - mz) * kt);
-      c_1 = exp2_fast((mb - mz) * k1);
-      // an empty side's sum is 0 whatever its factor
-      if (m == -INFINITY) c_t = c_1 = 1.f;
-      const float back = mt == -INFINITY ? 0.f : base_of(mt) - mz;
-      st = st * c_t + teach.st * exp2_fast(back * kt);
-      if (two) s1 = s1 * c_1 + teach.s1 * exp2_fast(back * k1);
+      const float et = base_of(teach.m, kt), e1 = POW == 2 ? 2.f * et : base_of(teach.m, k1);
+      b_t = fmaxf(c_t, et), b_1 = fmaxf(c_1, e1);
+      u_t = exp2_fast(c_t - b_t), u_1 = exp2_fast(c_1 - b_1);
+      st = st * u_t + teach.st * exp2_fast(et - b_t);
+      if (POW) s1 = s1 * u_1 + teach.s1 * exp2_fast(e1 - b_1);
     }
-    if (!two) s1 = st, c_1 = c_t;
-    const float log_st = __log2f(st) * kLn2, log_s1 = __log2f(s1) * kLn2;
+    if (!POW) s1 = st, b_1 = b_t, u_1 = u_t;
+    if (st == INFINITY) st = s1 = NAN;   // +inf among the logits
+    const float l_t = __log2f(st), l_1 = __log2f(s1);   // of the row's sums, less b_t and b_1
     const float rest = sr == 0.f ? 0.f : teach.rest;
     const float mass = teach.mass + rest;   // P
     if (wave == 0) {
       float soft = 0.f;
       for (int k = lane; k < a.k; k += 64) {
         const float p = s_p[k];
-        if (p != 0.f) soft += p * (s_lp[k] - ((s_z[k] - mz) / a.tau - log_st));
+        if (p != 0.f) soft += p * (s_lp[k] - kLn2 * (fmaf(s_z[k] - shift, kt, -b_t) - l_t));
       }
       soft = wave_sum(soft);
-      if (rest > 0.f)
-        soft += rest * (__log2f(rest) * kLn2 - (__log2f(sr) * kLn2 + (mb - mz) / a.tau - log_st));
+      if (rest > 0.f) soft += rest * kLn2 * (__log2f(rest) - (__log2f(sr) - l_t + (c_t - b_t)));
       if (lane == 0) {
         float loss = a.alpha * a.tau * a.tau * soft;
-        if (hard) loss += (1.f - a.alpha) * (log_s1 - (teach.z_label - mz));
+        if (hard) loss += (1.f - a.alpha) * kLn2 * (l_1 - fmaf(teach.z_label - shift, k1, -b_1));
         a.row_loss[row] = loss;
       }
     }
-    if (g) {
+    if constexpr (GRAD) {
       const float go = norm * (a.grad_out ? a.grad_out[a.grad_out_rows ? row : 0] : 1.f);
       const float cs = go * a.alpha * a.tau, ch = go * (1.f - a.alpha);
-      // factors of e_tau and e_1 (about mz at an entry, about mb elsewhere)
+      // factors of the exponentials: about the row's base at an entry, the block's elsewhere
       const float f_top = cs * mass / st, f_top1 = ch / s1;
-      const float f_t = f_top * c_t - (rest > 0.f ? cs * rest / sr : 0.f), f_1 = f_top1 * c_1;
-      auto grad_of = [&](float x) {
-        const float y = x - mb, et = exp2_fast(y * kt);
-        float d = f_t * et;
-        if (two)
-          d += f_1 * exp2_fast(y * k1);
-        else if (hard)
-          d += f_1 * et;
-        return d;
+      float f_t = f_top * u_t - (rest > 0.f ? cs * rest / sr : 0.f), f_1 = f_top1 * u_1;
+      if (!POW) f_t += f_1;   // one softmax for both terms (f_1 is 0 without labels' term)
+      const auto grad_of = [&](float x) {
+        const float et = exp2_fast(fmaf(x, kt, -c_t));
+        if (POW == 1) return fmaf(f_t, et, f_1 * exp2_fast(fmaf(x, k1, -c_1)));
+        if (POW == 2) return et * fmaf(f_1, et, f_t);
+        return f_t * et;
       };
-      auto grad8 = [&](const typename R::Raw& raw, int64_t j) {
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
+        const uint32_t vec = c * THREADS + tid;
         float x[8];
-        R::unpack(raw, x);
+        R::unpack(q[c], x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = grad_of(x[e]);
-        row_st<DT>(g, j, v, R::pack(x));
-      };
-      if constexpr (NV != kStream) {
-#pragma unroll
-        for (int c = 0; c < kN; ++c) grad8(q[c], 8 * ((int64_t)c * blockDim.x + tid));
-      } else {
-        for (int64_t c = tid; c < vecs; c += blockDim.x)
-          grad8(row_ld<DT>(z, 8 * c, v, R::kNegInf), 8 * c);
+        if (vec < vecs) R::st((T*)(g + vec * kBytes), R::pack(x));
       }
+      for (uint32_t vec = NV * THREADS + tid; vec < vecs; vec += THREADS) {
+        float x[8];
+        again8(vec, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = grad_of(x[e]);
+        R::st((T*)(g + vec * kBytes), R::pack(x));
+      }
+      if (tid < ragged) Elem<DT>::st((T*)g + vecs * 8 + tid, grad_of(xr));
       __syncthreads();   // the columns below are written again
       if (wave == 0) {
+        const auto top_of = [&](float x) {
+          const float et = exp2_fast(fmaf(x, kt, -b_t));
+          if (POW == 1) return fmaf(f_top, et, f_top1 * exp2_fast(fmaf(x, k1, -b_1)));
+          if (POW == 2) return et * fmaf(f_top1, et, f_top);
+          return (f_top + f_top1) * et;
+        };
         for (int k = lane; k < a.k; k += 64) {
           const int id = s_idx[k];
           if (id < 0) continue;
@@ -369,13 +462,10 @@ __global__ __launch_bounds__(1024) void distill_kernel(Args a) {
             p = 0.f;
             for (int i = 0; i < a.k; ++i) p += s_idx[i] == id ? s_p[i] : 0.f;
           }
-          const float y = s_z[k] - mz, et = exp2_fast(y * kt);
-          float x = f_top * et - cs * p;
-          if (hard) x += f_top1 * (two ? exp2_fast(y * k1) : et) - (id == label ? ch : 0.f);
-          Elem<DT>::st(g + id, x);
+          Elem<DT>::st((T*)g + id, top_of(s_z[k] - shift) - cs * p - (id == label ? ch : 0.f));
         }
         if (hard && lane == 0 && !(bits[label >> 5] >> (label & 31) & 1))
-          Elem<DT>::st(g + label, grad_of(teach.z_label) - ch);
+          Elem<DT>::st((T*)g + label, grad_of(teach.z_label - shift) - ch);
       }
     }
     if (wave == 0) {
@@ -385,25 +475,27 @@ __global__ __launch_bounds__(1024) void distill_kernel(Args a) {
     }
     // the first wavefront writes `teach` again for the next row: all have read it
     // before the barrier above, where there is one
-    if (!g) __syncthreads();
+    if (!GRAD) __syncthreads();
   }
 }
 
 constexpr int kSumThreads = 1024;
 
-// The rows' losses to one: their sum, over the rows that count for a mean.
-__global__ __launch_bounds__(kSumThreads) void total_kernel(Args a, float* loss) {
+// The rows' losses to one: their sum, or over the count that stands in its place.
+__global__ __launch_bounds__(kSumThreads) void total_kernel(Args a) {
   __shared__ float tmp[kMaxWaves];
-  const int64_t live = a.mean ? count_live(a, tmp) : 1;
+  const float count = a.mean && a.rows > 0 ? *a.loss : 1.f;
   float s = 0.f;
+#pragma unroll 8
   for (int64_t r = threadIdx.x; r < a.rows; r += kSumThreads) s += a.row_loss[r];
   s = wave_sum(s);
   if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x > 0) return;
   s = 0.f;
+#pragma unroll
   for (int w = 0; w < kMaxWaves; ++w) s += tmp[w];
-  *loss = s / (float)(live > 0 ? live : 1);
+  *a.loss = s / count;
 }
 
 // x[row] *= f (one factor, or one per row): nothing is read where it is 1.
@@ -428,18 +520,38 @@ __global__ __launch_bounds__(256) void scale_kernel(void* x, int64_t rows, int64
 
 inline int launched() { return hipGetLastError() == hipSuccess ? kOk : kErrLaunch; }
 
-// Columns up to 32768: four vectors a thread of as few threads as hold the row;
-// then eight of 1024 threads; wider rows are read twice.
-int vectors(int64_t v, int* threads) {
-  const int64_t vecs = (v + 7) / 8;
-  *threads = 1024;
-  if (vecs <= 256) return *threads = 256, 1;
-  if (vecs <= 512) return *threads = 256, 2;
-  if (vecs <= 1024) return *threads = 256, 4;
-  if (vecs <= 2048) return *threads = 512, 4;
-  if (vecs <= 4096) return 4;
-  if (vecs <= 8192) return 8;
-  return kStream;
+// Launches one shape of block.  As many blocks as can run at a time go over the rows.
+template <int DT, int NV, bool GRAD, int THREADS, int WAVES>
+int launch(const Args& a, hipStream_t st) {
+  const bool two = a.alpha != 1.f && a.tau != 1.f;
+  const int64_t most = 256 * (WAVES * 256 / THREADS);
+  const unsigned grid = (unsigned)(a.rows < most ? a.rows : most);
+  const size_t lds = 16 * (size_t)a.k + (size_t)(a.vocab + 31) / 32 * 4;
+  const auto kern = !two           ? distill_kernel<DT, NV, 0, GRAD, THREADS, WAVES>
+                    : a.tau == 2.f ? distill_kernel<DT, NV, 2, GRAD, THREADS, WAVES>
+                                   : distill_kernel<DT, NV, 1, GRAD, THREADS, WAVES>;
+  if (lds > 62 * 1024 &&
+      hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
+                          (int)lds) != hipSuccess)
+    return kErrLaunch;
+  kern<<<grid, THREADS, lds, st>>>(a);
+  return launched();
+}
+
+// Threads of a row's block and the vectors each keeps of it for the gradient.
+template <int DT>
+int launch(const Args& a, hipStream_t st) {
+  const int64_t vecs = a.vocab / 8;
+  if (!a.grad)
+    return vecs <= 1024 ? launch<DT, 0, false, 256, 8>(a, st)
+                        : launch<DT, 0, false, 512, 8>(a, st);
+  if (vecs <= 128) return launch<DT, 1, true, 128, 6>(a, st);
+  if (vecs <= 256) return launch<DT, 2, true, 128, 6>(a, st);
+  if (vecs <= 512) return launch<DT, 4, true, 128, 4>(a, st);
+  constexpr int kFull = DT == kF32 ? 4 : 8, kWide = DT == kF32 ? 2 : 1;
+  if (vecs <= 1024) return launch<DT, kFull, true, 128 * kWide, 4>(a, st);
+  if (vecs <= 2048) return launch<DT, kFull, true, 256 * kWide, 4>(a, st);
+  return launch<DT, kFull, true, 512 * kWide, 4>(a, st);
 }
 
 }  // namespace distill
@@ -462,7 +574,7 @@ int cpt_distill_topk(int dtype, const void* logits, int64_t rows, int64_t vocab,
       ld_batch < 0 || ld_row < 0 || gld_batch < 0 || gld_row < 0)
     return kErrShape;
   // LDS: 16 bytes an entry and a bit a column
-  if (k > kMaxEntries || vocab > kMaxVocab) return kErrTooLarge;
+  if (k > kMaxEntries || vocab > kMaxVocab || rows > 0x7FFFFFFF) return kErrTooLarge;
   if (reduction != 2 && !loss) return kErrShape;
   if (alpha != 1.f && !labels && rows > 0) return kErrShape;
   if (rows > 0 && (!logits || !row_loss || seq < 1 || (k > 0 && (!top_logits || !top_indices))))
@@ -471,40 +583,15 @@ int cpt_distill_topk(int dtype, const void* logits, int64_t rows, int64_t vocab,
   Args a{rows, vocab, logits, seq, ld_batch, ld_row, grad, gld_batch, gld_row, top_logits,
          top_indices, top_dtype, idx_wide, (int)k, (const float*)top_lse, labels, label_wide,
          ignore_index, temperature, alpha, grad_scale, (const float*)grad_out, reduction == 2,
-         reduction == 0, (float*)row_loss};
+         reduction == 0, (float*)row_loss, (float*)loss};
   if (rows > 0) {
-    int threads;
-    const int nv = vectors(vocab, &threads);
-    const int64_t most = 256 * (2048 / threads);   // as many blocks as can run at a time
-    const unsigned grid = (unsigned)(rows < most ? rows : most);
-    const size_t lds = 16 * (size_t)k + (size_t)(vocab + 31) / 32 * 4;
-#define CPT_DISTILL(DT, NV)                                                              \
-  do {                                                                                  \
-    if (lds > 62 * 1024 &&                                                              \
-        hipFuncSetAttribute((const void*)distill_kernel<DT, NV>,                        \
-                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) \
-      return kErrLaunch;                                                                \
-    distill_kernel<DT, NV><<<grid, threads, lds, st>>>(a);                              \
-  } while (0)
-#define CPT_DISTILL_NV(DT)                      \
-  switch (nv) {                                 \
-    case 1: CPT_DISTILL(DT, 1); break;          \
-    case 2: CPT_DISTILL(DT, 2); break;          \
-    case 4: CPT_DISTILL(DT, 4); break;          \
-    case 8: CPT_DISTILL(DT, 8); break;          \
-    default: CPT_DISTILL(DT, kStream); break;   \
-  }
-    if (dtype == kF32) {
-      CPT_DISTILL_NV(kF32)
-    } else if (dtype == kF16) {
-      CPT_DISTILL_NV(kF16)
-    } else {
-      CPT_DISTILL_NV(kBF16)
-    }
-    if (launched() != kOk) return kErrLaunch;
+    const int rc = dtype == kF32   ? launch<kF32>(a, st)
+                   : dtype == kF16 ? launch<kF16>(a, st)
+                                   : launch<kBF16>(a, st);
+    if (rc != kOk) return rc;
   }
   if (reduction != 2) {
-    total_kernel<<<1, kSumThreads, 0, st>>>(a, (float*)loss);
+    total_kernel<<<1, kSumThreads, 0, st>>>(a);
     return launched();
   }
   return kOk;

@@ -68,7 +68,19 @@ template <int DT> struct Row8Half {   // 16-bit formats
     }
     return r;
   }
-  static __device__ __forceinline__ Raw zero() { return Raw{u32x4{0, 0, 0, 0}}; }
+  static __device__ __forceinline__ Raw fill(uint32_t bits) {
+    const uint32_t w = bits | (bits << 16);
+    return Raw{u32x4{w, w, w, w}};
+  }
+  static __device__ __forceinline__ Raw zero() { return fill(0); }
+  // `bits` in the elements whose bit of `which` is set
+  static __device__ __forceinline__ void mask(Raw& r, uint32_t which, uint32_t bits) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (which >> (2 * j) & 1) r.w[j] = (r.w[j] & 0xFFFF0000u) | bits;
+      if (which >> (2 * j + 1) & 1) r.w[j] = (r.w[j] & 0xFFFFu) | (bits << 16);
+    }
+  }
 };
 template <> struct Row8<kBF16> : Row8Half<kBF16> {
   static constexpr uint32_t kNegInf = 0xFF80u;
@@ -121,8 +133,16 @@ template <> struct Row8<kF32> {
     }
     return r;
   }
-  static __device__ __forceinline__ Raw zero() {
-    return Raw{u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
+  static __device__ __forceinline__ Raw fill(uint32_t b) {
+    return Raw{u32x4{b, b, b, b}, u32x4{b, b, b, b}};
+  }
+  static __device__ __forceinline__ Raw zero() { return fill(0); }
+  static __device__ __forceinline__ void mask(Raw& r, uint32_t which, uint32_t bits) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (which >> j & 1) r.w[j] = bits;
+      if (which >> (4 + j) & 1) r.x[j] = bits;
+    }
   }
 };
 
