@@ -6,14 +6,15 @@
 // The lookup is HBM-bound: one thread per eight columns.
 //
 // The gradient adds no floats atomically.  The tokens' (id, position) pairs are
-// sorted by id with their order kept (a radix sort of 8 bits a pass, each pass
-// ranking 2048 pairs a block by ballots), so one id's tokens lie side by side in
-// the order of the batch.  The sorted list is cut into tiles of equal length,
-// whatever ids they hold, so a frequent token's rows are spread over as many
-// wavefronts as it needs: a wavefront sums 512 columns of one tile in fp32,
-// writes each id that lies wholly inside it, and leaves the sums of an id that
-// goes on over a tile's edge to be joined in tile order.  The result is the same
-// from run to run.  Bound by HBM: dy is read once, the table written once.
+// sorted by id with their order kept, so one id's tokens lie side by side in the
+// order of the batch: up to 16384 tokens by counting each one's smaller ids in one
+// launch, beyond by a radix sort of 8 bits a pass (a block ranks 2048 pairs by
+// ballots).  The table's zeros are written by further blocks of the same launches:
+// sorting is latency and compares, the zeros are HBM.  The sorted list is cut into
+// tiles of equal length, whatever ids they hold, so a frequent token's rows are
+// spread over as many wavefronts as it needs; sums of an id over several tiles are
+// joined in tile order.  The result is the same from run to run.  Bound by HBM: dy
+// is read once, the table written once (rows with tokens twice).
 
 #include "compact_amd.h"
 #include "row_ops.h"
@@ -76,36 +77,61 @@ __device__ __forceinline__ uint32_t token_key(const void* ids, int wide, int64_t
   return id >= 0 && id < vocab && id != padding ? (uint32_t)id : (uint32_t)vocab;
 }
 
-// counts[0][block][digit] of the lowest digit, and zeros for the later passes'.
-__global__ __launch_bounds__(kBlock) void count_kernel(const void* __restrict__ ids, int wide,
+// The share of the table's zeros that a launch of the sort writes beside it, in
+// blocks past its own.
+struct Zeros {
+  void* out;
+  int64_t begin, end;   // elements, of a row type
+  unsigned first;       // block
+};
+template <int OT>
+__device__ __forceinline__ bool zeros_here(const Zeros& z) {
+  if (blockIdx.x < z.first) return false;
+  using R = Row8<OT>;
+  const int64_t step = (int64_t)(gridDim.x - z.first) * blockDim.x * 8;
+  int64_t i = z.begin + 8 * ((int64_t)(blockIdx.x - z.first) * blockDim.x + threadIdx.x);
+  for (; i < z.end; i += step) row_st<OT>((typename R::T*)z.out, i, z.end, R::zero());
+  return true;
+}
+
+// counts[block][digit] of the pairs' digit (key >> shift) & 255 (of the tokens
+// themselves where `in` is null).
+template <int OT>
+__global__ __launch_bounds__(kBlock) void count_kernel(const Pair* __restrict__ in,
+                                                       const void* __restrict__ ids, int wide,
                                                        int64_t n, int64_t vocab, int64_t padding,
-                                                       int passes, uint32_t* counts) {
+                                                       int shift, uint32_t* __restrict__ counts,
+                                                       Zeros zeros) {
   __shared__ uint32_t hist[kRadix];
+  if (zeros_here<OT>(zeros)) return;
   hist[threadIdx.x] = 0;
   __syncthreads();
   const int64_t i0 = (int64_t)blockIdx.x * kSortTile;
+#pragma unroll
   for (int k = 0; k < kItems; ++k) {
     const int64_t i = i0 + k * kBlock + threadIdx.x;
-    if (i < n) atomicAdd(&hist[token_key(ids, wide, i, vocab, padding) & (kRadix - 1)], 1u);
+    if (i >= n) continue;
+    const uint32_t key = in ? in[i].id : token_key(ids, wide, i, vocab, padding);
+    atomicAdd(&hist[(key >> shift) & (kRadix - 1)], 1u);
   }
   __syncthreads();
-  for (int p = 0; p < passes; ++p)
-    counts[((int64_t)p * gridDim.x + blockIdx.x) * kRadix + threadIdx.x] =
-        p == 0 ? hist[threadIdx.x] : 0;
+  counts[(int64_t)blockIdx.x * kRadix + threadIdx.x] = hist[threadIdx.x];
 }
 
 // One pass of the sort: pairs of `in` (the tokens themselves in the first) to
 // their places by digit (key >> shift) & 255, equal digits in their order.
-// `next` (null in the last pass) collects the next digit's counts by block.
+template <int OT>
 __global__ __launch_bounds__(kBlock) void scatter_kernel(const Pair* __restrict__ in,
                                                          const void* __restrict__ ids, int wide,
                                                          int64_t n, int64_t vocab, int64_t padding,
                                                          int shift,
                                                          const uint32_t* __restrict__ counts,
-                                                         uint32_t* next, Pair* __restrict__ out) {
+                                                         unsigned blocks, Pair* __restrict__ out,
+                                                         Zeros zeros) {
   __shared__ uint32_t wave_count[kWaves][kRadix];
   __shared__ uint32_t base[kRadix];
   __shared__ uint32_t scan[kWaves];
+  if (zeros_here<OT>(zeros)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (int w = 0; w < kWaves; ++w) wave_count[w][tid] = 0;
   __syncthreads();
@@ -140,7 +166,7 @@ __global__ __launch_bounds__(kBlock) void scatter_kernel(const Pair* __restrict_
   // thread t: where digit t starts for this block
   uint32_t total = 0, mine = 0;
 #pragma unroll 8
-  for (unsigned b = 0; b < gridDim.x; ++b) {
+  for (unsigned b = 0; b < blocks; ++b) {
     const uint32_t c = counts[(int64_t)b * kRadix + tid];
     mine += b < blockIdx.x ? c : 0;
     total += c;
@@ -167,11 +193,58 @@ __global__ __launch_bounds__(kBlock) void scatter_kernel(const Pair* __restrict_
   for (int k = 0; k < kItems; ++k) {
     if (i0 + k * 64 >= n) continue;
     const uint32_t digit = (q[k].id >> shift) & (kRadix - 1);
-    const uint32_t to = base[digit] + wave_count[wave][digit] + rank[k];
-    out[to] = q[k];
-    if (next)
-      atomicAdd(&next[(int64_t)(to / kSortTile) * kRadix + ((q[k].id >> (shift + 8)) & 255)], 1u);
+    out[base[digit] + wave_count[wave][digit] + rank[k]] = q[k];
   }
+}
+
+// The sort of a short list in one launch, beside the table's zeros: a token's
+// place is the number of tokens with a smaller id, or the same one earlier.  Blocks
+// [0, rank_blocks) count for 64 tokens each, 64 compares an instruction and a
+// population count on the scalar unit (n^2 / 64 vector instructions in all: 1 us of
+// the chip at 8192 tokens), while the other blocks, bound by HBM, write zeros.
+constexpr int kRankThreads = 1024;
+constexpr int kRankWaves = kRankThreads / 64;
+constexpr int kRankChunks = 8;   // 64 keys each, held by a wavefront at a time
+
+template <int OT>
+__global__ __launch_bounds__(kRankThreads) void rank_kernel(const void* __restrict__ ids, int wide,
+                                                            int64_t n, int64_t vocab,
+                                                            int64_t padding,
+                                                            Pair* __restrict__ pairs,
+                                                            Zeros zeros) {
+  __shared__ int part[kRankWaves][64];
+  if (zeros_here<OT>(zeros)) return;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int chunks = (int)((n + 63) / 64), own = blockIdx.x;
+  const int64_t at = (int64_t)own * 64 + lane;
+  // past the end: a key above every other
+  const uint32_t key = at < n ? token_key(ids, wide, at, vocab, padding) : ~0u;
+  int rank = 0;
+  for (int c0 = wave * kRankChunks; c0 < chunks; c0 += kRankWaves * kRankChunks) {
+    uint32_t k[kRankChunks];
+#pragma unroll
+    for (int c = 0; c < kRankChunks; ++c) {
+      const int64_t i = (int64_t)(c0 + c) * 64 + lane;
+      // equal keys count where they come earlier: in the chunks before this one
+      k[c] = i < n ? token_key(ids, wide, i, vocab, padding) : ~0u;
+      if (c0 + c >= own && i < n) ++k[c];
+    }
+    for (int t = 0; t < 64; ++t) {
+      const uint32_t mine = (uint32_t)__builtin_amdgcn_readlane((int)key, t);
+      int below = 0;
+#pragma unroll
+      for (int c = 0; c < kRankChunks; ++c) below += __popcll(__ballot(k[c] <= mine));
+      if (lane == t) rank += below;
+    }
+  }
+  part[wave][lane] = rank;
+  __syncthreads();
+  if (wave > 0 || at >= n) return;
+  for (int w = 1; w < kRankWaves; ++w) rank += part[w][lane];
+  for (int t = 0; t < 64; ++t)   // the own chunk's equal keys
+    rank += (uint32_t)__builtin_amdgcn_readlane((int)key, t) == key && t < lane;
+  pairs[rank] = Pair{key, (uint32_t)at};
 }
 
 // ---------------------------------------------------------------------------
@@ -187,126 +260,192 @@ __global__ __launch_bounds__(kBlock) void zero_kernel(void* out, int64_t total) 
     row_st<DT>((typename R::T*)out, i, total, R::zero());
 }
 
-template <int OT>
-__device__ __forceinline__ void write_row(void* out, int64_t v, int64_t j, int64_t d, float scale,
-                                          int accumulate, const float acc[8]) {
+template <int OT, bool TINY, bool ADD>
+__device__ __forceinline__ void write_row(void* out, int64_t v, const Cols<OT, TINY>& cols,
+                                          int64_t d, float scale, const float acc[8]) {
   using R = Row8<OT>;
   typename R::T* row = (typename R::T*)out + v * d;
   float r[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) r[e] = acc[e] * scale;
-  if (accumulate) {
+  if (ADD) {
     float o[8];
-    R::unpack(row_ld<OT>(row, j, d, 0), o);
+    R::unpack(cols.ld(row), o);
 #pragma unroll
     for (int e = 0; e < 8; ++e) r[e] += o[e];
+    cols.st_own(row, R::pack(r));
+  } else {
+    cols.st(row, R::pack(r));
   }
-  row_st<OT>(row, j, d, R::pack(r));
 }
 
-// grid (tiles, columns / 512 / 4): a wavefront sums 512 columns of one tile.
-// edge: fp32 [tiles][2][d]: sums of the id that came in over the tile's first
-// edge (0), and of the id that starts inside and goes on past its end (1).
-template <int DT, int OT>
+// A wavefront sums 512 columns of the ids that begin in one tile of TILE sorted
+// tokens.  The tile's last id is followed to its end if that lies in the next
+// tile (which then leaves it out): 2 TILE pairs, one a lane.  An id that goes on
+// further is summed tile by tile; `edge` (fp32 [tiles][2][d]) takes the sums of
+// the tile that it begins in (1) and of those that it runs on into (0).
+constexpr int kAhead = 4;   // rows loaded while as many are added
+
+template <int DT, int OT, bool TINY, bool ADD, int TILE>
 __global__ __launch_bounds__(kBlock) void sum_kernel(const void* __restrict__ grad, int64_t ld,
                                                      const Pair* __restrict__ pairs, int64_t n,
-                                                     int64_t vocab, int64_t d, int tile,
-                                                     float scale, int accumulate, void* out,
-                                                     float* edge) {
+                                                     int64_t vocab, int64_t d, unsigned strips,
+                                                     float scale, void* out, float* edge) {
   using R = Row8<DT>;
   using T = typename R::T;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t j = ((int64_t)blockIdx.y * kWaves + wave) * kCols + 8 * lane;
-  if (j - 8 * lane >= d) return;
-  const int64_t i0 = (int64_t)blockIdx.x * tile;
-  const int64_t i1 = min(n, i0 + tile);
+  const int lane = threadIdx.x & 63;
+  const uint32_t unit = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t t = unit / strips, i0 = t * TILE;
+  const int64_t j = (unit - t * strips) * kCols + 8 * lane;
+  if (i0 >= n) return;
+  const Cols<DT, TINY> cols(j, d);
+  const Cols<OT, TINY> to(j, d);
+  const Cols<kF32, TINY> sums(j, d);
   const uint32_t none = (uint32_t)vocab;
-  uint32_t id = pairs[i0].id;
-  bool entered = i0 > 0 && pairs[i0 - 1].id == id;
-  float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  constexpr int kAhead = 8;
-  for (int64_t i = i0; i < i1 && id != none; i += kAhead) {
-    Pair p[kAhead];
-    typename R::Raw q[kAhead];
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      p[k] = i + k < i1 ? pairs[i + k] : Pair{none, 0};
-      q[k] = p[k].id != none ? row_ld<DT>((const T*)grad + (int64_t)p[k].pos * ld, j, d, 0)
-                             : R::zero();
+  const Pair p = lane < 2 * TILE && i0 + lane < n ? pairs[i0 + lane] : Pair{none, 0};
+  const uint32_t first = __builtin_amdgcn_readfirstlane(p.id);
+  if (first == none) return;
+  // three ids around the tile, each in its lane (none where there is no such pair)
+  const int64_t beside = lane == 0 ? i0 - 1 : lane == 1 ? i0 - TILE - 1 : i0 + 2 * TILE;
+  const uint32_t around = beside >= 0 && beside < n ? pairs[beside].id : none;
+  const bool entered = __builtin_amdgcn_readlane(around, 0) == first;
+  const bool older = __builtin_amdgcn_readlane(around, 1) == first;   // than the last tile
+  const uint32_t far = __builtin_amdgcn_readlane(around, 2);
+  const int live = __popcll(__ballot(p.id != none));
+  const int run = __popcll(__ballot(p.id == first));
+  int begin = 0, end = live < TILE ? live : TILE;
+  bool head = false, tail = false;   // of an id that goes over further tiles
+  if (entered) {
+    if (!older && run <= TILE) {
+      begin = run;                   // the last tile has it whole
+    } else {
+      head = true;
     }
+  }
+  if (live > TILE && !(entered && run > TILE)) {
+    const uint32_t id = __builtin_amdgcn_readlane(p.id, TILE - 1);
+    const int upto = __popcll(__ballot(p.id <= id));
+    if (upto > TILE) {
+      if (upto == 2 * TILE && far == id)
+        tail = true;
+      else
+        end = upto;
+    }
+  }
+  if (begin >= end) return;
+  const uint32_t before = __shfl_up(p.id, 1);
+  const uint64_t starts = __ballot(lane > 0 && p.id != before);
+  float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  typename R::Raw q[2][kAhead];
+  const auto load = [&](int k0, typename R::Raw (&r)[kAhead]) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      if (i + k >= i1) break;
-      if (p[k].id != id) {
-        if (entered)
-          row_st<kF32>(edge + 2 * blockIdx.x * d, j, d, Row8<kF32>::pack(acc));
-        else
-          write_row<OT>(out, id, j, d, scale, accumulate, acc);
-        entered = false;
-        id = p[k].id;
+      // past the end: the last row again, not added
+      const uint32_t pos = __builtin_amdgcn_readlane(p.pos, min(k0 + k, end - 1));
+      r[k] = cols.ld((const T*)grad + (int64_t)pos * ld);
+    }
+  };
+  const auto add = [&](int k0, const typename R::Raw (&r)[kAhead]) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-        if (id == none) break;
-      }
+    for (int k = 0; k < kAhead; ++k) {
+      const int at = k0 + k;
+      if (at >= end) break;
       float v[8];
-      R::unpack(q[k], v);
+      R::unpack(r[k], v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) acc[e] += v[e];
+      const bool stop = at + 1 == end;
+      if (!stop && !(starts >> (at + 1) & 1)) continue;
+      if ((stop && tail) || (head && at < run))
+        sums.st(edge + (2 * t + (head && at < run ? 0 : 1)) * d, Row8<kF32>::pack(acc));
+      else
+        write_row<OT, TINY, ADD>(out, __builtin_amdgcn_readlane(p.id, at), to, d, scale, acc);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = 0.f;
     }
+  };
+  load(begin, q[0]);
+  for (int k = begin; k < end; k += 2 * kAhead) {
+    load(k + kAhead, q[1]);
+    add(k, q[0]);
+    load(k + 2 * kAhead, q[0]);
+    add(k + kAhead, q[1]);
   }
-  if (id == none) return;
-  const bool leaves = i1 < n && pairs[i1].id == id;
-  if (entered || leaves)
-    row_st<kF32>(edge + (2 * blockIdx.x + (entered ? 0 : 1)) * d, j, d, Row8<kF32>::pack(acc));
-  else
-    write_row<OT>(out, id, j, d, scale, accumulate, acc);
 }
 
-// grid (tiles, columns / 512): the ids that start in a tile and end in a later
-// one.  Four wavefronts add a quarter of the tiles each, then in order.
-template <int OT>
-__global__ __launch_bounds__(kBlock) void join_kernel(const Pair* __restrict__ pairs, int64_t n,
-                                                      int64_t vocab, int64_t d, int tile,
-                                                      float scale, int accumulate, void* out,
-                                                      const float* __restrict__ edge) {
-  __shared__ float part[kWaves][8][64];
-  const int64_t t0 = blockIdx.x, i1 = (t0 + 1) * tile;
-  if (i1 >= n) return;
-  const uint32_t id = pairs[i1 - 1].id;
-  if (id == (uint32_t)vocab || pairs[i1].id != id) return;
-  if (pairs[i1 - tile].id == id && t0 > 0 && pairs[i1 - tile - 1].id == id) return;
-  // the last tile that the id reaches: the first later one that does not end with it
-  // still holds its last tokens
-  int64_t lo = t0 + 1, hi = (n + tile - 1) / tile - 1;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) / 2;
-    if (pairs[min(n, (mid + 1) * tile) - 1].id == id && (mid + 1) * tile < n &&
-        pairs[(mid + 1) * tile].id == id)
-      lo = mid + 1;
-    else
-      hi = mid;
-  }
-  const int64_t count = lo - t0 + 1, per = (count + kWaves - 1) / kWaves;
+// The ids that go over three tiles or more.  A block looks at four tiles, and for
+// each such id that begins in one of them adds the tiles' sums of 512 columns:
+// each wavefront a part of the tiles, then the parts in order.
+constexpr int kJoinTiles = 4;
+constexpr int kJoinThreads = 512;
+
+template <int OT, bool TINY, bool ADD, int TILE>
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(const Pair* __restrict__ pairs, int64_t n,
+                                                      int64_t vocab, int64_t d, float scale,
+                                                      void* out, const float* __restrict__ edge) {
+  constexpr int kParts = kJoinThreads / 64;
+  __shared__ float part[kParts][8][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t j = (int64_t)blockIdx.y * kCols + 8 * lane;
-  float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  const int64_t c0 = wave * per, c1 = min(count, c0 + per);
-#pragma unroll 4
-  for (int64_t c = c0; c < c1; ++c) {
-    float v[8];
-    Row8<kF32>::unpack(row_ld<kF32>(edge + (2 * (t0 + c) + (c == 0 ? 1 : 0)) * d, j, d, 0), v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] += v[e];
+  const Cols<OT, TINY> to(j, d);
+  const Cols<kF32, TINY> sums(j, d);
+  uint32_t id = 0;
+  bool is = false;
+  {
+    const int64_t t = (int64_t)blockIdx.x * kJoinTiles + lane, i = t * TILE;
+    if (lane < kJoinTiles && i + 2 * TILE < n) {
+      id = pairs[i + TILE].id;
+      is = id != (uint32_t)vocab && pairs[i + TILE - 1].id == id &&
+           pairs[i + 2 * TILE].id == id &&
+           !(pairs[i].id == id && i > 0 && pairs[i - 1].id == id);
+    }
   }
+  for (uint64_t heads = __ballot(is); heads; heads &= heads - 1) {
+    const int h = __builtin_ctzll(heads);
+    const int64_t t0 = (int64_t)blockIdx.x * kJoinTiles + h;
+    const uint32_t v = __builtin_amdgcn_readlane(id, h);
+    // the last tile that begins with the id, 64 tiles looked at together; a long
+    // run's first 4096 and 64 apart
+    int64_t last = t0 + 2;
+    const auto reach = [&](int64_t step) {
+      const int64_t t = last + (lane + 1) * step;
+      const int r = __popcll(__ballot(t * TILE < n && pairs[min(n - 1, t * TILE)].id == v));
+      last += r * step;
+      return r;
+    };
+    if (reach(1) == 64) {
+      while (reach(4096) == 64) {}
+      reach(64);
+      reach(1);
+    }
+    const int64_t count = last - t0 + 1, per = (count + kParts - 1) / kParts;
+    const int64_t c0 = wave * per, c1 = min(count, c0 + per);
+    float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 4
+    for (int64_t c = c0; c < c1; ++c) {
+      float x[8];
+      Row8<kF32>::unpack(sums.ld(edge + (2 * (t0 + c) + (c == 0 ? 1 : 0)) * d), x);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) part[wave][e][lane] = acc[e];
-  __syncthreads();
-  if (wave > 0) return;
+      for (int e = 0; e < 8; ++e) acc[e] += x[e];
+    }
+    __syncthreads();
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    for (int w = 1; w < kWaves; ++w) acc[e] += part[w][e][lane];
-  write_row<OT>(out, id, j, d, scale, accumulate, acc);
+    for (int e = 0; e < 8; ++e) part[wave][e][lane] = acc[e];
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        for (int w = 1; w < kParts; ++w) acc[e] += part[w][e][lane];
+      write_row<OT, TINY, ADD>(out, v, to, d, scale, acc);
+    }
+  }
 }
+
+// Tokens up to which the one-launch sort is the faster: with the table's zeros
+// beside it 12000 tokens take 52 us against the radix sort's 63, 20011 (in a small
+// table) 95 against 81.
+constexpr int64_t kRankTokens = 16384;
+constexpr int kZeroThreads = 1 << 20;   // of a launch's blocks of zeros
 
 inline int launched() { return hipGetLastError() == hipSuccess ? kOk : kErrLaunch; }
 
@@ -316,13 +455,10 @@ int passes_of(int64_t vocab) {   // keys 0 .. vocab
   return (bits + 7) / 8;
 }
 
-// Tokens of a tile: 32, more where the batch still gives 4096 wavefronts (each
-// edge costs an fp32 row written and read again).
+// 16 tokens a tile where 32 would leave the chip short of wavefronts: 8192 tokens
+// of 2048 columns 41 against 44 us, 32768 91 against 86.
 int tile_of(int64_t n, int64_t d) {
-  const int64_t strips = (d + kCols - 1) / kCols;
-  int tile = 32;
-  while (tile < 256 && n * strips / (2 * tile) >= 4096) tile *= 2;
-  return tile;
+  return n * ((d + kCols - 1) / kCols) <= 40000 ? 16 : 32;
 }
 
 struct Plan {
@@ -340,16 +476,17 @@ Plan plan(int64_t n, int64_t vocab, int64_t d) {
   p.sort_blocks = (n + kSortTile - 1) / kSortTile;
   p.tiles = (n + p.tile - 1) / p.tile;
   p.counts = 0;
-  p.pairs = up(p.passes * p.sort_blocks * kRadix * 4);
+  p.pairs = up(p.sort_blocks * kRadix * 4);
   p.edge = p.pairs + 2 * up(n * (int64_t)sizeof(Pair));
   p.bytes = p.edge + up(p.tiles * 2 * d * 4);
   return p;
 }
 
 bool sizes_ok(int64_t n, int64_t vocab, int64_t d) { return n >= 0 && vocab >= 0 && d >= 0; }
-// positions and keys are 32 bits wide, a grid's second extent 16
+// positions and keys are 32 bits wide, a grid's second extent 16, its first 31
 bool too_large(int64_t n, int64_t vocab, int64_t d) {
-  return n >= (1ll << 31) || vocab >= (1ll << 31) || d > 65535ll * kCols;
+  return n >= (1ll << 31) || vocab >= (1ll << 31) || d > 65535ll * kCols ||
+         (n / 16 + 1) * (d / kCols + 1) >= (1ll << 31);
 }
 
 }  // namespace embed
@@ -398,40 +535,69 @@ int cpt_embedding_backward(int dtype, int out_dtype, const void* grad, int64_t l
   if (vocab == 0 || d == 0) return kOk;
   if (!out || (n > 0 && (!grad || !ids || !workspace))) return kErrShape;
   const hipStream_t st = (hipStream_t)stream;
-  if (!accumulate) {
-    const int64_t total = vocab * d, want = (total + 8 * kBlock - 1) / (8 * kBlock);
+  const int64_t total = accumulate ? 0 : vocab * d;
+  if (n == 0) {
+    const int64_t want = (total + 8 * kBlock - 1) / (8 * kBlock);
     const unsigned grid = (unsigned)(want < 2048 ? want : 2048);
     const auto kern = out_dtype == kF32   ? zero_kernel<kF32>
                       : out_dtype == kF16 ? zero_kernel<kF16>
                                           : zero_kernel<kBF16>;
-    kern<<<grid, kBlock, 0, st>>>(out, total);
-    if (launched() != kOk) return kErrLaunch;
+    if (total > 0) kern<<<grid, kBlock, 0, st>>>(out, total);
+    return launched();
   }
-  if (n == 0) return kOk;
   const Plan p = plan(n, vocab, d);
   uint8_t* const ws = (uint8_t*)workspace;
   uint32_t* const counts = (uint32_t*)(ws + p.counts);
   Pair* pairs[2] = {(Pair*)(ws + p.pairs), (Pair*)(ws + p.pairs + up(n * sizeof(Pair)))};
   float* const edge = (float*)(ws + p.edge);
-  const unsigned sb = (unsigned)p.sort_blocks;
-  count_kernel<<<sb, kBlock, 0, st>>>(ids, ids_wide, n, vocab, padding_idx, p.passes, counts);
-  const Pair* in = nullptr;
-  for (int k = 0; k < p.passes; ++k) {
-    uint32_t* const c = counts + (int64_t)k * sb * kRadix;
-    scatter_kernel<<<sb, kBlock, 0, st>>>(in, ids, ids_wide, n, vocab, padding_idx, 8 * k, c,
-                                          k + 1 < p.passes ? c + (int64_t)sb * kRadix : nullptr,
-                                          pairs[k & 1]);
-    in = pairs[k & 1];
+  // part `k` of `parts` of the zeros, in blocks of `threads` after the first `own`
+  const auto zeros = [&](int k, int parts, unsigned own, int threads, unsigned* grid) {
+    const int64_t each = (total / parts + 7) / 8 * 8;
+    Zeros z{out, each * k, k + 1 == parts || each * (k + 1) > total ? total : each * (k + 1), own};
+    const int64_t want = z.end <= z.begin ? 0 : (z.end - z.begin + 8 * threads - 1) / (8 * threads);
+    *grid = own + (unsigned)(want < kZeroThreads / threads ? want : kZeroThreads / threads);
+    return z;
+  };
+  const Pair* in = pairs[0];
+  unsigned grid;
+  if (n <= kRankTokens) {
+    const unsigned own = (unsigned)((n + 63) / 64);
+    const Zeros z = zeros(0, 1, own, kRankThreads, &grid);
+    const auto kern = out_dtype == kF32   ? rank_kernel<kF32>
+                      : out_dtype == kF16 ? rank_kernel<kF16>
+                                          : rank_kernel<kBF16>;
+    kern<<<grid, kRankThreads, 0, st>>>(ids, ids_wide, n, vocab, padding_idx, pairs[0], z);
+  } else {
+    const unsigned own = (unsigned)p.sort_blocks;
+    const auto count = out_dtype == kF32   ? count_kernel<kF32>
+                       : out_dtype == kF16 ? count_kernel<kF16>
+                                           : count_kernel<kBF16>;
+    const auto scatter = out_dtype == kF32   ? scatter_kernel<kF32>
+                         : out_dtype == kF16 ? scatter_kernel<kF16>
+                                             : scatter_kernel<kBF16>;
+    in = nullptr;
+    for (int k = 0; k < p.passes; ++k) {
+      Zeros z = zeros(2 * k, 2 * p.passes, own, kBlock, &grid);
+      count<<<grid, kBlock, 0, st>>>(in, ids, ids_wide, n, vocab, padding_idx, 8 * k, counts, z);
+      z = zeros(2 * k + 1, 2 * p.passes, own, kBlock, &grid);
+      scatter<<<grid, kBlock, 0, st>>>(in, ids, ids_wide, n, vocab, padding_idx, 8 * k, counts,
+                                       own, pairs[k & 1], z);
+      in = pairs[k & 1];
+    }
   }
   if (launched() != kOk) return kErrLaunch;
-  const int64_t strips = (d + kCols - 1) / kCols;
-  const dim3 sums((unsigned)p.tiles, (unsigned)((strips + kWaves - 1) / kWaves));
-  const dim3 joins((unsigned)p.tiles, (unsigned)strips);
-#define CPT_SUM(DT, OT)                                                                          \
-  (sum_kernel<DT, OT><<<sums, kBlock, 0, st>>>(grad, ld_grad, in, n, vocab, d, p.tile, scale,     \
-                                               accumulate, out, edge),                           \
-   join_kernel<OT><<<joins, kBlock, 0, st>>>(in, n, vocab, d, p.tile, scale, accumulate, out,     \
-                                             edge))
+  const unsigned strips = (unsigned)((d + kCols - 1) / kCols);
+  const unsigned sums = (unsigned)((p.tiles * strips + kWaves - 1) / kWaves);
+  const dim3 joins((unsigned)((p.tiles + kJoinTiles - 1) / kJoinTiles), strips);
+#define CPT_SUM_T(DT, OT, TINY, ADD, TILE)                                                      \
+  (sum_kernel<DT, OT, TINY, ADD, TILE><<<sums, kBlock, 0, st>>>(                                \
+       grad, ld_grad, in, n, vocab, d, strips, scale, out, edge),                               \
+   join_kernel<OT, TINY, ADD, TILE><<<joins, kJoinThreads, 0, st>>>(in, n, vocab, d, scale, out, edge))
+#define CPT_SUM_A(DT, OT, TINY, TILE) \
+  (accumulate ? CPT_SUM_T(DT, OT, TINY, true, TILE) : CPT_SUM_T(DT, OT, TINY, false, TILE))
+#define CPT_SUM(DT, OT)                                                                         \
+  (d < 8 ? (p.tile == 16 ? CPT_SUM_A(DT, OT, true, 16) : CPT_SUM_A(DT, OT, true, 32))            \
+         : (p.tile == 16 ? CPT_SUM_A(DT, OT, false, 16) : CPT_SUM_A(DT, OT, false, 32)))
   if (dtype == kF32)
     CPT_SUM(kF32, kF32);
   else if (dtype == kF16)

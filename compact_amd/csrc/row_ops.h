@@ -44,6 +44,14 @@ template <int DT> struct Row8Half {   // 16-bit formats
       if (2 * j + 1 < n) p[2 * j + 1] = (uint16_t)(r.w[j] >> 16);
     }
   }
+  // elements k .. 7
+  static __device__ __forceinline__ void st_from(T* p, const Raw& r, int k) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (2 * j >= k) p[2 * j] = (uint16_t)(r.w[j] & 0xFFFFu);
+      if (2 * j + 1 >= k) p[2 * j + 1] = (uint16_t)(r.w[j] >> 16);
+    }
+  }
   static __device__ __forceinline__ void unpack(const Raw& r, float v[8]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -117,6 +125,13 @@ template <> struct Row8<kF32> {
       if (4 + j < n) p[4 + j] = __uint_as_float(r.x[j]);
     }
   }
+  static __device__ __forceinline__ void st_from(T* p, const Raw& r, int k) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j >= k) p[j] = __uint_as_float(r.w[j]);
+      if (4 + j >= k) p[4 + j] = __uint_as_float(r.x[j]);
+    }
+  }
   static __device__ __forceinline__ void unpack(const Raw& r, float v[8]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -162,6 +177,42 @@ __device__ __forceinline__ void row_st(typename Row8<DT>::T* row, int64_t j, int
   else if (j < d)
     Row8<DT>::st_n(row + j, r, (int)(d - j));
 }
+
+// A thread's eight columns [j, j + 8) of a row of d, without a branch before the
+// load (each would be waited for by itself): past the end the row's last eight are
+// taken, of which the first `skip` are other threads' too.  Rows of fewer than
+// eight columns (TINY) go element by element.
+template <int DT, bool TINY>
+struct Cols {
+  using R = Row8<DT>;
+  using T = typename R::T;
+  int64_t at;
+  int skip, n;
+  __device__ __forceinline__ Cols(int64_t j, int64_t d) {
+    at = TINY ? j : min(j, d - 8);
+    skip = (int)min(j - at, (int64_t)8);
+    n = (int)max(min(d - j, (int64_t)8), (int64_t)0);
+  }
+  __device__ __forceinline__ typename R::Raw ld(const T* row) const {
+    return TINY ? R::ld_n(row + at, n, 0) : R::ld(row + at);
+  }
+  // shared columns are stored by each that has them: with the same values
+  __device__ __forceinline__ void st(T* row, const typename R::Raw& r) const {
+    if (TINY)
+      R::st_n(row + at, r, n);
+    else if (skip < 8)
+      R::st(row + at, r);
+  }
+  // only the thread's own: where what is stored depends on what was there
+  __device__ __forceinline__ void st_own(T* row, const typename R::Raw& r) const {
+    if (TINY)
+      R::st_n(row + at, r, n);
+    else if (skip == 0)
+      R::st(row + at, r);
+    else
+      R::st_from(row + at, r, skip);
+  }
+};
 
 // Sum and maximum over a wavefront, in every lane: four shifts within rows of
 // 16 lanes and two broadcasts across them (DPP), a fixed order.
