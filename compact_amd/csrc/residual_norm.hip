@@ -39,14 +39,6 @@ struct Shape {
   float alpha, beta, eps;
 };
 
-// Eight weights of a type known at run time, `none` where there is no tensor.
-__device__ __forceinline__ void ld_weights(const void* w, int wdt, int64_t base, int64_t j,
-                                           int64_t d, float none, float v[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    v[e] = !w ? none : j + e < d ? ld_any(w, wdt, base + j + e) : 0.f;
-}
-
 // Sums of N values over the threads of each row group, in every thread.  One
 // barrier; `red` alternates between two buffers from call to call.
 template <int N>
@@ -68,13 +60,30 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float (*red)[kMaxWaves]
   }
 }
 
-template <int DT, int NV>
+// A thread's eight weights of DT or fp32, ones where there is no tensor.
+template <int DT, bool TINY>
+__device__ __forceinline__ void ld_weights(const void* w, int wdt, int64_t base, int64_t j,
+                                           int64_t d, float v[8]) {
+  if (!w) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 1.f;
+  } else if (wdt == DT) {
+    const Cols<DT, TINY> c(j, d);
+    Row8<DT>::unpack(c.ld((const typename Row8<DT>::T*)w + base), v);
+  } else {
+    const Cols<kF32, TINY> c(j, d);
+    Row8<kF32>::unpack(c.ld((const float*)w + base), v);
+  }
+}
+
+template <int DT, int NV, bool TINY>
 __global__ __launch_bounds__(kMaxThreads) void forward_kernel(
     Shape s, const void* __restrict__ residual, int64_t ld_res, const void* __restrict__ y,
     int64_t ld_y, const void* __restrict__ w_post, const void* __restrict__ w_pre,
     const void* __restrict__ gate, void* residual_out, void* x, float* stats) {
   using R = Row8<DT>;
   using T = typename R::T;
+  using C = Cols<DT, TINY>;
   __shared__ float red[2][2][kMaxWaves];
   const int group = threadIdx.x / s.tr, tid = threadIdx.x - group * s.tr;
   float a[NV][8], wp[NV][8];
@@ -82,26 +91,47 @@ __global__ __launch_bounds__(kMaxThreads) void forward_kernel(
   for (int c = 0; c < NV; ++c) {
     const int64_t j = 8 * ((int64_t)c * s.tr + tid);
     float g[8];
-    ld_weights(w_post, s.wdt, 0, j, s.d, 1.f, a[c]);
-    ld_weights(s.gate == kChannel ? gate : nullptr, s.wdt, 0, j, s.d, 1.f, g);
-    ld_weights(w_pre, s.wdt, 0, j, s.d, 1.f, wp[c]);
+    ld_weights<DT, TINY>(w_post, s.wdt, 0, j, s.d, a[c]);
+    ld_weights<DT, TINY>(s.gate == kChannel ? gate : nullptr, s.wdt, 0, j, s.d, g);
+    ld_weights<DT, TINY>(w_pre, s.wdt, 0, j, s.d, wp[c]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) a[c][e] *= s.alpha * g[e];
   }
+  const bool ragged = s.d % 8 != 0 || s.tr * NV * 8 != s.d;
   const float inv_d = 1.f / (float)s.d;
   int turn = 0;
   const int64_t step = (int64_t)gridDim.x * s.groups;
-  for (int64_t row0 = (int64_t)blockIdx.x * s.groups; row0 < s.rows; row0 += step, turn ^= 1) {
-    const int64_t row = row0 + group;
-    const bool in = row < s.rows;
-    const int64_t d = in ? s.d : 0;   // a group past the last row reads and writes nothing
-    typename R::Raw ry[NV], rr[NV];
+  struct Loaded {
+    typename R::Raw y[NV], r[NV];
+  };
+  const auto load = [&](int64_t row0, Loaded& q) {
+    const int64_t row = min(row0 + group, s.rows - 1);   // groups past it repeat the last row
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
-      const int64_t j = 8 * ((int64_t)c * s.tr + tid);
-      rr[c] = row_ld<DT>((const T*)residual + row * ld_res, j, d, 0);
-      if (y) ry[c] = row_ld<DT>((const T*)y + row * ld_y, j, d, 0);
+      const C cols(8 * ((int64_t)c * s.tr + tid), s.d);
+      q.y[c] = cols.ld((const T*)(y ? y : residual) + row * (y ? ld_y : ld_res));
+      q.r[c] = cols.ld((const T*)residual + row * ld_res);
     }
+  };
+  Loaded q;
+  int64_t row0 = (int64_t)blockIdx.x * s.groups;
+  load(row0, q);
+  for (; row0 < s.rows; row0 += step, turn ^= 1) {
+    const bool in = row0 + group < s.rows;
+    const int64_t row = in ? row0 + group : s.rows - 1;
+    // the next row's loads go ahead of this one's stores, which would be waited for
+    Loaded next;
+    load(row0 + step, next);
+    if (!TINY && ragged) {
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
+        const C cols(8 * ((int64_t)c * s.tr + tid), s.d);
+        R::mask(q.y[c], (1u << cols.skip) - 1, 0);
+        R::mask(q.r[c], (1u << cols.skip) - 1, 0);
+      }
+    }
+    const auto& ry = q.y;
+    const auto& rr = q.r;
     float r[NV][8];
     float rho1 = 1.f;
     if (y) {
@@ -118,21 +148,22 @@ __global__ __launch_bounds__(kMaxThreads) void forward_kernel(
         rho1 = 1.f / sqrtf(sum[0] * inv_d + s.eps);
       }
       float k = rho1;
-      if (s.gate == kToken && in) k *= ld_any(gate, s.wdt, row);
+      if (s.gate == kToken) k *= ld_any(gate, s.wdt, row);
 #pragma unroll
       for (int c = 0; c < NV; ++c) {
-        const int64_t j = 8 * ((int64_t)c * s.tr + tid);
+        const C cols(8 * ((int64_t)c * s.tr + tid), s.d);
         float v[8], g[8];
         R::unpack(rr[c], r[c]);
         R::unpack(ry[c], v);
-        if (s.gate == kSequence && in) {
-          ld_weights(gate, s.wdt, row / s.seq * s.d, j, s.d, 1.f, g);
+        if (s.gate == kSequence) {
+          ld_weights<DT, TINY>(gate, s.wdt, row / s.seq * s.d, 8 * ((int64_t)c * s.tr + tid), s.d,
+                               g);
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] *= g[e];
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) r[c][e] = s.beta * r[c][e] + a[c][e] * (v[e] * k);
-        row_st<DT>((T*)residual_out + row * s.d, j, d, R::pack(r[c]));
+        if (in) cols.st_own((T*)residual_out + row * s.d, R::pack(r[c]));
       }
     } else {
 #pragma unroll
@@ -149,24 +180,25 @@ __global__ __launch_bounds__(kMaxThreads) void forward_kernel(
       rho2 = 1.f / sqrtf(sum[0] * inv_d + s.eps);
 #pragma unroll
       for (int c = 0; c < NV; ++c) {
-        const int64_t j = 8 * ((int64_t)c * s.tr + tid);
+        const C cols(8 * ((int64_t)c * s.tr + tid), s.d);
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = r[c][e] * rho2 * wp[c][e];
-        row_st<DT>((T*)x + row * s.d, j, d, R::pack(v));
+        if (in) cols.st_own((T*)x + row * s.d, R::pack(v));
       }
     }
     if (tid == 0 && in) {
       stats[row] = rho1;
       stats[s.rows + row] = rho2;
     }
+    q = next;
   }
 }
 
 // grid (chunks of a sequence's rows, sequences).  Block (c, b) takes the row
 // groups c, c + chunks, ... of sequence b and leaves its sums over them in
 // partial[b * chunks + c]: dw_pre's columns, then G's.
-template <int DT, int NV>
+template <int DT, int NV, bool TINY>
 __global__ __launch_bounds__(kMaxThreads) void backward_kernel(
     Shape s, const void* __restrict__ d_res_out, int64_t ld_dro, const void* __restrict__ d_x,
     int64_t ld_dx, const void* __restrict__ res_out, int64_t ld_ro, const void* __restrict__ y,
@@ -175,6 +207,7 @@ __global__ __launch_bounds__(kMaxThreads) void backward_kernel(
     void* d_gate, float* partial) {
   using R = Row8<DT>;
   using T = typename R::T;
+  using C = Cols<DT, TINY>;
   extern __shared__ __align__(16) float combine[];
   __shared__ float red[2][3][kMaxWaves];
   const int group = threadIdx.x / s.tr, tid = threadIdx.x - group * s.tr;
@@ -184,47 +217,68 @@ __global__ __launch_bounds__(kMaxThreads) void backward_kernel(
   for (int c = 0; c < NV; ++c) {
     const int64_t j = 8 * ((int64_t)c * s.tr + tid);
     float g[8];
-    ld_weights(w_post, s.wdt, 0, j, s.d, 1.f, a[c]);
-    ld_weights(s.gate == kChannel || s.gate == kSequence ? gate : nullptr, s.wdt,
-               s.gate == kSequence ? b * s.d : 0, j, s.d, 1.f, g);
-    ld_weights(w_pre, s.wdt, 0, j, s.d, 1.f, wp[c]);
+    ld_weights<DT, TINY>(w_post, s.wdt, 0, j, s.d, a[c]);
+    ld_weights<DT, TINY>(s.gate == kChannel || s.gate == kSequence ? gate : nullptr, s.wdt,
+                         s.gate == kSequence ? b * s.d : 0, j, s.d, g);
+    ld_weights<DT, TINY>(w_pre, s.wdt, 0, j, s.d, wp[c]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       a[c][e] *= s.alpha * g[e];
       acc_pre[c][e] = acc_g[c][e] = 0.f;
     }
   }
+  const bool ragged = s.d % 8 != 0 || s.tr * NV * 8 != s.d;
   const float inv_d = 1.f / (float)s.d;
   const int64_t step = (int64_t)gridDim.x * s.groups;
-  int turn = 0;
-  for (int64_t row0 = (int64_t)blockIdx.x * s.groups; row0 < s.seq; row0 += step, turn ^= 1) {
-    const bool in = row0 + group < s.seq;
-    const int64_t row = b * s.seq + row0 + group;
-    const int64_t d = in ? s.d : 0;
-    typename R::Raw q_dr[NV], q_dx[NV], q_r[NV], q_y[NV];
+  struct Loaded {
+    typename R::Raw dr[NV], dx[NV], r[NV], y[NV];
+    float rho1, rho2, gate;
+  };
+  const auto load = [&](int64_t row0, Loaded& q) {
+    const int64_t row = b * s.seq + min(row0 + group, s.seq - 1);
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
-      const int64_t j = 8 * ((int64_t)c * s.tr + tid);
-      q_dr[c] = q_dx[c] = q_r[c] = q_y[c] = R::zero();
-      if (d_res_out) q_dr[c] = row_ld<DT>((const T*)d_res_out + row * ld_dro, j, d, 0);
+      const C cols(8 * ((int64_t)c * s.tr + tid), s.d);
+      q.dr[c] = q.dx[c] = q.r[c] = q.y[c] = R::zero();
+      if (d_res_out) q.dr[c] = cols.ld((const T*)d_res_out + row * ld_dro);
       if (d_x) {
-        q_dx[c] = row_ld<DT>((const T*)d_x + row * ld_dx, j, d, 0);
-        q_r[c] = row_ld<DT>((const T*)res_out + row * ld_ro, j, d, 0);
+        q.dx[c] = cols.ld((const T*)d_x + row * ld_dx);
+        q.r[c] = cols.ld((const T*)res_out + row * ld_ro);
       }
-      if (y) q_y[c] = row_ld<DT>((const T*)y + row * ld_y, j, d, 0);
+      if (y) q.y[c] = cols.ld((const T*)y + row * ld_y);
     }
-    const float rho1 = in ? stats[row] : 0.f, rho2 = in ? stats[s.rows + row] : 0.f;
-    const float gt = s.gate == kToken && in ? ld_any(gate, s.wdt, row) : 1.f;
+    q.rho1 = stats[row], q.rho2 = stats[s.rows + row];
+    q.gate = s.gate == kToken ? ld_any(gate, s.wdt, row) : 1.f;
+  };
+  int turn = 0;
+  Loaded q;
+  int64_t row0 = (int64_t)blockIdx.x * s.groups;
+  for (; row0 < s.seq; row0 += step, turn ^= 1) {
+    const bool in = row0 + group < s.seq;
+    const int64_t row = b * s.seq + row0 + group;
+    load(row0, q);
+    if (!in || (!TINY && ragged)) {   // a group past the last row adds nothing
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
+        const C cols(8 * ((int64_t)c * s.tr + tid), s.d);
+        const uint32_t off = !in ? 255 : TINY ? 0 : (1u << cols.skip) - 1;
+        R::mask(q.dr[c], off, 0);
+        R::mask(q.dx[c], off, 0);
+        R::mask(q.r[c], off, 0);
+        R::mask(q.y[c], off, 0);
+      }
+    }
+    const float rho1 = q.rho1, rho2 = q.rho2, gt = q.gate;
     // one reduction for both norms: with t = dr' + rho2 (dn2 - n2 m2) left open in m2,
     // sum a n1 t = sum a n1 (dr' + rho2 dn2) - rho2 m2 sum a n1 n2
     float sum[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
       float dr[8], dx[8], r[8], v[8];
-      R::unpack(q_dr[c], dr);
-      R::unpack(q_dx[c], dx);
-      R::unpack(q_r[c], r);
-      R::unpack(q_y[c], v);
+      R::unpack(q.dr[c], dr);
+      R::unpack(q.dx[c], dx);
+      R::unpack(q.r[c], r);
+      R::unpack(q.y[c], v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float n2 = r[e] * rho2, dn2 = dx[e] * wp[c][e], an1 = a[c][e] * (v[e] * rho1);
@@ -240,12 +294,12 @@ __global__ __launch_bounds__(kMaxThreads) void backward_kernel(
     if (s.gate == kToken && in && tid == 0) st_any(d_gate, s.wdt, row, dgt);
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
-      const int64_t j = 8 * ((int64_t)c * s.tr + tid);
+      const C cols(8 * ((int64_t)c * s.tr + tid), s.d);
       float dr[8], dx[8], r[8], v[8];
-      R::unpack(q_dr[c], dr);
-      R::unpack(q_dx[c], dx);
-      R::unpack(q_r[c], r);
-      R::unpack(q_y[c], v);
+      R::unpack(q.dr[c], dr);
+      R::unpack(q.dx[c], dx);
+      R::unpack(q.r[c], r);
+      R::unpack(q.y[c], v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float n2 = r[e] * rho2, n1 = v[e] * rho1;
@@ -255,8 +309,10 @@ __global__ __launch_bounds__(kMaxThreads) void backward_kernel(
         dr[e] = s.beta * t;
         v[e] = rho1 * (gt * a[c][e] * t - n1 * m1);
       }
-      row_st<DT>((T*)d_res + row * s.d, j, d, R::pack(dr));
-      if (y) row_st<DT>((T*)d_y + row * s.d, j, d, R::pack(v));
+      if (in) {
+        cols.st_own((T*)d_res + row * s.d, R::pack(dr));
+        if (y) cols.st_own((T*)d_y + row * s.d, R::pack(v));
+      }
     }
   }
   // the groups' sums, in group order
@@ -276,14 +332,15 @@ __global__ __launch_bounds__(kMaxThreads) void backward_kernel(
     if (group == 0) {
 #pragma unroll
       for (int c = 0; c < NV; ++c) {
-        const int64_t j = 8 * ((int64_t)c * s.tr + tid);
+        const Cols<kF32, TINY> cols(8 * ((int64_t)c * s.tr + tid), s.d);
+        float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          float v = acc[c][e];
+          v[e] = acc[c][e];
           for (int g = 1; g < s.groups; ++g)
-            v += combine[((g - 1) * NV + c) * 8 * s.tr + e * s.tr + tid];
-          if (j + e < s.d) out[which * s.d + j + e] = v;
+            v[e] += combine[((g - 1) * NV + c) * 8 * s.tr + e * s.tr + tid];
         }
+        cols.st_own(out + which * s.d, Row8<kF32>::pack(v));
       }
     }
   }
@@ -344,21 +401,28 @@ inline int launched() { return hipGetLastError() == hipSuccess ? kOk : kErrLaunc
 
 constexpr int64_t kMaxD = 8 * kMaxThreads * 2;
 
-// Vectors per thread, and the threads and row groups of a block.
-int plan(Shape& s) {
+// Vectors per thread, and the threads and row groups of a block of about `threads`.
+int plan(Shape& s, int threads) {
   const int64_t vecs = (s.d + 7) / 8;
   const int nv = vecs <= kMaxThreads ? 1 : 2;
   const int64_t t = (vecs + nv - 1) / nv;
   s.tr = (int)((t + 63) / 64 * 64);
-  s.groups = kMaxThreads / s.tr;
+  s.groups = threads / s.tr > 1 ? threads / s.tr : 1;
   if (s.groups > s.seq) s.groups = s.seq > 0 ? (int)s.seq : 1;
   return nv;
 }
 
-// Chunks of a sequence's rows in the backward: one block of 16 wavefronts per CU
+// The backward's blocks: two of 512 threads a CU, which wait for their barriers
+// apart (30000 x 512 bf16: 47 us, one of 1024 52); for rows of more than 2048
+// columns one of 1024, which leaves half the partial sums (4000 x 8192: 93 us,
+// against 102).
+int backward_threads(int64_t d) { return d <= 2048 ? 512 : 1024; }
+
+// Chunks of a sequence's rows in the backward: as many blocks as run at a time,
 // over all sequences, as far as there are rows.
 int64_t backward_chunks(const Shape& s, int64_t seqs) {
-  int64_t c = (256 + seqs - 1) / seqs;
+  const int64_t blocks = 256 * (1024 / backward_threads(s.d));
+  int64_t c = (blocks + seqs - 1) / seqs;
   const int64_t most = (s.seq + s.groups - 1) / s.groups;
   if (c > most) c = most;
   return c < 1 ? 1 : c;
@@ -395,16 +459,17 @@ int cpt_residual_norm(int dtype, int weight_dtype, const void* residual, int64_t
   if (!residual || !stats || ld_residual < 0 || ld_y < 0) return kErrShape;
   Shape s{rows, seq, d, 0, 0, gate_kind, weight_dtype, scale, residual_scale, eps};
   s.seq = rows;   // blocks take rows of any sequence
-  const int nv = plan(s);
+  const int nv = plan(s, 256);
   s.seq = seq;
   const int threads = s.tr * s.groups;
   const int64_t blocks = (rows + s.groups - 1) / s.groups;
   const int64_t most = 256 * (2048 / threads);   // as many as can run at a time
   const dim3 grid((unsigned)(blocks < most ? blocks : most));
-#define CPT_FWD(DT, NV)                                                                         \
-  forward_kernel<DT, NV><<<grid, threads, 0, (hipStream_t)stream>>>(                             \
+#define CPT_FWD(DT, NV, TINY)                                                                    \
+  forward_kernel<DT, NV, TINY><<<grid, threads, 0, (hipStream_t)stream>>>(                             \
       s, residual, ld_residual, y, ld_y, w_post, w_pre, gate, residual_out, x, (float*)stats)
-#define CPT_FWD_NV(DT) (nv == 1 ? CPT_FWD(DT, 1) : CPT_FWD(DT, 2))
+#define CPT_FWD_NV(DT) \
+  (d < 8 ? CPT_FWD(DT, 1, true) : nv == 1 ? CPT_FWD(DT, 1, false) : CPT_FWD(DT, 2, false))
   dtype == kF32 ? CPT_FWD_NV(kF32) : dtype == kF16 ? CPT_FWD_NV(kF16) : CPT_FWD_NV(kBF16);
   return launched();
 }
@@ -414,7 +479,7 @@ int64_t cpt_residual_norm_backward_workspace_bytes(int64_t rows, int64_t seq, in
   if (!shape_ok(rows, seq, d, gate_kind) || d > kMaxD) return -1;
   if (rows == 0) return 0;
   Shape s{rows, seq, d, 0, 0, gate_kind, kF32, 1.f, 1.f, 0.f};
-  plan(s);
+  plan(s, backward_threads(d));
   const int64_t seqs = rows / seq;
   return seqs * backward_chunks(s, seqs) * 2 * d * 4;
 }
@@ -443,18 +508,19 @@ int cpt_residual_norm_backward(int dtype, int weight_dtype, const void* d_residu
                    ld_dx < 0 || ld_ro < 0 || ld_y < 0))
     return kErrShape;
   Shape s{rows, seq, d, 0, 0, gate_kind, weight_dtype, scale, residual_scale, 0.f};
-  const int nv = plan(s);
+  const int nv = plan(s, backward_threads(d));
   const int64_t chunks = seqs == 0 ? 0 : backward_chunks(s, seqs);
   const hipStream_t st = (hipStream_t)stream;
   if (rows > 0) {
     const int threads = s.tr * s.groups;
     const dim3 grid((unsigned)chunks, (unsigned)seqs);
     const size_t lds = (size_t)(s.groups - 1) * s.tr * 8 * nv * 4;
-#define CPT_BWD(DT, NV)                                                                         \
-  backward_kernel<DT, NV><<<grid, threads, lds, st>>>(                                           \
+#define CPT_BWD(DT, NV, TINY)                                                                    \
+  backward_kernel<DT, NV, TINY><<<grid, threads, lds, st>>>(                                           \
       s, d_residual_out, ld_dro, d_x, ld_dx, residual_out, ld_ro, y, ld_y, (const float*)stats,  \
       w_post, w_pre, gate, d_residual, d_y, d_gate, (float*)workspace)
-#define CPT_BWD_NV(DT) (nv == 1 ? CPT_BWD(DT, 1) : CPT_BWD(DT, 2))
+#define CPT_BWD_NV(DT) \
+  (d < 8 ? CPT_BWD(DT, 1, true) : nv == 1 ? CPT_BWD(DT, 1, false) : CPT_BWD(DT, 2, false))
     dtype == kF32 ? CPT_BWD_NV(kF32) : dtype == kF16 ? CPT_BWD_NV(kF16) : CPT_BWD_NV(kBF16);
     const int rc = launched();
     if (rc != kOk) return rc;
