@@ -32,10 +32,22 @@ def _index_code(t: torch.Tensor, what: str) -> int:
     return _INDEX[t.dtype]
 
 
-def _same_device(first, *rest):
+def _on_device(first, *rest):
+    """All tensors (None: absent) on one HIP device."""
+    dev = first.get_device()
+    if dev < 0:
+        _require_device(first)
     for t in rest:
-        assert t is None or t.device == first.device, \
-            f"tensors on {first.device} and {t.device}"
+        if t is not None and t.get_device() != dev:
+            _require_device(t)
+            raise AssertionError(f"tensors on {first.device} and {t.device}")
+
+
+def _new_like(t):
+    """An uninitialised contiguous tensor of t's shape and type."""
+    if t.is_contiguous():
+        return torch.empty_like(t)
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _rows(t, d):
@@ -57,14 +69,13 @@ def _rows(t, d):
 def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """scale * weight[ids]: [*ids.shape, D] in weight's dtype.  ids: int32 or
     int64; an id outside the table gives a row of zeros."""
-    _require_device(ids, weight)
-    _same_device(weight, ids)
+    _on_device(weight, ids)
     assert weight.dim() == 2, f"weight [V, D] expected, got {tuple(weight.shape)}"
     wide = _index_code(ids, "ids")
     dt = _dtype_code(weight)
     weight, ids = weight.contiguous(), ids.contiguous()
     v, d = weight.shape
-    out = torch.empty((*ids.shape, d), dtype=weight.dtype, device=weight.device)
+    out = weight.new_empty((*ids.shape, d))
     with _timed("embedding"):
         rc = _lib.api().cpt_embedding(dt, weight.data_ptr(), v, d, ids.data_ptr(), wide,
                                       ids.numel(), float(scale), out.data_ptr(), _stream(weight))
@@ -80,8 +91,7 @@ def embedding_backward(grad: torch.Tensor, ids: torch.Tensor, num_embeddings: in
     table add nothing.  `out` [num_embeddings, D], in grad's dtype or float32,
     is added to instead (a gradient accumulated over micro-batches): only the
     rows that the tokens name are read and written."""
-    _require_device(grad, ids, out)
-    _same_device(grad, ids, out)
+    _on_device(grad, ids, out)
     wide = _index_code(ids, "ids")
     dt = _dtype_code(grad)
     assert grad.dim() >= 1 and grad.shape[:-1] == ids.shape, \
@@ -206,8 +216,7 @@ def residual_norm(residual, y=None, w_pre=None, *, w_post=None, gate=None, scale
     float32.  y None: x is the norm of `residual`, returned as it is.  Returns
     (residual_out, x, stats); stats, fp32 [2, rows], is what the backward
     needs."""
-    _require_device(residual, y, w_pre, w_post, gate)
-    _same_device(residual, y, w_pre, w_post, gate)
+    _on_device(residual, y, w_pre, w_post, gate)
     dt = _dtype_code(residual)
     assert residual.dim() >= 1 and residual.shape[-1] > 0, "residual_norm: [..., D] expected"
     assert y is not None or w_pre is not None, "residual_norm: y or w_pre expected"
@@ -219,9 +228,8 @@ def residual_norm(residual, y=None, w_pre=None, *, w_post=None, gate=None, scale
     w_pre, w_post, gate = _dense(w_pre), _dense(w_post), _dense(gate)
     res, ld_res = _rows(residual, d)
     y2, ld_y = _rows(y, d)
-    new = dict(dtype=residual.dtype, device=residual.device)
-    out = torch.empty(shape, **new) if y is not None else None
-    x = torch.empty(shape, **new) if w_pre is not None else None
+    out = _new_like(residual) if y is not None else None
+    x = _new_like(residual) if w_pre is not None else None
     stats = torch.empty((2, rows), dtype=torch.float32, device=residual.device)
     if rows == 0:
         return (residual if out is None else out), x, stats
@@ -241,8 +249,7 @@ def residual_norm_backward(d_residual_out, d_x, residual_out, y, stats, w_pre=No
     zeros) and x (None without w_pre), given residual_out, y and stats of the
     forward.  Returns (d_residual, d_y, d_w_pre, d_w_post, d_gate), None for
     what the forward had none of."""
-    _require_device(d_residual_out, d_x, residual_out, y, stats, w_pre, w_post, gate)
-    _same_device(residual_out, d_residual_out, d_x, y, stats, w_pre, w_post, gate)
+    _on_device(residual_out, d_residual_out, d_x, y, stats, w_pre, w_post, gate)
     dt = _dtype_code(residual_out)
     shape, d = residual_out.shape, residual_out.shape[-1]
     assert (d_x is None) == (w_pre is None), "d_x and w_pre belong together"
@@ -256,11 +263,12 @@ def residual_norm_backward(d_residual_out, d_x, residual_out, y, stats, w_pre=No
     assert tuple(stats.shape) == (2, rows) and stats.dtype == torch.float32 \
         and stats.is_contiguous(), f"stats: contiguous float32 {(2, rows)} expected"
     w_pre, w_post, gate = _dense(w_pre), _dense(w_post), _dense(gate)
-    new = dict(dtype=residual_out.dtype, device=residual_out.device)
-    d_res = torch.empty(shape, **new)
-    d_y = torch.empty(shape, **new) if y is not None else None
+    d_res = _new_like(residual_out)
+    d_y = _new_like(residual_out) if y is not None else None
     make = torch.empty_like if rows else torch.zeros_like
-    d_w_pre, d_w_post, d_gate = (None if w is None else make(w) for w in (w_pre, w_post, gate))
+    d_w_pre = None if w_pre is None else make(w_pre)
+    d_w_post = None if w_post is None else make(w_post)
+    d_gate = None if gate is None else make(gate)
     if rows == 0:
         return d_res, d_y, d_w_pre, d_w_post, d_gate
     dro, ld_dro = _rows(d_residual_out, d)
@@ -367,8 +375,7 @@ def distill_topk(logits, top_logits, top_indices, labels=None, *, top_lse=None,
     "none" one value per row).  `inplace` writes it over logits, which must be
     the caller's own.  A row-strided view such as logits[:, :-1] is read as it
     lies."""
-    _require_device(logits, top_logits, top_indices, labels, top_lse)
-    _same_device(logits, top_logits, top_indices, labels, top_lse)
+    _on_device(logits, top_logits, top_indices, labels, top_lse)
     dt, tdt = _dtype_code(logits), _dtype_code(top_logits)
     assert logits.dim() >= 1 and logits.shape[-1] > 0, "distill_topk: logits [..., V] expected"
     assert reduction in _REDUCTION, f"reduction={reduction!r}"
@@ -393,16 +400,15 @@ def distill_topk(logits, top_logits, top_indices, labels=None, *, top_lse=None,
     rows = logits.numel() // v
     dev = logits.device
 
-    def layout(t):
-        """(tensor, rows per batch, batch stride, row stride)"""
-        if not t.is_contiguous() and (v == 1 or t.stride(-1) == 1):
-            if t.dim() == 2:
-                return t, max(rows, 1), 0, t.stride(0)
-            if t.dim() == 3:
-                return t, max(t.shape[1], 1), t.stride(0), t.stride(1)
-        return t.contiguous(), max(rows, 1), 0, v
-
-    z, seq, ld_b, ld_s = layout(logits)
+    # rows per batch entry, and the strides of both
+    z, seq, ld_b, ld_s = logits, max(rows, 1), 0, v
+    if not z.is_contiguous():
+        if z.dim() == 2 and (v == 1 or z.stride(1) == 1):
+            ld_s = z.stride(0)
+        elif z.dim() == 3 and (v == 1 or z.stride(2) == 1):
+            seq, ld_b, ld_s = max(z.shape[1], 1), z.stride(0), z.stride(1)
+        else:
+            z = z.contiguous()
     grad, gld_b, gld_s = None, 0, 0
     if want_grad and inplace:
         assert z is logits and (seq <= 1 or ld_s >= v) and \
@@ -410,7 +416,7 @@ def distill_topk(logits, top_logits, top_indices, labels=None, *, top_lse=None,
             "inplace: logits of separate rows, whole along the vocabulary, expected"
         grad, gld_b, gld_s = logits, ld_b, ld_s
     elif want_grad:
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        grad = _new_like(logits)
         gld_b, gld_s = seq * v, v
     scale, gout = 1.0, None
     if isinstance(grad_out, torch.Tensor):
