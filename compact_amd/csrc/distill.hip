@@ -36,6 +36,7 @@ constexpr float kLn2 = 0.69314718055994530942f;
 constexpr int kMaxWaves = 16;
 constexpr int kMaxEntries = 2048;
 constexpr int64_t kMaxVocab = 1 << 19;
+constexpr int kBatch = 2;   // vectors in flight of a row that is read again
 
 struct Args {
   int64_t rows, vocab;
@@ -68,6 +69,13 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 constexpr float kFar = 268435456.f;
 __device__ __forceinline__ float base_of(float m, float k) {
   return rintf(fminf(fmaxf(m * k, -kFar), kFar));
+}
+
+// 1 / x to fp32's last place (one Newton step from the instruction's estimate)
+// in three instructions, where a correctly rounded division takes ten.
+__device__ __forceinline__ float inverse(float x) {
+  const float r = __builtin_amdgcn_rcpf(x);
+  return fmaf(r, fmaf(-x, r, 1.f), r);
 }
 
 __device__ __forceinline__ bool live_label(const Args& a, int64_t y) {
@@ -180,6 +188,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
   __syncthreads();
 
   const auto offset = [&](int64_t r, int64_t ld_b, int64_t ld_s) {
+    if (a.seq >= a.rows) return r * ld_s * (int64_t)sizeof(T);   // one batch
     const uint32_t rb = (uint32_t)r / (uint32_t)a.seq, rs = (uint32_t)r - rb * (uint32_t)a.seq;
     return (rb * ld_b + rs * ld_s) * (int64_t)sizeof(T);
   };
@@ -275,14 +284,20 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
       }
       if (tid < ragged && bits[vecs >> 2] >> (8 * (vecs & 3) + tid) & 1) xr = -INFINITY;
     }
-    // columns past the registers are read again: with a tail, without the entries'
+    // Columns past the registers are read again, kBatch vectors at a time: with a
+    // tail without the entries', and -inf past the row's end.
     float shift = 0.f;
-    const auto again8 = [&](uint32_t vec, float x[8]) {
-      Raw r = vec8(vec);
+    const auto load_batch = [&](uint32_t first, Raw (&r)[kBatch]) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) r[i] = vec8(min(first + i * THREADS, vecs - 1));
+    };
+    const auto unpack_again = [&](uint32_t vec, Raw& r, float x[8]) {
       if (tail) {
-        const uint32_t top = bits[vec >> 2] >> (8 * (vec & 3)) & 255;
+        const uint32_t at = min(vec, vecs - 1);
+        const uint32_t top = bits[at >> 2] >> (8 * (at & 3)) & 255;
         if (top) R::mask(r, top, R::kNegInf);
       }
+      if (vec >= vecs) r = R::fill(R::kNegInf);
       R::unpack(r, x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] -= shift;
@@ -317,27 +332,32 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
         for (int e = 0; e < 8; ++e) add(x[e]);
         repack<DT>(q[c]);
       }
-      for (uint32_t vec = NV * THREADS + tid; vec < vecs; vec += THREADS) {
-        float x[8], mc = m;
-        again8(vec, x);
+      for (uint32_t first = NV * THREADS + tid; first < vecs; first += kBatch * THREADS) {
+        Raw r[kBatch];
+        load_batch(first, r);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mc = fmaxf(mc, x[e]);
-        if (mc > m) {
-          const float nt = base_of(mc, kt), n1 = base_of(mc, k1);
-          st *= exp2_fast(ct - nt);
-          if (POW == 1) s1 *= exp2_fast(c1 - n1);
-          if (POW == 2) s1 *= exp2_fast(2.f * (ct - nt));
-          m = mc, ct = nt, c1 = n1;
+        for (int i = 0; i < kBatch; ++i) {
+          float x[8], mc = m;
+          unpack_again(first + i * THREADS, r[i], x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mc = fmaxf(mc, x[e]);
+          if (mc > m) {
+            const float nt = base_of(mc, kt), n1 = base_of(mc, k1);
+            st *= exp2_fast(ct - nt);
+            if (POW == 1) s1 *= exp2_fast(c1 - n1);
+            if (POW == 2) s1 *= exp2_fast(2.f * (ct - nt));
+            m = mc, ct = nt, c1 = n1;
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) add(x[e]);
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) add(x[e]);
       }
       add(xr);
       // over the wavefront, then the block: sums are brought to the common base
-      const float mw = wave_max(m), cw = base_of(mw, kt);
-      st = wave_sum(st * exp2_fast(ct - cw));
+      const float mw = wave_max(m), back = exp2_fast(ct - base_of(mw, kt));
+      st = wave_sum(st * back);
       if (POW == 1) s1 = wave_sum(s1 * exp2_fast(c1 - base_of(mw, k1)));
-      if (POW == 2) s1 = wave_sum(s1 * exp2_fast(2.f * (ct - cw)));
+      if (POW == 2) s1 = wave_sum(s1 * back * back);
       if (lane == 0) {
         red_m[turn][wave] = mw;
         red_t[turn][wave] = st;
@@ -365,10 +385,11 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
         const int w = lane & (kMaxWaves - 1);
         const float mw = red_m[turn][w];
         m = row16_max(mw);
-        c_t = base_of(m, kt), c_1 = POW == 2 ? 2.f * c_t : base_of(m, k1);
-        st = row16_sum(red_t[turn][w] * exp2_fast(base_of(mw, kt) - c_t));
+        c_t = base_of(m, kt), c_1 = POW == 2 ? 2.f * c_t : POW == 1 ? base_of(m, k1) : 0.f;
+        const float back = exp2_fast(base_of(mw, kt) - c_t);
+        st = row16_sum(red_t[turn][w] * back);
         if (POW == 1) s1 = row16_sum(red_1[turn][w] * exp2_fast(base_of(mw, k1) - c_1));
-        if (POW == 2) s1 = row16_sum(red_1[turn][w] * exp2_fast(2.f * (base_of(mw, kt) - c_t)));
+        if (POW == 2) s1 = row16_sum(red_1[turn][w] * back * back);
       }
       turn ^= 1;
       m_row = tail ? fmaxf(m, teach.m) : m;
@@ -399,10 +420,10 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
     }
     if (!POW) s1 = st, b_1 = b_t, u_1 = u_t;
     if (st == INFINITY) st = s1 = NAN;   // +inf among the logits
-    const float l_t = __log2f(st), l_1 = __log2f(s1);   // of the row's sums, less b_t and b_1
     const float rest = sr == 0.f ? 0.f : teach.rest;
     const float mass = teach.mass + rest;   // P
     if (wave == 0) {
+      const float l_t = __log2f(st), l_1 = __log2f(s1);   // of the row's sums, less b_t and b_1
       float soft = 0.f;
       for (int k = lane; k < a.k; k += 64) {
         const float p = s_p[k];
@@ -420,8 +441,9 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
       const float go = norm * (a.grad_out ? a.grad_out[a.grad_out_rows ? row : 0] : 1.f);
       const float cs = go * a.alpha * a.tau, ch = go * (1.f - a.alpha);
       // factors of the exponentials: about the row's base at an entry, the block's elsewhere
-      const float f_top = cs * mass / st, f_top1 = ch / s1;
-      float f_t = f_top * u_t - (rest > 0.f ? cs * rest / sr : 0.f), f_1 = f_top1 * u_1;
+      const float f_top = cs * mass * inverse(st), f_top1 = ch * inverse(s1);
+      float f_t = f_top * u_t, f_1 = f_top1 * u_1;
+      if (rest > 0.f) f_t -= cs * rest * inverse(sr);
       if (!POW) f_t += f_1;   // one softmax for both terms (f_1 is 0 without labels' term)
       const auto grad_of = [&](float x) {
         const float et = exp2_fast(fmaf(x, kt, -c_t));
@@ -438,12 +460,18 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
         for (int e = 0; e < 8; ++e) x[e] = grad_of(x[e]);
         if (vec < vecs) R::st((T*)(g + vec * kBytes), R::pack(x));
       }
-      for (uint32_t vec = NV * THREADS + tid; vec < vecs; vec += THREADS) {
-        float x[8];
-        again8(vec, x);
+      for (uint32_t first = NV * THREADS + tid; first < vecs; first += kBatch * THREADS) {
+        Raw r[kBatch];
+        load_batch(first, r);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = grad_of(x[e]);
-        R::st((T*)(g + vec * kBytes), R::pack(x));
+        for (int i = 0; i < kBatch; ++i) {
+          const uint32_t vec = first + i * THREADS;
+          float x[8];
+          unpack_again(vec, r[i], x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = grad_of(x[e]);
+          if (vec < vecs) R::st((T*)(g + vec * kBytes), R::pack(x));
+        }
       }
       if (tid < ragged) Elem<DT>::st((T*)g + vecs * 8 + tid, grad_of(xr));
       __syncthreads();   // the columns below are written again
