@@ -438,6 +438,8 @@ def distill_topk(logits, top_logits, top_indices, labels=None, *, top_lse=None,
             losses.data_ptr(), losses.data_ptr() + 4 * rows, _ptr(grad), gld_b, gld_s,
             _stream(logits))
     check(rc, "distill_topk")
+    if grad is logits:      # autograd refuses a graph that still needs the old values
+        torch.autograd.graph.increment_version(logits)
     return loss, grad
 
 

@@ -341,6 +341,43 @@ def test_function(device, dtype, reduction):
         assert not cpt.distill_loss(z, t, idx, y, alpha=0.5).requires_grad
 
 
+def test_widest(device):
+    """The widest vocabulary with the most entries (96 KiB of LDS)."""
+    z, t, idx, y, lse = _inputs(2, 524288, 2048, torch.bfloat16, device, tail=True)
+    y[0] = -100
+    check(z, t, idx, y, lse, 1.0, 0.5)
+    check(z, t, idx, y, None, 2.0, 0.5)
+
+
+def test_inplace_is_known_to_autograd(device):
+    """A graph that keeps the logits themselves cannot be used after they are gone."""
+    cpt = _cpt()
+    z, t, idx, _, _ = _inputs(4, 300, 5, torch.float32, device, labels=False)
+    leaf = z.clone().requires_grad_(True)
+    loss = cpt.distill_loss(torch.tanh(leaf), t, idx, inplace=True)
+    with pytest.raises(RuntimeError):
+        loss.backward()
+
+
+def test_graph(device):
+    """Captured and replayed, with other work between the replays."""
+    cpt = _cpt()
+    z, t, idx, y, _ = _inputs(40, 5003, 9, torch.bfloat16, device)
+    kw = dict(temperature=2.0, alpha=0.5)
+    cpt.distill_topk(z, t, idx, y, **kw)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, grad = cpt.distill_topk(z, t, idx, y, **kw)
+    for i in range(4):
+        z.copy_(z.roll(1, 0))
+        y.copy_(y.roll(1, 0))
+        want = cpt.distill_topk(z, t, idx, y, **kw)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(loss, want[0]) and torch.equal(grad, want[1])
+
+
 def test_another_stream(device):
     cpt = _cpt()
     z, t, idx, y, _ = _inputs(64, 9000, 5, torch.bfloat16, device)

@@ -107,6 +107,49 @@ def test_gradient_long(device, kind, n):
     assert torch.equal(got, cpt.embedding_backward(grad, ids, 32000))
 
 
+@pytest.mark.parametrize("n,v", [(16385, 32000), (20000, 200), (20000, 300000), (50000, 70000)])
+def test_gradient_radix(device, n, v):
+    """One to three passes of the sort, and the first length that takes it."""
+    cpt = _cpt()
+    g = torch.Generator().manual_seed(n + v)
+    ids = _ids("skewed", n, v, g).to(device)
+    grad = torch.randn(n, 40, device=device)
+    got = cpt.embedding_backward(grad, ids, v, padding_idx=1)
+    _check_grad(got, grad, ids, v, 1.0, 1)
+
+
+@pytest.mark.parametrize("d", [5, 515, 1001])
+def test_ragged_rows_added_to_a_buffer(device, d):
+    cpt = _cpt()
+    g = torch.Generator().manual_seed(d)
+    ids = _ids("skewed", 900, 50, g).to(device)
+    grad = torch.randn(900, d, generator=g).to(torch.bfloat16).to(device)
+    base = torch.randn(50, d, generator=g).to(device)
+    out = cpt.embedding_backward(grad, ids, 50, out=base.clone())
+    _check_grad(out, grad, ids, 50, 1.0, None, base)
+
+
+def test_graph(device):
+    """Captured and replayed, with other work between the replays."""
+    cpt = _cpt()
+    w = torch.randn(700, 264, device=device).to(torch.bfloat16)
+    for n in (3000, 17000):
+        ids = torch.randint(0, 700, (n,), device=device)
+        grad = torch.randn(n, 264, device=device).to(torch.bfloat16)
+        cpt.embedding_backward(grad, ids, 700)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = cpt.embedding(ids, w, 2.0)
+            dw = cpt.embedding_backward(grad, ids, 700)
+        for i in range(4):
+            ids.copy_(ids.roll(7) // (1 + i % 2))
+            want = cpt.embedding(ids, w, 2.0), cpt.embedding_backward(grad, ids, 700)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want[0]) and torch.equal(dw, want[1])
+
+
 @pytest.mark.parametrize("dtype,out_dtype", [(torch.bfloat16, torch.bfloat16),
                                              (torch.bfloat16, torch.float32),
                                              (torch.float16, torch.float32),

@@ -221,6 +221,43 @@ def test_zero_rows_and_large_values(device):
     assert out[1][2].isnan().all()
 
 
+@pytest.mark.parametrize("gate", ["none", "channel", "sequence", "token"])
+def test_narrow_rows(device, gate):
+    """Fewer columns than a vector."""
+    cpt = _cpt()
+    for shape in ((3, 4, 5), (2, 700, 7), (1, 9, 2)):
+        res, y, dro, dx, w_pre, w_post, g = _inputs(shape, torch.bfloat16, torch.float32, gate,
+                                                    True, device)
+        out = cpt.residual_norm(res, y, w_pre, w_post=w_post, gate=g, eps=EPS)
+        check_forward(out, res, y, w_pre, w_post, g, 1.0, 1.0, EPS)
+        grads = cpt.residual_norm_backward(dro, dx, out[0], y, out[2], w_pre, w_post=w_post, gate=g)
+        check_backward(grads, dro, dx, out[0], y, out[2], w_pre, w_post, g, 1.0, 1.0)
+
+
+def test_graph(device):
+    """Captured and replayed, with other work between the replays."""
+    cpt = _cpt()
+    res, y, dro, dx, w_pre, w_post, g = _inputs((2, 50, 2056), torch.bfloat16, torch.bfloat16,
+                                                "channel", True, device)
+
+    def step():
+        out = cpt.residual_norm(res, y, w_pre, w_post=w_post, gate=g)
+        return out + cpt.residual_norm_backward(dro, dx, out[0], y, out[2], w_pre, w_post=w_post,
+                                                gate=g)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(4):
+        y.copy_(y.roll(1, 1))
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_no_rows(device):
     cpt = _cpt()
     w = torch.ones(64, device=device, requires_grad=True)
