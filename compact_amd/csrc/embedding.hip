@@ -7,8 +7,8 @@
 //
 // The gradient adds no floats atomically.  The tokens' (id, position) pairs are
 // sorted by id with their order kept, so one id's tokens lie side by side in the
-// order of the batch: up to 16384 tokens by counting each one's smaller ids in one
-// launch, beyond by a radix sort of 8 bits a pass (a block ranks 2048 pairs by
+// order of the batch: up to some 8192 tokens by counting each one's smaller ids in
+// one launch, beyond by a radix sort of 8 bits a pass (a block ranks 2048 pairs by
 // ballots).  The table's zeros are written by further blocks of the same launches:
 // sorting is latency and compares, the zeros are HBM.  The sorted list is cut into
 // tiles of equal length, whatever ids they hold, so a frequent token's rows are
@@ -95,13 +95,13 @@ __device__ __forceinline__ bool zeros_here(const Zeros& z) {
 }
 
 // counts[block][digit] of the pairs' digit (key >> shift) & 255 (of the tokens
-// themselves where `in` is null).
+// themselves where `in` is null), and zeros for the `later` passes' counts.
 template <int OT>
 __global__ __launch_bounds__(kBlock) void count_kernel(const Pair* __restrict__ in,
                                                        const void* __restrict__ ids, int wide,
                                                        int64_t n, int64_t vocab, int64_t padding,
                                                        int shift, uint32_t* __restrict__ counts,
-                                                       Zeros zeros) {
+                                                       unsigned blocks, int later, Zeros zeros) {
   __shared__ uint32_t hist[kRadix];
   if (zeros_here<OT>(zeros)) return;
   hist[threadIdx.x] = 0;
@@ -115,25 +115,32 @@ __global__ __launch_bounds__(kBlock) void count_kernel(const Pair* __restrict__ 
     atomicAdd(&hist[(key >> shift) & (kRadix - 1)], 1u);
   }
   __syncthreads();
-  counts[(int64_t)blockIdx.x * kRadix + threadIdx.x] = hist[threadIdx.x];
+  for (int p = 0; p <= later; ++p)
+    counts[((int64_t)p * blocks + blockIdx.x) * kRadix + threadIdx.x] =
+        p == 0 ? hist[threadIdx.x] : 0;
 }
 
 // One pass of the sort: pairs of `in` (the tokens themselves in the first) to
-// their places by digit (key >> shift) & 255, equal digits in their order.
+// their places by digit (key >> shift) & 255, equal digits in their order.  `next`
+// (or null) takes the next digit's counts of the blocks that the pairs move to:
+// gathered in LDS (1 KiB a block), as a frequent token's pairs all add to one.
 template <int OT>
 __global__ __launch_bounds__(kBlock) void scatter_kernel(const Pair* __restrict__ in,
                                                          const void* __restrict__ ids, int wide,
                                                          int64_t n, int64_t vocab, int64_t padding,
                                                          int shift,
                                                          const uint32_t* __restrict__ counts,
-                                                         unsigned blocks, Pair* __restrict__ out,
-                                                         Zeros zeros) {
+                                                         unsigned blocks, uint32_t* next,
+                                                         Pair* __restrict__ out, Zeros zeros) {
+  extern __shared__ uint32_t moved[];   // [blocks][digit]
   __shared__ uint32_t wave_count[kWaves][kRadix];
   __shared__ uint32_t base[kRadix];
   __shared__ uint32_t scan[kWaves];
   if (zeros_here<OT>(zeros)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   for (int w = 0; w < kWaves; ++w) wave_count[w][tid] = 0;
+  if (next)
+    for (unsigned b = 0; b < blocks; ++b) moved[b * kRadix + tid] = 0;
   __syncthreads();
   // a wavefront ranks 512 consecutive pairs, 64 at a time
   const int64_t i0 = (int64_t)blockIdx.x * kSortTile + wave * (kSortTile / kWaves) + lane;
@@ -193,7 +200,16 @@ __global__ __launch_bounds__(kBlock) void scatter_kernel(const Pair* __restrict_
   for (int k = 0; k < kItems; ++k) {
     if (i0 + k * 64 >= n) continue;
     const uint32_t digit = (q[k].id >> shift) & (kRadix - 1);
-    out[base[digit] + wave_count[wave][digit] + rank[k]] = q[k];
+    const uint32_t to = base[digit] + wave_count[wave][digit] + rank[k];
+    out[to] = q[k];
+    if (next)
+      atomicAdd(&moved[to / kSortTile * kRadix + (q[k].id >> (shift + 8) & (kRadix - 1))], 1u);
+  }
+  if (!next) return;
+  __syncthreads();
+  for (unsigned b = 0; b < blocks; ++b) {
+    const uint32_t c = moved[b * kRadix + tid];
+    if (c) atomicAdd(&next[(int64_t)b * kRadix + tid], c);
   }
 }
 
@@ -441,10 +457,16 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const Pair* __restri
   }
 }
 
-// Tokens up to which the one-launch sort is the faster: with the table's zeros
-// beside it 12000 tokens take 52 us against the radix sort's 63, 20011 (in a small
-// table) 95 against 81.
-constexpr int64_t kRankTokens = 16384;
+// Whether the one-launch sort is the faster: its compares grow with the square of
+// the tokens (9 us at 8192, 21 at 12500), the radix sort's three launches take 20.
+// Zeros of 64 MiB or more hide it for longer.  us for the whole gradient, with the
+// one sort and the other: 8192 tokens into 32000 x 2048 bf16 40 and 48; 12500 into
+// the same 53 and 60; 9000 into 5000 x 1000 36 and 34; 16000 into that 50 and 37.
+bool rank_pays(int64_t n, int64_t zero_bytes) {
+  return n <= (zero_bytes >= (64 << 20) ? 12288 : 8192);
+}
+
+constexpr unsigned kMovedBlocks = 56;   // 56 KiB of LDS: 114688 tokens
 constexpr int kZeroThreads = 1 << 20;   // of a launch's blocks of zeros
 
 inline int launched() { return hipGetLastError() == hipSuccess ? kOk : kErrLaunch; }
@@ -476,7 +498,7 @@ Plan plan(int64_t n, int64_t vocab, int64_t d) {
   p.sort_blocks = (n + kSortTile - 1) / kSortTile;
   p.tiles = (n + p.tile - 1) / p.tile;
   p.counts = 0;
-  p.pairs = up(p.sort_blocks * kRadix * 4);
+  p.pairs = up(p.passes * p.sort_blocks * kRadix * 4);
   p.edge = p.pairs + 2 * up(n * (int64_t)sizeof(Pair));
   p.bytes = p.edge + up(p.tiles * 2 * d * 4);
   return p;
@@ -560,7 +582,7 @@ int cpt_embedding_backward(int dtype, int out_dtype, const void* grad, int64_t l
   };
   const Pair* in = pairs[0];
   unsigned grid;
-  if (n <= kRankTokens) {
+  if (rank_pays(n, total * (out_dtype == kF32 ? 4 : 2))) {
     const unsigned own = (unsigned)((n + 63) / 64);
     const Zeros z = zeros(0, 1, own, kRankThreads, &grid);
     const auto kern = out_dtype == kF32   ? rank_kernel<kF32>
@@ -576,12 +598,22 @@ int cpt_embedding_backward(int dtype, int out_dtype, const void* grad, int64_t l
                          : out_dtype == kF16 ? scatter_kernel<kF16>
                                              : scatter_kernel<kBF16>;
     in = nullptr;
+    // a pass counts for the next one where the blocks' counts fit LDS
+    const bool ahead = own <= kMovedBlocks;
+    const int parts = ahead ? p.passes + 1 : 2 * p.passes;
+    int part = 0;
     for (int k = 0; k < p.passes; ++k) {
-      Zeros z = zeros(2 * k, 2 * p.passes, own, kBlock, &grid);
-      count<<<grid, kBlock, 0, st>>>(in, ids, ids_wide, n, vocab, padding_idx, 8 * k, counts, z);
-      z = zeros(2 * k + 1, 2 * p.passes, own, kBlock, &grid);
-      scatter<<<grid, kBlock, 0, st>>>(in, ids, ids_wide, n, vocab, padding_idx, 8 * k, counts,
-                                       own, pairs[k & 1], z);
+      uint32_t* const c = counts + (ahead ? (int64_t)k * own * kRadix : 0);
+      if (k == 0 || !ahead) {
+        const Zeros z = zeros(part++, parts, own, kBlock, &grid);
+        count<<<grid, kBlock, 0, st>>>(in, ids, ids_wide, n, vocab, padding_idx, 8 * k, c, own,
+                                       ahead ? p.passes - 1 : 0, z);
+      }
+      const bool counts_next = ahead && k + 1 < p.passes;
+      const Zeros z = zeros(part++, parts, own, kBlock, &grid);
+      scatter<<<grid, kBlock, counts_next ? own * kRadix * 4 : 0, st>>>(
+          in, ids, ids_wide, n, vocab, padding_idx, 8 * k, c, own,
+          counts_next ? c + (int64_t)own * kRadix : nullptr, pairs[k & 1], z);
       in = pairs[k & 1];
     }
   }

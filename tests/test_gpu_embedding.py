@@ -107,9 +107,11 @@ def test_gradient_long(device, kind, n):
     assert torch.equal(got, cpt.embedding_backward(grad, ids, 32000))
 
 
-@pytest.mark.parametrize("n,v", [(16385, 32000), (20000, 200), (20000, 300000), (50000, 70000)])
+@pytest.mark.parametrize("n,v", [(8192, 500), (8193, 500), (12288, 850000), (12289, 850000),
+                                 (16385, 32000), (20000, 200), (20000, 300000), (50000, 70000),
+                                 (114688, 70000), (114689, 70000)])
 def test_gradient_radix(device, n, v):
-    """One to three passes of the sort, and the first length that takes it."""
+    """One to three passes of the sort; the lengths at which another one begins."""
     cpt = _cpt()
     g = torch.Generator().manual_seed(n + v)
     ids = _ids("skewed", n, v, g).to(device)
