@@ -181,22 +181,24 @@ def _gate_kind(gate, shape):
 
 
 def _norm_args(x, y, w_pre, w_post, gate, residual_scale):
-    """Checks shared by both directions; returns the weights' type."""
-    d = x.shape[-1]
-    assert y is None or (y.shape == x.shape and y.dtype == x.dtype), \
-        "residual and y share shape and dtype"
-    assert y is not None or (w_post is None and gate is None and residual_scale == 1.0), \
-        "w_post, gate and residual_scale belong to a block's output y"
-    wdt = None
-    for name, w in (("w_pre", w_pre), ("w_post", w_post), ("gate", gate)):
-        if w is None:
-            continue
-        assert wdt is None or w.dtype == wdt, "w_pre, w_post and gate share one dtype"
-        wdt = w.dtype
-        assert name == "gate" or tuple(w.shape) == (d,), f"{name} {tuple(w.shape)} for D={d}"
-    wdt = x.dtype if wdt is None else wdt
-    assert wdt in (x.dtype, torch.float32), f"weights of {wdt} with activations of {x.dtype}"
-    return wdt
+    """Checks shared by both directions; returns the weights' type code."""
+    shape = x.shape
+    if y is None:
+        assert w_post is None and gate is None and residual_scale == 1.0, \
+            "w_post, gate and residual_scale belong to a block's output y"
+    else:
+        assert y.shape == shape and y.dtype == x.dtype, "residual and y share shape and dtype"
+    wdt = x.dtype
+    first = w_pre if w_pre is not None else w_post if w_post is not None else gate
+    if first is not None:
+        wdt = first.dtype
+        assert wdt == x.dtype or wdt == torch.float32, \
+            f"weights of {wdt} with activations of {x.dtype}"
+    for w in (w_pre, w_post):
+        assert w is None or (w.dtype == wdt and w.dim() == 1 and w.shape[0] == shape[-1]), \
+            f"weights: {wdt} {(shape[-1],)} expected, got {w.dtype} {tuple(w.shape)}"
+    assert gate is None or gate.dtype == wdt, "w_pre, w_post and gate share one dtype"
+    return _DT[wdt]
 
 
 def _dense(t):
@@ -222,7 +224,8 @@ def residual_norm(residual, y=None, w_pre=None, *, w_post=None, gate=None, scale
     assert y is not None or w_pre is not None, "residual_norm: y or w_pre expected"
     assert eps >= 0, f"eps={eps}"
     wdt = _norm_args(residual, y, w_pre, w_post, gate, residual_scale)
-    shape, d = residual.shape, residual.shape[-1]
+    shape = residual.shape
+    d = shape[-1]
     kind, seq = _gate_kind(gate, shape)
     rows = residual.numel() // d
     w_pre, w_post, gate = _dense(w_pre), _dense(w_post), _dense(gate)
@@ -235,7 +238,7 @@ def residual_norm(residual, y=None, w_pre=None, *, w_post=None, gate=None, scale
         return (residual if out is None else out), x, stats
     with _timed("residual_norm"):
         rc = _lib.api().cpt_residual_norm(
-            dt, _DT[wdt], res.data_ptr(), ld_res, _ptr(y2), ld_y, _ptr(w_post), _ptr(w_pre),
+            dt, wdt, res.data_ptr(), ld_res, _ptr(y2), ld_y, _ptr(w_post), _ptr(w_pre),
             _ptr(gate), kind, rows, seq, d, float(scale), float(residual_scale), float(eps),
             _ptr(out), _ptr(x), stats.data_ptr(), _stream(residual))
     check(rc, "residual_norm")
@@ -281,7 +284,7 @@ def residual_norm_backward(d_residual_out, d_x, residual_out, y, stats, w_pre=No
     ws = torch.empty(nbytes // 4, dtype=torch.float32, device=residual_out.device)
     with _timed("residual_norm_backward"):
         rc = L.cpt_residual_norm_backward(
-            dt, _DT[wdt], _ptr(dro), ld_dro, _ptr(dx), ld_dx, ro.data_ptr(), ld_ro, _ptr(y2),
+            dt, wdt, _ptr(dro), ld_dro, _ptr(dx), ld_dx, ro.data_ptr(), ld_ro, _ptr(y2),
             ld_y, stats.data_ptr(), _ptr(w_post), _ptr(w_pre), _ptr(gate), kind, rows, seq, d,
             float(scale), float(residual_scale), d_res.data_ptr(), _ptr(d_y), _ptr(d_w_pre),
             _ptr(d_w_post), _ptr(d_gate), ws.data_ptr(), _stream(residual_out))
@@ -398,7 +401,6 @@ def distill_topk(logits, top_logits, top_indices, labels=None, *, top_lse=None,
         top_lse = top_lse.float().contiguous()
     top_logits, top_indices = top_logits.contiguous(), top_indices.contiguous()
     rows = logits.numel() // v
-    dev = logits.device
 
     # rows per batch entry, and the strides of both
     z, seq, ld_b, ld_s = logits, max(rows, 1), 0, v
@@ -428,7 +430,7 @@ def distill_topk(logits, top_logits, top_indices, labels=None, *, top_lse=None,
     elif grad_out is not None:
         scale = float(grad_out)
     # a row's loss each, then (one more) their sum or mean
-    losses = torch.empty(rows + 1, dtype=torch.float32, device=dev)
+    losses = torch.empty(rows + 1, dtype=torch.float32, device=logits.device)
     loss = losses[:rows].view(lead) if reduction == "none" else losses[rows]
     with _timed("distill_topk"):
         rc = _lib.api().cpt_distill_topk(
