@@ -7,14 +7,18 @@
 //
 // The gradient adds no floats atomically.  The tokens' (id, position) pairs are
 // sorted by id with their order kept, so one id's tokens lie side by side in the
-// order of the batch: up to some 8192 tokens by counting each one's smaller ids in
-// one launch, beyond by a radix sort of 8 bits a pass (a block ranks 2048 pairs by
-// ballots).  The table's zeros are written by further blocks of the same launches:
+// order of the batch: up to 32768 tokens in one launch, each of 32 blocks sorting a
+// range of ids in LDS; beyond by a radix sort of 8 bits a pass (a block ranks 2048
+// pairs by ballots).  The table's zeros are written by further blocks of the same launches:
 // sorting is latency and compares, the zeros are HBM.  The sorted list is cut into
 // tiles of equal length, whatever ids they hold, so a frequent token's rows are
 // spread over as many wavefronts as it needs; sums of an id over several tiles are
 // joined in tile order.  The result is the same from run to run.  Bound by HBM: dy
 // is read once, the table written once (rows with tokens twice).
+//
+// Measured on one MI355X: the lookup of 8192 x 2048 bf16 9.8 us (4.6 TB/s), its
+// gradient into 32000 rows 36 (4.5 TB/s of what it must read and write), of 65536
+// tokens 119.  The sums take 11 us of the first, 69 of the second, at 4.4 TB/s.
 
 #include "compact_amd.h"
 #include "row_ops.h"
@@ -213,54 +217,154 @@ __global__ __launch_bounds__(kBlock) void scatter_kernel(const Pair* __restrict_
   }
 }
 
-// The sort of a short list in one launch, beside the table's zeros: a token's
-// place is the number of tokens with a smaller id, or the same one earlier.  Blocks
-// [0, rank_blocks) count for 64 tokens each, 64 compares an instruction and a
-// population count on the scalar unit (n^2 / 64 vector instructions in all: 1 us of
-// the chip at 8192 tokens), while the other blocks, bound by HBM, write zeros.
-constexpr int kRankThreads = 1024;
-constexpr int kRankWaves = kRankThreads / 64;
-constexpr int kRankChunks = 8;   // 64 keys each, held by a wavefront at a time
+// The sort of up to 32768 tokens in one launch.  Each of 32 blocks takes a range of
+// ids: it reads all tokens, counts those below its range and packs those inside,
+// in their order, into LDS as (id - first id) << 15 | position; sorts them there
+// by the id's bits in stable passes of up to 8; and writes them behind the tokens
+// of the ranges below.  Tokens that are summed nowhere fill the list's end.  Bound by
+// latency and, in the reading of all tokens by each block, by the vector pipe: 18 us
+// at 8192 tokens beside 131 MB of zeros (which alone take 20), 20 to 24 at 20011.
+// The whole gradient against the radix sort's three launches: 8192 tokens into
+// 32000 x 2048 bf16 36 and 48 us, 16000 into 5000 x 1000 33 and 37, 20011 x 1001
+// fp32 48 and 52, 32768 into 32000 x 2048 86 and 84.
+constexpr int kRanges = 32;
+constexpr int kRangeThreads = 1024;
+constexpr int kRangeWaves = kRangeThreads / 64;
+constexpr int kPosBits = 15;
+constexpr int kRangeRounds = (1 << kPosBits) / kRangeThreads;   // of 64 tokens a wavefront
 
 template <int OT>
-__global__ __launch_bounds__(kRankThreads) void rank_kernel(const void* __restrict__ ids, int wide,
-                                                            int64_t n, int64_t vocab,
-                                                            int64_t padding,
-                                                            Pair* __restrict__ pairs,
-                                                            Zeros zeros) {
-  __shared__ int part[kRankWaves][64];
+__global__ __launch_bounds__(kRangeThreads) void range_sort_kernel(
+    const void* __restrict__ ids, int wide, int n, uint32_t vocab, int64_t padding, uint32_t span,
+    int bits, Pair* __restrict__ out, Zeros zeros) {
+  extern __shared__ uint32_t list[];   // [n]
+  __shared__ uint16_t count[kRangeWaves][kRadix];
+  __shared__ uint32_t base[kRadix], tmp[2][kRangeWaves];
   if (zeros_here<OT>(zeros)) return;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int chunks = (int)((n + 63) / 64), own = blockIdx.x;
-  const int64_t at = (int64_t)own * 64 + lane;
-  // past the end: a key above every other
-  const uint32_t key = at < n ? token_key(ids, wide, at, vocab, padding) : ~0u;
-  int rank = 0;
-  for (int c0 = wave * kRankChunks; c0 < chunks; c0 += kRankWaves * kRankChunks) {
-    uint32_t k[kRankChunks];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t lo = min(blockIdx.x * span, vocab), width_in = min(span, vocab - lo);
+  const uint64_t lower = (1ull << lane) - 1;
+  // a wavefront has consecutive tokens, 64 at a time; one compare each tells what lies
+  // inside the range and below it (a negative id of 32 bits is above every other)
+  int each = (n + kRangeThreads - 1) / kRangeThreads * 64, i0 = wave * each;
+  const int i1 = min(n, i0 + each);
+  constexpr int kAhead = 16;
+  const uint32_t pad = padding >= 0 ? (uint32_t)padding : ~0u;
+  const auto keys = [&](int i, uint32_t (&k)[kAhead]) {
+    uint32_t top[kAhead];
+    if (wide) {
 #pragma unroll
-    for (int c = 0; c < kRankChunks; ++c) {
-      const int64_t i = (int64_t)(c0 + c) * 64 + lane;
-      // equal keys count where they come earlier: in the chunks before this one
-      k[c] = i < n ? token_key(ids, wide, i, vocab, padding) : ~0u;
-      if (c0 + c >= own && i < n) ++k[c];
+      for (int t = 0; t < kAhead; ++t) {
+        const uint2 id = reinterpret_cast<const uint2*>(ids)[min(i + 64 * t + lane, n - 1)];
+        k[t] = id.x, top[t] = id.y;
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < kAhead; ++t) {
+        k[t] = reinterpret_cast<const uint32_t*>(ids)[min(i + 64 * t + lane, n - 1)];
+        top[t] = 0;
+      }
     }
-    for (int t = 0; t < 64; ++t) {
-      const uint32_t mine = (uint32_t)__builtin_amdgcn_readlane((int)key, t);
-      int below = 0;
 #pragma unroll
-      for (int c = 0; c < kRankChunks; ++c) below += __popcll(__ballot(k[c] <= mine));
-      if (lane == t) rank += below;
+    for (int t = 0; t < kAhead; ++t)
+      if (top[t] != 0 || i + 64 * t + lane >= i1 || k[t] == pad) k[t] = ~0u;
+  };
+  uint32_t inside = 0, below = 0;
+  for (int i = i0; i < i1; i += 64 * kAhead) {
+    uint32_t k[kAhead];
+    keys(i, k);
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) {
+      inside += __popcll(__ballot(k[t] - lo < width_in));
+      below += __popcll(__ballot(k[t] < lo));
     }
   }
-  part[wave][lane] = rank;
+  if (lane == 0) tmp[0][wave] = inside, tmp[1][wave] = below;
   __syncthreads();
-  if (wave > 0 || at >= n) return;
-  for (int w = 1; w < kRankWaves; ++w) rank += part[w][lane];
-  for (int t = 0; t < 64; ++t)   // the own chunk's equal keys
-    rank += (uint32_t)__builtin_amdgcn_readlane((int)key, t) == key && t < lane;
-  pairs[rank] = Pair{key, (uint32_t)at};
+  int to = 0, m = 0, first = 0;
+  for (int w = 0; w < kRangeWaves; ++w) {
+    to += w < wave ? tmp[0][w] : 0;
+    m += tmp[0][w];
+    first += tmp[1][w];
+  }
+  for (int i = i0; i < i1; i += 64 * kAhead) {
+    uint32_t k[kAhead];
+    keys(i, k);
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) {
+      const bool in = k[t] - lo < width_in;
+      const uint64_t mask = __ballot(in);
+      if (in) list[to + __popcll(mask & lower)] = (k[t] - lo) << kPosBits | (i + 64 * t + lane);
+      to += __popcll(mask);
+    }
+  }
+  // stable passes over the packed list, its pairs in registers between LDS and LDS
+  each = (m + kRangeThreads - 1) / kRangeThreads * 64, i0 = wave * each;
+  const int rounds = each / 64;
+  const int passes = (bits + 7) / 8, width = passes > 0 ? (bits + passes - 1) / passes : 0;
+  for (int p = 0; p < passes; ++p) {
+    const int shift = kPosBits + p * width;
+    for (int c = tid; c < kRangeWaves * kRadix / 2; c += kRangeThreads)
+      reinterpret_cast<uint32_t*>(&count[0][0])[c] = 0;
+    __syncthreads();
+    uint32_t q[kRangeRounds], rank[kRangeRounds];
+#pragma unroll
+    for (int r = 0; r < kRangeRounds; ++r) {
+      if (r >= rounds) break;
+      const int i = i0 + 64 * r + lane;
+      const bool live = i < m;
+      q[r] = live ? list[i] : 0;
+      const uint32_t digit = q[r] >> shift & ((1u << width) - 1);
+      uint64_t same = __ballot(live);
+      for (int b = 0; b < width; ++b) {
+        const uint64_t set = __ballot(digit >> b & 1);
+        same &= digit >> b & 1 ? set : ~set;
+      }
+      const uint32_t before = live ? count[wave][digit] : 0;
+      rank[r] = before + __popcll(same & lower);
+      // the wavefront's accesses to its own counters stay in order: read, then written
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (live && (same & lower) == 0) count[wave][digit] = (uint16_t)(before + __popcll(same));
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    __syncthreads();
+    // thread d: digit d's pairs by wavefront, and where they start
+    uint32_t total = 0, upto = 0;
+    if (tid < kRadix) {
+      for (int w = 0; w < kRangeWaves; ++w) {
+        const uint32_t c = count[w][tid];
+        count[w][tid] = (uint16_t)total;
+        total += c;
+      }
+      upto = total;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t u = __shfl_up(upto, off);
+        if (lane >= off) upto += u;
+      }
+      if (lane == 63) tmp[0][wave] = upto;
+    }
+    __syncthreads();
+    if (tid < kRadix) {
+      for (int w = 0; w < wave; ++w) upto += tmp[0][w];
+      base[tid] = upto - total;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kRangeRounds; ++r) {
+      if (r >= rounds) break;
+      if (i0 + 64 * r + lane >= m) continue;
+      const uint32_t digit = q[r] >> shift & ((1u << width) - 1);
+      list[base[digit] + count[wave][digit] + rank[r]] = q[r];
+    }
+    __syncthreads();
+  }
+  if (passes == 0) __syncthreads();
+  for (int i = tid; i < m; i += kRangeThreads)
+    out[first + i] = Pair{lo + (list[i] >> kPosBits), list[i] & ((1u << kPosBits) - 1)};
+  if (blockIdx.x == kRanges - 1)
+    for (int i = first + m + tid; i < n; i += kRangeThreads) out[i] = Pair{vocab, 0};
 }
 
 // ---------------------------------------------------------------------------
@@ -457,13 +561,15 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const Pair* __restri
   }
 }
 
-// Whether the one-launch sort is the faster: its compares grow with the square of
-// the tokens (9 us at 8192, 21 at 12500), the radix sort's three launches take 20.
-// Zeros of 64 MiB or more hide it for longer.  us for the whole gradient, with the
-// one sort and the other: 8192 tokens into 32000 x 2048 bf16 40 and 48; 12500 into
-// the same 53 and 60; 9000 into 5000 x 1000 36 and 34; 16000 into that 50 and 37.
-bool rank_pays(int64_t n, int64_t zero_bytes) {
-  return n <= (zero_bytes >= (64 << 20) ? 12288 : 8192);
+// The ids of a range, and whether the tokens' places fit beside their bits.
+uint32_t range_span(int64_t vocab) { return (uint32_t)((vocab + kRanges - 1) / kRanges); }
+int bits_of(uint32_t v) {   // 0 .. v
+  int b = 0;
+  while (b < 32 && (v >> b) != 0) ++b;
+  return b;
+}
+bool by_ranges(int64_t n, int64_t vocab) {
+  return n <= (1 << kPosBits) && bits_of(range_span(vocab) - 1) <= 32 - kPosBits;
 }
 
 constexpr unsigned kMovedBlocks = 56;   // 56 KiB of LDS: 114688 tokens
@@ -582,13 +688,19 @@ int cpt_embedding_backward(int dtype, int out_dtype, const void* grad, int64_t l
   };
   const Pair* in = pairs[0];
   unsigned grid;
-  if (rank_pays(n, total * (out_dtype == kF32 ? 4 : 2))) {
-    const unsigned own = (unsigned)((n + 63) / 64);
-    const Zeros z = zeros(0, 1, own, kRankThreads, &grid);
-    const auto kern = out_dtype == kF32   ? rank_kernel<kF32>
-                      : out_dtype == kF16 ? rank_kernel<kF16>
-                                          : rank_kernel<kBF16>;
-    kern<<<grid, kRankThreads, 0, st>>>(ids, ids_wide, n, vocab, padding_idx, pairs[0], z);
+  if (by_ranges(n, vocab)) {
+    const Zeros z = zeros(0, 1, kRanges, kRangeThreads, &grid);
+    const auto kern = out_dtype == kF32   ? range_sort_kernel<kF32>
+                      : out_dtype == kF16 ? range_sort_kernel<kF16>
+                                          : range_sort_kernel<kBF16>;
+    const size_t lds = 4 * (size_t)n;
+    if (lds > 32 * 1024 &&
+        hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
+                            (int)lds) != hipSuccess)
+      return kErrLaunch;
+    const uint32_t span = range_span(vocab);
+    kern<<<grid, kRangeThreads, lds, st>>>(ids, ids_wide, (int)n, (uint32_t)vocab, padding_idx,
+                                           span, bits_of(span - 1), pairs[0], z);
   } else {
     const unsigned own = (unsigned)p.sort_blocks;
     const auto count = out_dtype == kF32   ? count_kernel<kF32>
