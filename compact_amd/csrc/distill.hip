@@ -124,6 +124,19 @@ struct Teacher {
   float m, st, s1; // with a tail: maximum and sums over the entries' columns
 };
 
+// A teacher's entry as it is stored: the words of its index and of its logit.
+struct Entry {
+  uint32_t index, index_high;
+  uint16_t low, high;
+  __device__ __forceinline__ int id(uint32_t vocab, int wide) const {
+    return (wide ? index_high == 0 : true) && index < vocab ? (int)index : -1;
+  }
+  __device__ __forceinline__ float logit(int dt) const {
+    if (dt == kF32) return __uint_as_float((uint32_t)high << 16 | low);
+    return dt == kF16 ? f16_bits_to_f32(low) : bf16_to_f32(low);
+  }
+};
+
 // The compiler would keep every unpacked column of one pass over the registers
 // for the next: eight registers a vector more than it has.
 template <int DT>
@@ -219,15 +232,17 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
       }
       continue;
     }
-    // loads come back in order: the first entries', needed first, lead
-    const auto entry = [&](int k, int* id, float* t) {
-      const int64_t i = ld_index(a.idx, a.idx_wide, row * a.k + k);
-      *t = ld_any(a.top, a.top_dtype, row * a.k + k);
-      *id = i >= 0 && i < v ? (int)i : -1;
+    // Loads come back in order: the first entries', needed first, lead.  They are
+    // loaded as words of either width without a branch, which would be waited for.
+    const auto load_entry = [&](int k) {
+      const int64_t i = row * a.k + k;
+      const int64_t w = i << a.idx_wide, h = i << (a.top_dtype == kF32);
+      const uint32_t* const idx = (const uint32_t*)a.idx;
+      const uint16_t* const top = (const uint16_t*)a.top;
+      return Entry{idx[w], idx[w + a.idx_wide], top[h], top[h + (a.top_dtype == kF32)]};
     };
-    int e_id = -1;
-    float e_t = 0.f;
-    if (wave == 0 && lane < a.k) entry(lane, &e_id, &e_t);
+    Entry first{};
+    if (wave == 0 && a.k > 0) first = load_entry(min(lane, a.k - 1));
     Raw q[NV > 0 ? NV : 1];
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
@@ -241,8 +256,9 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
       float m = -INFINITY;
       int again = 0;
       for (int k = lane; k < a.k; k += 64) {
-        if (k >= 64) entry(k, &e_id, &e_t);
-        const float t = e_id >= 0 ? e_t / a.tau : -INFINITY;
+        if (k >= 64) first = load_entry(k);
+        const int e_id = first.id(v, a.idx_wide);
+        const float t = e_id >= 0 ? first.logit(a.top_dtype) / a.tau : -INFINITY;
         s_idx[k] = e_id;
         s_z[k] = e_id >= 0 ? elem(e_id) : 0.f;
         s_lp[k] = t;

@@ -9,12 +9,12 @@
 // sorted by id with their order kept, so one id's tokens lie side by side in the
 // order of the batch: up to 32768 tokens in one launch, each of 32 blocks sorting a
 // range of ids in LDS; beyond by a radix sort of 8 bits a pass (a block ranks 2048
-// pairs by ballots).  The table's zeros are written by further blocks of the same launches:
-// sorting is latency and compares, the zeros are HBM.  The sorted list is cut into
-// tiles of equal length, whatever ids they hold, so a frequent token's rows are
-// spread over as many wavefronts as it needs; sums of an id over several tiles are
-// joined in tile order.  The result is the same from run to run.  Bound by HBM: dy
-// is read once, the table written once (rows with tokens twice).
+// pairs by ballots).  The table's zeros are written by further blocks of the same
+// launches: sorting is latency and compares, the zeros are HBM.  The sorted list is
+// cut into tiles of equal length, whatever ids they hold, so a frequent token's rows
+// are spread over as many wavefronts as it needs; sums of an id over several tiles
+// are joined in tile order.  The result is the same from run to run.  Bound by HBM:
+// dy is read once, the table written once (rows with tokens twice).
 //
 // Measured on one MI355X: the lookup of 8192 x 2048 bf16 9.8 us (4.6 TB/s), its
 // gradient into 32000 rows 36 (4.5 TB/s of what it must read and write), of 65536
