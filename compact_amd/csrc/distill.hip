@@ -137,14 +137,6 @@ struct Entry {
   }
 };
 
-// The compiler would keep every unpacked column of one pass over the registers
-// for the next: eight registers a vector more than it has.
-template <int DT>
-__device__ __forceinline__ void repack(typename Row8<DT>::Raw& r) {
-  asm volatile("" : "+v"(r.w));
-  if constexpr (DT == kF32) asm volatile("" : "+v"(r.x));
-}
-
 // Whether entry k is the first of its index.
 __device__ __forceinline__ bool first_of(const int* idx, int k) {
   for (int i = 0; i < k; ++i)

@@ -18,12 +18,12 @@
 // reads four and writes two.  A group of `tr` threads holds a row in registers,
 // eight columns per thread and vector; a block has `groups` of them side by
 // side and goes over its rows with the weights (and the backward's sums over
-// tokens) kept in registers.
+// tokens, those of more than 8192 columns in LDS) kept in registers.
 //
 // Measured on one MI355X: forward of 8192 x 2048 bf16 with both norms 27 us (5.0
 // TB/s), of 8192 x 4096 49 (5.5); backward of 8192 x 4096 82 us and 5 for the
-// partial sums (4.6 TB/s), of 3009 x 1999 fp32, every row unaligned, 31 and 4.  A
-// large copy reaches 5.0.
+// partial sums (4.6 TB/s), of 3009 x 1999 fp32, every row unaligned, 31 and 4, of
+// 2000 x 16000 bf16 127 in all (3.0 TB/s).  A large copy reaches 5.0.
 
 #include "compact_amd.h"
 #include "row_ops.h"
@@ -217,7 +217,21 @@ __global__ __launch_bounds__(kMaxThreads) void backward_kernel(
   __shared__ float red[2][3][kMaxWaves];
   const int group = threadIdx.x / s.tr, tid = threadIdx.x - group * s.tr;
   const int64_t b = blockIdx.y;
-  float a[NV][8], wp[NV][8], acc_pre[NV][8], acc_g[NV][8];
+  // Two vectors a thread leave no registers for the weights' sums: LDS has them, a
+  // slot of its own for each thread (such a block has one group).  2000 x 16000 bf16
+  // with all of it in registers, which spill: 268 us; so 127.
+  constexpr bool kInLds = NV > 1;
+  float a[NV][8], wp[NV][8], acc_pre[kInLds ? 1 : NV][8], acc_g[kInLds ? 1 : NV][8];
+  float4* const slot = reinterpret_cast<float4*>(combine) + tid;
+  const auto take = [&](int i, float (&v)[8]) {
+    const float4 lo = slot[2 * i * s.tr], hi = slot[(2 * i + 1) * s.tr];
+    v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w;
+    v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+  };
+  const auto put = [&](int i, const float (&v)[8]) {
+    slot[2 * i * s.tr] = make_float4(v[0], v[1], v[2], v[3]);
+    slot[(2 * i + 1) * s.tr] = make_float4(v[4], v[5], v[6], v[7]);
+  };
 #pragma unroll
   for (int c = 0; c < NV; ++c) {
     const int64_t j = 8 * ((int64_t)c * s.tr + tid);
@@ -229,8 +243,9 @@ __global__ __launch_bounds__(kMaxThreads) void backward_kernel(
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       a[c][e] *= s.alpha * g[e];
-      acc_pre[c][e] = acc_g[c][e] = 0.f;
+      acc_pre[kInLds ? 0 : c][e] = acc_g[kInLds ? 0 : c][e] = 0.f;
     }
+    if (kInLds) put(c, acc_pre[0]), put(NV + c, acc_g[0]);
   }
   const bool ragged = s.d % 8 != 0 || s.tr * NV * 8 != s.d;
   const float inv_d = 1.f / (float)s.d;
@@ -293,6 +308,13 @@ __global__ __launch_bounds__(kMaxThreads) void backward_kernel(
       }
     }
     group_sum<3>(sum, red[turn], s.tr);
+    if (kInLds) {
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
+        repack<DT>(q.dr[c]), repack<DT>(q.dx[c]);
+        repack<DT>(q.r[c]), repack<DT>(q.y[c]);
+      }
+    }
     const float m2 = sum[0] * inv_d;
     const float dgt = sum[1] - rho2 * m2 * sum[2];
     const float m1 = w_post ? gt * dgt * inv_d : 0.f;
@@ -305,47 +327,60 @@ __global__ __launch_bounds__(kMaxThreads) void backward_kernel(
       R::unpack(q.dx[c], dx);
       R::unpack(q.r[c], r);
       R::unpack(q.y[c], v);
+      float(&sum_pre)[8] = acc_pre[kInLds ? 0 : c];
+      float(&sum_g)[8] = acc_g[kInLds ? 0 : c];
+      if (kInLds) take(c, sum_pre), take(NV + c, sum_g);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float n2 = r[e] * rho2, n1 = v[e] * rho1;
         const float t = dr[e] + rho2 * (dx[e] * wp[c][e] - n2 * m2);
-        acc_pre[c][e] += dx[e] * n2;
-        acc_g[c][e] += gt * t * n1;
+        sum_pre[e] += dx[e] * n2;
+        sum_g[e] += gt * t * n1;
         dr[e] = s.beta * t;
         v[e] = rho1 * (gt * a[c][e] * t - n1 * m1);
       }
+      if (kInLds) put(c, sum_pre), put(NV + c, sum_g);
       if (in) {
         cols.st_own((T*)d_res + row * s.d, R::pack(dr));
         if (y) cols.st_own((T*)d_y + row * s.d, R::pack(v));
       }
     }
   }
-  // the groups' sums, in group order
   float* out = partial + (b * gridDim.x + blockIdx.x) * 2 * s.d;
+  if constexpr (kInLds) {
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    auto& acc = which ? acc_g : acc_pre;
-    __syncthreads();
-    if (group > 0) {
-#pragma unroll
-      for (int c = 0; c < NV; ++c)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          combine[((group - 1) * NV + c) * 8 * s.tr + e * s.tr + tid] = acc[c][e];
+    for (int i = 0; i < 2 * NV; ++i) {
+      const Cols<kF32, TINY> cols(8 * ((int64_t)(i % NV) * s.tr + tid), s.d);
+      take(i, acc_pre[0]);
+      cols.st_own(out + i / NV * s.d, Row8<kF32>::pack(acc_pre[0]));
     }
-    __syncthreads();
-    if (group == 0) {
+  } else {
+    // the groups' sums, in group order
 #pragma unroll
-      for (int c = 0; c < NV; ++c) {
-        const Cols<kF32, TINY> cols(8 * ((int64_t)c * s.tr + tid), s.d);
-        float v[8];
+    for (int which = 0; which < 2; ++which) {
+      auto& acc = which ? acc_g : acc_pre;
+      __syncthreads();
+      if (group > 0) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[e] = acc[c][e];
-          for (int g = 1; g < s.groups; ++g)
-            v[e] += combine[((g - 1) * NV + c) * 8 * s.tr + e * s.tr + tid];
+        for (int c = 0; c < NV; ++c)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            combine[((group - 1) * NV + c) * 8 * s.tr + e * s.tr + tid] = acc[c][e];
+      }
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+          const Cols<kF32, TINY> cols(8 * ((int64_t)c * s.tr + tid), s.d);
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            v[e] = acc[c][e];
+            for (int g = 1; g < s.groups; ++g)
+              v[e] += combine[((g - 1) * NV + c) * 8 * s.tr + e * s.tr + tid];
+          }
+          cols.st_own(out + which * s.d, Row8<kF32>::pack(v));
         }
-        cols.st_own(out + which * s.d, Row8<kF32>::pack(v));
       }
     }
   }
@@ -519,7 +554,7 @@ int cpt_residual_norm_backward(int dtype, int weight_dtype, const void* d_residu
   if (rows > 0) {
     const int threads = s.tr * s.groups;
     const dim3 grid((unsigned)chunks, (unsigned)seqs);
-    const size_t lds = (size_t)(s.groups - 1) * s.tr * 8 * nv * 4;
+    const size_t lds = (size_t)(nv > 1 ? 2 * nv : s.groups - 1) * s.tr * 8 * 4;
 #define CPT_BWD(DT, NV, TINY)                                                                    \
   backward_kernel<DT, NV, TINY><<<grid, threads, lds, st>>>(                                           \
       s, d_residual_out, ld_dro, d_x, ld_dx, residual_out, ld_ro, y, ld_y, (const float*)stats,  \

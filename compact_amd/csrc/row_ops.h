@@ -161,6 +161,14 @@ template <> struct Row8<kF32> {
   }
 };
 
+// The compiler would keep the columns that it unpacked for one pass over a row in
+// registers for the next pass: eight a vector more.  This makes it unpack again.
+template <int DT>
+__device__ __forceinline__ void repack(typename Row8<DT>::Raw& r) {
+  asm volatile("" : "+v"(r.w));
+  if constexpr (DT == kF32) asm volatile("" : "+v"(r.x));
+}
+
 // Elements [j, j + 8) of a row of d columns: `fill` past its end.
 template <int DT>
 __device__ __forceinline__ typename Row8<DT>::Raw row_ld(const typename Row8<DT>::T* row, int64_t j,
