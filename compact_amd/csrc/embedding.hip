@@ -251,33 +251,32 @@ __global__ __launch_bounds__(kRangeThreads) void range_sort_kernel(
   const int i1 = min(n, i0 + each);
   constexpr int kAhead = 16;
   const uint32_t pad = padding >= 0 ? (uint32_t)padding : ~0u;
-  const auto keys = [&](int i, uint32_t (&k)[kAhead]) {
+  uint32_t key[kRangeRounds];
+  uint32_t inside = 0, below = 0;
+#pragma unroll
+  for (int h = 0; h < kRangeRounds; h += kAhead) {
+    if (i0 + 64 * h >= i1) break;
     uint32_t top[kAhead];
     if (wide) {
 #pragma unroll
       for (int t = 0; t < kAhead; ++t) {
-        const uint2 id = reinterpret_cast<const uint2*>(ids)[min(i + 64 * t + lane, n - 1)];
-        k[t] = id.x, top[t] = id.y;
+        const uint2 id =
+            reinterpret_cast<const uint2*>(ids)[min(i0 + 64 * (h + t) + lane, n - 1)];
+        key[h + t] = id.x, top[t] = id.y;
       }
     } else {
 #pragma unroll
       for (int t = 0; t < kAhead; ++t) {
-        k[t] = reinterpret_cast<const uint32_t*>(ids)[min(i + 64 * t + lane, n - 1)];
+        key[h + t] = reinterpret_cast<const uint32_t*>(ids)[min(i0 + 64 * (h + t) + lane, n - 1)];
         top[t] = 0;
       }
     }
 #pragma unroll
-    for (int t = 0; t < kAhead; ++t)
-      if (top[t] != 0 || i + 64 * t + lane >= i1 || k[t] == pad) k[t] = ~0u;
-  };
-  uint32_t inside = 0, below = 0;
-  for (int i = i0; i < i1; i += 64 * kAhead) {
-    uint32_t k[kAhead];
-    keys(i, k);
-#pragma unroll
     for (int t = 0; t < kAhead; ++t) {
-      inside += __popcll(__ballot(k[t] - lo < width_in));
-      below += __popcll(__ballot(k[t] < lo));
+      uint32_t& k = key[h + t];
+      if (top[t] != 0 || i0 + 64 * (h + t) + lane >= i1 || k == pad) k = ~0u;
+      inside += __popcll(__ballot(k - lo < width_in));
+      below += __popcll(__ballot(k < lo));
     }
   }
   if (lane == 0) tmp[0][wave] = inside, tmp[1][wave] = below;
@@ -288,16 +287,13 @@ __global__ __launch_bounds__(kRangeThreads) void range_sort_kernel(
     m += tmp[0][w];
     first += tmp[1][w];
   }
-  for (int i = i0; i < i1; i += 64 * kAhead) {
-    uint32_t k[kAhead];
-    keys(i, k);
 #pragma unroll
-    for (int t = 0; t < kAhead; ++t) {
-      const bool in = k[t] - lo < width_in;
-      const uint64_t mask = __ballot(in);
-      if (in) list[to + __popcll(mask & lower)] = (k[t] - lo) << kPosBits | (i + 64 * t + lane);
-      to += __popcll(mask);
-    }
+  for (int t = 0; t < kRangeRounds; ++t) {
+    if (i0 + 64 * t >= i1) break;
+    const bool in = key[t] - lo < width_in;
+    const uint64_t mask = __ballot(in);
+    if (in) list[to + __popcll(mask & lower)] = (key[t] - lo) << kPosBits | (i0 + 64 * t + lane);
+    to += __popcll(mask);
   }
   // stable passes over the packed list, its pairs in registers between LDS and LDS
   each = (m + kRangeThreads - 1) / kRangeThreads * 64, i0 = wave * each;
