@@ -17,7 +17,7 @@
 // dy is read once, the table written once (rows with tokens twice).
 //
 // Measured on one MI355X: the lookup of 8192 x 2048 bf16 9.8 us (4.6 TB/s), its
-// gradient into 32000 rows 36 (4.5 TB/s of what it must read and write), of 65536
+// gradient into 32000 rows 35 (4.6 TB/s of what it must read and write), of 65536
 // tokens 119.  The sums take 11 us of the first, 69 of the second, at 4.4 TB/s.
 
 #include "compact_amd.h"
@@ -218,15 +218,16 @@ __global__ __launch_bounds__(kBlock) void scatter_kernel(const Pair* __restrict_
 }
 
 // The sort of up to 32768 tokens in one launch.  Each of 32 blocks takes a range of
-// ids: it reads all tokens, counts those below its range and packs those inside,
-// in their order, into LDS as (id - first id) << 15 | position; sorts them there
-// by the id's bits in stable passes of up to 8; and writes them behind the tokens
-// of the ranges below.  Tokens that are summed nowhere fill the list's end.  Bound by
+// ids: it reads all tokens into registers, counts those below its range and packs
+// those inside, in their order, into LDS as (id - first id) << 15 | position; sorts
+// them there by the id's bits in stable passes of up to 8; and writes them behind the
+// tokens of the ranges below.  Tokens that are summed nowhere fill the list's end.  Bound by
 // latency and, in the reading of all tokens by each block, by the vector pipe: 18 us
-// at 8192 tokens beside 131 MB of zeros (which alone take 20), 20 to 24 at 20011.
-// The whole gradient against the radix sort's three launches: 8192 tokens into
-// 32000 x 2048 bf16 36 and 48 us, 16000 into 5000 x 1000 33 and 37, 20011 x 1001
-// fp32 48 and 52, 32768 into 32000 x 2048 86 and 84.
+// at 8192 tokens beside 131 MB of zeros (which alone take 20), 16 at 20011 (20 where
+// the tokens are read a second time to be packed).  The whole gradient against the
+// radix sort's three launches: 8192 tokens into 32000 x 2048 bf16 35 and 48 us, 16000
+// into 5000 x 1000 31 and 37, 20011 x 1001 fp32 44 and 52, 32768 into 32000 x 2048 82
+// and 84.
 constexpr int kRanges = 32;
 constexpr int kRangeThreads = 1024;
 constexpr int kRangeWaves = kRangeThreads / 64;
