@@ -630,7 +630,7 @@ int cpt_distill_topk(int dtype, const void* logits, int64_t rows, int64_t vocab,
     return kErrShape;
   const hipStream_t st = (hipStream_t)stream;
   Args a{rows, vocab, logits, seq, ld_batch, ld_row, grad, gld_batch, gld_row, top_logits,
-         top_indices, top_dtype, idx_wide, (int)k, (const float*)top_lse, labels, label_wide,
+         top_indices, top_dtype, idx_wide != 0, (int)k, (const float*)top_lse, labels, label_wide,
          ignore_index, temperature, alpha, grad_scale, (const float*)grad_out, reduction == 2,
          reduction == 0, (float*)row_loss, (float*)loss};
   if (rows > 0) {
