@@ -23,7 +23,8 @@
 // Measured on one MI355X: forward of 8192 x 2048 bf16 with both norms 27 us (5.0
 // TB/s), of 8192 x 4096 49 (5.5); backward of 8192 x 4096 82 us and 5 for the
 // partial sums (4.6 TB/s), of 3009 x 1999 fp32, every row unaligned, 31 and 4, of
-// 2000 x 16000 bf16 127 in all (3.0 TB/s).  A large copy reaches 5.0.
+// 2000 x 16000 bf16 127 in all (3.0 TB/s), of 49923 x 128 fp16 23 in all (3.4
+// TB/s).  A large copy reaches 5.0.
 
 #include "compact_amd.h"
 #include "row_ops.h"
@@ -44,10 +45,22 @@ struct Shape {
   float alpha, beta, eps;
 };
 
-// Sums of N values over the threads of each row group, in every thread.  One
-// barrier; `red` alternates between two buffers from call to call.
+// Sums of N values over the threads of each row group, in every thread: of 16 or 32
+// threads by rotations within 16 lanes, of more with one barrier; `red` alternates
+// between two buffers from call to call.
 template <int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float (*red)[kMaxWaves], int tr) {
+  if (tr < 64) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] += dpp<0x128, 0xF>(0.f, v[i]);   // row_ror:8
+      v[i] += dpp<0x124, 0xF>(0.f, v[i]);
+      v[i] += dpp<0x122, 0xF>(0.f, v[i]);
+      v[i] += dpp<0x121, 0xF>(0.f, v[i]);
+      if (tr == 32) v[i] += __shfl_xor(v[i], 16);
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
   const int wave = threadIdx.x >> 6, per = tr >> 6;
@@ -347,40 +360,41 @@ __global__ __launch_bounds__(kMaxThreads) void backward_kernel(
     }
   }
   float* out = partial + (b * gridDim.x + blockIdx.x) * 2 * s.d;
-  if constexpr (kInLds) {
 #pragma unroll
-    for (int i = 0; i < 2 * NV; ++i) {
-      const Cols<kF32, TINY> cols(8 * ((int64_t)(i % NV) * s.tr + tid), s.d);
-      take(i, acc_pre[0]);
-      cols.st_own(out + i / NV * s.d, Row8<kF32>::pack(acc_pre[0]));
-    }
-  } else {
-    // the groups' sums, in group order
+  for (int which = 0; which < 2; ++which) {
+    auto& acc = which ? acc_g : acc_pre;
+    if (s.groups == 1) {
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      auto& acc = which ? acc_g : acc_pre;
+      for (int c = 0; c < NV; ++c) {
+        const Cols<kF32, TINY> cols(8 * ((int64_t)c * s.tr + tid), s.d);
+        if (kInLds) take(which * NV + c, acc[0]);
+        cols.st_own(out + which * s.d, Row8<kF32>::pack(acc[kInLds ? 0 : c]));
+      }
+    } else if constexpr (!kInLds) {
+      // the groups' sums, a column a thread, in group order
+      const int64_t pitch = (s.d + 7) / 8 * 8;
       __syncthreads();
-      if (group > 0) {
 #pragma unroll
-        for (int c = 0; c < NV; ++c)
+      for (int c = 0; c < NV; ++c) {
+        const C cols(8 * ((int64_t)c * s.tr + tid), s.d);
+        float* const to = combine + group * pitch + cols.at;
+        if (!TINY && cols.skip == 0) {   // aligned: 8 floats a thread
+          reinterpret_cast<float4*>(to)[0] =
+              make_float4(acc[c][0], acc[c][1], acc[c][2], acc[c][3]);
+          reinterpret_cast<float4*>(to)[1] =
+              make_float4(acc[c][4], acc[c][5], acc[c][6], acc[c][7]);
+        } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            combine[((group - 1) * NV + c) * 8 * s.tr + e * s.tr + tid] = acc[c][e];
+            if (e >= cols.skip && e < cols.skip + cols.n) to[e] = acc[c][e];
+        }
       }
       __syncthreads();
-      if (group == 0) {
-#pragma unroll
-        for (int c = 0; c < NV; ++c) {
-          const Cols<kF32, TINY> cols(8 * ((int64_t)c * s.tr + tid), s.d);
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            v[e] = acc[c][e];
-            for (int g = 1; g < s.groups; ++g)
-              v[e] += combine[((g - 1) * NV + c) * 8 * s.tr + e * s.tr + tid];
-          }
-          cols.st_own(out + which * s.d, Row8<kF32>::pack(v));
-        }
+      for (int64_t j = threadIdx.x; j < s.d; j += blockDim.x) {
+        float v = combine[j];
+#pragma unroll 8
+        for (int g = 1; g < s.groups; ++g) v += combine[g * pitch + j];
+        out[which * s.d + j] = v;
       }
     }
   }
@@ -442,11 +456,15 @@ inline int launched() { return hipGetLastError() == hipSuccess ? kOk : kErrLaunc
 constexpr int64_t kMaxD = 8 * kMaxThreads * 2;
 
 // Vectors per thread, and the threads and row groups of a block of about `threads`.
+// Rows of up to 256 columns share a wavefront, so that its lanes all have columns
+// (16 or 32 threads a row against 64: forward of 100000 x 128 bf16 19 and 52 us, of
+// 64000 x 256 26 and 36; backward of 49923 x 128 fp16 23 and 50, half of that from
+// the groups' sums being added a column a thread).
 int plan(Shape& s, int threads) {
   const int64_t vecs = (s.d + 7) / 8;
   const int nv = vecs <= kMaxThreads ? 1 : 2;
   const int64_t t = (vecs + nv - 1) / nv;
-  s.tr = (int)((t + 63) / 64 * 64);
+  s.tr = t <= 16 ? 16 : t <= 32 ? 32 : (int)((t + 63) / 64 * 64);
   s.groups = threads / s.tr > 1 ? threads / s.tr : 1;
   if (s.groups > s.seq) s.groups = s.seq > 0 ? (int)s.seq : 1;
   return nv;
@@ -554,7 +572,7 @@ int cpt_residual_norm_backward(int dtype, int weight_dtype, const void* d_residu
   if (rows > 0) {
     const int threads = s.tr * s.groups;
     const dim3 grid((unsigned)chunks, (unsigned)seqs);
-    const size_t lds = (size_t)(nv > 1 ? 2 * nv : s.groups - 1) * s.tr * 8 * 4;
+    const size_t lds = 4 * (size_t)(nv > 1 ? 2 * nv * s.tr * 8 : s.groups > 1 ? s.groups * ((d + 7) / 8 * 8) : 0);
 #define CPT_BWD(DT, NV, TINY)                                                                    \
   backward_kernel<DT, NV, TINY><<<grid, threads, lds, st>>>(                                           \
       s, d_residual_out, ld_dro, d_x, ld_dx, residual_out, ld_ro, y, ld_y, (const float*)stats,  \

@@ -349,3 +349,24 @@ def test_refusals(device):
             bad()
     with pytest.raises(RuntimeError):
         cpt.residual_norm(r.cpu(), r, w)
+
+
+# rows of 16 or 32 threads, several to a wavefront, and the first width beyond them;
+# row groups past the last row, blocks of a few rows, sums over several groups
+NARROW = [(1, 1, 121), (3, 5, 16), (3, 37, 9), (2, 70, 128), (1, 333, 129), (3, 100, 200),
+          (2, 2001, 256), (1, 3000, 257), (1, 20000, 72), (2, 35, 1000)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gate", ["none", "channel", "sequence", "token"])
+@pytest.mark.parametrize("shape", NARROW)
+def test_narrow_rows(device, dtype, gate, shape):
+    cpt = _cpt()
+    res, y, dro, dx, w_pre, w_post, g = _inputs(shape, dtype, dtype, gate, True, device, seed=3)
+    out = cpt.residual_norm(res, y, w_pre, w_post=w_post, gate=g, scale=0.7, residual_scale=1.25,
+                            eps=EPS)
+    check_forward(out, res, y, w_pre, w_post, g, 0.7, 1.25, EPS)
+    ro, _, stats = out
+    back = cpt.residual_norm_backward(dro, dx, ro, y, stats, w_pre, w_post=w_post, gate=g,
+                                      scale=0.7, residual_scale=1.25)
+    check_backward(back, dro, dx, ro, y, stats, w_pre, w_post, g, 0.7, 1.25)
