@@ -226,7 +226,7 @@ __global__ __launch_bounds__(kBlock) void scatter_kernel(const Pair* __restrict_
 // at 8192 tokens beside 131 MB of zeros (which alone take 20), 16 at 20011 (20 where
 // the tokens are read a second time to be packed).  The whole gradient against the
 // radix sort's three launches: 8192 tokens into 32000 x 2048 bf16 35 and 48 us, 16000
-// into 5000 x 1000 31 and 37, 20011 x 1001 fp32 44 and 52, 32768 into 32000 x 2048 82
+// into 5000 x 1000 31 and 37, 20011 x 1001 fp32 43 and 52, 32768 into 32000 x 2048 82
 // and 84.
 constexpr int kRanges = 32;
 constexpr int kRangeThreads = 1024;
@@ -495,6 +495,10 @@ __global__ __launch_bounds__(kBlock) void sum_kernel(const void* __restrict__ gr
 // each wavefront a part of the tiles, then the parts in order.
 constexpr int kJoinTiles = 4;
 constexpr int kJoinThreads = 512;
+// Sums loaded together, and added without a branch: one that left the loop would
+// draw each load behind it, to be waited for by itself (90000 x 100 bf16 55 us, 50
+// so; 4 together 50.5).
+constexpr int kJoinAhead = 8;
 
 template <int OT, bool TINY, bool ADD, int TILE>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(const Pair* __restrict__ pairs, int64_t n,
@@ -502,48 +506,65 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const Pair* __restri
                                                       void* out, const float* __restrict__ edge) {
   constexpr int kParts = kJoinThreads / 64;
   __shared__ float part[kParts][8][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t j = (int64_t)blockIdx.y * kCols + 8 * lane;
   const Cols<OT, TINY> to(j, d);
   const Cols<kF32, TINY> sums(j, d);
   uint32_t id = 0;
   bool is = false;
   {
-    const int64_t t = (int64_t)blockIdx.x * kJoinTiles + lane, i = t * TILE;
-    if (lane < kJoinTiles && i + 2 * TILE < n) {
-      id = pairs[i + TILE].id;
-      is = id != (uint32_t)vocab && pairs[i + TILE - 1].id == id &&
-           pairs[i + 2 * TILE].id == id &&
-           !(pairs[i].id == id && i > 0 && pairs[i - 1].id == id);
-    }
+    const int64_t i = ((int64_t)blockIdx.x * kJoinTiles + (lane & (kJoinTiles - 1))) * TILE;
+    const auto at = [&](int64_t k) { return pairs[min(max(k, (int64_t)0), n - 1)].id; };
+    const uint32_t before = at(i - 1), head = at(i), end = at(i + TILE - 1), far = at(i + 2 * TILE);
+    id = at(i + TILE);
+    is = (lane < kJoinTiles) & (i + 2 * TILE < n) & (id != (uint32_t)vocab) & (end == id) &
+         (far == id) & !((head == id) & (i > 0) & (before == id));
   }
   for (uint64_t heads = __ballot(is); heads; heads &= heads - 1) {
     const int h = __builtin_ctzll(heads);
     const int64_t t0 = (int64_t)blockIdx.x * kJoinTiles + h;
     const uint32_t v = __builtin_amdgcn_readlane(id, h);
-    // the last tile that begins with the id, 64 tiles looked at together; a long
-    // run's first 4096 and 64 apart
+    // the last tile that begins with the id: 64 tiles looked at together, and of a
+    // long run every 64th of 4096, beyond every 4096th
     int64_t last = t0 + 2;
-    const auto reach = [&](int64_t step) {
-      const int64_t t = last + (lane + 1) * step;
-      const int r = __popcll(__ballot(t * TILE < n && pairs[min(n - 1, t * TILE)].id == v));
+    const auto runs_to = [&](int64_t step) {
+      const int64_t i = (last + (lane + 1) * step) * TILE;
+      const uint32_t there = pairs[min(n - 1, i)].id;
+      return (there == v) & (i < n);
+    };
+    const auto reach = [&](bool in, int64_t step) {
+      const int r = __popcll(__ballot(in));
       last += r * step;
       return r;
     };
-    if (reach(1) == 64) {
-      while (reach(4096) == 64) {}
-      reach(64);
-      reach(1);
+    const bool near = runs_to(1), far = runs_to(64);
+    if (__popcll(__ballot(near)) < 64) {
+      reach(near, 1);
+    } else {
+      if (reach(far, 64) == 64) {
+        while (reach(runs_to(4096), 4096) == 64) {}
+        reach(runs_to(64), 64);
+      }
+      reach(runs_to(1), 1);
     }
     const int64_t count = last - t0 + 1, per = (count + kParts - 1) / kParts;
     const int64_t c0 = wave * per, c1 = min(count, c0 + per);
     float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll 4
-    for (int64_t c = c0; c < c1; ++c) {
-      float x[8];
-      Row8<kF32>::unpack(sums.ld(edge + (2 * (t0 + c) + (c == 0 ? 1 : 0)) * d), x);
+    for (int64_t c = c0; c < c1; c += kJoinAhead) {
+      Row8<kF32>::Raw q[kJoinAhead];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] += x[e];
+      for (int i = 0; i < kJoinAhead; ++i) {
+        const int64_t at = min(c + i, c1 - 1);   // past the end: the last one again, not added
+        q[i] = sums.ld(edge + (2 * (t0 + at) + (at == 0 ? 1 : 0)) * d);
+      }
+#pragma unroll
+      for (int i = 0; i < kJoinAhead; ++i) {
+        float x[8];
+        Row8<kF32>::unpack(q[i], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] += c + i < c1 ? x[e] : 0.f;
+      }
     }
     __syncthreads();
 #pragma unroll
