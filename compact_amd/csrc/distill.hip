@@ -425,17 +425,25 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
     // st, s1: the whole row's, about b_t and b_1, u_t and u_1 apart
     sr = st;
     float b_t = c_t, b_1 = c_1, u_t = 1.f, u_1 = 1.f;
+    float q_top = 0.f;   // the student's share of the entries' columns, with a tail
     if (tail) {
       const float et = base_of(teach.m, kt), e1 = POW == 2 ? 2.f * et : base_of(teach.m, k1);
       b_t = fmaxf(c_t, et), b_1 = fmaxf(c_1, e1);
       u_t = exp2_fast(c_t - b_t), u_1 = exp2_fast(c_1 - b_1);
-      st = st * u_t + teach.st * exp2_fast(et - b_t);
+      q_top = teach.st * exp2_fast(et - b_t);
+      st = st * u_t + q_top;
+      q_top *= inverse(st);
       if (POW) s1 = s1 * u_1 + teach.s1 * exp2_fast(e1 - b_1);
     }
     if (!POW) s1 = st, b_1 = b_t, u_1 = u_t;
     if (st == INFINITY) st = s1 = NAN;   // +inf among the logits
     const float rest = sr == 0.f ? 0.f : teach.rest;
     const float mass = teach.mass + rest;   // P
+    // Of a large rest, two shares near 1 (many classes, a high temperature), only the
+    // difference counts, and it is taken between the entries' shares instead:
+    //   log(rest / q_rest) = log(1 + (q_top - p_top) / (1 - q_top))
+    //   P q_rest - rest = p_top - P q_top
+    const bool large_rest = tail && q_top < 0.5f && teach.mass < 0.5f;
     if (wave == 0) {
       const float l_t = __log2f(st), l_1 = __log2f(s1);   // of the row's sums, less b_t and b_1
       float soft = 0.f;
@@ -444,7 +452,9 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
         if (p != 0.f) soft += p * (s_lp[k] - kLn2 * (fmaf(s_z[k] - shift, kt, -b_t) - l_t));
       }
       soft = wave_sum(soft);
-      if (rest > 0.f) soft += rest * kLn2 * (__log2f(rest) - (__log2f(sr) - l_t + (c_t - b_t)));
+      if (rest > 0.f)
+        soft += rest * (large_rest ? log1pf((q_top - teach.mass) / (1.f - q_top))
+                                   : kLn2 * (__log2f(rest) - (__log2f(sr) - l_t + (c_t - b_t))));
       if (lane == 0) {
         float loss = a.alpha * a.tau * a.tau * soft;
         if (hard) loss += (1.f - a.alpha) * kLn2 * (l_1 - fmaf(teach.z_label - shift, k1, -b_1));
@@ -457,7 +467,9 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
       // factors of the exponentials: about the row's base at an entry, the block's elsewhere
       const float f_top = cs * mass * inverse(st), f_top1 = ch * inverse(s1);
       float f_t = f_top * u_t, f_1 = f_top1 * u_1;
-      if (rest > 0.f) f_t -= cs * rest * inverse(sr);
+      if (rest > 0.f)
+        f_t = large_rest ? cs * (teach.mass - mass * q_top) * inverse(sr)
+                         : f_t - cs * rest * inverse(sr);
       if (!POW) f_t += f_1;   // one softmax for both terms (f_1 is 0 without labels' term)
       const auto grad_of = [&](float x) {
         const float et = exp2_fast(fmaf(x, kt, -c_t));

@@ -415,3 +415,42 @@ def test_refusals(device):
             bad()
     with pytest.raises(RuntimeError):
         cpt.distill_topk(z.cpu(), t, i)
+
+
+@pytest.mark.parametrize("k", [1, 19])
+@pytest.mark.parametrize("tau", [1.0, 4.0, 8.0])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_small_shares_keep_their_digits(device, dtype, tau, k):
+    """Entries that hold a small part of both softmaxes: the rest's term and the
+    columns' gradient are differences between shares near 1.  With s = sum (p + q)
+    over the entries' columns, L the largest |log p|, |log q| there, each share is
+    good to (2 L + 200) e of itself, and the loss is of first order in them:
+    |error| <= tau^2 (4 L + 400) e s (L + 1).  A column outside the entries has
+    tau (p_top - P q_top) q / q_rest."""
+    g = torch.Generator().manual_seed(k)
+    n, v = 40, 24001
+    z = torch.randn(n, v, generator=g).to(dtype)
+    t = z.float() * 0.5 + torch.randn(n, v, generator=g)
+    top = 0.2 * t[:, 100:100 + k]   # not the largest: the entries' share stays small
+    idx = torch.arange(100, 100 + k).expand(n, k).contiguous()
+    lse = torch.logsumexp(t.double() / tau, 1).float()
+    lq = torch.log_softmax(z.double() / tau, 1)
+    lp = top.double() / tau - lse.double()[:, None]
+    p, q = lp.exp(), lq[:, 100:100 + k].exp()
+    a, b = p.sum(1), q.sum(1)
+    assert (a < 0.1).all() and (b < 0.1).all()
+    want = tau ** 2 * ((p * (lp - q.log())).sum(1) + (1 - a) * (torch.log1p(-a) - torch.log1p(-b)))
+    big = torch.maximum(lp.abs().amax(1), q.log().abs().amax(1))
+    bound = tau ** 2 * (4 * big + 400) * E * (a + b) * (big + 1)
+    loss, grad = _cpt().distill_topk(z.to(device), top.to(device), idx.to(device),
+                                     top_lse=lse.to(device), temperature=tau, alpha=1.0,
+                                     reduction="none",
+                                     grad_out=torch.full((n,), 2.0 ** 12, device=device))
+    assert ((loss.cpu().double() - want).abs() <= bound).all()
+    out = torch.ones(v, dtype=torch.bool)
+    out[100:100 + k] = False
+    cond = (lq - torch.log1p(-b)[:, None]).exp()[:, out]
+    exact = 2.0 ** 12 * tau * (a - b)[:, None] * cond
+    slack = 2.0 ** 12 * tau * (4 * big + 400 + 200)[:, None] * E * (a + b)[:, None] * cond
+    off = (grad.cpu().double()[:, out] - exact).abs()
+    assert (off <= UNIT[dtype] * exact.abs() + TINY[dtype] + slack).all()
