@@ -23,7 +23,8 @@
 // (maximum, sum of exponentials): one exchange over the block per row.  With a
 // tail the columns outside the entries are summed about their own maximum, so
 // q_rest keeps its digits however small it is; where nothing is left outside (all
-// of it -inf), the p_rest term falls away.
+// of it -inf), the p_rest term falls away.  Where the entries hold little, p_rest
+// and q_rest are both near 1 and what counts is taken from the entries' shares.
 //
 // Measured on one MI355X: 8192 rows of 32000 bf16 columns (15% left out, both
 // terms, tau 2) 226 us, 4.3 TB/s of rows read and gradients written; a large copy
@@ -597,7 +598,7 @@ int launch(const Args& a, hipStream_t st) {
 // several rows are in flight on a CU and few wavefronts wait for each other (8000
 // rows of 8000 bf16 columns: 69 us with 128 threads, 102 with 256 and half the
 // vectors).  Rows past 32768 columns do not fit; a few more registers each then pay
-// (1500 x 50000 fp32 131 us, 139 with 4 vectors; 1531 x 50021 bf16 82, 86 with 8),
+// (1500 x 50000 fp32 131 us, 139 with 4 vectors; 1531 x 50021 bf16 84, 86 with 8),
 // and the rest is read twice.  Without a gradient nothing is kept: one pass.
 template <int DT>
 int launch(const Args& a, hipStream_t st) {
