@@ -408,8 +408,10 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
       }
       turn ^= 1;
       m_row = tail ? fmaxf(m, teach.m) : m;
-      if (shift != 0.f || fabsf(base_of(m_row, kt)) < kFar || fabsf(m_row) == INFINITY) break;
-      // a row of nothing but far values (masked by the type's lowest): move it to 0
+      // a row of nothing but far values (masked by the type's lowest), far at the larger
+      // of the scales: move it to 0
+      const float k_most = POW == 1 ? fmaxf(kt, k1) : kt;
+      if (shift != 0.f || fabsf(base_of(m_row, k_most)) < kFar || fabsf(m_row) == INFINITY) break;
       shift = m_row;
 #pragma unroll
       for (int c = 0; c < NV; ++c) {

@@ -454,3 +454,24 @@ def test_small_shares_keep_their_digits(device, dtype, tau, k):
     slack = 2.0 ** 12 * tau * (4 * big + 400 + 200)[:, None] * E * (a + b)[:, None] * cond
     off = (grad.cpu().double()[:, out] - exact).abs()
     assert (off <= UNIT[dtype] * exact.abs() + TINY[dtype] + slack).all()
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("tau", [0.5, 1.0, 1.5, 2.0, 8.0])
+@pytest.mark.parametrize("value", [-1e9, -2.5e8, 1e9])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_of_far_values(device, dtype, value, tau, tail):
+    """Rows that lie wholly beyond what a base of the exponentials reaches, at the
+    temperature or at temperature 1 alone: all one value, or a few steps apart (so
+    that exact gradients lie below the smallest normal number, 2^-126, too)."""
+    for v in (200, 70001):
+        z, t, idx, y, lse = _inputs(4, v, 6, dtype, device, tau=tau, tail=tail)
+        y[:] = idx[:, 1]
+        z[1] = value
+        z[2] = (value + 64.0 * (torch.arange(v, device=device) % 3)).to(dtype)
+        want = definition(z, t, idx, y, lse, tau, 0.5, -100, "none", 1.0)
+        loss, grad = _cpt().distill_topk(z, t, idx, y, top_lse=lse, temperature=tau, alpha=0.5,
+                                         reduction="none")
+        assert loss.isfinite().all() and grad.isfinite().all()
+        _close(loss, want[0], want[2] + 2.0 ** -23 * want[0].abs(), "loss")
+        _close(grad, want[1], UNIT[dtype] * want[1].abs() + want[3] + 2.0 ** -126, "gradient")
