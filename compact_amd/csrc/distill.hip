@@ -22,9 +22,10 @@
 // written over the general one after a barrier.  Statistics are fp32, kept as
 // (maximum, sum of exponentials): one exchange over the block per row.  With a
 // tail the columns outside the entries are summed about their own maximum, so
-// q_rest keeps its digits however small it is; where nothing is left outside (all
-// of it -inf), the p_rest term falls away.  Where the entries hold little, p_rest
-// and q_rest are both near 1 and what counts is taken from the entries' shares.
+// q_rest keeps its digits however small it is (a finite logit counts however low it
+// lies); where nothing is left outside (all of it -inf), the p_rest term falls away.
+// Where the entries hold little, p_rest and q_rest are both near 1 and what counts is
+// taken from the entries' shares.
 //
 // Measured on one MI355X: 8192 rows of 32000 bf16 columns (15% left out, both
 // terms, tau 2) 226 us, 4.3 TB/s of rows read and gradients written; a large copy
@@ -87,6 +88,11 @@ __device__ __forceinline__ float inverse(float x) {
 
 __device__ __forceinline__ bool live_label(const Args& a, int64_t y) {
   return y != a.ignore && y >= 0 && y < a.vocab;
+}
+
+// A value that all lanes share, in a scalar register.
+__device__ __forceinline__ float uniform(float x) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
 }
 
 // Rows that count, over the whole batch (each block for itself: the labels are
@@ -186,6 +192,9 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
   const bool tail = a.lse != nullptr;
   const bool hard = a.alpha != 1.f;
   const float kt = kLog2e / a.tau, k1 = kLog2e;
+  // well before a base stops, at the temperature or at temperature 1
+  const uint32_t far_from =
+      __float_as_uint(uniform(0.5f * kFar / (POW == 1 ? fmaxf(kt, k1) : kt)));
   for (uint32_t w = tid; w < (v + 31) / 32; w += THREADS) bits[w] = 0;
   if (tid < 2 * kMaxWaves && tid % kMaxWaves >= THREADS / 64) {   // wavefronts there are not
     red_m[tid / kMaxWaves][tid % kMaxWaves] = -INFINITY;
@@ -301,7 +310,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
     }
     // Columns past the registers are read again, kBatch vectors at a time: with a
     // tail without the entries', and -inf past the row's end.
-    float shift = 0.f;
+    float shift = 0.f, below = 0.f;   // taken off the entries and the label; off the columns
     const auto load_batch = [&](uint32_t first, Raw (&r)[kBatch]) {
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) r[i] = vec8(min(first + i * THREADS, vecs - 1));
@@ -315,11 +324,11 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
       if (vec >= vecs) r = R::fill(R::kNegInf);
       R::unpack(r, x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] -= shift;
+      for (int e = 0; e < 8; ++e) x[e] -= below;
     };
 
-    float m, st, s1, c_t, c_1, sr, m_row;
-    for (;;) {
+    float m, st, s1, c_t, c_1, sr;
+    for (bool moved = false;; moved = true) {
       // maximum and sums over the thread's columns
       m = xr;
       st = s1 = 0.f;
@@ -407,32 +416,40 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
         if (POW == 2) s1 = row16_sum(red_1[turn][w] * back * back);
       }
       turn ^= 1;
-      m_row = tail ? fmaxf(m, teach.m) : m;
-      // a row of nothing but far values (masked by the type's lowest), far at the larger
-      // of the scales: move it to 0
-      const float k_most = POW == 1 ? fmaxf(kt, k1) : kt;
-      if (shift != 0.f || fabsf(base_of(m_row, k_most)) < kFar || fabsf(m_row) == INFINITY) break;
-      shift = m_row;
+      // values that are far (masked by the type's lowest) are moved to 0 and summed again:
+      // a row of nothing else, and with a tail what lies outside the entries, each by its
+      // own maximum
+      const auto far = [&](float x) {   // in scalar registers, as all share x
+        const uint32_t size = __float_as_uint(uniform(x)) & 0x7FFFFFFFu;
+        return size - far_from < 0x7F800000u - far_from;   // and finite
+      };
+      if (moved || !(far(m) || (tail && far(fmaxf(m, teach.m))))) break;
+      const float m_row = tail ? fmaxf(m, teach.m) : m;
+      shift = uniform(fabsf(m_row) == INFINITY ? 0.f : m_row);
+      below = uniform(m == -INFINITY ? shift : m);
 #pragma unroll
       for (int c = 0; c < NV; ++c) {
         float x[8];
         R::unpack(q[c], x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] -= shift;
+        for (int e = 0; e < 8; ++e) x[e] -= below;
         q[c] = R::pack(x);
       }
-      xr -= shift;
+      xr -= below;
       __syncthreads();   // `teach` is written again
     }
     // c_t, c_1: the base of the block's sums.  sr: its sum (the rest's, with a tail);
-    // st, s1: the whole row's, about b_t and b_1, u_t and u_1 apart
+    // st, s1: the whole row's, about b_t and b_1, u_t and u_1 apart; `apart` is how far
+    // the columns were moved more than the entries
     sr = st;
     float b_t = c_t, b_1 = c_1, u_t = 1.f, u_1 = 1.f;
+    const float apart = below - shift;
     float q_top = 0.f;   // the student's share of the entries' columns, with a tail
     if (tail) {
       const float et = base_of(teach.m, kt), e1 = POW == 2 ? 2.f * et : base_of(teach.m, k1);
-      b_t = fmaxf(c_t, et), b_1 = fmaxf(c_1, e1);
-      u_t = exp2_fast(c_t - b_t), u_1 = exp2_fast(c_1 - b_1);
+      const float r_t = fmaf(apart, kt, c_t), r_1 = fmaf(apart, k1, c_1);
+      b_t = fmaxf(r_t, et), b_1 = fmaxf(r_1, e1);
+      u_t = exp2_fast(r_t - b_t), u_1 = exp2_fast(r_1 - b_1);
       q_top = teach.st * exp2_fast(et - b_t);
       st = st * u_t + q_top;
       q_top *= inverse(st);
@@ -457,7 +474,8 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
       soft = wave_sum(soft);
       if (rest > 0.f)
         soft += rest * (large_rest ? log1pf((q_top - teach.mass) / (1.f - q_top))
-                                   : kLn2 * (__log2f(rest) - (__log2f(sr) - l_t + (c_t - b_t))));
+                                   : kLn2 * (__log2f(rest) - (__log2f(sr) - l_t + (c_t - b_t))) -
+                                         apart * (kt * kLn2));
       if (lane == 0) {
         float loss = a.alpha * a.tau * a.tau * soft;
         if (hard) loss += (1.f - a.alpha) * kLn2 * (l_1 - fmaf(teach.z_label - shift, k1, -b_1));
@@ -522,7 +540,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
           Elem<DT>::st((T*)g + id, top_of(s_z[k] - shift) - cs * p - (id == label ? ch : 0.f));
         }
         if (hard && lane == 0 && !(bits[label >> 5] >> (label & 31) & 1))
-          Elem<DT>::st((T*)g + label, grad_of(teach.z_label - shift) - ch);
+          Elem<DT>::st((T*)g + label, grad_of(teach.z_label - below) - ch);
       }
     }
     if (wave == 0) {

@@ -475,3 +475,52 @@ def test_rows_of_far_values(device, dtype, value, tau, tail):
         assert loss.isfinite().all() and grad.isfinite().all()
         _close(loss, want[0], want[2] + 2.0 ** -23 * want[0].abs(), "loss")
         _close(grad, want[1], UNIT[dtype] * want[1].abs() + want[3] + 2.0 ** -126, "gradient")
+
+
+@pytest.mark.parametrize("tau", [1.0, 1.5, 2.0])
+@pytest.mark.parametrize("value", [-1e9, -2.5e8, "lowest"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_far_values_outside_the_entries(device, dtype, value, tau):
+    """With a tail, finite logits far below the entries count as the formula has them
+    (q_rest about exp(value / tau)); only -inf leaves nothing.  Bounds as above, with
+    the range of the entries and of the rest each by itself: 150 at most; a gradient
+    may lie below the smallest normal number."""
+    value = torch.finfo(dtype).min if value == "lowest" else value
+    n, k, alpha = 4, 6, 0.5
+    for v in (200, 70001):
+        z, t, idx, y, lse = _inputs(n, v, k, dtype, device, tau=tau, tail=True)
+        lse += 0.5
+        y[:] = idx[:, 1]
+        at = z.gather(1, idx)
+        z[1:3] = value
+        if value > -1e30:
+            z[2] = (value + 64.0 * (torch.arange(v, device=device) % 3)).to(dtype)
+        z[1:3] = z[1:3].scatter(1, idx[1:3], at[1:3])
+        z[3] -= 5e8 if dtype == torch.float32 else 0   # the whole row, entries and rest
+        z64, lp = z.double(), t.double() / tau - lse.double()[:, None]
+        lq = torch.log_softmax(z64 / tau, 1)
+        p, lqj = lp.exp(), lq.gather(1, idx)
+        top = torch.zeros_like(z64).scatter_(1, idx, 1.0) > 0
+        lo = torch.logsumexp(lq.masked_fill(top, -math.inf), 1)
+        rest = 1 - p.sum(1)
+        assert (rest > 0.1).all()
+        soft = (p * (lp - lqj)).sum(1) + rest * (rest.log() - lo)
+        size = (p * (lp.abs() + lqj.abs() + 1)).sum(1) + rest * (rest.log().abs() + lo.abs() + 1)
+        l1 = torch.log_softmax(z64, 1)
+        hard = -l1.gather(1, y[:, None])[:, 0]
+        loss, grad = _cpt().distill_topk(z, t, idx, y, top_lse=lse, temperature=tau, alpha=alpha,
+                                         reduction="none")
+        off = (12 * (lse.double().abs() + lp.abs().amax(1)) + 8 + k) * E
+        want = alpha * tau ** 2 * soft + (1 - alpha) * hard
+        bound = 2.0 ** -23 * want.abs() + (1 - alpha) * 550 * E * (hard + 1) \
+            + alpha * tau ** 2 * (550 * E * size + off * (lo.abs() + rest.log().abs() + 2))
+        _close(loss, want, bound, "loss")
+        # 64 bits do not hold log(v) beside the lowest value: not exp(lq - lo)
+        cond = torch.softmax((z64 / tau).masked_fill(top, -math.inf), 1)
+        dense = torch.zeros_like(z64).scatter_(1, idx, p)
+        hot = torch.zeros_like(z64).scatter_(1, y[:, None], 1.0)
+        exact = alpha * tau * (lq.exp() - dense - rest[:, None] * cond) \
+            + (1 - alpha) * (l1.exp() - hot)
+        terms = tau * (lq.exp() + dense + rest[:, None] * cond) + l1.exp() + hot
+        _close(grad, exact, UNIT[dtype] * exact.abs() + 550 * E * terms
+               + tau * off[:, None] * (dense + cond + lq.exp()) + 2.0 ** -126, "gradient")
