@@ -260,7 +260,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
       for (int k = lane; k < a.k; k += 64) {
         if (k >= 64) first = load_entry(k);
         const int e_id = first.id(v, a.idx_wide);
-        const float t = e_id >= 0 ? first.logit(a.top_dtype) / a.tau : -INFINITY;
+        const float t = e_id >= 0 ? first.logit(a.top_dtype) : -INFINITY;
         s_idx[k] = e_id;
         s_z[k] = e_id >= 0 ? elem(e_id) : 0.f;
         s_lp[k] = t;
@@ -269,19 +269,22 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
           again |= atomicOr(&bits[e_id >> 5], 1u << (e_id & 31)) >> (e_id & 31) & 1;
       }
       again = __ballot(again) != 0;
-      float base, sum = 0.f;
+      // log p = (t - base) / tau - ls: the difference of two logits rounded once, so that
+      // log p is good about 0 however large the logits are
+      float base, ls = 0.f, sum = 0.f;
       if (tail) {
-        base = a.lse[row];
+        base = a.lse[row];   // at the temperature
       } else {
         m = wave_max(m);
         m = m == -INFINITY ? 0.f : m;
-        for (int k = lane; k < a.k; k += 64) sum += exp2_fast((s_lp[k] - m) * kLog2e);
+        for (int k = lane; k < a.k; k += 64) sum += exp2_fast((s_lp[k] - m) * kt);
         sum = wave_sum(sum);
-        base = m + __log2f(sum) * kLn2;
+        base = m, ls = __log2f(sum) * kLn2;
       }
       float mass = 0.f;
       for (int k = lane; k < a.k; k += 64) {
-        const float lp = s_lp[k] - base;
+        const float t = s_lp[k];
+        const float lp = (tail ? fmaf(-base, a.tau, t) : t - base) / a.tau - ls;
         const float p = s_idx[k] < 0 || (!tail && sum == 0.f) ? 0.f : exp2_fast(lp * kLog2e);
         s_lp[k] = lp;
         s_p[k] = p;

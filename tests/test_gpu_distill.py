@@ -524,3 +524,36 @@ def test_far_values_outside_the_entries(device, dtype, value, tau):
         terms = tau * (lq.exp() + dense + rest[:, None] * cond) + l1.exp() + hot
         _close(grad, exact, UNIT[dtype] * exact.abs() + 550 * E * terms
                + tau * off[:, None] * (dense + cond + lq.exp()) + 2.0 ** -126, "gradient")
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("tau", [1.0, 3.0])
+def test_large_teacher_logits(device, tau, tail):
+    """Teacher logits about 32768 (a unit in the last place is 2^-8): log p is rounded
+    about 0, not about them.  A difference of two of them is exact or rounded once, so
+    log p has an error of (4 |log p| + 8) e; with R the rows' ranges of teacher and
+    student and sums of fewer than 60 roundings, the loss has
+    tau^2 (4 R + 100) e * its terms, and p_rest = 1 - sum p an error of (4 R + 100) e."""
+    g = torch.Generator().manual_seed(11)
+    n, v, k = 20, 1000, 40
+    z = 2 * torch.randn(n, v, generator=g)
+    t = 32768 - torch.randint(0, 2000, (n, k), generator=g) / 256.0
+    idx = torch.argsort(torch.rand(n, v, generator=g), 1)[:, :k].contiguous()
+    t64, lq = t.double() / tau, torch.log_softmax(z.double() / tau, 1)
+    base = torch.logsumexp(t64, 1)
+    lse = (base + 0.25).float() if tail else None
+    lp = t64 - (lse.double() if tail else base)[:, None]
+    p, lqj = lp.exp(), lq.gather(1, idx)
+    soft, size = (p * (lp - lqj)).sum(1), (p * (lp.abs() + lqj.abs() + 1)).sum(1)
+    err = (4 * (1 + (z.amax(1) - z.amin(1)).double() + 8) + 100) * E
+    bound = err * size
+    if tail:
+        rest = 1 - p.sum(1)
+        lo = torch.logsumexp(lq.scatter(1, idx, -math.inf), 1)
+        soft = soft + rest * (rest.log() - lo)
+        bound = bound + err * (rest.log().abs() + lo.abs() + 2)
+    loss, _ = _cpt().distill_topk(z.to(device), t.to(device), idx.to(device),
+                                  top_lse=lse.to(device) if tail else None, temperature=tau,
+                                  reduction="none", want_grad=False)
+    _close(loss.cpu(), tau ** 2 * soft, tau ** 2 * bound + 2.0 ** -23 * tau ** 2 * soft.abs(),
+           "loss")
