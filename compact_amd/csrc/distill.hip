@@ -336,11 +336,20 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
       m = xr;
       st = s1 = 0.f;
       float ct = 0.f, c1 = 0.f;
-      const auto add = [&](float x) {
+      const auto add = [&](float x, float& to_t, float& to_1) {
         const float et = exp2_fast(fmaf(x, kt, -ct));
-        st += et;
-        if (POW == 1) s1 += exp2_fast(fmaf(x, k1, -c1));
-        if (POW == 2) s1 = fmaf(et, et, s1);
+        to_t += et;
+        if (POW == 1) to_1 += exp2_fast(fmaf(x, k1, -c1));
+        if (POW == 2) to_1 = fmaf(et, et, to_1);
+      };
+      // a vector's eight first by themselves: the chain of the widest row (65536 vectors)
+      // has 137 terms, not 1024
+      const auto add_vec = [&](const float x[8]) {
+        float vt = 0.f, v1 = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) add(x[e], vt, v1);
+        st += vt;
+        if (POW) s1 += v1;
       };
 #pragma unroll
       for (int c = 0; c < NV; ++c) {
@@ -355,8 +364,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
       for (int c = 0; c < NV; ++c) {
         float x[8];
         R::unpack(q[c], x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) add(x[e]);
+        add_vec(x);
         repack<DT>(q[c]);
       }
       for (uint32_t first = NV * THREADS + tid; first < vecs; first += kBatch * THREADS) {
@@ -375,11 +383,10 @@ __global__ __launch_bounds__(THREADS, WAVES) void distill_kernel(Args a) {
             if (POW == 2) s1 *= exp2_fast(2.f * (ct - nt));
             m = mc, ct = nt, c1 = n1;
           }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) add(x[e]);
+          add_vec(x);
         }
       }
-      add(xr);
+      add(xr, st, s1);
       // over the wavefront, then the block: sums are brought to the common base
       const float mw = wave_max(m), back = exp2_fast(ct - base_of(mw, kt));
       st = wave_sum(st * back);

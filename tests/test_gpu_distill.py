@@ -557,3 +557,17 @@ def test_large_teacher_logits(device, tau, tail):
                                   reduction="none", want_grad=False)
     _close(loss.cpu(), tau ** 2 * soft, tau ** 2 * bound + 2.0 ** -23 * tau ** 2 * soft.abs(),
            "loss")
+
+
+def test_sum_over_the_widest_row(device):
+    """A sum of equal exponentials 1 + 2^-15 - 2^-20, which a chain of 1024 of them
+    rounds down by half a unit at every other step.  With chains of at most 150 terms,
+    the block's exchange (16) and the logarithm's and products' roundings (60 at this
+    size), log sum exp - z = log v is off by 230 e at most."""
+    v = 524288
+    value = math.log(1 + 2.0 ** -15 - 2.0 ** -20)
+    z = torch.full((3, v), value, device=device)
+    t, idx = torch.zeros(3, 1, device=device), torch.zeros(3, 1, dtype=torch.int64, device=device)
+    y = torch.arange(3, device=device)
+    loss, _ = _cpt().distill_topk(z, t, idx, y, alpha=0.0, reduction="none", want_grad=False)
+    assert ((loss.double() - math.log(v)).abs() <= 230 * E).all()
