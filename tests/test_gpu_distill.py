@@ -571,3 +571,24 @@ def test_sum_over_the_widest_row(device):
     y = torch.arange(3, device=device)
     loss, _ = _cpt().distill_topk(z, t, idx, y, alpha=0.0, reduction="none", want_grad=False)
     assert ((loss.double() - math.log(v)).abs() <= 230 * E).all()
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("tau", [1.0, 1.5, 2.0])
+@pytest.mark.parametrize("n,v,dtype", [(7000, 515, torch.bfloat16), (7000, 515, torch.float32),
+                                       (2200, 8209, torch.float16), (1100, 8209, torch.float32),
+                                       (600, 33001, torch.float32)])
+def test_many_rows_a_block(device, n, v, dtype, tau, tail):
+    """More rows than blocks: each goes over several, ignored ones between them, with
+    entries that occur twice or not at all."""
+    z, t, idx, y, lse = _inputs(n, v, 9, dtype, device, tau=tau, tail=tail)
+    idx[::5, 1] = idx[::5, 0]
+    idx[3::7, 2] = -1
+    if tail:
+        lse += 0.5
+    gout = 4096.0 if dtype == torch.float16 else 1.0
+    loss, grad = check(z, t, idx, y, lse, tau, 0.5, reduction="none", gout=gout)
+    only, _ = _cpt().distill_topk(z, t, idx, y, top_lse=lse, temperature=tau, alpha=0.5,
+                                  reduction="none", want_grad=False)
+    want = definition(z, t, idx, y, lse, tau, 0.5, -100, "none", 1.0)
+    _close(only, want[0], want[2] + 2.0 ** -23 * want[0].abs(), "loss alone")
