@@ -402,18 +402,18 @@ __global__ __launch_bounds__(kMaxThreads) void backward_kernel(
 
 constexpr int kFinCols = 64, kFinSlices = 16;
 
-// grid (columns / 64, 2 + sequences with a gate of their own): the chunks'
-// sums of 64 columns, sixteen slices of them added side by side and then in
-// order.  y = 0: dw_pre; y = 1: dw_post, and dg of a channel gate from the same
-// sum; y = 2 + b: dg of sequence b.
+// grid (columns / 64, results from `base`, 0 or 2): the chunks' sums of 64 columns,
+// sixteen slices of them added side by side and then in order.  Result 0: dw_pre; 1:
+// dw_post, and dg of a channel gate from the same sum; 2 + b: dg of sequence b, where
+// it has a gate of its own.
 __global__ __launch_bounds__(kFinCols* kFinSlices) void finish_kernel(
-    Shape s, const float* __restrict__ partial, int64_t chunks, int64_t seqs,
+    Shape s, int base, const float* __restrict__ partial, int64_t chunks, int64_t seqs,
     const void* __restrict__ w_post, const void* __restrict__ gate, void* d_w_pre, void* d_w_post,
     void* d_gate) {
   __shared__ float part[kFinSlices][kFinCols];
   const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
   const int64_t j = (int64_t)blockIdx.x * kFinCols + lane;
-  const int what = blockIdx.y;
+  const int what = base + blockIdx.y;
   const bool in = j < s.d;
   const int64_t first = what >= 2 ? (what - 2) * chunks : 0;
   const int64_t n = what >= 2 ? chunks : chunks * seqs;
@@ -454,6 +454,13 @@ __global__ __launch_bounds__(kFinCols* kFinSlices) void finish_kernel(
 inline int launched() { return hipGetLastError() == hipSuccess ? kOk : kErrLaunch; }
 
 constexpr int64_t kMaxD = 8 * kMaxThreads * 2;
+
+// Of a grid's second extent (16 bits wide): more sequences take further launches.
+constexpr int64_t kMaxExtent = 65535;
+unsigned extent(int64_t n) { return (unsigned)(n < kMaxExtent ? n : kMaxExtent); }
+void* from(const void* p, int64_t element, int type) {
+  return p ? (char*)p + element * (type == kF32 ? 4 : 2) : nullptr;
+}
 
 // Vectors per thread, and the threads and row groups of a block of about `threads`.
 // Rows of up to 256 columns share a wavefront, so that its lanes all have columns
@@ -561,7 +568,6 @@ int cpt_residual_norm_backward(int dtype, int weight_dtype, const void* d_residu
   if (!y && (w_post || gate || residual_scale != 1.f)) return kErrShape;
   if (!y && !d_x) return kErrShape;
   const int64_t seqs = rows == 0 ? 0 : rows / seq;
-  if (seqs > 65533) return kErrTooLarge;   // a grid's second extent
   if (rows > 0 && (!stats || !d_residual || !workspace || (d_x && !residual_out) || ld_dro < 0 ||
                    ld_dx < 0 || ld_ro < 0 || ld_y < 0))
     return kErrShape;
@@ -571,24 +577,37 @@ int cpt_residual_norm_backward(int dtype, int weight_dtype, const void* d_residu
   const hipStream_t st = (hipStream_t)stream;
   if (rows > 0) {
     const int threads = s.tr * s.groups;
-    const dim3 grid((unsigned)chunks, (unsigned)seqs);
     const size_t lds = 4 * (size_t)(nv > 1 ? 2 * nv * s.tr * 8 : s.groups > 1 ? s.groups * ((d + 7) / 8 * 8) : 0);
+    for (int64_t seq0 = 0; seq0 < seqs; seq0 += kMaxExtent) {   // tensors from sequence seq0 on
+      const int64_t row0 = seq0 * seq;
+      const dim3 grid((unsigned)chunks, extent(seqs - seq0));
 #define CPT_BWD(DT, NV, TINY)                                                                    \
-  backward_kernel<DT, NV, TINY><<<grid, threads, lds, st>>>(                                           \
-      s, d_residual_out, ld_dro, d_x, ld_dx, residual_out, ld_ro, y, ld_y, (const float*)stats,  \
-      w_post, w_pre, gate, d_residual, d_y, d_gate, (float*)workspace)
+  backward_kernel<DT, NV, TINY><<<grid, threads, lds, st>>>(                                     \
+      s, from(d_residual_out, row0 * ld_dro, dtype), ld_dro, from(d_x, row0 * ld_dx, dtype),     \
+      ld_dx, from(residual_out, row0 * ld_ro, dtype), ld_ro, from(y, row0 * ld_y, dtype), ld_y,  \
+      (const float*)stats + row0, w_post, w_pre, from(gate, seq0 * d, weight_dtype),             \
+      from(d_residual, row0 * d, dtype), from(d_y, row0 * d, dtype), d_gate,                     \
+      (float*)workspace + seq0 * chunks * 2 * d)
 #define CPT_BWD_NV(DT) \
   (d < 8 ? CPT_BWD(DT, 1, true) : nv == 1 ? CPT_BWD(DT, 1, false) : CPT_BWD(DT, 2, false))
-    dtype == kF32 ? CPT_BWD_NV(kF32) : dtype == kF16 ? CPT_BWD_NV(kF16) : CPT_BWD_NV(kBF16);
-    const int rc = launched();
-    if (rc != kOk) return rc;
+      dtype == kF32 ? CPT_BWD_NV(kF32) : dtype == kF16 ? CPT_BWD_NV(kF16) : CPT_BWD_NV(kBF16);
+      const int rc = launched();
+      if (rc != kOk) return rc;
+    }
   }
   if (d_w_pre || d_w_post || gate_kind == kChannel || gate_kind == kSequence) {
-    const dim3 grid((unsigned)((d + kFinCols - 1) / kFinCols),
-                    (unsigned)(gate_kind == kSequence ? 2 + seqs : 2));
-    finish_kernel<<<grid, kFinCols * kFinSlices, 0, st>>>(s, (const float*)workspace, chunks, seqs,
-                                                          w_post, gate, d_w_pre, d_w_post, d_gate);
-    return launched();
+    const auto finish = [&](int base, int64_t seq0, unsigned results) {
+      const dim3 grid((unsigned)((d + kFinCols - 1) / kFinCols), results);
+      finish_kernel<<<grid, kFinCols * kFinSlices, 0, st>>>(
+          s, base, (const float*)workspace + seq0 * chunks * 2 * d, chunks, seqs, w_post, gate,
+          d_w_pre, d_w_post, from(d_gate, seq0 * d, weight_dtype));
+      return launched();
+    };
+    const int64_t gated = gate_kind == kSequence ? seqs : 0;
+    int rc = finish(0, 0, extent(2 + gated));
+    for (int64_t seq0 = kMaxExtent - 2; rc == kOk && seq0 < gated; seq0 += kMaxExtent)
+      rc = finish(2, seq0, extent(gated - seq0));
+    return rc;
   }
   return kOk;
 }

@@ -370,3 +370,15 @@ def test_narrow_rows(device, dtype, gate, shape):
     back = cpt.residual_norm_backward(dro, dx, ro, y, stats, w_pre, w_post=w_post, gate=g,
                                       scale=0.7, residual_scale=1.25)
     check_backward(back, dro, dx, ro, y, stats, w_pre, w_post, g, 0.7, 1.25)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(66000, 1, 8), (65540, 2, 40), (131080, 1, 5)])
+def test_many_sequences_with_a_gate_each(device, dtype, shape):
+    """More sequences than a grid's second extent."""
+    cpt = _cpt()
+    res, y, dro, dx, w_pre, w_post, g = _inputs(shape, dtype, dtype, "sequence", True, device)
+    out = cpt.residual_norm(res, y, w_pre, w_post=w_post, gate=g, eps=EPS)
+    check_forward(out, res, y, w_pre, w_post, g, 1.0, 1.0, EPS)
+    grads = cpt.residual_norm_backward(dro, dx, out[0], y, out[2], w_pre, w_post=w_post, gate=g)
+    check_backward(grads, dro, dx, out[0], y, out[2], w_pre, w_post, g, 1.0, 1.0)
