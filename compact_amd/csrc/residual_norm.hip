@@ -400,6 +400,13 @@ __global__ __launch_bounds__(kMaxThreads) void backward_kernel(
   }
 }
 
+template <int DT>
+auto backward_of(int64_t d, int nv) {
+  return d < 8     ? backward_kernel<DT, 1, true>
+         : nv == 1 ? backward_kernel<DT, 1, false>
+                   : backward_kernel<DT, 2, false>;
+}
+
 constexpr int kFinCols = 64, kFinSlices = 16;
 
 // grid (columns / 64, results from `base`, 0 or 2): the chunks' sums of 64 columns,
@@ -577,20 +584,27 @@ int cpt_residual_norm_backward(int dtype, int weight_dtype, const void* d_residu
   const hipStream_t st = (hipStream_t)stream;
   if (rows > 0) {
     const int threads = s.tr * s.groups;
-    const size_t lds = 4 * (size_t)(nv > 1 ? 2 * nv * s.tr * 8 : s.groups > 1 ? s.groups * ((d + 7) / 8 * 8) : 0);
+    const auto kern = dtype == kF32   ? backward_of<kF32>(d, nv)
+                      : dtype == kF16 ? backward_of<kF16>(d, nv)
+                                      : backward_of<kBF16>(d, nv);
+    // the sums over tokens of rows with two vectors a thread; the groups' of others
+    const int64_t floats = nv > 1         ? 2 * nv * s.tr * 8
+                           : s.groups > 1 ? s.groups * ((d + 7) / 8 * 8)
+                                          : 0;
+    const size_t lds = 4 * (size_t)floats;
+    if (lds > 62 * 1024 &&
+        hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
+                            (int)lds) != hipSuccess)
+      return kErrLaunch;
     for (int64_t seq0 = 0; seq0 < seqs; seq0 += kMaxExtent) {   // tensors from sequence seq0 on
       const int64_t row0 = seq0 * seq;
       const dim3 grid((unsigned)chunks, extent(seqs - seq0));
-#define CPT_BWD(DT, NV, TINY)                                                                    \
-  backward_kernel<DT, NV, TINY><<<grid, threads, lds, st>>>(                                     \
-      s, from(d_residual_out, row0 * ld_dro, dtype), ld_dro, from(d_x, row0 * ld_dx, dtype),     \
-      ld_dx, from(residual_out, row0 * ld_ro, dtype), ld_ro, from(y, row0 * ld_y, dtype), ld_y,  \
-      (const float*)stats + row0, w_post, w_pre, from(gate, seq0 * d, weight_dtype),             \
-      from(d_residual, row0 * d, dtype), from(d_y, row0 * d, dtype), d_gate,                     \
-      (float*)workspace + seq0 * chunks * 2 * d)
-#define CPT_BWD_NV(DT) \
-  (d < 8 ? CPT_BWD(DT, 1, true) : nv == 1 ? CPT_BWD(DT, 1, false) : CPT_BWD(DT, 2, false))
-      dtype == kF32 ? CPT_BWD_NV(kF32) : dtype == kF16 ? CPT_BWD_NV(kF16) : CPT_BWD_NV(kBF16);
+      kern<<<grid, threads, lds, st>>>(
+          s, from(d_residual_out, row0 * ld_dro, dtype), ld_dro, from(d_x, row0 * ld_dx, dtype),
+          ld_dx, from(residual_out, row0 * ld_ro, dtype), ld_ro, from(y, row0 * ld_y, dtype), ld_y,
+          (const float*)stats + row0, w_post, w_pre, from(gate, seq0 * d, weight_dtype),
+          from(d_residual, row0 * d, dtype), from(d_y, row0 * d, dtype), d_gate,
+          (float*)workspace + seq0 * chunks * 2 * d);
       const int rc = launched();
       if (rc != kOk) return rc;
     }
