@@ -222,7 +222,7 @@ def test_zero_rows_and_large_values(device):
 
 
 @pytest.mark.parametrize("gate", ["none", "channel", "sequence", "token"])
-def test_narrow_rows(device, gate):
+def test_rows_of_less_than_a_vector(device, gate):
     """Fewer columns than a vector."""
     cpt = _cpt()
     for shape in ((3, 4, 5), (2, 700, 7), (1, 9, 2)):
