@@ -382,3 +382,25 @@ def test_many_sequences_with_a_gate_each(device, dtype, shape):
     check_forward(out, res, y, w_pre, w_post, g, 1.0, 1.0, EPS)
     grads = cpt.residual_norm_backward(dro, dx, out[0], y, out[2], w_pre, w_post=w_post, gate=g)
     check_backward(grads, dro, dx, out[0], y, out[2], w_pre, w_post, g, 1.0, 1.0)
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "sequence", "token"])
+@pytest.mark.parametrize("shape,dtype", [((2, 2500, 2048), torch.bfloat16),
+                                         ((6, 700, 2048), torch.float16),
+                                         ((2, 600, 4097), torch.float32),
+                                         ((2, 600, 4097), torch.bfloat16),
+                                         ((1, 900, 8200), torch.float16),
+                                         ((2, 300, 16384), torch.float32),
+                                         ((2, 400, 16383), torch.bfloat16),
+                                         ((2, 20000, 5), torch.float32)])
+def test_many_rows_a_block(device, shape, dtype, gate):
+    """More rows than blocks: each goes over several, in both directions."""
+    cpt = _cpt()
+    res, y, dro, dx, w_pre, w_post, g = _inputs(shape, dtype, dtype, gate, True, device, seed=5)
+    out = cpt.residual_norm(res, y, w_pre, w_post=w_post, gate=g, scale=0.7, residual_scale=1.25,
+                            eps=EPS)
+    check_forward(out, res, y, w_pre, w_post, g, 0.7, 1.25, EPS)
+    ro, _, stats = out
+    back = cpt.residual_norm_backward(dro, dx, ro, y, stats, w_pre, w_post=w_post, gate=g,
+                                      scale=0.7, residual_scale=1.25)
+    check_backward(back, dro, dx, ro, y, stats, w_pre, w_post, g, 0.7, 1.25)
