@@ -244,3 +244,23 @@ def test_refusals(device):
             bad()
     with pytest.raises(RuntimeError):
         cpt.embedding(ids.cpu(), w)
+
+
+@pytest.mark.parametrize("d", [5, 100, 515])
+@pytest.mark.parametrize("kind", ["uniform", "one", "skewed", "outside"])
+@pytest.mark.parametrize("n,v", [(9000, 500), (20011, 37), (40000, 3000), (100352, 32000)])
+def test_gradient_of_whole_numbers(device, n, v, kind, d):
+    """Sums of small whole numbers are exact in fp32 in any order: equal, so that no
+    tile of a long run is lost, added twice or put to another id."""
+    cpt = _cpt()
+    g = torch.Generator().manual_seed(n + d)
+    ids = _ids(kind, n, v, g).to(device)
+    grad = torch.randint(-8, 9, (n, d), generator=g).to(device)
+    ok = (ids >= 0) & (ids < v) & (ids != 1)
+    want = torch.zeros(v, d, dtype=torch.float64, device=device)
+    want.index_add_(0, ids[ok], grad[ok].double())
+    got = cpt.embedding_backward(grad.float(), ids, v, padding_idx=1)
+    assert torch.equal(got.double(), want)
+    base = torch.randint(-50, 50, (v, d), generator=g).float().to(device)
+    got = cpt.embedding_backward(grad.bfloat16(), ids, v, padding_idx=1, out=base.clone())
+    assert torch.equal(got.double(), want + base.double())
