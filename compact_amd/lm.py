@@ -62,6 +62,29 @@ def _rows(t, d):
     return t, t.stride(0)
 
 
+class _Once(torch.autograd.Function):
+    """The first `n` of the tensors as they are: gradients, as a function of them all
+    that cannot be differentiated."""
+
+    @staticmethod
+    def forward(ctx, what, n, *tensors):
+        ctx.what = what
+        return tuple(None if t is None else t.view_as(t) for t in tensors[:n])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.what} is differentiable once: its gradient has no gradient")
+
+
+def _differentiable_once(what, grads, *inputs):
+    """What a Function's backward returns: the gradients that a kernel computed from
+    `inputs`.  Under create_graph they are tied to the inputs, so that a second
+    derivative through them is an error and no term of it is left out."""
+    if not torch.is_grad_enabled():
+        return grads
+    return _Once.apply(what, len(grads), *grads, *inputs)
+
+
 # ---------------------------------------------------------------------------
 # embedding
 # ---------------------------------------------------------------------------
@@ -125,7 +148,8 @@ def embedding_backward(grad: torch.Tensor, ids: torch.Tensor, num_embeddings: in
 
 
 class EmbeddingFunction(torch.autograd.Function):
-    """scale * weight[ids] with the table's gradient by sorted tokens."""
+    """scale * weight[ids] with the table's gradient by sorted tokens; differentiable
+    once."""
 
     @staticmethod
     def forward(ctx, ids, weight, scale=1.0, padding_idx=None):
@@ -140,6 +164,7 @@ class EmbeddingFunction(torch.autograd.Function):
         dw = None
         if ctx.needs_input_grad[1]:
             dw = embedding_backward(grad, ids, v, scale, padding_idx=padding_idx)
+            dw, = _differentiable_once("EmbeddingFunction", (dw,), grad)
         return None, dw, None, None
 
 
@@ -295,7 +320,7 @@ def residual_norm_backward(d_residual_out, d_x, residual_out, y, stats, w_pre=No
 class ResidualNormFunction(torch.autograd.Function):
     """residual_norm as an autograd Function: (residual_out, x) of (residual, y,
     ...), or with y None (residual, x); x is None without w_pre.  Saves
-    residual_out, y and two fp32 values a token."""
+    residual_out, y and two fp32 values a token.  Differentiable once."""
 
     @staticmethod
     def forward(ctx, residual, y, w_pre, w_post=None, gate=None, scale=1.0, residual_scale=1.0,
@@ -317,10 +342,10 @@ class ResidualNormFunction(torch.autograd.Function):
             if y is None:
                 return d_out, None, torch.zeros_like(w_pre), None, None, None, None, None
             d_x = torch.zeros_like(out)
-        dr, dy, dwp, dwq, dg = residual_norm_backward(
-            d_out, d_x, out, y, stats, w_pre, w_post=w_post, gate=gate, scale=scale,
-            residual_scale=residual_scale)
-        return dr, dy, dwp, dwq, dg, None, None, None
+        grads = residual_norm_backward(d_out, d_x, out, y, stats, w_pre, w_post=w_post, gate=gate,
+                                       scale=scale, residual_scale=residual_scale)
+        return *_differentiable_once("ResidualNormFunction", grads, d_out, d_x, out, y, w_pre,
+                                     w_post, gate), None, None, None
 
 
 class ResidualNorm(nn.Module):
@@ -461,7 +486,8 @@ class DistillTopKFunction(torch.autograd.Function):
     the loss's incoming gradient, which touches nothing where that is 1; another
     factor than a power of two rounds a second time.  float16: a mean's gradient
     underflows before a loss scale reaches it, so the backward computes it from
-    the logits with the incoming gradient.  One backward per forward."""
+    the logits with the incoming gradient.  One backward per forward; differentiable
+    once, so create_graph is refused."""
 
     @staticmethod
     def forward(ctx, logits, top_logits, top_indices, labels=None, top_lse=None, temperature=1.0,
@@ -483,6 +509,8 @@ class DistillTopKFunction(torch.autograd.Function):
     def backward(ctx, grad_out):
         if ctx.done:
             raise RuntimeError("DistillTopKFunction: one backward per forward")
+        if torch.is_grad_enabled():     # the logits may be gone: nothing to tie it to
+            raise RuntimeError("DistillTopKFunction is differentiable once: no create_graph")
         ctx.done = True
         grad_out = grad_out.float().contiguous()
         if ctx.grad is None:

@@ -159,3 +159,39 @@ def test_no_work_is_no_launch(c_abi):
     assert L.cpt_residual_norm(2, 2, None, 8, None, 8, None, 4096, None, 0, 0, 0, 8, 1.0, 1.0, 0.0,
                                None, 4096, None, None) == _lib.OK
     assert L.cpt_scale_rows(2, None, 0, 50, None, 0, None) == _lib.OK
+
+
+def test_second_derivatives_are_refused(library):
+    """Under create_graph a gradient knows what it came from, and what would need its
+    own gradient is an error, not a term left out; first derivatives are as ever."""
+    ids = torch.tensor([1, 0, 1])
+    table = torch.randn(4, 8, requires_grad=True)
+    square = lambda t: (t * t).sum()
+    out = lm.EmbeddingFunction.apply(ids, table, 2.0)
+    grad, = torch.autograd.grad(square(out), table, create_graph=True)
+    assert grad.requires_grad
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        square(grad).backward()
+    # a gradient that does not depend on the table has none
+    grad, = torch.autograd.grad(lm.EmbeddingFunction.apply(ids, table).sum(), table,
+                                create_graph=True)
+    assert not grad.requires_grad
+
+    w, r, y = (torch.randn(s, requires_grad=True) for s in ((8,), (3, 8), (3, 8)))
+    for args in ((r, None, w), (r, y, w), (r, y, w, w, w), (r, y, None, w)):
+        ro, x = lm.ResidualNormFunction.apply(*args)
+        grads = torch.autograd.grad((ro if x is None else x).sum(), [r, w],
+                                    create_graph=True)
+        assert grads[1].requires_grad
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            square(grads[1]).backward()
+        ro, x = lm.ResidualNormFunction.apply(*args)
+        ((ro if x is None else x).sum()).backward()
+        assert library.calls[-1][0] == "cpt_residual_norm_backward"
+
+    z = torch.randn(3, 9, requires_grad=True)
+    t, i = torch.zeros(3, 2), torch.zeros(3, 2, dtype=torch.int64)
+    for dtype in (torch.float32, torch.float16):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(lm.distill_loss(z.to(dtype), t, i), z, create_graph=True)
+        lm.distill_loss(z.to(dtype), t, i).backward()
