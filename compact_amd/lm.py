@@ -447,7 +447,7 @@ def distill_topk(logits, top_logits, top_indices, labels=None, *, top_lse=None,
         gld_b, gld_s = seq * v, v
     scale, gout = 1.0, None
     if isinstance(grad_out, torch.Tensor):
-        _require_device(grad_out)
+        _on_device(logits, grad_out)
         assert grad_out.dtype == torch.float32 and grad_out.numel() == \
             (rows if reduction == "none" else 1), \
             f"grad_out: float32 of the loss's shape expected, got {tuple(grad_out.shape)}"

@@ -195,3 +195,13 @@ def test_second_derivatives_are_refused(library):
         with pytest.raises(RuntimeError, match="differentiable once"):
             torch.autograd.grad(lm.distill_loss(z.to(dtype), t, i), z, create_graph=True)
         lm.distill_loss(z.to(dtype), t, i).backward()
+
+
+def test_grad_out_lies_with_the_logits(library, monkeypatch):
+    z, t, i = torch.zeros(4, 50), torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int64)
+    there = torch.ones(4)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 1 if self is there else 0)
+    with pytest.raises(AssertionError, match="tensors on"):
+        lm.distill_topk(z, t, i, reduction="none", grad_out=there)
+    assert not library.calls
+    lm.distill_topk(z, t, i, reduction="none", grad_out=torch.ones(4))
