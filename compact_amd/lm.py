@@ -176,6 +176,18 @@ class ScaledEmbedding(nn.Embedding):
         super().__init__(num_embeddings, embedding_dim, padding_idx, device=device, dtype=dtype)
         self.scale = scale
 
+    @classmethod
+    def from_pretrained(cls, embeddings: torch.Tensor, freeze: bool = True, padding_idx=None,
+                        scale: float = 1.0):
+        """A module over the table `embeddings` [V, D] itself, trained unless `freeze`."""
+        assert embeddings.dim() == 2, f"table [V, D] expected, got {tuple(embeddings.shape)}"
+        m = cls(*embeddings.shape, padding_idx, scale, device="meta")
+        m.weight = nn.Parameter(embeddings, requires_grad=not freeze)
+        return m
+
+    def extra_repr(self):
+        return f"{super().extra_repr()}, scale={self.scale}"
+
     def forward(self, ids):
         return EmbeddingFunction.apply(ids, self.weight, self.scale, self.padding_idx)
 

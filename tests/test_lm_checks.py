@@ -205,3 +205,17 @@ def test_grad_out_lies_with_the_logits(library, monkeypatch):
         lm.distill_topk(z, t, i, reduction="none", grad_out=there)
     assert not library.calls
     lm.distill_topk(z, t, i, reduction="none", grad_out=torch.ones(4))
+
+
+def test_embedding_module_of_a_given_table(library):
+    table = torch.arange(12.0).view(4, 3)
+    m = lm.ScaledEmbedding.from_pretrained(table, padding_idx=-1, scale=3.0)
+    assert m.weight.data_ptr() == table.data_ptr() and not m.weight.requires_grad
+    assert (m.num_embeddings, m.embedding_dim, m.padding_idx, m.scale) == (4, 3, 3, 3.0)
+    assert torch.equal(table, torch.arange(12.0).view(4, 3))
+    m(torch.tensor([1, 2]))
+    assert library.calls[-1][1][1] == table.data_ptr() and library.calls[-1][1][7] == 3.0
+    assert lm.ScaledEmbedding.from_pretrained(table, freeze=False).weight.requires_grad
+    assert "scale=3.0" in repr(m) and "padding_idx=3" in repr(m)
+    with pytest.raises(AssertionError):
+        lm.ScaledEmbedding.from_pretrained(table[0])
