@@ -379,6 +379,7 @@ class ResidualNorm(nn.Module):
 
     def forward(self, residual, y=None, gate=None):
         assert gate is None or self.gate is None, "two gates"
+        assert gate is None or y is not None, "a gate belongs to a block's output y"
         if y is None:
             return ResidualNormFunction.apply(residual, None, self.w_pre, None, None, 1.0, 1.0,
                                               self.eps)

@@ -219,3 +219,13 @@ def test_embedding_module_of_a_given_table(library):
     assert "scale=3.0" in repr(m) and "padding_idx=3" in repr(m)
     with pytest.raises(AssertionError):
         lm.ScaledEmbedding.from_pretrained(table[0])
+
+
+def test_module_refuses_a_gate_of_nothing(library):
+    m, h = lm.ResidualNorm(8), torch.zeros(2, 3, 8)
+    with pytest.raises(AssertionError, match="block's output"):
+        m(h, gate=torch.ones(2, 3, 1))
+    assert not library.calls
+    m(h)
+    m(h, h, gate=torch.ones(2, 3, 1))
+    assert [c[0] for c in library.calls] == ["cpt_residual_norm"] * 2
