@@ -592,3 +592,21 @@ def test_many_rows_a_block(device, n, v, dtype, tau, tail):
                                   reduction="none", want_grad=False)
     want = definition(z, t, idx, y, lse, tau, 0.5, -100, "none", 1.0)
     _close(only, want[0], want[2] + 2.0 ** -23 * want[0].abs(), "loss alone")
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("tau", [1.0, 1.5, 2.0, 8.0])
+def test_far_values_without_a_gradient(device, tau, tail):
+    """Rows that are moved to 0, whose columns are all read again, give the losses that
+    the pass with the gradient gives (the same sums in another order)."""
+    for v in (200, 70001):
+        z, t, idx, y, lse = _inputs(4, v, 6, torch.float32, device, tau=tau, tail=tail)
+        y[:] = idx[:, 1]
+        at = z.gather(1, idx)
+        z[1:3] = -1e9
+        z[2] = z[2].scatter(0, idx[2], at[2])
+        kw = dict(top_lse=lse, temperature=tau, alpha=0.5, reduction="none")
+        with_grad, _ = _cpt().distill_topk(z, t, idx, y, **kw)
+        alone, _ = _cpt().distill_topk(z, t, idx, y, want_grad=False, **kw)
+        assert alone.isfinite().all()
+        assert ((alone - with_grad).abs() <= 2 * 550 * E * (1 + with_grad.abs())).all()
