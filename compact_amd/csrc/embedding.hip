@@ -17,8 +17,9 @@
 // dy is read once, the table written once (rows with tokens twice).
 //
 // Measured on one MI355X: the lookup of 8192 x 2048 bf16 9.8 us (4.6 TB/s), its
-// gradient into 32000 rows 35 (4.6 TB/s of what it must read and write), of 65536
-// tokens 119.  The sums take 11 us of the first, 69 of the second, at 4.4 TB/s.
+// gradient into 32000 rows 43 (3.7 TB/s of what it must read and write; 35 where dy
+// lies in the Infinity Cache), of 65536 tokens 118.  The sums take 11 us of the first,
+// 71 of the second, at 4.3 TB/s; the second's three launches of the sort 37.
 
 #include "compact_amd.h"
 #include "row_ops.h"
@@ -224,10 +225,10 @@ __global__ __launch_bounds__(kBlock) void scatter_kernel(const Pair* __restrict_
 // tokens of the ranges below.  Tokens that are summed nowhere fill the list's end.  Bound by
 // latency and, in the reading of all tokens by each block, by the vector pipe: 18 us
 // at 8192 tokens beside 131 MB of zeros (which alone take 20), 16 at 20011 (20 where
-// the tokens are read a second time to be packed).  The whole gradient against the
-// radix sort's three launches: 8192 tokens into 32000 x 2048 bf16 35 and 48 us, 16000
-// into 5000 x 1000 31 and 37, 20011 x 1001 fp32 43 and 52, 32768 into 32000 x 2048 82
-// and 84.
+// the tokens are read a second time to be packed).  The whole gradient, dy in the
+// Infinity Cache, against the radix sort's three launches: 8192 tokens into 32000 x
+// 2048 bf16 35 and 48 us, 16000 into 5000 x 1000 31 and 37, 20011 x 1001 fp32 43 and
+// 52, 32768 into 32000 x 2048 82 and 84.
 constexpr int kRanges = 32;
 constexpr int kRangeThreads = 1024;
 constexpr int kRangeWaves = kRangeThreads / 64;

@@ -23,7 +23,7 @@
 // Measured on one MI355X: forward of 8192 x 2048 bf16 with both norms 27 us (5.0
 // TB/s), of 8192 x 4096 49 (5.5); backward of 8192 x 4096 82 us and 5 for the
 // partial sums (4.6 TB/s), of 3009 x 1999 fp32, every row unaligned, 31 and 4, of
-// 2000 x 16000 bf16 127 in all (3.0 TB/s), of 49923 x 128 fp16 23 in all (3.4
+// 2000 x 16000 bf16 125 in all (3.1 TB/s), of 49923 x 128 fp16 23 in all (3.4
 // TB/s).  A large copy reaches 5.0.
 
 #include "compact_amd.h"
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(kMaxThreads) void backward_kernel(
   const int64_t b = blockIdx.y;
   // Two vectors a thread leave no registers for the weights' sums: LDS has them, a
   // slot of its own for each thread (such a block has one group).  2000 x 16000 bf16
-  // with all of it in registers, which spill: 268 us; so 127.
+  // with all of it in registers, which spill: 268 us; so 125.
   constexpr bool kInLds = NV > 1;
   float a[NV][8], wp[NV][8], acc_pre[kInLds ? 1 : NV][8], acc_g[kInLds ? 1 : NV][8];
   float4* const slot = reinterpret_cast<float4*>(combine) + tid;

@@ -405,7 +405,8 @@ def distill_topk(logits, top_logits, top_indices, labels=None, *, top_lse=None,
 
     top_lse [...]: the teacher's log-sum-exp of all its logits / T; then
     p = exp(top_logits / T - top_lse), and what it leaves (1 - sum p) is held
-    against what q leaves outside the entries.  top_indices: int32 or int64; an
+    against what q leaves outside the entries (nothing only where all of that is
+    -inf: finite logits count, however low).  top_indices: int32 or int64; an
     index outside [0, V) is no entry, and a row without entries has no soft term.
     Rows labelled ignore_index, or outside [0, V), have no loss and a zero
     gradient; alpha < 1 needs labels.  "mean" is over the rows left in (0 where
