@@ -63,13 +63,14 @@ def _rows(t, d):
 
 
 class _Once(torch.autograd.Function):
-    """The first `n` of the tensors as they are: gradients, as a function of them all
-    that cannot be differentiated."""
+    """The first `n` of the tensors themselves: new gradients, as a function of them all
+    that cannot be differentiated.  No views, which may not be changed in place."""
 
     @staticmethod
     def forward(ctx, what, n, *tensors):
         ctx.what = what
-        return tuple(None if t is None else t.view_as(t) for t in tensors[:n])
+        ctx.mark_dirty(*[t for t in tensors[:n] if t is not None])
+        return tensors[:n]
 
     @staticmethod
     def backward(ctx, *grads):

@@ -229,3 +229,15 @@ def test_module_refuses_a_gate_of_nothing(library):
     m(h)
     m(h, h, gate=torch.ones(2, 3, 1))
     assert [c[0] for c in library.calls] == ["cpt_residual_norm"] * 2
+
+
+def test_gradients_of_create_graph_are_ones_own(library):
+    """They can be changed in place, as other gradients can."""
+    ids, table = torch.tensor([1, 0, 1]), torch.randn(4, 8, requires_grad=True)
+    w, r, y = (torch.randn(s, requires_grad=True) for s in ((8,), (3, 8), (3, 8)))
+    ro, x = lm.ResidualNormFunction.apply(r, y, w, w)
+    out = lm.EmbeddingFunction.apply(ids, table)
+    loss = (out * out).sum() + ro.sum() + (x * x).sum()
+    for grad in torch.autograd.grad(loss, [table, r, y], create_graph=True):
+        grad.mul_(0.5)
+        assert grad.requires_grad
