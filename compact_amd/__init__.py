@@ -26,3 +26,12 @@ from .lm import (  # noqa: F401
     residual_norm, residual_norm_backward, ResidualNormFunction, ResidualNorm,
     distill_topk, DistillTopKFunction, distill_loss,
 )
+from .rope import (  # noqa: F401
+    qk_rope, qk_rope_backward, QKRopeFunction, QKNormRope,
+)
+from .scoring import (  # noqa: F401
+    TokenLogprobs, token_logprobs, token_logprobs_backward, TokenLogprobsFunction, token_scores,
+)
+from .optim import (  # noqa: F401
+    adamw_step, grad_norm, adamw_8bit_values, AdamW,
+)

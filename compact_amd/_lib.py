@@ -105,6 +105,21 @@ SIGNATURES = {
                          ctypes.c_float, ctypes.c_float, _I, ctypes.c_float, _P, _P, _P, _P, _L,
                          _L, _P],
     "cpt_scale_rows": [_I, _P, _L, _L, _P, _I, _P],
+    "cpt_qk_rope": [_I, _I, _I, _I, _P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _I, _L, _P, _L, _L,
+                    _L, _L, _L, _L, ctypes.c_float, ctypes.c_float, _P, _L, _L, _L, _P, _L, _L, _L,
+                    _P],
+    "cpt_qk_rope_backward": [_I, _I, _I, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L,
+                             _L, _L, _P, _P, _P, _I, _L, _P, _L, _L, _L, _L, _L, _L,
+                             ctypes.c_float, ctypes.c_float, _P, _P, _P, _P, _P, _P],
+    "cpt_token_logprobs": [_I, _P, _L, _L, _L, _L, _L, _I, _P, _L, ctypes.c_float, _L, _P, _P, _P,
+                           _P, _P, _P, _P],
+    "cpt_token_logprobs_backward": [_I, _P, _L, _L, _L, _L, _L, _I, _P, _L, ctypes.c_float, _P, _P,
+                                    _P, _P, _P, _P, _L, _L, _P],
+    "cpt_adamw": [_I, _I, _I, _I, _P, _L, ctypes.c_double, _P, ctypes.c_double, ctypes.c_double,
+                  ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, _I, _L, _P,
+                  _P, _P],
+    "cpt_grad_norm": [_I, _P, _L, ctypes.c_float, _P, _P, _P],
+    "cpt_adamw_8bit_values": [_P, _L, _P],
 }
 
 # size queries: name -> argument types (restype int64)
@@ -116,6 +131,8 @@ SIZE_QUERIES = {
     "cpt_gemm_bf16_skinny_dual_workspace_bytes": [_L, _L, _L, _I],
     "cpt_embedding_backward_workspace_bytes": [_L, _L, _L],
     "cpt_residual_norm_backward_workspace_bytes": [_L, _L, _L, _I],
+    "cpt_qk_rope_backward_workspace_bytes": [_L, _L, _L, _L],
+    "cpt_adamw_workspace_bytes": [_L, _L],
 }
 
 CACHE_NONE, CACHE_BF16, CACHE_INT4, CACHE_INT8 = 0, 1, 4, 8

@@ -101,6 +101,15 @@ PyMethodDef methods[] = {
     CPT_ENTRY(cpt_residual_norm_backward_workspace_bytes),
     CPT_ENTRY(cpt_distill_topk),
     CPT_ENTRY(cpt_scale_rows),
+    CPT_ENTRY(cpt_qk_rope),
+    CPT_ENTRY(cpt_qk_rope_backward),
+    CPT_ENTRY(cpt_qk_rope_backward_workspace_bytes),
+    CPT_ENTRY(cpt_token_logprobs),
+    CPT_ENTRY(cpt_token_logprobs_backward),
+    CPT_ENTRY(cpt_adamw),
+    CPT_ENTRY(cpt_adamw_workspace_bytes),
+    CPT_ENTRY(cpt_grad_norm),
+    CPT_ENTRY(cpt_adamw_8bit_values),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_capi", "compact_amd's C ABI", -1, methods,

@@ -1,0 +1,499 @@
+// The queries' and keys' norms and position rotation, and their gradient.
+//
+// Per head of d columns, at position t:
+//   n = x / sqrt(mean x^2 + eps) * w            (no weights: n = x)
+//   the first R columns turn by pairs (a, b) -> (a c - b s, b c + a s) with
+//   c, s = scaling * cos, sin(t * inv_freq[pair]); a pair is two neighbours
+//   (interleaved) or column i of each half of the R.
+// Backward, with dn = the gradient turned back and rho = 1 / sqrt(mean x^2 + eps):
+//   dw = sum over tokens and heads of dn * x * rho
+//   dx = rho * (dn w - x rho^2 mean(dn w x))
+// Nothing is kept between the two: a head's row is in registers when rho is needed.
+//
+// Bound: HBM, two (backward with norms three) passes over q and k.  A lane holds
+// eight pairs, so a head is d / 16 lanes and the norm's sums are a few exchanges
+// within them.  All d columns are pairs here: those past R with c = 1, s = 0.
+// Angles are products in 64 bits reduced to a turn (a position of 10^6 times a
+// frequency rounded in 32 bits is 0.03 off), once per token and pair into LDS for
+// all heads.
+
+#include <algorithm>
+
+#include "compact_amd.h"
+#include "row_ops.h"
+
+namespace cpt {
+namespace {
+
+constexpr int kRopeThreads = 256;
+constexpr int kRopeTableBytes = 16384;    // cos and sin of a tile of tokens
+constexpr int kRopeMaxTile = 64;          // tokens a tile
+constexpr int kRopeBlocks = 1024;         // blocks of the backward, each with a partial sum
+
+struct RopeSide {                         // queries or keys
+  const void* x;
+  const void* dy;
+  void* out;
+  const void* w;
+  float* partial;                         // [blocks, d]
+  int64_t xs[3], ys[3], os[3];            // elements between sequences, tokens, heads
+  FastDivU32 heads;
+  int blocks, tile;
+};
+
+struct RopeArgs {
+  RopeSide side[2];
+  const void* positions;
+  const float* inv_freq;
+  int64_t pos_stride;
+  FastDivU32 seq;
+  int tokens, d, rot, lanes, pos_wide, wdt;
+  float eps, scaling;
+};
+
+// A lane's eight pairs of a head: pair(t) for t = 0 .. 7.  VEC: eight neighbours,
+// moved 16 bytes at a time; otherwise (d or R not a multiple of 16) every
+// `lanes`-th, an element at a time.
+template <int DT, bool VEC, bool INTER>
+struct HeadLane {
+  using R = Row8<DT>;
+  using T = typename R::T;
+  int lane, lanes, pairs, rot, d;
+
+  __device__ __forceinline__ bool on(int t) const {
+    return VEC ? lane * 8 < pairs : lane + t * lanes < pairs;
+  }
+  // pairs past the end are taken as the last one(s)
+  __device__ __forceinline__ int pair(int t) const {
+    return VEC ? min(lane * 8, pairs - 8) + t : min(lane + t * lanes, pairs - 1);
+  }
+  __device__ __forceinline__ int col_a(int i) const {
+    if (INTER) return 2 * i;
+    return i < rot / 2 ? i : i + rot / 2;
+  }
+  __device__ __forceinline__ int col_b(int i) const {
+    if (INTER) return 2 * i + 1;
+    return i < rot / 2 ? i + rot / 2 : i + d / 2;
+  }
+  __device__ __forceinline__ void ld(const T* row, float a[8], float b[8]) const {
+    if constexpr (VEC) {
+      const int i = pair(0);
+      if constexpr (INTER) {
+        float v[16];
+        R::unpack(R::ld(row + 2 * i), v);
+        R::unpack(R::ld(row + 2 * i + 8), v + 8);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) a[t] = v[2 * t], b[t] = v[2 * t + 1];
+      } else {
+        const auto ra = R::ld(row + col_a(i)), rb = R::ld(row + col_b(i));
+        R::unpack(ra, a);
+        R::unpack(rb, b);
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const int i = pair(t);
+        a[t] = Elem<DT>::ld(row + col_a(i));
+        b[t] = Elem<DT>::ld(row + col_b(i));
+      }
+    }
+  }
+  __device__ __forceinline__ void st(T* row, const float a[8], const float b[8]) const {
+    if constexpr (VEC) {
+      if (!on(0)) return;
+      const int i = lane * 8;
+      if constexpr (INTER) {
+        float v[16];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) v[2 * t] = a[t], v[2 * t + 1] = b[t];
+        R::st(row + 2 * i, R::pack(v));
+        R::st(row + 2 * i + 8, R::pack(v + 8));
+      } else {
+        R::st(row + col_a(i), R::pack(a));
+        R::st(row + col_b(i), R::pack(b));
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+        if (on(t)) {
+          Elem<DT>::st(row + col_a(pair(t)), a[t]);
+          Elem<DT>::st(row + col_b(pair(t)), b[t]);
+        }
+    }
+  }
+};
+
+// The sum over a head's lanes, in each of them.
+__device__ __forceinline__ float head_sum(float v, int lanes) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// cos and sin of a tile's tokens, and where their rows start.
+template <bool BWD>
+__device__ __forceinline__ void rope_table(const RopeArgs& A, const RopeSide& S, int t0, int nt,
+                                           float2* table, int64_t (*base)[kRopeMaxTile]) {
+  const int pairs = A.d / 2, turning = A.rot / 2;
+  for (int i = threadIdx.x; i < nt * pairs; i += kRopeThreads) {
+    const int tok = i / pairs, p = i - tok * pairs;
+    float c = 1.f, s = 0.f;
+    if (p < turning) {
+      const uint32_t b = A.seq.div(t0 + tok), n = t0 + tok - b * A.seq.d;
+      const int64_t pos = A.positions ? ld_index(A.positions, A.pos_wide, b * A.pos_stride + n)
+                                      : (int64_t)n;
+      double turn = (double)pos * ((double)A.inv_freq[p] * 0.15915494309189533577);
+      turn -= rint(turn);
+      sincospif(2.f * (float)turn, &s, &c);
+      c *= A.scaling;
+      s *= A.scaling;
+    }
+    table[i] = make_float2(c, s);
+  }
+  if (threadIdx.x < nt) {
+    const uint32_t b = A.seq.div(t0 + threadIdx.x), n = t0 + threadIdx.x - b * A.seq.d;
+    base[0][threadIdx.x] = b * S.xs[0] + n * S.xs[1];
+    base[1][threadIdx.x] = b * S.os[0] + n * S.os[1];
+    if (BWD) base[2][threadIdx.x] = b * S.ys[0] + n * S.ys[1];
+  }
+}
+
+// INVERSE turns back (the gradient without norms).
+template <int DT, bool VEC, bool INTER, bool NORM>
+__global__ __launch_bounds__(kRopeThreads) void rope_forward(const RopeArgs A, int inverse) {
+  extern __shared__ float2 table[];
+  __shared__ int64_t base[2][kRopeMaxTile];
+  using T = typename Elem<DT>::T;
+  const int k_side = blockIdx.x >= A.side[0].blocks;
+  const RopeSide& S = A.side[k_side];
+  const int block = blockIdx.x - (k_side ? A.side[0].blocks : 0);
+  const int group = threadIdx.x / A.lanes, groups = kRopeThreads / A.lanes, pairs = A.d / 2;
+  const HeadLane<DT, VEC, INTER> io{(int)threadIdx.x & (A.lanes - 1), A.lanes, pairs, A.rot, A.d};
+  float wa[8], wb[8];
+  if (NORM) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      wa[t] = ld_any(S.w, A.wdt, io.col_a(io.pair(t)));
+      wb[t] = ld_any(S.w, A.wdt, io.col_b(io.pair(t)));
+    }
+  }
+  const int t0 = block * S.tile, nt = min(S.tile, A.tokens - t0);
+  rope_table<false>(A, S, t0, nt, table, base);
+  __syncthreads();
+  const int items = nt * S.heads.d;
+  for (int it = group; it < items; it += groups) {
+    const uint32_t tok = S.heads.div(it), h = it - tok * S.heads.d;
+    float a[8], b[8];
+    io.ld((const T*)S.x + base[0][tok] + h * S.xs[2], a, b);
+    if (NORM) {
+      float ss = 0.f;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) ss += io.on(t) ? a[t] * a[t] + b[t] * b[t] : 0.f;
+      const float rho = rsqrtf(head_sum(ss, A.lanes) / A.d + A.eps);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) a[t] *= rho * wa[t], b[t] *= rho * wb[t];
+    }
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const float2 cs = table[tok * pairs + io.pair(t)];
+      const float s = inverse ? -cs.y : cs.y;
+      const float u = a[t] * cs.x - b[t] * s;
+      b[t] = b[t] * cs.x + a[t] * s;
+      a[t] = u;
+    }
+    io.st((T*)S.out + base[1][tok] + h * S.os[2], a, b);
+  }
+}
+
+template <int DT, bool VEC, bool INTER>
+__global__ __launch_bounds__(kRopeThreads) void rope_norm_backward(const RopeArgs A) {
+  extern __shared__ float2 table[];
+  __shared__ int64_t base[3][kRopeMaxTile];
+  using T = typename Elem<DT>::T;
+  const int k_side = blockIdx.x >= A.side[0].blocks;
+  const RopeSide& S = A.side[k_side];
+  const int block = blockIdx.x - (k_side ? A.side[0].blocks : 0);
+  const int group = threadIdx.x / A.lanes, groups = kRopeThreads / A.lanes, pairs = A.d / 2;
+  const HeadLane<DT, VEC, INTER> io{(int)threadIdx.x & (A.lanes - 1), A.lanes, pairs, A.rot, A.d};
+  float wa[8], wb[8], da[8], db[8];
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    wa[t] = ld_any(S.w, A.wdt, io.col_a(io.pair(t)));
+    wb[t] = ld_any(S.w, A.wdt, io.col_b(io.pair(t)));
+    da[t] = db[t] = 0.f;
+  }
+  const float inv_d = 1.f / A.d;
+  for (int64_t t0 = (int64_t)block * S.tile; t0 < A.tokens; t0 += (int64_t)S.blocks * S.tile) {
+    const int nt = (int)min((int64_t)S.tile, A.tokens - t0);
+    rope_table<true>(A, S, (int)t0, nt, table, base);
+    __syncthreads();
+    const int items = nt * S.heads.d;
+    for (int it = group; it < items; it += groups) {
+      const uint32_t tok = S.heads.div(it), h = it - tok * S.heads.d;
+      float a[8], b[8], ga[8], gb[8];
+      io.ld((const T*)S.x + base[0][tok] + h * S.xs[2], a, b);
+      io.ld((const T*)S.dy + base[2][tok] + h * S.ys[2], ga, gb);
+      float ss = 0.f, sd = 0.f;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const float2 cs = table[tok * pairs + io.pair(t)];
+        const float u = ga[t] * cs.x + gb[t] * cs.y;
+        gb[t] = gb[t] * cs.x - ga[t] * cs.y;
+        ga[t] = u;
+        const float xa = io.on(t) ? a[t] : 0.f, xb = io.on(t) ? b[t] : 0.f;
+        ss += xa * xa + xb * xb;
+        sd += ga[t] * wa[t] * xa + gb[t] * wb[t] * xb;
+      }
+      ss = head_sum(ss, A.lanes);
+      sd = head_sum(sd, A.lanes);
+      const float rho = rsqrtf(ss * inv_d + A.eps);
+      const float m = rho * rho * (sd * inv_d);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        da[t] += ga[t] * (a[t] * rho);
+        db[t] += gb[t] * (b[t] * rho);
+        a[t] = rho * (ga[t] * wa[t] - a[t] * m);
+        b[t] = rho * (gb[t] * wb[t] - b[t] * m);
+      }
+      io.st((T*)S.out + base[1][tok] + h * S.os[2], a, b);
+    }
+    __syncthreads();
+  }
+  // the groups' sums: within a wavefront by exchange, then one row a wavefront in LDS
+  for (int o = A.lanes; o < 64; o <<= 1)
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      da[t] += __shfl_xor(da[t], o);
+      db[t] += __shfl_xor(db[t], o);
+    }
+  float* sums = reinterpret_cast<float*>(table);    // [4, d]
+  if ((threadIdx.x & 63) < A.lanes) {
+    float* mine = sums + (threadIdx.x >> 6) * A.d;
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+      if (io.on(t)) {
+        mine[io.col_a(io.pair(t))] = da[t];
+        mine[io.col_b(io.pair(t))] = db[t];
+      }
+  }
+  __syncthreads();
+  for (int j = threadIdx.x; j < A.d; j += kRopeThreads)
+    S.partial[(int64_t)block * A.d + j] =
+        (sums[j] + sums[A.d + j]) + (sums[2 * A.d + j] + sums[3 * A.d + j]);
+}
+
+// dw[j] = the blocks' partial sums, 16 columns a block, 16 threads each.
+__global__ __launch_bounds__(256) void rope_weight_sums(const float* pq, int nq, void* dwq,
+                                                        const float* pk, int nk, void* dwk, int d,
+                                                        int wdt) {
+  __shared__ float part[16][17];
+  const float* p = blockIdx.y ? pk : pq;
+  const int n = blockIdx.y ? nk : nq;
+  const int c = threadIdx.x & 15, r = threadIdx.x >> 4, j = blockIdx.x * 16 + c;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (j < d) {
+    int i = r;
+    for (; i + 48 < n; i += 64)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s[u] += p[(int64_t)(i + 16 * u) * d + j];
+    for (; i < n; i += 16) s[0] += p[(int64_t)i * d + j];
+  }
+  part[r][c] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  if (r == 0 && j < d) {
+    float t = 0.f;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) t += part[u][c];
+    st_any(blockIdx.y ? dwk : dwq, wdt, j, t);
+  }
+}
+
+int pow2_at_least(int n) {
+  int l = 1;
+  while (l < n) l <<= 1;
+  return l;
+}
+
+// Lanes a head, and whether it moves 16 bytes at a time.
+bool rope_vec(int64_t d, int64_t rot, bool inter) {
+  return d % 16 == 0 && (inter || rot % 16 == 0);
+}
+int rope_lanes(int64_t d) { return pow2_at_least((int)((d / 2 + 7) / 8)); }
+
+// Tokens a tile: enough that the block's groups take about four heads each, as many as
+// the table holds, and no more than leaves a block for every CU (four).
+int rope_tile(int64_t tokens, int64_t heads, int64_t d) {
+  const int64_t groups = kRopeThreads / rope_lanes(d);
+  int64_t t = (4 * groups + heads - 1) / heads;
+  t = std::min<int64_t>(t, kRopeTableBytes / (d / 2 * 8));
+  t = std::min<int64_t>(t, (tokens + 1023) / 1024);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(t, kRopeMaxTile));
+}
+
+int64_t rope_blocks(int64_t tokens, int tile, bool bounded) {
+  const int64_t n = (tokens + tile - 1) / tile;
+  return bounded ? std::min<int64_t>(n, kRopeBlocks) : n;
+}
+
+int rope_check(int dtype, int wdt, int64_t batch, int64_t seq, int64_t hq, int64_t hk, int64_t d,
+               int64_t rot) {
+  if (dtype < 0 || dtype > 2 || (wdt != dtype && wdt != kF32)) return kErrDType;
+  if (batch < 0 || seq < 0 || hq < 0 || hk < 0 || d < 2 || d % 2 || rot < 2 || rot % 2 || rot > d)
+    return kErrShape;
+  if (d > 1024 || hq > 65536 || hk > 65536) return kErrTooLarge;
+  if (seq > 0 && batch > ((1ll << 30) - 1) / seq) return kErrTooLarge;
+  return kOk;
+}
+
+RopeSide rope_side(const void* x, const int64_t* xs, const void* dy, const int64_t* ys, void* out,
+                   const int64_t* os, const void* w, int64_t heads) {
+  RopeSide s{};
+  s.x = x, s.dy = dy, s.out = out, s.w = w;
+  for (int i = 0; i < 3; ++i) {
+    s.xs[i] = xs[i];
+    s.ys[i] = ys ? ys[i] : 0;
+    s.os[i] = os[i];
+  }
+  s.heads = FastDivU32::make((uint32_t)std::max<int64_t>(heads, 1));
+  return s;
+}
+
+template <int DT>
+int launch_forward(const RopeArgs& A, bool vec, bool inter, bool norm, int inverse, size_t lds,
+                   hipStream_t st) {
+  const int grid = A.side[0].blocks + A.side[1].blocks;
+#define CPT_ROPE(V, I, N) \
+  rope_forward<DT, V, I, N><<<grid, kRopeThreads, lds, st>>>(A, inverse)
+  if (vec) {
+    if (inter) { if (norm) CPT_ROPE(true, true, true); else CPT_ROPE(true, true, false); }
+    else { if (norm) CPT_ROPE(true, false, true); else CPT_ROPE(true, false, false); }
+  } else {
+    if (inter) { if (norm) CPT_ROPE(false, true, true); else CPT_ROPE(false, true, false); }
+    else { if (norm) CPT_ROPE(false, false, true); else CPT_ROPE(false, false, false); }
+  }
+#undef CPT_ROPE
+  return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
+}
+
+template <int DT>
+int launch_backward(const RopeArgs& A, bool vec, bool inter, size_t lds, hipStream_t st) {
+  const int grid = A.side[0].blocks + A.side[1].blocks;
+#define CPT_ROPE(V, I) rope_norm_backward<DT, V, I><<<grid, kRopeThreads, lds, st>>>(A)
+  if (vec) { if (inter) CPT_ROPE(true, true); else CPT_ROPE(true, false); }
+  else { if (inter) CPT_ROPE(false, true); else CPT_ROPE(false, false); }
+#undef CPT_ROPE
+  return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
+}
+
+}  // namespace
+}  // namespace cpt
+
+using namespace cpt;
+
+extern "C" {
+
+int cpt_qk_rope(int dtype, int weight_dtype, int interleaved, int inverse, const void* q,
+                int64_t q_batch, int64_t q_token, int64_t q_head, const void* k, int64_t k_batch,
+                int64_t k_token, int64_t k_head, const void* w_q, const void* w_k,
+                const void* positions, int pos_wide, int64_t pos_batch, const void* inv_freq,
+                int64_t batch, int64_t seq, int64_t heads_q, int64_t heads_k, int64_t d,
+                int64_t rotary, float eps, float scaling, void* q_out, int64_t qo_batch,
+                int64_t qo_token, int64_t qo_head, void* k_out, int64_t ko_batch, int64_t ko_token,
+                int64_t ko_head, void* stream) {
+  const int rc = rope_check(dtype, weight_dtype, batch, seq, heads_q, heads_k, d, rotary);
+  if (rc) return rc;
+  if ((w_q == nullptr) != (w_k == nullptr) || (w_q && inverse) || !inv_freq || !(eps >= 0.f))
+    return kErrShape;
+  const int64_t tokens = batch * seq;
+  if (tokens == 0 || heads_q + heads_k == 0) return kOk;
+  if ((heads_q && (!q || !q_out)) || (heads_k && (!k || !k_out))) return kErrShape;
+  RopeArgs A{};
+  const int64_t xq[3] = {q_batch, q_token, q_head}, xk[3] = {k_batch, k_token, k_head};
+  const int64_t oq[3] = {qo_batch, qo_token, qo_head}, ok[3] = {ko_batch, ko_token, ko_head};
+  A.side[0] = rope_side(q, xq, nullptr, nullptr, q_out, oq, w_q, heads_q);
+  A.side[1] = rope_side(k, xk, nullptr, nullptr, k_out, ok, w_k, heads_k);
+  const int64_t heads[2] = {heads_q, heads_k};
+  int most = 1;
+  for (int i = 0; i < 2; ++i) {
+    A.side[i].tile = rope_tile(tokens, std::max<int64_t>(heads[i], 1), d);
+    A.side[i].blocks = heads[i] ? (int)rope_blocks(tokens, A.side[i].tile, false) : 0;
+    if (heads[i]) most = std::max(most, A.side[i].tile);
+  }
+  A.positions = positions, A.pos_wide = pos_wide, A.pos_stride = pos_batch;
+  A.inv_freq = (const float*)inv_freq;
+  A.seq = FastDivU32::make((uint32_t)seq);
+  A.tokens = (int)tokens, A.d = (int)d, A.rot = (int)rotary, A.lanes = rope_lanes(d);
+  A.wdt = weight_dtype, A.eps = eps, A.scaling = scaling;
+  const size_t lds = (size_t)most * (d / 2) * 8;
+  const bool vec = rope_vec(d, rotary, interleaved), norm = w_q != nullptr;
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == kF32) return launch_forward<kF32>(A, vec, interleaved, norm, inverse, lds, st);
+  if (dtype == kF16) return launch_forward<kF16>(A, vec, interleaved, norm, inverse, lds, st);
+  return launch_forward<kBF16>(A, vec, interleaved, norm, inverse, lds, st);
+}
+
+int64_t cpt_qk_rope_backward_workspace_bytes(int64_t tokens, int64_t heads_q, int64_t heads_k,
+                                             int64_t d) {
+  if (tokens < 0 || heads_q < 0 || heads_k < 0 || d < 2 || d > 1024 || tokens >= 1ll << 30)
+    return -1;
+  int64_t n = 0;
+  if (tokens > 0) {
+    if (heads_q) n += rope_blocks(tokens, rope_tile(tokens, heads_q, d), true);
+    if (heads_k) n += rope_blocks(tokens, rope_tile(tokens, heads_k, d), true);
+  }
+  return n * d * 4;
+}
+
+int cpt_qk_rope_backward(int dtype, int weight_dtype, int interleaved, const void* d_q,
+                         int64_t dq_batch, int64_t dq_token, int64_t dq_head, const void* d_k,
+                         int64_t dk_batch, int64_t dk_token, int64_t dk_head, const void* q,
+                         int64_t q_batch, int64_t q_token, int64_t q_head, const void* k,
+                         int64_t k_batch, int64_t k_token, int64_t k_head, const void* w_q,
+                         const void* w_k, const void* positions, int pos_wide, int64_t pos_batch,
+                         const void* inv_freq, int64_t batch, int64_t seq, int64_t heads_q,
+                         int64_t heads_k, int64_t d, int64_t rotary, float eps, float scaling,
+                         void* q_grad, void* k_grad, void* dw_q, void* dw_k, void* workspace,
+                         void* stream) {
+  const int rc = rope_check(dtype, weight_dtype, batch, seq, heads_q, heads_k, d, rotary);
+  if (rc) return rc;
+  const int64_t tokens = batch * seq;
+  if (!w_q || !w_k || !dw_q || !dw_k || !inv_freq || !(eps >= 0.f)) return kErrShape;
+  if (tokens == 0 || heads_q == 0 || heads_k == 0) return kErrShape;
+  if (!q || !k || !d_q || !d_k || !q_grad || !k_grad || !workspace) return kErrShape;
+  RopeArgs A{};
+  const int64_t xq[3] = {q_batch, q_token, q_head}, xk[3] = {k_batch, k_token, k_head};
+  const int64_t yq[3] = {dq_batch, dq_token, dq_head}, yk[3] = {dk_batch, dk_token, dk_head};
+  const int64_t oq[3] = {seq * heads_q * d, heads_q * d, d};
+  const int64_t ok[3] = {seq * heads_k * d, heads_k * d, d};
+  A.side[0] = rope_side(q, xq, d_q, yq, q_grad, oq, w_q, heads_q);
+  A.side[1] = rope_side(k, xk, d_k, yk, k_grad, ok, w_k, heads_k);
+  const int64_t heads[2] = {heads_q, heads_k};
+  float* ws = (float*)workspace;
+  int most = 1;
+  for (int i = 0; i < 2; ++i) {
+    RopeSide& s = A.side[i];
+    s.tile = rope_tile(tokens, heads[i], d);
+    s.blocks = (int)rope_blocks(tokens, s.tile, true);
+    s.partial = ws;
+    ws += (int64_t)s.blocks * d;
+    most = std::max(most, s.tile);
+  }
+  A.positions = positions, A.pos_wide = pos_wide, A.pos_stride = pos_batch;
+  A.inv_freq = (const float*)inv_freq;
+  A.seq = FastDivU32::make((uint32_t)seq);
+  A.tokens = (int)tokens, A.d = (int)d, A.rot = (int)rotary, A.lanes = rope_lanes(d);
+  A.wdt = weight_dtype, A.eps = eps, A.scaling = scaling;
+  // the table, and at the end four rows of sums in its place
+  const size_t lds = std::max<size_t>((size_t)most * (d / 2) * 8, (size_t)d * 16);
+  const bool vec = rope_vec(d, rotary, interleaved);
+  const hipStream_t st = (hipStream_t)stream;
+  const int err = dtype == kF32   ? launch_backward<kF32>(A, vec, interleaved, lds, st)
+                  : dtype == kF16 ? launch_backward<kF16>(A, vec, interleaved, lds, st)
+                                  : launch_backward<kBF16>(A, vec, interleaved, lds, st);
+  if (err) return err;
+  rope_weight_sums<<<dim3((unsigned)((d + 15) / 16), 2), 256, 0, st>>>(
+      A.side[0].partial, A.side[0].blocks, dw_q, A.side[1].partial, A.side[1].blocks, dw_k, (int)d,
+      weight_dtype);
+  return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
+}
+
+}  // extern "C"

@@ -106,6 +106,14 @@ def _timed(name):
     return _UNTIMED if KernelTimer.active is None else _Timed(name)
 
 
+def _guard(t):
+    """t's device as the current one, for the launches inside: the default stream is the
+    current device's."""
+    if t.get_device() == torch.cuda.current_device():
+        return _UNTIMED
+    return torch.cuda.device(t.device)
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 

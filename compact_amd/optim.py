@@ -1,0 +1,379 @@
+"""AdamW over many tensors in few launches, moments in float32 or in 8 bits.
+
+  adamw_step, grad_norm, adamw_8bit_values    AdamW
+
+`adamw_step` steps lists of tensors in place; `AdamW` is the torch optimizer
+around it.  Parameters are float32, float16 or bfloat16, gradients of their type or
+float32, an fp32 copy of 16-bit parameters optional.  Gradients can be clipped to
+their global norm within the step, which costs one more read of them and no
+synchronisation.  The reference leaves the optimizer to torch.  There is no CPU
+path.
+
+8-bit moments take 2 bytes and 1/64 an element in place of 8.  128 consecutive
+elements share a power of two (a byte each for both moments); a code has three
+bits of mantissa and four (first moment, signed) or five (second) of exponent, and
+values are rounded up or down at random, in proportion, so that averages that
+move by less than a code's step a time still move.
+"""
+
+from __future__ import annotations
+
+from array import array
+
+import torch
+
+from . import _lib
+from ._lib import check
+from .kernels import _DT, _guard, _ptr, _require_device, _stream, _timed
+
+BLOCK = 128         # elements of an 8-bit moment that share a scale
+_ENTRY = 10         # 8-byte fields of a cpt_adamw_tensor
+
+
+def _dense_layout(t):
+    """Whether t's elements fill its memory once, in whatever order of its axes."""
+    if t.is_contiguous():
+        return True
+    extent = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if stride != extent:
+            return False
+        extent = stride * size
+    return True
+
+
+def _same_layout(a, b):
+    """Whether dense a and b of one shape lie alike in memory."""
+    return (a.is_contiguous() and b.is_contiguous()) or a.stride() == b.stride()
+
+
+def _one_kind(tensors, what):
+    """All tensors of one dtype on one HIP device."""
+    first = tensors[0]
+    dt, dev = first.dtype, first.get_device()
+    if dev < 0:
+        _require_device(first)
+    for t in tensors:
+        if t.dtype != dt or t.get_device() != dev:
+            raise AssertionError(f"{what}: {dt} on {first.device} and {t.dtype} on {t.device}")
+    return dt, dev
+
+
+def _lists(params, **lists):
+    """As many of each as there are parameters."""
+    for name, ts in lists.items():
+        assert ts is None or len(ts) == len(params), \
+            f"{name}: {len(params)} tensors expected, got {len(ts)}"
+
+
+def _like(params, tensors, what, dtype, dev):
+    """Addresses of `tensors`: dtype, shaped and laid out as the parameters."""
+    out = []
+    for p, t in zip(params, tensors):
+        if t.dtype != dtype or t.get_device() != dev or t.shape != p.shape \
+                or not _same_layout(p, t):
+            raise AssertionError(
+                f"{what}: {dtype} {tuple(p.shape)} {p.stride()} on {p.device} expected, got "
+                f"{t.dtype} {tuple(t.shape)} {t.stride()} on {t.device}")
+        out.append(t.data_ptr())
+    return out
+
+
+def _bytes(counts, tensors, what, dev):
+    """Addresses of `tensors`: contiguous uint8 with so many elements."""
+    out = []
+    for n, t in zip(counts, tensors):
+        if t.dtype != torch.uint8 or t.get_device() != dev or t.numel() != n \
+                or not t.is_contiguous():
+            raise AssertionError(f"{what}: contiguous uint8 of {n} expected, got {t.dtype} "
+                                 f"{tuple(t.shape)} on {t.device}")
+        out.append(t.data_ptr())
+    return out
+
+
+def _scalar(t, dev, what):
+    assert t.dtype == torch.float32 and t.numel() == 1 and t.get_device() == dev, \
+        f"{what}: one float32 on the parameters' device expected"
+    return t.data_ptr()
+
+
+def _steps(step, count, dev):
+    """(host step numbers or None, device counts' addresses or None)."""
+    if isinstance(step, torch.Tensor):
+        assert step.dtype == torch.int64 and step.numel() == count and step.is_contiguous() \
+            and step.get_device() == dev, \
+            f"step: {count} contiguous int64 on the parameters' device expected"
+        return None, [step.data_ptr() + 8 * i for i in range(count)]
+    if isinstance(step, int):
+        assert step >= 1, f"step={step}: the first is 1"
+        return [step] * count, None
+    assert len(step) == count, f"step: {count} expected, got {len(step)}"
+    if count and isinstance(step[0], torch.Tensor):
+        for t in step:
+            assert isinstance(t, torch.Tensor) and t.dtype == torch.int64 and t.numel() == 1 \
+                and t.get_device() == dev, "step: one int64 on the parameters' device each expected"
+        at = [t.data_ptr() for t in step]
+        assert len(set(at)) == count, "step: a count of its own for each parameter expected"
+        return None, at
+    for t in step:
+        assert isinstance(t, int) and t >= 1, f"step={t}: whole numbers from 1 on expected"
+    return list(step), None
+
+
+def _table(count, columns):
+    """The C ABI's array of tensors, from columns of addresses and numbers."""
+    rows = array("q", bytes(8 * _ENTRY * count))
+    for i, c in columns.items():
+        if c is not None:
+            rows[i::_ENTRY] = array("q", c)
+    return rows
+
+
+def grad_norm(grads, *, grad_scale: float = 1.0, out=None) -> torch.Tensor:
+    """The 2-norm of grad_scale times all gradients as one vector, a float32 scalar on
+    their device; squares are summed in 64 bits.  One dtype and device."""
+    grads = list(grads)
+    assert grads, "grad_norm: no gradients"
+    dt, dev = _one_kind(grads, "grads")
+    assert dt in _DT, f"unsupported dtype {dt}"
+    grads = [g if _dense_layout(g) else g.contiguous() for g in grads]
+    sizes = [g.numel() for g in grads]
+    if out is None:
+        out = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    L = _lib.api()
+    nbytes = L.cpt_adamw_workspace_bytes(len(grads), sum(sizes))
+    assert nbytes >= 0, "grad_norm: sizes out of range"
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=grads[0].device)
+    table = _table(len(grads), {1: [g.data_ptr() for g in grads], 8: sizes})
+    with _guard(grads[0]), _timed("grad_norm"):
+        rc = L.cpt_grad_norm(_DT[dt], table.buffer_info()[0], len(grads), float(grad_scale),
+                             _scalar(out, dev, "out"), ws.data_ptr(), _stream(grads[0]))
+    check(rc, "grad_norm")
+    return out
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.9, 0.999),
+               eps: float = 1e-8, weight_decay: float = 1e-2, m_scales=None, v_scales=None,
+               masters=None, grad_scale: float = 1.0, max_norm: float | None = None, norm=None,
+               seed: int = 0):
+    """One AdamW step over lists of tensors, in place:
+
+        g = grad * grad_scale * min(1, max_norm / (norm + 1e-6))
+        m = b1 m + (1 - b1) g;   v = b2 v + (1 - b2) g^2
+        p = p - lr weight_decay p - lr (m / (1 - b1^step)) / (sqrt(v / (1 - b2^step)) + eps)
+
+    params: one dtype and device, any dense layout; grads: their dtype or float32 (one
+    that lies otherwise than its parameter is copied); exp_avgs, exp_avg_sqs: float32,
+    laid out as the parameters.  With m_scales and v_scales (uint8, one a 128 elements)
+    the moments are 8-bit codes (uint8 [numel], in the order of the parameter's memory)
+    rounded by `seed`.  masters: float32 parameters that are stepped in the place of
+    16-bit ones, which become their rounding.  Zeros are a valid start for all moments,
+    codes and scales.
+
+    step: this step's number, from 1 (for all, or a list), or int64 counts of the steps
+    done on the device (one tensor of len(params), or one each), which the call
+    increases: what a captured graph needs.  lr: a number, or a float32 scalar on the
+    device.
+
+    max_norm clips by the global norm of grad_scale * grads, which is returned (float32
+    scalar on the device; else None); `norm` gives it where it is known, as for more
+    tensors than these.  A norm that is not finite leaves parameters, moments and
+    counts as they were."""
+    params, grads = list(params), list(grads)
+    exp_avgs, exp_avg_sqs = list(exp_avgs), list(exp_avg_sqs)
+    _lists(params, grads=grads, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs, m_scales=m_scales,
+           v_scales=v_scales, masters=masters)
+    assert (m_scales is None) == (v_scales is None), "m_scales and v_scales belong together"
+    b1, b2 = betas
+    assert 0 <= b1 < 1 and 0 <= b2 < 1, f"betas={betas}"
+    assert eps >= 0 and weight_decay >= 0, f"eps={eps}, weight_decay={weight_decay}"
+    assert max_norm is None or 0 < max_norm < float("inf"), f"max_norm={max_norm}"
+    assert norm is None or max_norm is not None, "norm goes with max_norm"
+    if not params:
+        return norm
+    dt, dev = _one_kind(params, "params")
+    gdt, gdev = _one_kind(grads, "grads")
+    assert dt in _DT, f"unsupported dtype {dt}"
+    assert gdev == dev and gdt in (dt, torch.float32), \
+        f"grads: {dt} or float32 beside the parameters expected, got {gdt} on {grads[0].device}"
+    for i, (p, g) in enumerate(zip(params, grads)):
+        assert g.shape == p.shape, f"gradient {tuple(g.shape)} for {tuple(p.shape)}"
+        if not p.is_contiguous():
+            assert _dense_layout(p), f"parameter {tuple(p.shape)} {p.stride()}: dense expected"
+        if not _same_layout(p, g):
+            grads[i] = torch.empty_like(p, dtype=gdt).copy_(g)
+    count = len(params)
+    sizes = [p.numel() for p in params]
+    at = [p.data_ptr() for p in params]
+    assert len({a for a, n in zip(at, sizes) if n}) == sum(n > 0 for n in sizes), \
+        "a parameter is there twice"
+    bits8 = m_scales is not None
+    cols = {0: at, 1: [g.data_ptr() for g in grads], 8: sizes}
+    if bits8:
+        blocks = [-(-n // BLOCK) for n in sizes]
+        cols[2] = _bytes(sizes, exp_avgs, "exp_avgs", dev)
+        cols[3] = _bytes(sizes, exp_avg_sqs, "exp_avg_sqs", dev)
+        cols[4] = _bytes(blocks, m_scales, "m_scales", dev)
+        cols[5] = _bytes(blocks, v_scales, "v_scales", dev)
+    else:
+        cols[2] = _like(params, exp_avgs, "exp_avgs", torch.float32, dev)
+        cols[3] = _like(params, exp_avg_sqs, "exp_avg_sqs", torch.float32, dev)
+    if masters is not None:
+        assert dt != torch.float32, "masters: of 16-bit parameters"
+        cols[6] = _like(params, masters, "masters", torch.float32, dev)
+    cols[9], cols[7] = _steps(step, count, dev)
+    lr_at = None
+    if isinstance(lr, torch.Tensor):
+        lr_at, lr = _scalar(lr, dev, "lr"), 0.0
+    assert lr >= 0, f"lr={lr}"
+    L = _lib.api()
+    ws = norm_at = None
+    given = norm is not None
+    if max_norm is not None:
+        if not given:
+            norm = torch.empty((), dtype=torch.float32, device=params[0].device)
+        norm_at = _scalar(norm, dev, "norm")
+    if max_norm is not None or cols[7] is not None:
+        nbytes = L.cpt_adamw_workspace_bytes(count, sum(sizes))
+        assert nbytes >= 0, "adamw_step: sizes out of range"
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=params[0].device)
+    table = _table(count, cols)
+    with _guard(params[0]), _timed("adamw_step"):
+        rc = L.cpt_adamw(_DT[dt], _DT[gdt], int(bits8), int(masters is not None),
+                         table.buffer_info()[0], count, float(lr), lr_at, float(b1), float(b2),
+                         float(eps), float(weight_decay), float(grad_scale),
+                         0.0 if max_norm is None else float(max_norm), int(given),
+                         seed & 0xFFFFFFFF, norm_at, _ptr(ws), _stream(params[0]))
+    check(rc, "adamw_step")
+    # autograd refuses a graph that still needs the old parameters
+    torch.autograd.graph.increment_version(params)
+    return norm
+
+
+def adamw_8bit_values(exp_avgs, exp_avg_sqs, m_scales, v_scales):
+    """What 8-bit moments stand for: two lists of bfloat16 tensors, shaped as the codes,
+    which hold the values exactly (NaN for a block with a value that was not finite)."""
+    exp_avgs, exp_avg_sqs = list(exp_avgs), list(exp_avg_sqs)
+    m_scales, v_scales = list(m_scales), list(v_scales)
+    _lists(exp_avgs, exp_avg_sqs=exp_avg_sqs, m_scales=m_scales, v_scales=v_scales)
+    if not exp_avgs:
+        return [], []
+    _, dev = _one_kind(exp_avgs, "exp_avgs")
+    sizes = [t.numel() for t in exp_avgs]
+    blocks = [-(-n // BLOCK) for n in sizes]
+    m = [torch.empty(t.shape, dtype=torch.bfloat16, device=t.device) for t in exp_avgs]
+    v = [torch.empty(t.shape, dtype=torch.bfloat16, device=t.device) for t in exp_avgs]
+    table = _table(len(sizes), {
+        0: [t.data_ptr() for t in m], 6: [t.data_ptr() for t in v],
+        2: _bytes(sizes, exp_avgs, "exp_avgs", dev),
+        3: _bytes(sizes, exp_avg_sqs, "exp_avg_sqs", dev),
+        4: _bytes(blocks, m_scales, "m_scales", dev),
+        5: _bytes(blocks, v_scales, "v_scales", dev), 8: sizes})
+    with _guard(m[0]), _timed("adamw_8bit_values"):
+        rc = _lib.api().cpt_adamw_8bit_values(table.buffer_info()[0], len(sizes), _stream(m[0]))
+    check(rc, "adamw_8bit_values")
+    return m, v
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's step by adamw_step.
+
+    state: "float32" or "8bit" moments.  master: keep an fp32 copy of 16-bit
+    parameters and step that.  max_norm clips all gradients by their global norm; the
+    last step's norm is in `norm` (on the device), and a step whose norm is not finite
+    changes nothing.  seed: of the 8-bit moments' rounding.  capturable: step counts
+    on the device, so that a step can be captured into a graph (give lr as a float32
+    tensor there to change it); the step before has to be an eager one, which makes the
+    state."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, *, state: str = "float32", master: bool = False,
+                 max_norm: float | None = None, seed: int = 0, capturable: bool = False):
+        assert state in ("float32", "8bit"), f"state={state!r}: 'float32' or '8bit' expected"
+        assert isinstance(lr, torch.Tensor) or lr >= 0, f"lr={lr}"
+        assert 0 <= betas[0] < 1 and 0 <= betas[1] < 1, f"betas={betas}"
+        assert eps >= 0 and weight_decay >= 0, f"eps={eps}, weight_decay={weight_decay}"
+        assert max_norm is None or max_norm > 0, f"max_norm={max_norm}"
+        self.max_norm, self.seed, self.norm = max_norm, seed, None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+                                      state=state, master=master, capturable=capturable))
+
+    def _init_state(self, p, group):
+        s = self.state[p]
+        if s:
+            return s
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: the state has to be there before a step is captured")
+        if not _dense_layout(p):
+            raise AssertionError(f"parameter {tuple(p.shape)} {p.stride()}: dense expected")
+        dev = p.device
+        s["step"] = torch.zeros((), dtype=torch.int64, device=dev) if group["capturable"] else 0
+        if group["state"] == "8bit":
+            n, blocks = p.numel(), -(-p.numel() // BLOCK)
+            for name, size in (("exp_avg", n), ("exp_avg_sq", n), ("m_scale", blocks),
+                               ("v_scale", blocks)):
+                s[name] = torch.zeros(size, dtype=torch.uint8, device=dev)
+        else:
+            s["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
+            s["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
+        if group["master"] and p.dtype != torch.float32:
+            s["master"] = p.detach().to(torch.float32, copy=True)
+        return s
+
+    @torch.no_grad()
+    def step(self, closure=None, *, grad_scale: float = 1.0):
+        """One step over the parameters that have gradients; grad_scale multiplies these
+        (the inverse of a loss scale)."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        buckets = {}
+        for gi, group in enumerate(self.param_groups):
+            for p in group["params"]:
+                if p.grad is not None:
+                    buckets.setdefault((gi, p.device, p.dtype, p.grad.dtype), []).append(p)
+        norm = None
+        if self.max_norm is not None and len(buckets) > 1:
+            norms = [grad_norm([p.grad for p in ps], grad_scale=grad_scale)
+                     for ps in buckets.values()]
+            norm = torch.linalg.vector_norm(torch.stack([n.to(norms[0].device) for n in norms]))
+        for k, ((gi, dev, dt, _), ps) in enumerate(buckets.items()):
+            group = self.param_groups[gi]
+            states = [self._init_state(p, group) for p in ps]
+            if group["capturable"]:
+                steps = [s["step"] for s in states]
+            else:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("AdamW: a captured step needs capturable=True")
+                steps = [s["step"] + 1 for s in states]
+            bits8 = group["state"] == "8bit"
+            lists = {n: [s[n] for s in states]
+                     for n in (("m_scale", "v_scale") if bits8 else ())}
+            got = adamw_step(
+                ps, [p.grad for p in ps], [s["exp_avg"] for s in states],
+                [s["exp_avg_sq"] for s in states], steps, lr=group["lr"], betas=group["betas"],
+                eps=group["eps"], weight_decay=group["weight_decay"],
+                m_scales=lists.get("m_scale"), v_scales=lists.get("v_scale"),
+                masters=[s["master"] for s in states] if "master" in states[0] else None,
+                grad_scale=grad_scale, max_norm=self.max_norm,
+                norm=None if norm is None else norm.to(dev), seed=self.seed + k)
+            if not group["capturable"]:
+                for s, n in zip(states, steps):
+                    s["step"] = n
+            if norm is None:
+                self.norm = got
+        if norm is not None:
+            self.norm = norm
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """As torch's, with every part of the state in the type that it was saved in."""
+        super().load_state_dict(state_dict)
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(ids, params):
+            saved = state_dict["state"].get(i)
+            if saved is not None:
+                self.state[p] = {n: t.detach().to(p.device, copy=True)
+                                 if isinstance(t, torch.Tensor) else t for n, t in saved.items()}

@@ -640,6 +640,109 @@ int cpt_distill_topk(int dtype, const void* logits, int64_t rows, int64_t vocab,
 int cpt_scale_rows(int dtype, void* x, int64_t rows, int64_t cols, const void* factor,
                    int per_row, void* stream);
 
+/* Norms of queries' and keys' heads and their position rotation (qk_rope.hip has
+ * the formulas).  q [batch, seq, heads_q, d] and k [batch, seq, heads_k, d], their
+ * columns contiguous, sequences, tokens and heads any number of elements apart;
+ * outputs likewise, and may be the inputs.  The first `rotary` columns turn, by
+ * pairs of neighbours (interleaved) or of halves; d even, at most 1024.  w_q, w_k
+ * [d] of weight_dtype (dtype or fp32): both norms, or NULL: none.  positions:
+ * int64 (pos_wide = 1) or int32, pos_batch elements between sequences, or NULL:
+ * 0 .. seq - 1.  inv_freq fp32 [rotary / 2]; cos and sin are multiplied by
+ * `scaling`.  inverse: turns back (the gradient where there are no norms). */
+int cpt_qk_rope(int dtype, int weight_dtype, int interleaved, int inverse, const void* q,
+                int64_t q_batch, int64_t q_token, int64_t q_head, const void* k, int64_t k_batch,
+                int64_t k_token, int64_t k_head, const void* w_q, const void* w_k,
+                const void* positions, int pos_wide, int64_t pos_batch, const void* inv_freq,
+                int64_t batch, int64_t seq, int64_t heads_q, int64_t heads_k, int64_t d,
+                int64_t rotary, float eps, float scaling, void* q_out, int64_t qo_batch,
+                int64_t qo_token, int64_t qo_head, void* k_out, int64_t ko_batch, int64_t ko_token,
+                int64_t ko_head, void* stream);
+
+/* Its gradient with norms, from those of the outputs and the forward's q and k:
+ * q_grad, k_grad contiguous, dw_q, dw_k [d] of the weights' type.  There has to be
+ * a token and a head of each.  workspace:
+ * cpt_qk_rope_backward_workspace_bytes(...) bytes of fp32 partial sums. */
+int64_t cpt_qk_rope_backward_workspace_bytes(int64_t tokens, int64_t heads_q, int64_t heads_k,
+                                             int64_t d);
+int cpt_qk_rope_backward(int dtype, int weight_dtype, int interleaved, const void* d_q,
+                         int64_t dq_batch, int64_t dq_token, int64_t dq_head, const void* d_k,
+                         int64_t dk_batch, int64_t dk_token, int64_t dk_head, const void* q,
+                         int64_t q_batch, int64_t q_token, int64_t q_head, const void* k,
+                         int64_t k_batch, int64_t k_token, int64_t k_head, const void* w_q,
+                         const void* w_k, const void* positions, int pos_wide, int64_t pos_batch,
+                         const void* inv_freq, int64_t batch, int64_t seq, int64_t heads_q,
+                         int64_t heads_k, int64_t d, int64_t rotary, float eps, float scaling,
+                         void* q_grad, void* k_grad, void* dw_q, void* dw_k, void* workspace,
+                         void* stream);
+
+/* Log probabilities of given tokens (logprobs.hip has the formulas) over logits of
+ * `rows` rows of `vocab` columns; row i starts at (i / seq) * ld_batch + (i % seq) *
+ * ld_row elements.  targets [rows] int64 (target_wide = 1) or int32, or NULL (then
+ * logprobs is NULL too).  Rows whose target is ignore_index or outside [0, vocab)
+ * are left out: zeros, and alternatives of -inf at column -1.  logprobs, entropy,
+ * lse fp32 [rows]; stats fp32 [2, rows] or NULL: the row's maximum and the log of
+ * its sum of e^((x - max) / T).  k <= 128: top_logprobs fp32 and top_indices int64
+ * [rows, k].  A row of -inf alone has entropy 0 and log probabilities of -inf; NaN
+ * or +inf make a row NaN. */
+int cpt_token_logprobs(int dtype, const void* logits, int64_t rows, int64_t vocab, int64_t seq,
+                       int64_t ld_batch, int64_t ld_row, int target_wide, const void* targets,
+                       int64_t ignore_index, float temperature, int64_t k, void* logprobs,
+                       void* entropy, void* lse, void* stats, void* top_logprobs,
+                       void* top_indices, void* stream);
+
+/* The logits' gradient from those of logprobs (d_logprobs fp32 [rows] or NULL) and
+ * of entropy (d_entropy, or NULL), given lse or stats, and entropy, of the forward.
+ * grad may be the logits themselves.  A row of -inf alone has a zero gradient. */
+int cpt_token_logprobs_backward(int dtype, const void* logits, int64_t rows, int64_t vocab,
+                                int64_t seq, int64_t ld_batch, int64_t ld_row, int target_wide,
+                                const void* targets, int64_t ignore_index, float temperature,
+                                const void* lse, const void* stats, const void* entropy,
+                                const void* d_logprobs, const void* d_entropy, void* grad,
+                                int64_t gld_batch, int64_t gld_row, void* stream);
+
+/* One tensor of an AdamW step: n elements each of parameters p, gradients g and
+ * moments m, v.  8-bit moments: codes, and a scale byte for each 128 elements in
+ * m_scale and v_scale (adamw.hip has the format).  master: fp32 parameters, or
+ * NULL.  step_device: int64, steps done before this one, or NULL: `step` is this
+ * step's number, from 1. */
+typedef struct {
+  void* p;
+  const void* g;
+  void* m;
+  void* v;
+  void* m_scale;
+  void* v_scale;
+  void* master;
+  void* step_device;
+  int64_t n;
+  int64_t step;
+} cpt_adamw_tensor;
+
+/* An AdamW step over `count` tensors of one type (dtype; gradients grad_dtype: dtype
+ * or fp32), in place (adamw.hip has the formulas).  `tensors` is host memory, read
+ * before the call returns.  Moments are fp32, or with bits8 in 8 bits, rounded at
+ * random by `seed`; with has_master the fp32 parameters are stepped and p is their
+ * rounding.  Gradients are multiplied by grad_scale and, with max_norm > 0, clipped
+ * to that global norm, which is written to `norm` (fp32 [1]) or, with norm_given,
+ * read there; a norm that is not finite leaves everything as it was.  step_device is given for all tensors or none:
+ * such counts are increased by one.  lr_device: fp32 [1] in lr's place, or NULL.
+ * workspace, for clipping or counts on the device, 16-byte aligned:
+ * cpt_adamw_workspace_bytes(count, elements of all tensors) bytes. */
+int64_t cpt_adamw_workspace_bytes(int64_t count, int64_t elements);
+int cpt_adamw(int dtype, int grad_dtype, int bits8, int has_master, const cpt_adamw_tensor* tensors,
+              int64_t count, double lr, const void* lr_device, double beta1, double beta2,
+              double eps, double weight_decay, double grad_scale, double max_norm, int norm_given,
+              int64_t seed, void* norm, void* workspace, void* stream);
+
+/* norm (fp32 [1]): the root of the sum of squares of grad_scale * g over all
+ * tensors' g; the sum is held in 64 bits.  workspace as cpt_adamw's. */
+int cpt_grad_norm(int grad_dtype, const cpt_adamw_tensor* tensors, int64_t count, float grad_scale,
+                  void* norm, void* workspace, void* stream);
+
+/* What 8-bit moments m, v (with their scales) stand for, as bf16, which holds them
+ * exactly: m's written to `p`, v's to `master`. */
+int cpt_adamw_8bit_values(const cpt_adamw_tensor* tensors, int64_t count, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
