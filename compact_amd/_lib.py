@@ -16,6 +16,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_build", "libcompact_amd.so")
 CAPI_PATH = os.path.join(_HERE, "_build", "_capi.so")
+LISTS_PATH = os.path.join(_HERE, "_build", "_lists.so")
 
 F32, F16, BF16 = 0, 1, 2
 
@@ -172,24 +173,39 @@ def lib():
     return _lib
 
 
+def _extension(name, path):
+    """A CPython extension built with the library.  Raises as lib()."""
+    lib()
+    if not os.path.exists(path):
+        raise LibraryMissing(f"{path} not found: build it with `python -m compact_amd.build`")
+    loader = importlib.machinery.ExtensionFileLoader(name, path)
+    spec = importlib.util.spec_from_file_location(name, path, loader=loader)
+    mod = importlib.util.module_from_spec(spec)
+    loader.exec_module(mod)
+    return mod
+
+
 _api = None
+_lists = None
 
 
 def api():
-    """The same entry points through the CPython binding (_build/_capi.so, built
-    with the library): what every step calls.  Loaded once; raises as lib()."""
+    """The same entry points through the CPython binding (_build/_capi.so): what every
+    step calls.  Loaded once; raises as lib()."""
     global _api
     if _api is None:
-        lib()
-        if not os.path.exists(CAPI_PATH):
-            raise LibraryMissing(f"{CAPI_PATH} not found: build it with "
-                                 "`python -m compact_amd.build`")
-        loader = importlib.machinery.ExtensionFileLoader("_capi", CAPI_PATH)
-        spec = importlib.util.spec_from_file_location("_capi", CAPI_PATH, loader=loader)
-        mod = importlib.util.module_from_spec(spec)
-        loader.exec_module(mod)
-        _api = mod
+        _api = _extension("_capi", CAPI_PATH)
     return _api
+
+
+def lists():
+    """The helper that turns lists of tensors into the C ABI's tables
+    (_build/_lists.so).  Loaded once; raises as lib()."""
+    global _lists
+    if _lists is None:
+        import torch  # noqa: F401  (its libraries come first)
+        _lists = _extension("_lists", LISTS_PATH)
+    return _lists
 
 
 # status codes (include/compact_amd.h)

@@ -24,6 +24,7 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_build")
 LIB = os.path.join(OUT_DIR, "libcompact_amd.so")
 CAPI = os.path.join(OUT_DIR, "_capi.so")
+LISTS = os.path.join(OUT_DIR, "_lists.so")
 ARCH = os.environ.get("CPT_OFFLOAD_ARCH", "gfx950")
 
 COMMON = [
@@ -67,11 +68,32 @@ def _build_capi() -> None:
     os.replace(tmp, CAPI)
 
 
+def _build_lists() -> None:
+    """The helper for lists of tensors (csrc/tensor_lists.cpp), on torch's C++ API."""
+    import torch
+    from torch.utils import cpp_extension
+    tmp = LISTS + ".tmp"
+    # headers of no accelerator: the file has no device code
+    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-I{sysconfig.get_paths()['include']}", f"-I{os.path.join(ROOT, 'include')}",
+           *(f"-I{p}" for p in cpp_extension.include_paths()),
+           os.path.join(CSRC, "tensor_lists.cpp"), "-o", tmp,
+           *(f"-L{p}" for p in cpp_extension.library_paths()), "-ltorch_python", "-ltorch_cpu",
+           "-ltorch", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"list helper failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, LISTS)
+
+
 def build(verbose: bool = False) -> str:
     os.makedirs(OUT_DIR, exist_ok=True)
     srcs = sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hip"))
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+        lists = ex.submit(_build_lists)
         objs = list(ex.map(_compile, srcs))
+        lists.result()
     tmp = LIB + ".tmp"
     cmd = [hipcc(), "-shared", "-fPIC", f"--offload-arch={ARCH}", "-Wl,-soname,libcompact_amd.so",
            "-o", tmp] + objs

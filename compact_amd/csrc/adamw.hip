@@ -21,7 +21,7 @@
 //
 // Bound: HBM, 22 bytes an element with 16-bit parameters and gradients and fp32
 // moments, 28 with an fp32 copy of the parameters, 10 with 8-bit moments.  The
-// tensors' pointers are kernel arguments, 48 a launch: no table to upload or keep.
+// tensors' pointers are kernel arguments, up to 80 a launch: no table to upload or keep.
 
 #include <algorithm>
 #include <cmath>
@@ -33,44 +33,60 @@ namespace cpt {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kStepTensors = 48;      // 80 bytes each in 4 KB of kernel arguments
-constexpr int kChunk = 8192;          // elements a block of the step, a multiple of 128
+constexpr int kArgBytes = 4096;       // of a kernel
+constexpr int kPass = kThreads * 8;   // elements a block has in registers at a time
 constexpr int kBlockLog = 7;          // 128 elements share a scale
 constexpr int kScaleBias = 134;
-constexpr int kNormBlocks = 2048;     // blocks that the squares' sum is cut into, about
 
-struct Tensor {
-  void* p;
-  const void* g;
-  void* m;
-  void* v;
-  uint8_t* ms;
-  uint8_t* vs;
-  float* master;
-  int64_t n;
-  int first;            // first block of this tensor
-  uint32_t key;         // the dither's
-  float inv1, inv2;     // 1 / (1 - b^t)
-};
-
-// What a step on the device decides: one float4 for all tensors {clip, skip}, then
-// {inv1, inv2, key} a tensor where the step counts are on the device.
+// Whether a step clips and goes ahead, decided on the device.
 struct Control {
   float clip;
   int skip;
 };
+// A tensor's bias corrections 1 / (1 - b^t) and its dither's key, likewise.
 struct DeviceStep {
   float inv1, inv2;
   uint32_t key;
 };
 
-struct StepArgs {
-  Tensor t[kStepTensors];
+// A tensor of a launch; what a kind of step has none of takes no room, so that one
+// launch has as many tensors as fit (84 with fp32 moments alone).
+template <bool BITS8>
+struct ScaleAddress {};
+template <>
+struct ScaleAddress<true> {
+  uint8_t* ms;
+  uint8_t* vs;
+};
+template <bool MASTER>
+struct MasterAddress {};
+template <>
+struct MasterAddress<true> {
+  float* master;
+};
+template <bool BITS8, bool MASTER>
+struct Tensor : ScaleAddress<BITS8>, MasterAddress<MASTER> {
+  void* p;
+  const void* g;
+  void* m;
+  void* v;
+  int64_t n;
+};
+struct StepCommon {
   const Control* control;         // null: no clipping
-  const DeviceStep* device_step;  // null: the tensors' own
+  const DeviceStep* device_step;  // null: inv1, inv2, and keys of seed and step
   const float* lr_device;         // null: lr
-  int count;
-  float lr, wd, b1, b2, c1, c2, eps, grad_scale;   // c = 1 - b
+  int64_t chunk;                  // elements a block, a multiple of 2048
+  int count, base;                // tensors, and the first one's place in the call
+  uint32_t seed, step;
+  float lr, wd, b1, b2, c1, c2, eps, grad_scale, inv1, inv2;   // c = 1 - b
+};
+template <bool BITS8, bool MASTER>
+struct StepArgs : StepCommon {
+  static constexpr int kTensors =
+      (kArgBytes - (int)sizeof(StepCommon) - 16) / ((int)sizeof(Tensor<BITS8, MASTER>) + 4);
+  int first[kTensors];            // first block
+  Tensor<BITS8, MASTER> t[kTensors];
 };
 
 __host__ __device__ __forceinline__ uint32_t mix(uint32_t h) {
@@ -85,11 +101,13 @@ __host__ __device__ __forceinline__ uint32_t tensor_key(uint32_t seed, uint32_t 
 }
 
 // The tensor that a block works on: the last whose first block is not past it.
-template <class Args>
-__device__ __forceinline__ int find_tensor(const Args& A, int block) {
-  const int lane = threadIdx.x & 63;
-  const int first = lane < A.count ? A.t[lane].first : 0x7FFFFFFF;
-  return __builtin_amdgcn_readfirstlane(__popcll(__ballot(first <= block)) - 1);
+__device__ __forceinline__ int find_tensor(const int* first, int count, int block) {
+  int n = 0;
+  for (int i = 0; i < count; i += 64) {
+    const int at = i + (threadIdx.x & 63);
+    n += __popcll(__ballot(at < count && first[min(at, count - 1)] <= block));
+  }
+  return __builtin_amdgcn_readfirstlane(n - 1);
 }
 
 __device__ __forceinline__ float mul(float a, float b) { return __fmul_rn(a, b); }
@@ -157,19 +175,28 @@ __device__ __forceinline__ int block_scale(uint32_t bits, int top) {
   return max((int)(bits >> 23) - 127 - top, 1 - kScaleBias);
 }
 
+// m / (sqrt(v) + eps).  Beside moments of three bits the hardware's root and reciprocal,
+// good to one unit in the last place (and a root of a denormal to nothing) are exact
+// enough; the IEEE ones are 25 instructions of about 80 an element there.
+template <bool BITS8>
+__device__ __forceinline__ float quotient(float m, float v, float eps) {
+  if (!BITS8 || eps < 1e-18f) return m / (sqrtf(v) + eps);
+  return m * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) + eps);
+}
+
 // PD: the parameters' type, GD: the gradients', BITS8: moments in 8 bits, MASTER: an
 // fp32 copy of the parameters that is stepped in their place.
 template <int PD, int GD, bool BITS8, bool MASTER>
-__global__ __launch_bounds__(kThreads) void adamw_kernel(const StepArgs A) {
-  const int ti = find_tensor(A, blockIdx.x);
-  const Tensor& T = A.t[ti];
+__global__ __launch_bounds__(kThreads) void adamw_kernel(const StepArgs<BITS8, MASTER> A) {
+  const int ti = find_tensor(A.first, A.count, blockIdx.x);
+  const auto& T = A.t[ti];
   float clip = 1.f;
   if (A.control) {
     if (A.control->skip) return;
     clip = A.control->clip;
   }
-  float inv1 = T.inv1, inv2 = T.inv2;
-  uint32_t key = T.key;
+  float inv1 = A.inv1, inv2 = A.inv2;
+  uint32_t key = tensor_key(A.seed, A.step, A.base + ti);
   if (A.device_step) {
     inv1 = A.device_step[ti].inv1;
     inv2 = A.device_step[ti].inv2;
@@ -177,12 +204,12 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const StepArgs A) {
   }
   const float lr = A.lr_device ? *A.lr_device : A.lr;
   const float step = lr * inv1, decay = -lr * A.wd;
-  const int64_t start = (int64_t)(blockIdx.x - T.first) * kChunk;
+  const int64_t start = (int64_t)(blockIdx.x - A.first[ti]) * A.chunk;
   const int64_t n = T.n;
-  int64_t end = min(start + kChunk, n);
+  int64_t end = min(start + A.chunk, n);
   // the 16 lanes of a block of moments stay together: each takes part in its maximum
   if (BITS8) end = (end + 127) & ~(int64_t)127;
-  for (int64_t i = start + threadIdx.x * 8; i < end; i += kThreads * 8) {
+  for (int64_t i = start + threadIdx.x * 8; i < end; i += kPass) {
     const auto rg = ld8<GD>(T.g, i, n);
     typename Row8<MASTER ? kF32 : PD>::Raw rp;
     if constexpr (MASTER)
@@ -214,8 +241,7 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const StepArgs A) {
       const float x = mul(mul(g[j], A.grad_scale), clip);
       m[j] = add(mul(A.b1, m[j]), mul(A.c1, x));
       v[j] = add(mul(A.b2, v[j]), mul(A.c2, mul(x, x)));
-      const float den = sqrtf(v[j] * inv2) + A.eps;
-      p[j] = fmaf(decay, p[j], p[j]) - step * m[j] / den;
+      p[j] = fmaf(decay, p[j], p[j]) - step * quotient<BITS8>(m[j], v[j] * inv2, A.eps);
     }
     if constexpr (BITS8) {
       // what lies past the tensor's end is zero and stays so
@@ -262,35 +288,58 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const StepArgs A) {
 struct NormTensor {
   const void* g;
   int64_t n;
-  int first;
 };
-constexpr int kNormTensors = 64;      // a lane each in find_tensor
 struct NormArgs {
-  NormTensor t[kNormTensors];
-  int count;
-  int64_t chunk;
-  float grad_scale;
+  static constexpr int kTensors = (kArgBytes - 48) / 20;
+  int64_t chunk;        // elements a block, a multiple of 2048
   double* partial;      // one a block
+  int count;
+  float grad_scale;
+  int first[kTensors];
+  NormTensor t[kTensors];
 };
 
-// Squares are summed in 64 bits: no gradient's square is out of range, and the order
-// of the sum does not show.
+// Eight squares' sum in fp32, the sums in 64 bits: their order does not show.  Squares
+// near the ends of fp32's range (a gradient past 2e19, all under 1e-15) in 64 bits too.
+__device__ __forceinline__ double squares(const float g[8], float scale) {
+  float x[8], s = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    x[j] = mul(g[j], scale);
+    s = fmaf(x[j], x[j], s);
+  }
+  if (s >= 1e-30f && s < INFINITY) return s;
+  double d = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) d = fma((double)x[j], (double)x[j], d);
+  return d;
+}
+
 template <int GD>
 __global__ __launch_bounds__(kThreads) void grad_squares(const NormArgs A) {
   __shared__ double part[kThreads / 64];
-  const NormTensor& T = A.t[find_tensor(A, blockIdx.x)];
-  const int64_t start = (blockIdx.x - T.first) * A.chunk, end = min(start + A.chunk, T.n);
-  double s[2] = {0, 0};
-  for (int64_t i = start + threadIdx.x * 8; i < end; i += kThreads * 8) {
-    float g[8];
-    Row8<GD>::unpack(ld8<GD>(T.g, i, T.n), g);
+  const int ti = find_tensor(A.first, A.count, blockIdx.x);
+  const NormTensor& T = A.t[ti];
+  const int64_t start = (blockIdx.x - A.first[ti]) * A.chunk, end = min(start + A.chunk, T.n);
+  double sum = 0;
+  int64_t i = start + threadIdx.x * 8;
+  for (; i + 3 * kPass + 8 <= end; i += 4 * kPass) {
+    typename Row8<GD>::Raw r[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const double x = mul(g[j], A.grad_scale);
-      s[j & 1] += x * x;
+    for (int u = 0; u < 4; ++u)
+      r[u] = Row8<GD>::ld((const typename Row8<GD>::T*)T.g + i + u * kPass);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float g[8];
+      Row8<GD>::unpack(r[u], g);
+      sum += squares(g, A.grad_scale);
     }
   }
-  double sum = s[0] + s[1];
+  for (; i < end; i += kPass) {
+    float g[8];
+    Row8<GD>::unpack(ld8<GD>(T.g, i, T.n), g);
+    sum += squares(g, A.grad_scale);
+  }
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
   __syncthreads();
@@ -327,15 +376,16 @@ __global__ __launch_bounds__(1024) void norm_kernel(const double* partial, int n
 // step counts on the device
 // ---------------------------------------------------------------------------
 
+constexpr int kCounts = 256;
 struct CountArgs {
-  int64_t* step[kStepTensors];
+  int64_t* step[kCounts];
   const Control* control;
   DeviceStep* out;
   int count, base;
   uint32_t seed;
   double b1, b2;
 };
-__global__ __launch_bounds__(64) void count_kernel(const CountArgs A) {
+__global__ __launch_bounds__(kCounts) void count_kernel(const CountArgs A) {
   const int i = threadIdx.x;
   if (i >= A.count || (A.control && A.control->skip)) return;
   const int64_t t = *A.step[i] + 1;
@@ -357,19 +407,21 @@ struct ValueTensor {
   uint16_t* om;
   uint16_t* ov;
   int64_t n;
-  int first;
 };
-constexpr int kValueTensors = 56;
 struct ValueArgs {
-  ValueTensor t[kValueTensors];
+  static constexpr int kTensors = (kArgBytes - 24) / 60;
+  int64_t chunk;
   int count;
+  int first[kTensors];
+  ValueTensor t[kTensors];
 };
 // Every value is a bf16 number: four bits times a power of two.
 __global__ __launch_bounds__(kThreads) void values_kernel(const ValueArgs A) {
-  const ValueTensor& T = A.t[find_tensor(A, blockIdx.x)];
-  const int64_t start = (int64_t)(blockIdx.x - T.first) * kChunk;
-  const int64_t n = T.n, end = min(start + kChunk, n);
-  for (int64_t i = start + threadIdx.x * 8; i < end; i += kThreads * 8) {
+  const int ti = find_tensor(A.first, A.count, blockIdx.x);
+  const ValueTensor& T = A.t[ti];
+  const int64_t start = (blockIdx.x - A.first[ti]) * A.chunk;
+  const int64_t n = T.n, end = min(start + A.chunk, n);
+  for (int64_t i = start + threadIdx.x * 8; i < end; i += kPass) {
     uint32_t cm[2], cv[2];
     ld_codes(T.m, i, n, cm);
     ld_codes(T.v, i, n, cv);
@@ -388,28 +440,34 @@ __global__ __launch_bounds__(kThreads) void values_kernel(const ValueArgs A) {
 int ok() { return hipGetLastError() == hipSuccess ? kOk : kErrLaunch; }
 int64_t chunks(int64_t n, int64_t c) { return (n + c - 1) / c; }
 
-// Elements a block of the norm's first launch: all gradients in about kNormBlocks.
-int64_t norm_chunk(int64_t total) {
-  return std::max<int64_t>(kThreads * 8, (total / kNormBlocks + 2047) / 2048 * 2048);
+// Elements a block, so that all of a call's are about `blocks` blocks: a multiple of a
+// pass, `most` passes at most.
+int64_t chunk_for(int64_t total, int64_t blocks, int64_t most) {
+  return std::min(std::max<int64_t>(total / blocks / kPass, 1), most) * kPass;
 }
+// The step's: a pass while that is under eight blocks a CU (230 k elements: 3.9 us, 7.9
+// in blocks of four passes), four passes of large calls.
+int64_t step_chunk(int64_t total) { return chunk_for(total, 2048, 4); }
+// The norm's, four passes together: its blocks' sums are added by one block.
+int64_t norm_chunk(int64_t total) { return 4 * chunk_for(total, 8192, 1 << 30); }
 
 struct Sizes {
-  int64_t total = 0, live = 0;
+  int64_t total = 0;
 };
 int tensor_sizes(const cpt_adamw_tensor* t, int64_t count, Sizes* s) {
   for (int64_t i = 0; i < count; ++i) {
     if (t[i].n < 0) return kErrShape;
     if (t[i].n > 1ll << 40) return kErrTooLarge;
     s->total += t[i].n;
-    s->live += t[i].n > 0;
   }
   return s->total > 1ll << 42 ? kErrTooLarge : kOk;
 }
 
-// Workspace: {Control, 16 bytes}, a DeviceStep a tensor of a launch's, partial sums.
+// Workspace: a Control, a DeviceStep a tensor, partial sums.
+constexpr int64_t kControlBytes = 16;
+int64_t step_bytes(int64_t count) { return (count * (int64_t)sizeof(DeviceStep) + 15) / 16 * 16; }
 int64_t workspace_bytes(int64_t count, int64_t total) {
-  const int64_t steps = (count + kStepTensors) * 16;
-  return 16 + steps + 8 * (count + chunks(total, norm_chunk(total)) + 1);
+  return kControlBytes + step_bytes(count) + 8 * (count + chunks(total, norm_chunk(total)) + 1);
 }
 
 template <int GD>
@@ -421,9 +479,10 @@ int launch_squares(const cpt_adamw_tensor* t, int64_t count, int64_t chunk, floa
     A.count = 0;
     A.chunk = chunk, A.grad_scale = grad_scale, A.partial = partial + done;
     int64_t grid = 0;
-    for (; i < count && A.count < kNormTensors; ++i) {
+    for (; i < count && A.count < NormArgs::kTensors; ++i) {
       if (t[i].n == 0) continue;
-      A.t[A.count++] = NormTensor{t[i].g, t[i].n, (int)grid};
+      A.first[A.count] = (int)grid;
+      A.t[A.count++] = NormTensor{t[i].g, t[i].n};
       grid += chunks(t[i].n, chunk);
     }
     if (A.count == 0) break;
@@ -448,19 +507,49 @@ int grad_norm(int gd, const cpt_adamw_tensor* t, int64_t count, int64_t total, f
   return ok();
 }
 
-template <int PD, int GD>
-void launch_step(const StepArgs& A, int64_t grid, bool bits8, bool master, hipStream_t st) {
-  const unsigned b = (unsigned)grid;
-  if (bits8) {
-    if (master && PD != kF32)
-      adamw_kernel<PD, GD, true, PD != kF32><<<b, kThreads, 0, st>>>(A);
-    else
-      adamw_kernel<PD, GD, true, false><<<b, kThreads, 0, st>>>(A);
-  } else if (master && PD != kF32) {
-    adamw_kernel<PD, GD, false, PD != kF32><<<b, kThreads, 0, st>>>(A);
-  } else {
-    adamw_kernel<PD, GD, false, false><<<b, kThreads, 0, st>>>(A);
+// All launches of a step of one kind, a run of tensors with one step number each.
+template <int PD, int GD, bool BITS8, bool MASTER>
+int launch_step(StepCommon C, const cpt_adamw_tensor* t, int64_t count, double beta1, double beta2,
+                hipStream_t st) {
+  using Args = StepArgs<BITS8, MASTER>;
+  static_assert(sizeof(Args) <= kArgBytes);
+  const DeviceStep* steps = C.device_step;
+  for (int64_t i = 0; i < count;) {
+    Args A;
+    static_cast<StepCommon&>(A) = C;
+    A.count = 0;
+    A.base = (int)i;
+    A.device_step = steps ? steps + i : nullptr;
+    if (!steps) {
+      A.step = (uint32_t)t[i].step;
+      A.inv1 = (float)(1.0 / (1.0 - std::pow(beta1, (double)t[i].step)));
+      A.inv2 = (float)(1.0 / (1.0 - std::pow(beta2, (double)t[i].step)));
+    }
+    int64_t grid = 0;
+    // an empty tensor keeps its place (keys and device steps go by it) and has no block
+    for (const int64_t step = t[i].step; i < count && A.count < Args::kTensors; ++i) {
+      if (!steps && t[i].step != step) break;
+      auto& T = A.t[A.count];
+      A.first[A.count++] = (int)grid;
+      T.p = t[i].p, T.g = t[i].g, T.m = t[i].m, T.v = t[i].v, T.n = t[i].n;
+      if constexpr (BITS8) T.ms = (uint8_t*)t[i].m_scale, T.vs = (uint8_t*)t[i].v_scale;
+      if constexpr (MASTER) T.master = (float*)t[i].master;
+      grid += chunks(t[i].n, C.chunk);
+    }
+    if (grid == 0) continue;
+    adamw_kernel<PD, GD, BITS8, MASTER><<<(unsigned)grid, kThreads, 0, st>>>(A);
+    if (ok()) return kErrLaunch;
   }
+  return kOk;
+}
+template <int PD, int GD>
+int launch_kind(const StepCommon& C, const cpt_adamw_tensor* t, int64_t count, double beta1,
+                double beta2, bool bits8, bool master, hipStream_t st) {
+  if (PD != kF32 && master)
+    return bits8 ? launch_step<PD, GD, true, PD != kF32>(C, t, count, beta1, beta2, st)
+                 : launch_step<PD, GD, false, PD != kF32>(C, t, count, beta1, beta2, st);
+  return bits8 ? launch_step<PD, GD, true, false>(C, t, count, beta1, beta2, st)
+               : launch_step<PD, GD, false, false>(C, t, count, beta1, beta2, st);
 }
 
 }  // namespace
@@ -514,7 +603,7 @@ int cpt_adamw(int dtype, int grad_dtype, int bits8, int has_master, const cpt_ad
   DeviceStep* steps = nullptr;
   if (clip) {
     control = (Control*)workspace;
-    double* partial = (double*)((char*)workspace + 16 + (count + kStepTensors) * 16);
+    double* partial = (double*)((char*)workspace + kControlBytes + step_bytes(count));
     if (norm_given) {
       decide_kernel<<<1, 1, 0, st>>>((const float*)norm, (float)max_norm, control);
       if (ok()) return kErrLaunch;
@@ -523,56 +612,30 @@ int cpt_adamw(int dtype, int grad_dtype, int bits8, int has_master, const cpt_ad
       return rc;
     }
   }
-  if (on_device) steps = (DeviceStep*)((char*)workspace + 16);
-  StepArgs A;
-  A.control = control;
-  A.lr_device = (const float*)lr_device;
-  A.lr = (float)lr, A.wd = (float)weight_decay;
-  A.b1 = (float)beta1, A.b2 = (float)beta2;
-  A.c1 = (float)(1 - beta1), A.c2 = (float)(1 - beta2);
-  A.eps = (float)eps, A.grad_scale = (float)grad_scale;
-  int64_t last_step = 0;
-  float inv1 = 0, inv2 = 0;
-  for (int64_t i = 0; i < count;) {
-    CountArgs C;
-    A.count = 0;
-    A.device_step = steps;
-    C.base = (int)i;
-    int64_t grid = 0;
-    for (int k = 0; i < count && k < kStepTensors; ++i, ++k) {
-      const cpt_adamw_tensor& t = tensors[i];
-      C.step[k] = (int64_t*)t.step_device;
-      C.count = k + 1;
-      if (!on_device && t.step != last_step) {
-        last_step = t.step;
-        inv1 = (float)(1.0 / (1.0 - std::pow(beta1, (double)t.step)));
-        inv2 = (float)(1.0 / (1.0 - std::pow(beta2, (double)t.step)));
-      }
-      // an empty tensor keeps its place (the device's step counts go by it) and no block
-      A.t[A.count++] = Tensor{t.p, t.g, t.m, t.v, (uint8_t*)t.m_scale, (uint8_t*)t.v_scale,
-                              (float*)t.master, t.n, (int)grid,
-                              tensor_key((uint32_t)seed, (uint32_t)t.step, (uint32_t)i), inv1,
-                              inv2};
-      grid += chunks(t.n, kChunk);
-    }
-    if (on_device) {
-      C.control = control, C.out = steps, C.seed = (uint32_t)seed, C.b1 = beta1, C.b2 = beta2;
-      count_kernel<<<1, 64, 0, st>>>(C);
+  if (on_device) {
+    steps = (DeviceStep*)((char*)workspace + kControlBytes);
+    for (int64_t i = 0; i < count; i += kCounts) {
+      CountArgs N;
+      N.count = (int)std::min<int64_t>(count - i, kCounts);
+      for (int k = 0; k < N.count; ++k) N.step[k] = (int64_t*)tensors[i + k].step_device;
+      N.control = control, N.out = steps + i, N.base = (int)i, N.seed = (uint32_t)seed;
+      N.b1 = beta1, N.b2 = beta2;
+      count_kernel<<<1, kCounts, 0, st>>>(N);
       if (ok()) return kErrLaunch;
-      steps += C.count;
     }
-    if (grid == 0) continue;
-#define CPT_STEP(PD, GD) launch_step<PD, GD>(A, grid, bits8, has_master, st)
-    if (dtype == kF32)
-      CPT_STEP(kF32, kF32);
-    else if (dtype == kF16)
-      grad_dtype == kF32 ? CPT_STEP(kF16, kF32) : CPT_STEP(kF16, kF16);
-    else
-      grad_dtype == kF32 ? CPT_STEP(kBF16, kF32) : CPT_STEP(kBF16, kBF16);
-#undef CPT_STEP
-    if (ok()) return kErrLaunch;
   }
-  return kOk;
+  StepCommon C{};
+  C.control = control, C.device_step = steps, C.lr_device = (const float*)lr_device;
+  C.chunk = step_chunk(s.total), C.seed = (uint32_t)seed;
+  C.lr = (float)lr, C.wd = (float)weight_decay, C.b1 = (float)beta1, C.b2 = (float)beta2;
+  C.c1 = (float)(1 - beta1), C.c2 = (float)(1 - beta2);
+  C.eps = (float)eps, C.grad_scale = (float)grad_scale;
+#define CPT_STEP(PD, GD) \
+  launch_kind<PD, GD>(C, tensors, count, beta1, beta2, bits8, has_master, st)
+  if (dtype == kF32) return CPT_STEP(kF32, kF32);
+  if (dtype == kF16) return grad_dtype == kF32 ? CPT_STEP(kF16, kF32) : CPT_STEP(kF16, kF16);
+  return grad_dtype == kF32 ? CPT_STEP(kBF16, kF32) : CPT_STEP(kBF16, kBF16);
+#undef CPT_STEP
 }
 
 int cpt_adamw_8bit_values(const cpt_adamw_tensor* tensors, int64_t count, void* stream) {
@@ -581,18 +644,20 @@ int cpt_adamw_8bit_values(const cpt_adamw_tensor* tensors, int64_t count, void* 
   if (const int rc = tensor_sizes(tensors, count, &s)) return rc;
   for (int64_t i = 0; i < count; ++i) {
     const cpt_adamw_tensor& t = tensors[i];
-    if (t.n && (!t.p || !t.master || !t.m || !t.v || !t.m_scale || !t.v_scale)) return kErrShape;
+    if (t.n && (!t.p || !t.g || !t.m || !t.v || !t.m_scale || !t.v_scale)) return kErrShape;
   }
   for (int64_t i = 0; i < count;) {
     ValueArgs A;
     A.count = 0;
+    A.chunk = step_chunk(s.total);
     int64_t grid = 0;
-    for (; i < count && A.count < kValueTensors; ++i) {
+    for (; i < count && A.count < ValueArgs::kTensors; ++i) {
       const cpt_adamw_tensor& t = tensors[i];
       if (t.n == 0) continue;
+      A.first[A.count] = (int)grid;
       A.t[A.count++] = ValueTensor{t.m, t.v, (const uint8_t*)t.m_scale, (const uint8_t*)t.v_scale,
-                                   (uint16_t*)t.p, (uint16_t*)t.master, t.n, (int)grid};
-      grid += chunks(t.n, kChunk);
+                                   (uint16_t*)t.p, (uint16_t*)t.g, t.n};
+      grid += chunks(t.n, A.chunk);
     }
     if (A.count == 0) break;
     values_kernel<<<(unsigned)grid, kThreads, 0, (hipStream_t)stream>>>(A);

@@ -17,7 +17,7 @@
 // looked at again, dealt out over the block.  Where a bound leaves too many (constant
 // rows, rows with little but -inf, NaN), a radix selection takes its place.
 
-#include <type_traits>
+#include <algorithm>
 
 #include "compact_amd.h"
 #include "row_ops.h"
@@ -26,7 +26,7 @@ namespace cpt {
 namespace {
 
 constexpr int kMaxTop = 128;          // alternatives
-constexpr int kMaxCand = 1024;        // candidates that are sorted
+constexpr int kSlots = 4;             // of a thread: four maxima each, of some of its vectors
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct LogArgs {
@@ -38,8 +38,9 @@ struct LogArgs {
   float* stats;
   float* top_logp;
   int64_t* top_idx;
-  int64_t rows, seq, ld_b, ld_s, ignore;
-  int v, k, wide;
+  int64_t rows, ld_b, ld_s, ignore;
+  FastDivU32 seq;
+  int v, k, wide, shift;              // 1 << shift vectors a maximum
   float inv_t;
 };
 
@@ -56,39 +57,127 @@ __device__ __forceinline__ float order_value(uint64_t key) {
   return __uint_as_float(b >> 31 ? b & 0x7FFFFFFFu : ~b);
 }
 
-// max, sum of 2^(t - max) and of 2^(t - max) (t - max) over t = x log2(e) / T, the max
-// kept as x.
+// A maximum m, and the sums of 2^(t - base) and of 2^(t - base) (t - base) over t = x c,
+// c = log2(e) / T.  base is the whole number next to m c: then t - base is one fused
+// multiply-add, and bases differ exactly.  Past 2^22 (`wide`; whole numbers end at
+// 2^24) it is m c itself, and t - base is (x - m) c.
 struct Stats {
-  float m, s, w;
+  float m, base, s, w;
+  bool wide;
 };
-__device__ __forceinline__ void rebase(Stats& a, float m, float k) {
-  if (a.m == -INFINITY) {
-    a.m = m;                  // s and w are 0 (or NaN)
-    return;
+__device__ __forceinline__ bool is_wide(float m, float c) { return !(fabsf(m * c) < 4194304.f); }
+__device__ __forceinline__ void rebase(Stats& a, float m, float c) {
+  const bool wide = is_wide(m, c);
+  const float base = wide ? 0.f : rintf(m * c);
+  float d = a.base - base;
+  if (wide || a.wide)
+    d = wide && a.wide ? (a.m - m) * c : wide ? fmaf(-c, m, a.base) : fmaf(c, a.m, -base);
+  if (a.m > -INFINITY) {        // else s and w are 0, or NaN
+    const float f = exp2f(d);
+    a.w = (a.w + fmaxf(d, -1024.f) * a.s) * f;    // far below: 0, not 0 * inf
+    a.s *= f;
   }
-  const float d = (a.m - m) * k, f = exp2f(d);
-  // far below: 0, not 0 * inf
-  a.w = (a.w + fmaxf(d, -1024.f) * a.s) * f;
-  a.s *= f;
-  a.m = m;
+  a.m = m, a.base = base, a.wide = wide;
 }
 
+// One wavefront's rows are narrow: its block is kept small, so that many run side by side.
 template <int NT>
 struct Shared {
+  static constexpr int kCand = NT == 64 ? 256 : 1024;   // candidates that are sorted
+  static constexpr int kList = NT == 64 ? 128 : 1024;   // maxima that reach the bound
   float red[3][NT / 64];
   float bound[NT / 64];
   int count, active, need;
   uint32_t prefix;
-  int hist[256];
   int scan[NT / 64];
-  uint16_t list[NT];
-  uint64_t cand[kMaxCand];
+  uint16_t list[kList];
+  union {
+    uint2 top[kSlots][NT];
+    int hist[256];
+  };
+  uint64_t cand[kCand];
 };
 
 template <int DT>
 __device__ __forceinline__ typename Row8<DT>::Raw ld_vec(const typename Row8<DT>::T* row, int vec,
                                                          int v) {
   return row_ld<DT>(row, (int64_t)vec * 8, v, Row8<DT>::kNegInf);
+}
+
+// Four vectors of a row, `step` apart, from the whole ones below `n` (past them the last
+// again).
+template <int DT>
+struct Four {
+  typename Row8<DT>::Raw raw[4];
+  __device__ __forceinline__ void ld(const typename Row8<DT>::T* row, int i, int step, int n) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      raw[u] = Row8<DT>::ld(row + (int64_t)min(i + u * step, n - 1) * 8);
+  }
+};
+
+// N vectors into a thread's statistics, and their maxima into those of the slot.  CUT: the
+// first `count` of them, the others being other threads'.
+template <int DT, int N, bool CUT>
+__device__ __forceinline__ void take(Stats& st, const typename Row8<DT>::Raw* raw, float c,
+                                     float slot[N], bool first, int count) {
+  float top = -INFINITY, low = INFINITY;
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    float x[8];
+    Row8<DT>::unpack(raw[u], x);
+    float most = x[0];
+    low = fminf(low, x[0]);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) most = fmaxf(most, x[j]), low = fminf(low, x[j]);
+    if (CUT && u >= count) most = -INFINITY;
+    slot[u] = first ? most : fmaxf(slot[u], most);
+    top = fmaxf(top, most);
+  }
+  if (top > st.m) rebase(st, top, c);
+  if (low * c > -1e38f && !st.wide) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      float x[8], s = CUT ? 0.f : st.s, w = CUT ? 0.f : st.w;
+      Row8<DT>::unpack(raw[u], x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float t = fmaf(x[j], c, -st.base);
+        const float e = __builtin_amdgcn_exp2f(t);
+        s += e;
+        w = fmaf(e, t, w);
+      }
+      st.s = !CUT ? s : u < count ? st.s + s : st.s;
+      st.w = !CUT ? w : u < count ? st.w + w : st.w;
+    }
+  } else {                      // -inf among them (0 * inf), or far from 0
+    const float m = st.m == -INFINITY ? 0.f : st.m;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      if (CUT && u >= count) break;
+      float x[8];
+      Row8<DT>::unpack(raw[u], x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float t = st.wide ? (x[j] - m) * c : fmaf(x[j], c, -st.base);
+        const float e = __builtin_amdgcn_exp2f(t);
+        st.s += e;
+        st.w = fmaf(e, fmaxf(t, -256.f), st.w);
+      }
+    }
+  }
+}
+
+// A maximum in 16 bits: the type's own, of fp32 the next bf16 number from it upwards.
+template <int DT>
+__device__ __forceinline__ uint32_t top_bits(float x) {
+  const uint32_t b = __float_as_uint(x);
+  if (DT == kF16) return f32_to_f16_bits(x);
+  return (b + (DT == kF32 && !(b >> 31) ? 0xFFFFu : 0u)) >> 16;
+}
+template <int DT>
+__device__ __forceinline__ float top_value(uint32_t b) {
+  return DT == kF16 ? f16_bits_to_f32((uint16_t)b) : __uint_as_float(b << 16);
 }
 
 // Candidates by radix selection: the k largest keys' columns into S.cand.
@@ -179,49 +268,39 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LogArgs A) {
       return;
     }
   }
-  const int64_t b = r / A.seq;
-  const auto* row = (const typename R::T*)A.x + b * A.ld_b + (r - b * A.seq) * A.ld_s;
+  const uint32_t b = A.seq.div((uint32_t)r), n = (uint32_t)r - b * A.seq.d;
+  const auto* row = (const typename R::T*)A.x + b * A.ld_b + n * A.ld_s;
   const float c = A.inv_t * kLog2e;
   const float chosen = threadIdx.x == 0 && A.targets ? Elem<DT>::ld(row + y) : 0.f;
   const int vecs = (v + 7) / 8, whole = v / 8;
 
-  // 1. maximum, sum and weighted sum of this thread's columns
-  Stats st{-INFINITY, 0.f, 0.f};
-  auto take = [&](const typename R::Raw* raw, auto count) {
-    constexpr int N = decltype(count)::value;
-    float top = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-      float x[8];
-      R::unpack(raw[u], x);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = fmaxf(top, x[j]);
-    }
-    if (top > st.m) rebase(st, top, c);
-    const float base = st.m == -INFINITY ? 0.f : st.m;
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-      float x[8];
-      R::unpack(raw[u], x);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float t = (x[j] - base) * c;     // exact near the maximum, of any size
-        const float e = __builtin_amdgcn_exp2f(t);
-        st.s += e;
-        st.w = fmaf(e, fmaxf(t, -256.f), st.w);
+  // 1. maximum, sum and weighted sum of this thread's columns: four vectors at a time, the
+  // next four on their way
+  Stats st{-INFINITY, 0.f, 0.f, 0.f, false};
+  if (whole > 0) {
+    Four<DT> cur;
+    const int first = threadIdx.x & ~63;      // the wave's: branches on it are uniform
+    float slot[4];
+    int group = 0;
+    for (int i = threadIdx.x, w = first; w < whole; i += 4 * NT, w += 4 * NT) {
+      cur.ld(row, i, NT, whole);
+      const bool fresh = (group & ((1 << A.shift) - 1)) == 0;
+      if (w + 3 * NT + 63 < whole)
+        take<DT, 4, false>(st, cur.raw, c, slot, fresh, 4);
+      else if (i < whole)
+        take<DT, 4, true>(st, cur.raw, c, slot, fresh, (whole - i + NT - 1) / NT);
+      if (k > 0) {
+        S.top[group >> A.shift][threadIdx.x] =
+            make_uint2(top_bits<DT>(slot[0]) | top_bits<DT>(slot[1]) << 16,
+                       top_bits<DT>(slot[2]) | top_bits<DT>(slot[3]) << 16);
+        ++group;
       }
     }
-  };
-  int i = threadIdx.x;
-  for (; i + 3 * NT < whole; i += 4 * NT) {
-    typename R::Raw raw[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) raw[u] = R::ld(row + (int64_t)(i + u * NT) * 8);
-    take(raw, std::integral_constant<int, 4>{});
   }
-  for (; i < vecs; i += NT) {
-    const typename R::Raw raw = ld_vec<DT>(row, i, v);
-    take(&raw, std::integral_constant<int, 1>{});
+  if (threadIdx.x == 0 && whole < vecs) {
+    const typename R::Raw raw = ld_vec<DT>(row, whole, v);
+    float slot[1];
+    take<DT, 1, false>(st, &raw, c, slot, true, 1);
   }
 
   // 2. the row's
@@ -229,14 +308,25 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LogArgs A) {
   const float wm = wave_max(mine);
   if (lane == 0) S.red[0][wave] = wm;
   // wavefronts whose lanes all have columns, and the first
-  const int full = max(1, min(kWaves, vecs / 64));
+  const int full = max(1, min(kWaves, whole / 64));
   if (k > 0) {
-    // the wave's k / full-th largest maximum of a lane (rounded up)
-    float left = mine, bound = wm;
-    for (int n = (k + full - 1) / full; n > 1 && bound > -INFINITY; --n) {
-      const uint64_t who = __ballot(left == bound);
-      if (lane == (int)__builtin_ctzll(who)) left = -INFINITY;
-      bound = wave_max(left);
+    // a number that k / full of the wave's maxima reach and, in eight halvings, few more
+    const int want = (k + full - 1) / full;
+    float bound = wm;
+    if (want > 1) {
+      const uint64_t has = __ballot(mine > -INFINITY);
+      bound = __popcll(has) < want ? -INFINITY : -wave_max(mine > -INFINITY ? -mine : -INFINITY);
+      float high = wm;
+      for (int n = 0; n < 8 && bound < high && bound > -INFINITY; ++n) {
+        const float mid = 0.5f * bound + 0.5f * high;
+        const int reach = __popcll(__ballot(mine >= mid));
+        if (reach < want) {
+          high = mid;
+        } else {
+          bound = mid;
+          if (reach == want) break;
+        }
+      }
     }
     if (lane == 0) S.bound[wave] = bound;
     if (threadIdx.x == 0) S.count = S.active = 0;
@@ -253,10 +343,11 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LogArgs A) {
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) s += S.red[1][w], w2 += S.red[2][w];
   const bool empty = m == -INFINITY && s == 0.f;      // -inf alone
-  const float log_s = logf(s);
+  // of e^(z - m / T)
+  const float log_s = logf(s) - (st.wide ? 0.f : fmaf(m, c, -st.base) * kLn2);
   if (threadIdx.x == 0) {
     A.lse[r] = empty ? -INFINITY : fmaf(m, A.inv_t, log_s);
-    A.entropy[r] = empty ? 0.f : log_s - (w2 / s) * kLn2;
+    A.entropy[r] = empty ? 0.f : logf(s) - (w2 / s) * kLn2;
     if (A.targets)
       A.logp[r] = empty ? -INFINITY : (chosen - m) * A.inv_t - log_s;
     if (A.stats) {
@@ -271,23 +362,52 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LogArgs A) {
   for (int w = 1; w < full; ++w) bound = fminf(bound, S.bound[w]);
   bool far = !(s < INFINITY) || bound == -INFINITY;   // NaN, or too few
   if (!far) {
-    if (mine >= bound) S.list[atomicAdd(&S.active, 1)] = (uint16_t)threadIdx.x;
+    // the maxima that reach it
+    if (mine >= bound)
+      for (int g = 0, w = threadIdx.x; w < whole; ++g, w += (4 * NT) << A.shift) {
+        const uint2 tops = S.top[g][threadIdx.x];
+        const uint32_t bits[4] = {tops.x & 0xFFFFu, tops.x >> 16, tops.y & 0xFFFFu, tops.y >> 16};
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (top_value<DT>(bits[u]) >= bound) {
+            const int at = atomicAdd(&S.active, 1);
+            if (at < S.kList) S.list[at] = (uint16_t)((g * 4 + u) * NT + threadIdx.x);
+          }
+      }
     __syncthreads();
-    const int per = (vecs + NT - 1) / NT, total = S.active * per;
-    for (int q = threadIdx.x; q < total; q += NT) {
-      const int a = q / per, vec = S.list[a] + (q - a * per) * NT;
-      if (vec >= vecs) continue;
+    // and their vectors again: every fourth of the thread's from the slot's start on
+    const int per = A.shift, active = S.active;
+    far = active > S.kList;
+    for (int q = threadIdx.x; !far && q < active << per; q += NT) {
+      const int entry = S.list[q >> per], slot = entry / NT;
+      const int nth = ((slot >> 2 << per) + (q & ((1 << per) - 1))) * 4 + (slot & 3);
+      const int vec = (entry & (NT - 1)) + nth * NT;
+      if (vec >= whole) continue;
       float x[8];
-      R::unpack(ld_vec<DT>(row, vec, v), x);
+      R::unpack(R::ld(row + (int64_t)vec * 8), x);
+      uint32_t hits = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) hits |= x[j] >= bound ? 1u << j : 0u;
+      if (hits == 0) continue;
+      int at = atomicAdd(&S.count, __popc(hits));
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (x[j] >= bound && vec * 8 + j < v) {
-          const int at = atomicAdd(&S.count, 1);
-          if (at < kMaxCand) S.cand[at] = order_key(x[j], vec * 8 + j);
+        if (hits >> j & 1) {
+          if (at < S.kCand) S.cand[at] = order_key(x[j], vec * 8 + j);
+          ++at;
         }
     }
+    // columns past the last whole vector
+    const int rest = whole * 8 + (int)threadIdx.x;
+    if (threadIdx.x < 8 && rest < v) {
+      const float x = Elem<DT>::ld(row + rest);
+      if (x >= bound) {
+        const int at = atomicAdd(&S.count, 1);
+        if (at < S.kCand) S.cand[at] = order_key(x, rest);
+      }
+    }
     __syncthreads();
-    far = S.count > kMaxCand;
+    far = far || S.count > S.kCand;
     __syncthreads();
   }
   if (far) radix_candidates<DT, NT>(row, v, k, S);
@@ -297,6 +417,7 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LogArgs A) {
   for (int a = threadIdx.x; a < count; a += NT) {
     const uint64_t key = S.cand[a];
     int rank = 0;
+#pragma unroll 8
     for (int o = 0; o < count; ++o) rank += S.cand[o] > key;
     if (rank < k) {
       const float x = order_value(key);
@@ -316,8 +437,9 @@ struct LogGradArgs {
   const float* d_logp;
   const float* d_entropy;
   void* grad;
-  int64_t rows, seq, ld_b, ld_s, gld_b, gld_s, ignore;
-  int v, wide, chunks;
+  int64_t rows, ld_b, ld_s, gld_b, gld_s, ignore;
+  FastDivU32 seq, chunks;
+  int v, wide;
   float inv_t;
 };
 
@@ -326,9 +448,8 @@ constexpr int kGradThreads = 256, kGradVecs = 4;
 template <int DT>
 __global__ __launch_bounds__(kGradThreads) void logprobs_grad_kernel(const LogGradArgs A) {
   using R = Row8<DT>;
-  const int64_t r = blockIdx.x / A.chunks;
-  const int chunk = (int)(blockIdx.x - r * A.chunks), v = A.v;
-  const int64_t b = r / A.seq, n = r - b * A.seq;
+  const uint32_t r = A.chunks.div(blockIdx.x), b = A.seq.div(r), n = r - b * A.seq.d;
+  const int chunk = (int)(blockIdx.x - r * A.chunks.d), v = A.v;
   const auto* row = (const typename R::T*)A.x + b * A.ld_b + n * A.ld_s;
   auto* out = (typename R::T*)A.grad + b * A.gld_b + n * A.gld_s;
   int64_t y = -1;
@@ -401,15 +522,22 @@ int cpt_token_logprobs(int dtype, const void* logits, int64_t rows, int64_t voca
   if (!entropy || !lse || (targets != nullptr) != (logprobs != nullptr) ||
       (k && (!top_logprobs || !top_indices)))
     return kErrShape;
+  // A row is one wavefront's where it is short: nothing to wait for (30000 x 4096 bf16, 20
+  // alternatives: 61 us, with 256 threads 129; 8192 x 32000: 108 and 98), unless so many
+  // alternatives are asked that its lanes' maxima are a weak bound.  A row for each CU
+  // or fewer: the chain of loads is shorter with more threads.
+  const int threads = vocab <= 8192 && k <= 48 ? 64 : rows <= 256 && vocab > 8192 ? 1024 : 256;
+  int shift = 0;
+  while ((vocab / 8 + ((4 * threads) << shift) - 1) / ((4 * threads) << shift) > kSlots) ++shift;
   const LogArgs A{logits, targets, (float*)logprobs, (float*)entropy, (float*)lse,
-                  (float*)stats, (float*)top_logprobs, (int64_t*)top_indices, rows, seq, ld_batch, ld_row,
-                  ignore_index, (int)vocab, (int)k, target_wide, 1.f / temperature};
+                  (float*)stats, (float*)top_logprobs, (int64_t*)top_indices, rows, ld_batch, ld_row,
+                  ignore_index, FastDivU32::make((uint32_t)std::min<int64_t>(seq, 0x7FFFFFFF)), (int)vocab, (int)k, target_wide, shift, 1.f / temperature};
   const hipStream_t st = (hipStream_t)stream;
   const unsigned grid = (unsigned)rows;
-  // few rows: a row is a chain of loads, shorter with more threads
-  const bool wide = rows <= 512 && vocab > 4096;
-#define CPT_LP(DT) \
-  (wide ? logprobs_kernel<DT, 1024><<<grid, 1024, 0, st>>>(A) : logprobs_kernel<DT, 256><<<grid, 256, 0, st>>>(A))
+#define CPT_LP(DT)                                                           \
+  (threads == 64    ? logprobs_kernel<DT, 64><<<grid, 64, 0, st>>>(A)        \
+   : threads == 256 ? logprobs_kernel<DT, 256><<<grid, 256, 0, st>>>(A)      \
+                    : logprobs_kernel<DT, 1024><<<grid, 1024, 0, st>>>(A))
   if (dtype == kF32)
     CPT_LP(kF32);
   else if (dtype == kF16)
@@ -430,11 +558,13 @@ int cpt_token_logprobs_backward(int dtype, const void* logits, int64_t rows, int
   if (rows == 0) return kOk;
   if ((!lse && !stats) || !grad || (d_logprobs && !targets) || (d_entropy && !entropy)) return kErrShape;
   LogGradArgs A{logits, targets, (const float*)lse, (const float*)stats, (const float*)entropy,
-                (const float*)d_logprobs, (const float*)d_entropy, grad, rows, seq, ld_batch,
-                ld_row, gld_batch, gld_row, ignore_index, (int)vocab, target_wide, 0,
-                1.f / temperature};
-  A.chunks = (int)((vocab + kGradThreads * kGradVecs * 8 - 1) / (kGradThreads * kGradVecs * 8));
-  const int64_t grid = rows * A.chunks;
+                (const float*)d_logprobs, (const float*)d_entropy, grad, rows, ld_batch,
+                ld_row, gld_batch, gld_row, ignore_index,
+                FastDivU32::make((uint32_t)std::min<int64_t>(seq, 0x7FFFFFFF)), {}, (int)vocab,
+                target_wide, 1.f / temperature};
+  const int64_t chunks = (vocab + kGradThreads * kGradVecs * 8 - 1) / (kGradThreads * kGradVecs * 8);
+  A.chunks = FastDivU32::make((uint32_t)chunks);
+  const int64_t grid = rows * chunks;
   if (grid > 0x7FFFFFFF) return kErrTooLarge;
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == kF32)

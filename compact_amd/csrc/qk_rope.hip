@@ -28,7 +28,8 @@ namespace {
 constexpr int kRopeThreads = 256;
 constexpr int kRopeTableBytes = 16384;    // cos and sin of a tile of tokens
 constexpr int kRopeMaxTile = 64;          // tokens a tile
-constexpr int kRopeBlocks = 1024;         // blocks of the backward, each with a partial sum
+constexpr int kRopeBlocks = 2048;         // of the backward, each with a partial sum
+constexpr int kSumThreads = 1024;
 
 struct RopeSide {                         // queries or keys
   const void* x;
@@ -123,6 +124,19 @@ struct HeadLane {
   }
 };
 
+// A head's weights as a lane has its columns: one branch, then loads alone (a load
+// under a branch of its own is waited for by itself).
+template <int DT, bool VEC, bool INTER>
+__device__ __forceinline__ void ld_weights(const HeadLane<DT, VEC, INTER>& io, const void* w,
+                                           int wdt, float a[8], float b[8]) {
+  if (DT != kF32 && wdt == kF32) {
+    const HeadLane<kF32, VEC, INTER> wide{io.lane, io.lanes, io.pairs, io.rot, io.d};
+    wide.ld((const float*)w, a, b);
+  } else {
+    io.ld((const typename Elem<DT>::T*)w, a, b);
+  }
+}
+
 // The sum over a head's lanes, in each of them.
 __device__ __forceinline__ float head_sum(float v, int lanes) {
   for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
@@ -169,13 +183,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_forward(const RopeArgs A, i
   const int group = threadIdx.x / A.lanes, groups = kRopeThreads / A.lanes, pairs = A.d / 2;
   const HeadLane<DT, VEC, INTER> io{(int)threadIdx.x & (A.lanes - 1), A.lanes, pairs, A.rot, A.d};
   float wa[8], wb[8];
-  if (NORM) {
-#pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      wa[t] = ld_any(S.w, A.wdt, io.col_a(io.pair(t)));
-      wb[t] = ld_any(S.w, A.wdt, io.col_b(io.pair(t)));
-    }
-  }
+  if (NORM) ld_weights(io, S.w, A.wdt, wa, wb);
   const int t0 = block * S.tile, nt = min(S.tile, A.tokens - t0);
   rope_table<false>(A, S, t0, nt, table, base);
   __syncthreads();
@@ -215,12 +223,9 @@ __global__ __launch_bounds__(kRopeThreads) void rope_norm_backward(const RopeArg
   const int group = threadIdx.x / A.lanes, groups = kRopeThreads / A.lanes, pairs = A.d / 2;
   const HeadLane<DT, VEC, INTER> io{(int)threadIdx.x & (A.lanes - 1), A.lanes, pairs, A.rot, A.d};
   float wa[8], wb[8], da[8], db[8];
+  ld_weights(io, S.w, A.wdt, wa, wb);
 #pragma unroll
-  for (int t = 0; t < 8; ++t) {
-    wa[t] = ld_any(S.w, A.wdt, io.col_a(io.pair(t)));
-    wb[t] = ld_any(S.w, A.wdt, io.col_b(io.pair(t)));
-    da[t] = db[t] = 0.f;
-  }
+  for (int t = 0; t < 8; ++t) da[t] = db[t] = 0.f;
   const float inv_d = 1.f / A.d;
   for (int64_t t0 = (int64_t)block * S.tile; t0 < A.tokens; t0 += (int64_t)S.blocks * S.tile) {
     const int nt = (int)min((int64_t)S.tile, A.tokens - t0);
@@ -281,29 +286,35 @@ __global__ __launch_bounds__(kRopeThreads) void rope_norm_backward(const RopeArg
         (sums[j] + sums[A.d + j]) + (sums[2 * A.d + j] + sums[3 * A.d + j]);
 }
 
-// dw[j] = the blocks' partial sums, 16 columns a block, 16 threads each.
-__global__ __launch_bounds__(256) void rope_weight_sums(const float* pq, int nq, void* dwq,
-                                                        const float* pk, int nk, void* dwk, int d,
-                                                        int wdt) {
-  __shared__ float part[16][17];
+// dw[j] = the blocks' partial sums, 16 columns a block, 64 threads each.
+__global__ __launch_bounds__(kSumThreads) void rope_weight_sums(const float* pq, int nq, void* dwq,
+                                                                const float* pk, int nk, void* dwk,
+                                                                int d, int wdt) {
+  __shared__ float part[kSumThreads / 16][17];
   const float* p = blockIdx.y ? pk : pq;
   const int n = blockIdx.y ? nk : nq;
-  const int c = threadIdx.x & 15, r = threadIdx.x >> 4, j = blockIdx.x * 16 + c;
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
-  if (j < d) {
-    int i = r;
-    for (; i + 48 < n; i += 64)
+  const int c = threadIdx.x & 15, r = threadIdx.x >> 4, j = min((int)blockIdx.x * 16 + c, d - 1);
+  float s[8];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) s[u] += p[(int64_t)(i + 16 * u) * d + j];
-    for (; i < n; i += 16) s[0] += p[(int64_t)i * d + j];
+  for (int u = 0; u < 8; ++u) s[u] = 0.f;
+  for (int i = r; i < n; i += 512) {
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = p[(int64_t)min(i + 64 * u, n - 1) * d + j];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s[u] += i + 64 * u < n ? v[u] : 0.f;
   }
-  part[r][c] = (s[0] + s[1]) + (s[2] + s[3]);
+  part[r][c] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
   __syncthreads();
-  if (r == 0 && j < d) {
+  // 16 columns' 64 sums: four lanes a column, then those four
+  if (threadIdx.x < 64) {
     float t = 0.f;
 #pragma unroll
-    for (int u = 0; u < 16; ++u) t += part[u][c];
-    st_any(blockIdx.y ? dwk : dwq, wdt, j, t);
+    for (int u = 0; u < 16; ++u) t += part[(threadIdx.x >> 4) * 16 + u][c];
+    t += __shfl_xor(t, 16);
+    t += __shfl_xor(t, 32);
+    if (threadIdx.x < 16 && (int)blockIdx.x * 16 + c < d)
+      st_any(blockIdx.y ? dwk : dwq, wdt, j, t);
   }
 }
 
@@ -319,19 +330,22 @@ bool rope_vec(int64_t d, int64_t rot, bool inter) {
 }
 int rope_lanes(int64_t d) { return pow2_at_least((int)((d / 2 + 7) / 8)); }
 
-// Tokens a tile: enough that the block's groups take about four heads each, as many as
-// the table holds, and no more than leaves a block for every CU (four).
+// Tokens a tile: as many as give every group of the block a head, and up to four times
+// that where there are tokens for 1024 blocks all the same, as far as the table holds.
+// (3009 tokens of 3 heads x 80: 10 a tile; with 3, two thirds of the block had none.)
 int rope_tile(int64_t tokens, int64_t heads, int64_t d) {
   const int64_t groups = kRopeThreads / rope_lanes(d);
-  int64_t t = (4 * groups + heads - 1) / heads;
-  t = std::min<int64_t>(t, kRopeTableBytes / (d / 2 * 8));
-  t = std::min<int64_t>(t, (tokens + 1023) / 1024);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(t, kRopeMaxTile));
+  const int64_t once = std::max<int64_t>(1, groups / heads);
+  const int64_t rounds = std::min<int64_t>(4, std::max<int64_t>(1, tokens / (once * 1024)));
+  const int64_t most = std::min<int64_t>(kRopeTableBytes / (d / 2 * 8), kRopeMaxTile);
+  return (int)std::max<int64_t>(1, std::min(std::min(once * rounds, most), tokens));
 }
 
-int64_t rope_blocks(int64_t tokens, int tile, bool bounded) {
-  const int64_t n = (tokens + tile - 1) / tile;
-  return bounded ? std::min<int64_t>(n, kRopeBlocks) : n;
+int64_t rope_blocks(int64_t tokens, int tile) { return (tokens + tile - 1) / tile; }
+// The backward's, which loop over tiles: kRopeBlocks by the sides' heads.
+int64_t rope_blocks_bounded(int64_t tokens, int tile, int64_t heads, int64_t all_heads) {
+  return std::min(rope_blocks(tokens, tile),
+                  std::max<int64_t>(1, kRopeBlocks * heads / all_heads));
 }
 
 int rope_check(int dtype, int wdt, int64_t batch, int64_t seq, int64_t hq, int64_t hk, int64_t d,
@@ -415,7 +429,7 @@ int cpt_qk_rope(int dtype, int weight_dtype, int interleaved, int inverse, const
   int most = 1;
   for (int i = 0; i < 2; ++i) {
     A.side[i].tile = rope_tile(tokens, std::max<int64_t>(heads[i], 1), d);
-    A.side[i].blocks = heads[i] ? (int)rope_blocks(tokens, A.side[i].tile, false) : 0;
+    A.side[i].blocks = heads[i] ? (int)rope_blocks(tokens, A.side[i].tile) : 0;
     if (heads[i]) most = std::max(most, A.side[i].tile);
   }
   A.positions = positions, A.pos_wide = pos_wide, A.pos_stride = pos_batch;
@@ -435,12 +449,11 @@ int64_t cpt_qk_rope_backward_workspace_bytes(int64_t tokens, int64_t heads_q, in
                                              int64_t d) {
   if (tokens < 0 || heads_q < 0 || heads_k < 0 || d < 2 || d > 1024 || tokens >= 1ll << 30)
     return -1;
-  int64_t n = 0;
-  if (tokens > 0) {
-    if (heads_q) n += rope_blocks(tokens, rope_tile(tokens, heads_q, d), true);
-    if (heads_k) n += rope_blocks(tokens, rope_tile(tokens, heads_k, d), true);
-  }
-  return n * d * 4;
+  if (tokens == 0 || heads_q == 0 || heads_k == 0) return 0;
+  const int64_t all = heads_q + heads_k;
+  return (rope_blocks_bounded(tokens, rope_tile(tokens, heads_q, d), heads_q, all) +
+          rope_blocks_bounded(tokens, rope_tile(tokens, heads_k, d), heads_k, all)) *
+         d * 4;
 }
 
 int cpt_qk_rope_backward(int dtype, int weight_dtype, int interleaved, const void* d_q,
@@ -472,7 +485,7 @@ int cpt_qk_rope_backward(int dtype, int weight_dtype, int interleaved, const voi
   for (int i = 0; i < 2; ++i) {
     RopeSide& s = A.side[i];
     s.tile = rope_tile(tokens, heads[i], d);
-    s.blocks = (int)rope_blocks(tokens, s.tile, true);
+    s.blocks = (int)rope_blocks_bounded(tokens, s.tile, heads[i], heads_q + heads_k);
     s.partial = ws;
     ws += (int64_t)s.blocks * d;
     most = std::max(most, s.tile);
@@ -490,7 +503,7 @@ int cpt_qk_rope_backward(int dtype, int weight_dtype, int interleaved, const voi
                   : dtype == kF16 ? launch_backward<kF16>(A, vec, interleaved, lds, st)
                                   : launch_backward<kBF16>(A, vec, interleaved, lds, st);
   if (err) return err;
-  rope_weight_sums<<<dim3((unsigned)((d + 15) / 16), 2), 256, 0, st>>>(
+  rope_weight_sums<<<dim3((unsigned)((d + 15) / 16), 2), kSumThreads, 0, st>>>(
       A.side[0].partial, A.side[0].blocks, dw_q, A.side[1].partial, A.side[1].blocks, dw_k, (int)d,
       weight_dtype);
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;

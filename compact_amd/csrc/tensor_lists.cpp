@@ -1,0 +1,281 @@
+// Lists of tensors as the C ABI takes them: an optimizer step has hundreds of tensors
+// in five lists, and a look at each from Python costs more than the step (320 adapter
+// factors: 550 us of checks and addresses, 25 here).  Everything that the kernels rely
+// on is checked: types, devices, sizes, layouts.
+
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
+
+#include <cstring>
+#include <string>
+#include <unordered_set>
+#include <vector>
+
+#include "compact_amd.h"
+
+namespace {
+
+// A violated condition: AssertionError, as the wrappers' other checks.
+struct Refused {
+  std::string why;
+};
+[[noreturn]] void refuse(const std::string& why) { throw Refused{why}; }
+
+std::string describe(const at::Tensor& t) {
+  std::string s = std::string(c10::toString(t.scalar_type())) + " [";
+  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+  s += "] strides [";
+  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.stride(i));
+  return s + "] on " + t.device().str();
+}
+
+// A list or tuple of tensors (borrowed).
+class List {
+ public:
+  List(PyObject* o, const char* name) : name_(name) {
+    if (o == Py_None) return;
+    fast_ = PySequence_Fast(o, "a sequence of tensors expected");
+    if (!fast_) throw python_error();
+    n_ = PySequence_Fast_GET_SIZE(fast_);
+    items_ = PySequence_Fast_ITEMS(fast_);
+  }
+  List(const List&) = delete;
+  ~List() { Py_XDECREF(fast_); }
+  explicit operator bool() const { return fast_ != nullptr; }
+  int64_t size() const { return n_; }
+  const char* name() const { return name_; }
+  PyObject* object(int64_t i) const { return items_[i]; }
+  const at::Tensor& operator[](int64_t i) const {
+    if (!THPVariable_Check(items_[i])) refuse(std::string(name_) + ": tensors expected");
+    const at::Tensor& t = THPVariable_Unpack(items_[i]);
+    if (t.layout() != at::kStrided || t.is_complex())
+      refuse(std::string(name_) + ": dense real tensors expected");
+    return t;
+  }
+
+ private:
+  const char* name_;
+  PyObject* fast_ = nullptr;
+  Py_ssize_t n_ = 0;
+  PyObject** items_ = nullptr;
+};
+
+// Whether a tensor's elements fill its memory once, in whatever order of its axes.
+bool dense(const at::Tensor& t) {
+  return t.is_contiguous() || t.unsafeGetTensorImpl()->is_non_overlapping_and_dense_default();
+}
+// Whether dense tensors of one shape lie alike.
+bool alike(const at::Tensor& a, const at::Tensor& b) {
+  return (a.is_contiguous() && b.is_contiguous()) || a.strides() == b.strides();
+}
+
+int code(at::ScalarType t) {
+  return t == at::kFloat ? 0 : t == at::kHalf ? 1 : t == at::kBFloat16 ? 2 : -1;
+}
+
+int64_t address(const at::Tensor& t) { return reinterpret_cast<int64_t>(t.data_ptr()); }
+
+void expect(const at::Tensor& t, const at::Tensor& p, at::ScalarType type, const char* name) {
+  if (t.scalar_type() != type || t.device() != p.device() || t.sizes() != p.sizes() || !alike(p, t))
+    refuse(std::string(name) + ": " + c10::toString(type) + " that lies as " + describe(p) +
+           " expected, got " + describe(t));
+}
+void expect_bytes(const at::Tensor& t, const at::Tensor& p, int64_t n, const char* name) {
+  if (t.scalar_type() != at::kByte || t.device() != p.device() || t.numel() != n ||
+      !t.is_contiguous())
+    refuse(std::string(name) + ": contiguous Byte of " + std::to_string(n) + " on " +
+           p.device().str() + " expected, got " + describe(t));
+}
+
+constexpr int64_t kBlock = 128;   // elements of an 8-bit moment that share a scale
+
+template <class F>
+PyObject* guarded(F&& f) {
+  try {
+    return f();
+  } catch (const Refused& r) {
+    PyErr_SetString(PyExc_AssertionError, r.why.c_str());
+  } catch (python_error& e) {
+    e.persist();
+    e.restore();
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  }
+  return nullptr;
+}
+
+// {table, its address, elements, more...}
+PyObject* result(const std::vector<cpt_adamw_tensor>& rows, int64_t elements, int dtype,
+                 int grad_dtype, PyObject* more) {
+  PyObject* table = PyBytes_FromStringAndSize(reinterpret_cast<const char*>(rows.data()),
+                                              rows.size() * sizeof(cpt_adamw_tensor));
+  if (!table) throw python_error();
+  return Py_BuildValue("(NLLiiN)", table,
+                       static_cast<long long>(reinterpret_cast<intptr_t>(PyBytes_AS_STRING(table))),
+                       static_cast<long long>(elements), dtype, grad_dtype, more);
+}
+
+// The steps' numbers, or addresses of counts on the device.
+void steps(PyObject* step, std::vector<cpt_adamw_tensor>& rows, const at::Device& device) {
+  const int64_t n = rows.size();
+  auto number = [](PyObject* o) {
+    if (!PyLong_Check(o)) refuse("step: whole numbers expected");
+    const long long v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) throw python_error();
+    if (v < 1) refuse("step=" + std::to_string(v) + ": the first is 1");
+    return v;
+  };
+  auto counts = [&](PyObject* o, int64_t m) -> int64_t* {
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (t.scalar_type() != at::kLong || t.numel() != m || !t.is_contiguous() ||
+        t.device() != device)
+      refuse("step: " + std::to_string(m) + " contiguous Long on " + device.str() +
+             " expected, got " + describe(t));
+    return static_cast<int64_t*>(t.data_ptr());
+  };
+  if (THPVariable_Check(step)) {
+    int64_t* at = counts(step, n);
+    for (int64_t i = 0; i < n; ++i) rows[i].step_device = at + i;
+    return;
+  }
+  if (PyLong_Check(step)) {
+    const long long v = number(step);
+    for (auto& r : rows) r.step = v;
+    return;
+  }
+  const List list(step, "step");
+  if (list.size() != n) refuse("step: " + std::to_string(n) + " expected");
+  const bool on_device = n && THPVariable_Check(list.object(0));
+  std::unordered_set<void*> seen;
+  for (int64_t i = 0; i < n; ++i) {
+    if (!on_device) {
+      rows[i].step = number(list.object(i));
+      continue;
+    }
+    if (!THPVariable_Check(list.object(i))) refuse("step: a count each expected");
+    rows[i].step_device = counts(list.object(i), 1);
+    if (!seen.insert(rows[i].step_device).second)
+      refuse("step: a count of its own for each parameter expected");
+  }
+}
+
+// adamw_table(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales, masters, step):
+// (table, address, elements, dtype, grads' dtype, [indices of gradients that lie
+// otherwise than their parameters])
+PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 8) refuse("eight arguments expected");
+    const List p(a[0], "params"), g(a[1], "grads"), m(a[2], "exp_avgs"), v(a[3], "exp_avg_sqs"),
+        ms(a[4], "m_scales"), vs(a[5], "v_scales"), w(a[6], "masters");
+    for (const List* l : {&g, &m, &v, &ms, &vs, &w})
+      if (*l && l->size() != p.size())
+        refuse(std::string(l->name()) + ": " + std::to_string(p.size()) + " tensors expected, got " +
+               std::to_string(l->size()));
+    const int64_t count = p.size();
+    std::vector<cpt_adamw_tensor> rows(count);
+    std::unordered_set<void*> seen;
+    seen.reserve(count);
+    const at::ScalarType type = p[0].scalar_type(), grad_type = g[0].scalar_type();
+    const at::Device device = p[0].device();
+    if (code(type) < 0) refuse("params: unsupported " + describe(p[0]));
+    if (grad_type != type && grad_type != at::kFloat)
+      refuse("grads: the parameters' type or Float expected, got " + describe(g[0]));
+    if (w && type == at::kFloat) refuse("masters: of 16-bit parameters");
+    THPObjectPtr otherwise(PyList_New(0));
+    if (!otherwise) throw python_error();
+    int64_t total = 0;
+    for (int64_t i = 0; i < count; ++i) {
+      const at::Tensor &pi = p[i], &gi = g[i];
+      cpt_adamw_tensor& r = rows[i];
+      if (pi.scalar_type() != type || pi.device() != device)
+        refuse("params: " + describe(p[0]) + " and " + describe(pi));
+      if (gi.scalar_type() != grad_type || gi.device() != device)
+        refuse("grads: " + describe(g[0]) + " and " + describe(gi));
+      if (gi.sizes() != pi.sizes())
+        refuse("grads: " + describe(gi) + " for " + describe(pi));
+      if (!dense(pi)) refuse("params: dense memory expected, got " + describe(pi));
+      r.n = pi.numel();
+      total += r.n;
+      r.p = pi.data_ptr();
+      if (r.n && !seen.insert(r.p).second) refuse("a parameter is there twice");
+      if (alike(pi, gi)) {
+        r.g = gi.data_ptr();
+      } else {
+        THPObjectPtr at(PyLong_FromLongLong(i));
+        if (!at || PyList_Append(otherwise.get(), at.get())) throw python_error();
+      }
+      if (ms) {
+        const int64_t blocks = (r.n + kBlock - 1) / kBlock;
+        expect_bytes(m[i], pi, r.n, m.name());
+        expect_bytes(v[i], pi, r.n, v.name());
+        expect_bytes(ms[i], pi, blocks, ms.name());
+        expect_bytes(vs[i], pi, blocks, vs.name());
+        r.m_scale = ms[i].data_ptr();
+        r.v_scale = vs[i].data_ptr();
+      } else {
+        expect(m[i], pi, at::kFloat, m.name());
+        expect(v[i], pi, at::kFloat, v.name());
+      }
+      r.m = m[i].data_ptr();
+      r.v = v[i].data_ptr();
+      if (w) {
+        expect(w[i], pi, at::kFloat, w.name());
+        r.master = w[i].data_ptr();
+      }
+    }
+    steps(a[7], rows, device);
+    return result(rows, total, code(type), code(grad_type), otherwise.release());
+  });
+}
+
+// grads_table(grads): (table, address, elements, dtype, dtype, [indices of gradients that
+// do not fill their memory once])
+PyObject* grads_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 1) refuse("one argument expected");
+    const List g(a[0], "grads");
+    std::vector<cpt_adamw_tensor> rows(g.size());
+    const at::ScalarType type = g[0].scalar_type();
+    const at::Device device = g[0].device();
+    if (code(type) < 0) refuse("grads: unsupported " + describe(g[0]));
+    THPObjectPtr otherwise(PyList_New(0));
+    if (!otherwise) throw python_error();
+    int64_t total = 0;
+    for (int64_t i = 0; i < g.size(); ++i) {
+      const at::Tensor& t = g[i];
+      if (t.scalar_type() != type || t.device() != device)
+        refuse("grads: " + describe(g[0]) + " and " + describe(t));
+      rows[i].n = t.numel();
+      rows[i].g = t.data_ptr();
+      total += rows[i].n;
+      if (!dense(t)) {
+        THPObjectPtr at(PyLong_FromLongLong(i));
+        if (!at || PyList_Append(otherwise.get(), at.get())) throw python_error();
+      }
+    }
+    return result(rows, total, code(type), code(type), otherwise.release());
+  });
+}
+
+// bump_versions(tensors): they were written to
+PyObject* bump_versions(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 1) refuse("one argument expected");
+    const List l(a[0], "tensors");
+    for (int64_t i = 0; i < l.size(); ++i)
+      if (!l[i].is_inference()) l[i].unsafeGetTensorImpl()->bump_version();
+    Py_RETURN_NONE;
+  });
+}
+
+#define ENTRY(name) \
+  {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&name)), METH_FASTCALL, nullptr}
+PyMethodDef methods[] = {ENTRY(adamw_table), ENTRY(grads_table), ENTRY(bump_versions),
+                         {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_lists", "lists of tensors for the C ABI", -1,
+                      methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__lists(void) { return PyModule_Create(&module); }

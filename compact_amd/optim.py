@@ -18,136 +18,53 @@ move by less than a code's step a time still move.
 
 from __future__ import annotations
 
-from array import array
-
 import torch
 
 from . import _lib
 from ._lib import check
-from .kernels import _DT, _guard, _ptr, _require_device, _stream, _timed
+from .kernels import _guard, _ptr, _require_device, _stream, _timed
 
 BLOCK = 128         # elements of an 8-bit moment that share a scale
-_ENTRY = 10         # 8-byte fields of a cpt_adamw_tensor
 
 
-def _dense_layout(t):
-    """Whether t's elements fill its memory once, in whatever order of its axes."""
-    if t.is_contiguous():
-        return True
-    extent = 1
-    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
-        if stride != extent:
-            return False
-        extent = stride * size
-    return True
-
-
-def _same_layout(a, b):
-    """Whether dense a and b of one shape lie alike in memory."""
-    return (a.is_contiguous() and b.is_contiguous()) or a.stride() == b.stride()
-
-
-def _one_kind(tensors, what):
-    """All tensors of one dtype on one HIP device."""
-    first = tensors[0]
-    dt, dev = first.dtype, first.get_device()
+def _first(tensors):
+    """The device index of a list's first tensor, which the others have to share."""
+    dev = tensors[0].get_device()
     if dev < 0:
-        _require_device(first)
-    for t in tensors:
-        if t.dtype != dt or t.get_device() != dev:
-            raise AssertionError(f"{what}: {dt} on {first.device} and {t.dtype} on {t.device}")
-    return dt, dev
-
-
-def _lists(params, **lists):
-    """As many of each as there are parameters."""
-    for name, ts in lists.items():
-        assert ts is None or len(ts) == len(params), \
-            f"{name}: {len(params)} tensors expected, got {len(ts)}"
-
-
-def _like(params, tensors, what, dtype, dev):
-    """Addresses of `tensors`: dtype, shaped and laid out as the parameters."""
-    out = []
-    for p, t in zip(params, tensors):
-        if t.dtype != dtype or t.get_device() != dev or t.shape != p.shape \
-                or not _same_layout(p, t):
-            raise AssertionError(
-                f"{what}: {dtype} {tuple(p.shape)} {p.stride()} on {p.device} expected, got "
-                f"{t.dtype} {tuple(t.shape)} {t.stride()} on {t.device}")
-        out.append(t.data_ptr())
-    return out
-
-
-def _bytes(counts, tensors, what, dev):
-    """Addresses of `tensors`: contiguous uint8 with so many elements."""
-    out = []
-    for n, t in zip(counts, tensors):
-        if t.dtype != torch.uint8 or t.get_device() != dev or t.numel() != n \
-                or not t.is_contiguous():
-            raise AssertionError(f"{what}: contiguous uint8 of {n} expected, got {t.dtype} "
-                                 f"{tuple(t.shape)} on {t.device}")
-        out.append(t.data_ptr())
-    return out
+        _require_device(tensors[0])
+    return dev
 
 
 def _scalar(t, dev, what):
     assert t.dtype == torch.float32 and t.numel() == 1 and t.get_device() == dev, \
-        f"{what}: one float32 on the parameters' device expected"
+        f"{what}: one float32 on the tensors' device expected"
     return t.data_ptr()
 
 
-def _steps(step, count, dev):
-    """(host step numbers or None, device counts' addresses or None)."""
-    if isinstance(step, torch.Tensor):
-        assert step.dtype == torch.int64 and step.numel() == count and step.is_contiguous() \
-            and step.get_device() == dev, \
-            f"step: {count} contiguous int64 on the parameters' device expected"
-        return None, [step.data_ptr() + 8 * i for i in range(count)]
-    if isinstance(step, int):
-        assert step >= 1, f"step={step}: the first is 1"
-        return [step] * count, None
-    assert len(step) == count, f"step: {count} expected, got {len(step)}"
-    if count and isinstance(step[0], torch.Tensor):
-        for t in step:
-            assert isinstance(t, torch.Tensor) and t.dtype == torch.int64 and t.numel() == 1 \
-                and t.get_device() == dev, "step: one int64 on the parameters' device each expected"
-        at = [t.data_ptr() for t in step]
-        assert len(set(at)) == count, "step: a count of its own for each parameter expected"
-        return None, at
-    for t in step:
-        assert isinstance(t, int) and t >= 1, f"step={t}: whole numbers from 1 on expected"
-    return list(step), None
-
-
-def _table(count, columns):
-    """The C ABI's array of tensors, from columns of addresses and numbers."""
-    rows = array("q", bytes(8 * _ENTRY * count))
-    for i, c in columns.items():
-        if c is not None:
-            rows[i::_ENTRY] = array("q", c)
-    return rows
+def _workspace(like, count, elements):
+    nbytes = _lib.api().cpt_adamw_workspace_bytes(count, elements)
+    assert nbytes >= 0, f"{count} tensors of {elements} elements: out of range"
+    return like.new_empty(nbytes, dtype=torch.uint8)
 
 
 def grad_norm(grads, *, grad_scale: float = 1.0, out=None) -> torch.Tensor:
     """The 2-norm of grad_scale times all gradients as one vector, a float32 scalar on
-    their device; squares are summed in 64 bits.  One dtype and device."""
+    their device; it is summed in 64 bits.  One dtype and device."""
     grads = list(grads)
     assert grads, "grad_norm: no gradients"
-    dt, dev = _one_kind(grads, "grads")
-    assert dt in _DT, f"unsupported dtype {dt}"
-    grads = [g if _dense_layout(g) else g.contiguous() for g in grads]
-    sizes = [g.numel() for g in grads]
+    dev = _first(grads)
+    table, at, total, _, dt, loose = _lib.lists().grads_table(grads)
+    if loose:
+        for i in loose:
+            grads[i] = grads[i].contiguous()
+        table, at, total, _, dt, _ = _lib.lists().grads_table(grads)
     if out is None:
-        out = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    L = _lib.api()
-    nbytes = L.cpt_adamw_workspace_bytes(len(grads), sum(sizes))
-    assert nbytes >= 0, "grad_norm: sizes out of range"
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=grads[0].device)
-    table = _table(len(grads), {1: [g.data_ptr() for g in grads], 8: sizes})
+        out = grads[0].new_empty((), dtype=torch.float32)
+    out_at = _scalar(out, dev, "out")
+    ws = _workspace(grads[0], len(grads), total)
     with _guard(grads[0]), _timed("grad_norm"):
-        rc = L.cpt_grad_norm(_DT[dt], table.buffer_info()[0], len(grads), float(grad_scale),
-                             _scalar(out, dev, "out"), ws.data_ptr(), _stream(grads[0]))
+        rc = _lib.api().cpt_grad_norm(dt, at, len(grads), float(grad_scale), out_at, ws.data_ptr(),
+                                      _stream(grads[0]))
     check(rc, "grad_norm")
     return out
 
@@ -180,97 +97,60 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.
     tensors than these.  A norm that is not finite leaves parameters, moments and
     counts as they were."""
     params, grads = list(params), list(grads)
-    exp_avgs, exp_avg_sqs = list(exp_avgs), list(exp_avg_sqs)
-    _lists(params, grads=grads, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs, m_scales=m_scales,
-           v_scales=v_scales, masters=masters)
-    assert (m_scales is None) == (v_scales is None), "m_scales and v_scales belong together"
     b1, b2 = betas
+    assert (m_scales is None) == (v_scales is None), "m_scales and v_scales belong together"
     assert 0 <= b1 < 1 and 0 <= b2 < 1, f"betas={betas}"
     assert eps >= 0 and weight_decay >= 0, f"eps={eps}, weight_decay={weight_decay}"
     assert max_norm is None or 0 < max_norm < float("inf"), f"max_norm={max_norm}"
     assert norm is None or max_norm is not None, "norm goes with max_norm"
     if not params:
+        assert not grads, "gradients without parameters"
         return norm
-    dt, dev = _one_kind(params, "params")
-    gdt, gdev = _one_kind(grads, "grads")
-    assert dt in _DT, f"unsupported dtype {dt}"
-    assert gdev == dev and gdt in (dt, torch.float32), \
-        f"grads: {dt} or float32 beside the parameters expected, got {gdt} on {grads[0].device}"
-    for i, (p, g) in enumerate(zip(params, grads)):
-        assert g.shape == p.shape, f"gradient {tuple(g.shape)} for {tuple(p.shape)}"
-        if not p.is_contiguous():
-            assert _dense_layout(p), f"parameter {tuple(p.shape)} {p.stride()}: dense expected"
-        if not _same_layout(p, g):
-            grads[i] = torch.empty_like(p, dtype=gdt).copy_(g)
-    count = len(params)
-    sizes = [p.numel() for p in params]
-    at = [p.data_ptr() for p in params]
-    assert len({a for a, n in zip(at, sizes) if n}) == sum(n > 0 for n in sizes), \
-        "a parameter is there twice"
-    bits8 = m_scales is not None
-    cols = {0: at, 1: [g.data_ptr() for g in grads], 8: sizes}
-    if bits8:
-        blocks = [-(-n // BLOCK) for n in sizes]
-        cols[2] = _bytes(sizes, exp_avgs, "exp_avgs", dev)
-        cols[3] = _bytes(sizes, exp_avg_sqs, "exp_avg_sqs", dev)
-        cols[4] = _bytes(blocks, m_scales, "m_scales", dev)
-        cols[5] = _bytes(blocks, v_scales, "v_scales", dev)
-    else:
-        cols[2] = _like(params, exp_avgs, "exp_avgs", torch.float32, dev)
-        cols[3] = _like(params, exp_avg_sqs, "exp_avg_sqs", torch.float32, dev)
-    if masters is not None:
-        assert dt != torch.float32, "masters: of 16-bit parameters"
-        cols[6] = _like(params, masters, "masters", torch.float32, dev)
-    cols[9], cols[7] = _steps(step, count, dev)
-    lr_at = None
+    assert grads, "parameters without gradients"
+    dev = _first(params)
+    lists = _lib.lists()
+    args = exp_avgs, exp_avg_sqs, m_scales, v_scales, masters, step
+    table, at, total, dt, gdt, loose = lists.adamw_table(params, grads, *args)
+    if loose:
+        for i in loose:
+            grads[i] = torch.empty_like(params[i], dtype=grads[i].dtype).copy_(grads[i])
+        table, at, total, dt, gdt, _ = lists.adamw_table(params, grads, *args)
+    lr_at = norm_at = ws = None
     if isinstance(lr, torch.Tensor):
         lr_at, lr = _scalar(lr, dev, "lr"), 0.0
     assert lr >= 0, f"lr={lr}"
-    L = _lib.api()
-    ws = norm_at = None
-    given = norm is not None
+    given, p0, count = norm is not None, params[0], len(params)
     if max_norm is not None:
         if not given:
-            norm = torch.empty((), dtype=torch.float32, device=params[0].device)
+            norm = p0.new_empty((), dtype=torch.float32)
         norm_at = _scalar(norm, dev, "norm")
-    if max_norm is not None or cols[7] is not None:
-        nbytes = L.cpt_adamw_workspace_bytes(count, sum(sizes))
-        assert nbytes >= 0, "adamw_step: sizes out of range"
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=params[0].device)
-    table = _table(count, cols)
-    with _guard(params[0]), _timed("adamw_step"):
-        rc = L.cpt_adamw(_DT[dt], _DT[gdt], int(bits8), int(masters is not None),
-                         table.buffer_info()[0], count, float(lr), lr_at, float(b1), float(b2),
-                         float(eps), float(weight_decay), float(grad_scale),
-                         0.0 if max_norm is None else float(max_norm), int(given),
-                         seed & 0xFFFFFFFF, norm_at, _ptr(ws), _stream(params[0]))
+    if max_norm is not None or not isinstance(step if isinstance(step, int) else step[0], int):
+        ws = _workspace(p0, count, total)
+    with _guard(p0), _timed("adamw_step"):
+        rc = _lib.api().cpt_adamw(dt, gdt, int(m_scales is not None), int(masters is not None), at,
+                                  count, float(lr), lr_at, float(b1), float(b2), float(eps),
+                                  float(weight_decay), float(grad_scale),
+                                  0.0 if max_norm is None else float(max_norm), int(given),
+                                  seed & 0xFFFFFFFF, norm_at, _ptr(ws), _stream(p0))
     check(rc, "adamw_step")
     # autograd refuses a graph that still needs the old parameters
-    torch.autograd.graph.increment_version(params)
+    lists.bump_versions(params)
     return norm
 
 
 def adamw_8bit_values(exp_avgs, exp_avg_sqs, m_scales, v_scales):
     """What 8-bit moments stand for: two lists of bfloat16 tensors, shaped as the codes,
     which hold the values exactly (NaN for a block with a value that was not finite)."""
-    exp_avgs, exp_avg_sqs = list(exp_avgs), list(exp_avg_sqs)
-    m_scales, v_scales = list(m_scales), list(v_scales)
-    _lists(exp_avgs, exp_avg_sqs=exp_avg_sqs, m_scales=m_scales, v_scales=v_scales)
+    exp_avgs = list(exp_avgs)
     if not exp_avgs:
         return [], []
-    _, dev = _one_kind(exp_avgs, "exp_avgs")
-    sizes = [t.numel() for t in exp_avgs]
-    blocks = [-(-n // BLOCK) for n in sizes]
-    m = [torch.empty(t.shape, dtype=torch.bfloat16, device=t.device) for t in exp_avgs]
-    v = [torch.empty(t.shape, dtype=torch.bfloat16, device=t.device) for t in exp_avgs]
-    table = _table(len(sizes), {
-        0: [t.data_ptr() for t in m], 6: [t.data_ptr() for t in v],
-        2: _bytes(sizes, exp_avgs, "exp_avgs", dev),
-        3: _bytes(sizes, exp_avg_sqs, "exp_avg_sqs", dev),
-        4: _bytes(blocks, m_scales, "m_scales", dev),
-        5: _bytes(blocks, v_scales, "v_scales", dev), 8: sizes})
+    _first(exp_avgs)
+    m = [t.new_empty(t.shape, dtype=torch.bfloat16) for t in exp_avgs]
+    v = [t.new_empty(t.shape, dtype=torch.bfloat16) for t in exp_avgs]
+    table, at, *_ = _lib.lists().adamw_table(m, v, exp_avgs, exp_avg_sqs, m_scales, v_scales, None,
+                                             1)
     with _guard(m[0]), _timed("adamw_8bit_values"):
-        rc = _lib.api().cpt_adamw_8bit_values(table.buffer_info()[0], len(sizes), _stream(m[0]))
+        rc = _lib.api().cpt_adamw_8bit_values(at, len(m), _stream(m[0]))
     check(rc, "adamw_8bit_values")
     return m, v
 
@@ -304,8 +184,6 @@ class AdamW(torch.optim.Optimizer):
             return s
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: the state has to be there before a step is captured")
-        if not _dense_layout(p):
-            raise AssertionError(f"parameter {tuple(p.shape)} {p.stride()}: dense expected")
         dev = p.device
         s["step"] = torch.zeros((), dtype=torch.int64, device=dev) if group["capturable"] else 0
         if group["state"] == "8bit":

@@ -18,53 +18,54 @@ import torch.nn as nn
 from . import _lib
 from ._lib import check
 from .kernels import _DT, _dtype_code, _guard, _ptr, _stream, _timed
-from .lm import _dense, _differentiable_once, _index_code, _on_device
+from .lm import _dense, _differentiable_once, _index_code, _new_like, _on_device
 
 
-def _heads(t, what):
-    """t [..., S, H, D] with contiguous columns: (t, its strides between sequences,
-    tokens and heads, batch, seq, heads, D)."""
-    assert t.dim() in (3, 4), f"{what} [B, S, H, D] or [S, H, D] expected, got {tuple(t.shape)}"
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
+def _strides(t):
+    """t [..., S, H, D] with contiguous columns, and the elements between its sequences,
+    tokens and heads."""
+    st = t.stride()
+    if st[-1] != 1 and t.shape[-1] > 1:
         t = t.contiguous()
-    if t.dim() == 3:
-        (s, h, d), st = t.shape, (0, *t.stride()[:2])
-        return t, st, 1, s, h, d
-    b, s, h, d = t.shape
-    return t, t.stride()[:3], b, s, h, d
+        st = t.stride()
+    return t, (st[:3] if len(st) == 4 else (0, st[0], st[1]))
 
 
 def _rope_args(q, k, positions, inv_freq, w_q, w_k, eps):
-    """Checks shared by both directions: (positions, its code and stride, weights' type)."""
-    assert q.dtype == k.dtype and q.dim() == k.dim() and q.shape[:-2] == k.shape[:-2] \
-        and q.shape[-1] == k.shape[-1], \
-        f"q {q.dtype} {tuple(q.shape)} and k {k.dtype} {tuple(k.shape)} share all but their heads"
-    assert q.shape[-2] > 0 and k.shape[-2] > 0, "q and k have a head at least"
-    d = q.shape[-1]
+    """Checks shared by both directions: (batch, seq, q's heads, k's, D, frequencies,
+    positions, their code and stride, weights' type)."""
+    qs, ks = q.shape, k.shape
+    assert len(qs) in (3, 4), f"q [B, S, H, D] or [S, H, D] expected, got {tuple(qs)}"
+    *lead, hq, d = qs
+    *lead_k, hk, dk = ks
+    assert lead == lead_k and d == dk and q.dtype == k.dtype, \
+        f"q {q.dtype} {tuple(qs)} and k {k.dtype} {tuple(ks)} share all but their heads"
+    assert hq > 0 and hk > 0, "q and k have a head at least"
     assert d % 2 == 0 and d > 0, f"head width {d}: even expected"
-    assert inv_freq.dtype == torch.float32 and inv_freq.dim() == 1 \
-        and 0 < 2 * inv_freq.shape[0] <= d, \
-        f"inv_freq: float32 of at most {d // 2} expected, got {inv_freq.dtype} " \
-        f"{tuple(inv_freq.shape)}"
+    assert inv_freq.dtype == torch.float32 and inv_freq.dim() == 1, \
+        f"inv_freq: float32 [R / 2] expected, got {inv_freq.dtype} {tuple(inv_freq.shape)}"
+    half = inv_freq.shape[0]
+    assert 0 < 2 * half <= d, f"inv_freq: at most {d // 2} frequencies expected, got {half}"
     assert (w_q is None) == (w_k is None), "w_q and w_k belong together"
     assert eps >= 0, f"eps={eps}"
     wdt = q.dtype
     if w_q is not None:
         wdt = w_q.dtype
-        assert wdt in (q.dtype, torch.float32), f"weights of {wdt} with heads of {q.dtype}"
+        assert wdt == q.dtype or wdt == torch.float32, f"weights of {wdt} with heads of {q.dtype}"
         for w in (w_q, w_k):
-            assert w.dtype == wdt and w.dim() == 1 and w.shape[0] == d, \
+            assert w.dtype == wdt and w.shape == (d,), \
                 f"weights: {wdt} {(d,)} expected, got {w.dtype} {tuple(w.shape)}"
-    if positions is None:
-        return None, 0, 0, _DT[wdt]
-    wide = _index_code(positions, "positions")
-    lead = q.shape[:-2]
-    if positions.dim() == 2 and positions.shape[0] == 1 and lead[-1] == positions.shape[1]:
-        positions = positions[0]
-    assert positions.shape in (lead, lead[-1:]), \
-        f"positions {tuple(positions.shape)}: {tuple(lead)} or {tuple(lead[-1:])} expected"
-    positions = positions.contiguous()
-    return positions, wide, (positions.shape[1] if positions.dim() == 2 else 0), _DT[wdt]
+    b, s = lead if len(lead) == 2 else (1, lead[0])
+    wide = pos_batch = 0
+    if positions is not None:
+        wide = _index_code(positions, "positions")
+        at = tuple(positions.shape)
+        assert at in ((b, s), (1, s), (s,)) and (len(at) == 1 or len(lead) == 2), \
+            f"positions {at}: {tuple(lead)} or {(s,)} expected"
+        if at == (b, s):
+            pos_batch = s
+        positions = positions.contiguous()
+    return b, s, hq, hk, d, 2 * half, positions, wide, pos_batch, _DT[wdt]
 
 
 def _distinct(t):
@@ -94,24 +95,24 @@ def qk_rope(q: torch.Tensor, k: torch.Tensor, positions, inv_freq: torch.Tensor,
     be the caller's own.  `inverse` turns back, without norms: the gradient."""
     _on_device(q, k, positions, inv_freq, w_q, w_k)
     dt = _dtype_code(q)
-    pos, wide, pos_batch, wdt = _rope_args(q, k, positions, inv_freq, w_q, w_k, eps)
+    b, s, hq, hk, d, rot, pos, wide, pos_batch, wdt = _rope_args(q, k, positions, inv_freq, w_q,
+                                                                 w_k, eps)
     assert not (inverse and w_q is not None), "inverse: of heads without norms"
     inv_freq, w_q, w_k = inv_freq.contiguous(), _dense(w_q), _dense(w_k)
-    q2, sq, b, s, hq, d = _heads(q, "q")
-    k2, sk, _, _, hk, _ = _heads(k, "k")
+    q2, sq = _strides(q)
+    k2, sk = _strides(k)
     if inplace:
         assert q2 is q and k2 is k and _distinct(q) and _distinct(k), \
             "inplace: heads with contiguous columns, no two elements in one place, expected"
         q_out, k_out, oq, ok = q, k, sq, sk
     else:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        q_out, k_out = _new_like(q), _new_like(k)
         oq, ok = (s * hq * d, hq * d, d), (s * hk * d, hk * d, d)
     with _guard(q), _timed("qk_rope"):
         rc = _lib.api().cpt_qk_rope(
             dt, wdt, int(interleaved), int(inverse), q2.data_ptr(), *sq, k2.data_ptr(), *sk,
             _ptr(w_q), _ptr(w_k), _ptr(pos), wide, pos_batch, inv_freq.data_ptr(), b, s, hq, hk, d,
-            2 * inv_freq.shape[0], float(eps), float(scaling), q_out.data_ptr(), *oq,
+            rot, float(eps), float(scaling), q_out.data_ptr(), *oq,
             k_out.data_ptr(), *ok, _stream(q))
     check(rc, "qk_rope")
     if inplace:
@@ -133,14 +134,14 @@ def qk_rope_backward(d_q, d_k, q, k, positions, inv_freq, *, w_q=None, w_k=None,
     for g, t in ((d_q, q), (d_k, k)):
         assert g.shape == t.shape and g.dtype == t.dtype, "gradients share q's and k's shapes " \
             "and dtype"
-    pos, wide, pos_batch, wdt = _rope_args(q, k, positions, inv_freq, w_q, w_k, eps)
+    b, s, hq, hk, d, rot, pos, wide, pos_batch, wdt = _rope_args(q, k, positions, inv_freq, w_q,
+                                                                 w_k, eps)
     inv_freq, w_q, w_k = inv_freq.contiguous(), _dense(w_q), _dense(w_k)
-    q2, sq, b, s, hq, d = _heads(q, "q")
-    k2, sk, _, _, hk, _ = _heads(k, "k")
-    gq, sgq, *_ = _heads(d_q, "d_q")
-    gk, sgk, *_ = _heads(d_k, "d_k")
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    q2, sq = _strides(q)
+    k2, sk = _strides(k)
+    gq, sgq = _strides(d_q)
+    gk, sgk = _strides(d_k)
+    dq, dk = _new_like(q), _new_like(k)
     if b * s == 0:
         return dq, dk, torch.zeros_like(w_q), torch.zeros_like(w_k)
     dw_q, dw_k = torch.empty_like(w_q), torch.empty_like(w_k)
@@ -152,7 +153,7 @@ def qk_rope_backward(d_q, d_k, q, k, positions, inv_freq, *, w_q=None, w_k=None,
         rc = L.cpt_qk_rope_backward(
             dt, wdt, int(interleaved), gq.data_ptr(), *sgq, gk.data_ptr(), *sgk, q2.data_ptr(), *sq,
             k2.data_ptr(), *sk, w_q.data_ptr(), w_k.data_ptr(), _ptr(pos), wide, pos_batch,
-            inv_freq.data_ptr(), b, s, hq, hk, d, 2 * inv_freq.shape[0], float(eps),
+            inv_freq.data_ptr(), b, s, hq, hk, d, rot, float(eps),
             float(scaling), dq.data_ptr(), dk.data_ptr(), dw_q.data_ptr(), dw_k.data_ptr(),
             ws.data_ptr(), _stream(q))
     check(rc, "qk_rope_backward")

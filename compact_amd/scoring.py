@@ -25,14 +25,15 @@ MAX_TOP = 128
 
 class TokenLogprobs(NamedTuple):
     """What token_logprobs returns; fp32 of the logits' leading shape, top_* one axis
-    more.  stats [2, rows], each row's maximum and the log of its sum, is what the
-    backward needs where lse is too coarse (logits in the thousands)."""
+    more.  stats [2, rows], where asked for: each row's maximum and the log of its sum,
+    which the backward takes in the place of lse where that is too coarse (logits in the
+    thousands)."""
     logprobs: Optional[torch.Tensor]
     entropy: torch.Tensor
     lse: torch.Tensor
     top_logprobs: Optional[torch.Tensor]
     top_indices: Optional[torch.Tensor]
-    stats: torch.Tensor
+    stats: Optional[torch.Tensor]
 
 
 def _logit_rows(z):
@@ -64,11 +65,11 @@ def _check_logits(logits, temperature):
 
 
 def token_logprobs(logits, targets=None, *, temperature: float = 1.0, top_k: int = 0,
-                   ignore_index: int = -100) -> TokenLogprobs:
+                   ignore_index: int = -100, stats: bool = False) -> TokenLogprobs:
     """Over rows of logits [..., V] with p = softmax(logits / temperature): log
     p[targets], the entropy -sum p log p, the log-sum-exp of logits / temperature, and
     the top_k <= 128 largest log p with their columns (int64), in falling order, equal
-    logits by rising column.
+    logits by rising column; with `stats` what a backward needs besides.
 
     targets: int32 or int64 [...], or None (no logprobs).  Rows whose target is
     ignore_index or outside [0, V) are left out: zeros, and alternatives of -inf at
@@ -82,21 +83,21 @@ def token_logprobs(logits, targets=None, *, temperature: float = 1.0, top_k: int
     top_k = int(top_k)
     assert 0 <= top_k <= min(v, MAX_TOP), f"top_k={top_k} of {v} (at most {MAX_TOP})"
     z, rows, seq, ld_b, ld_s = _logit_rows(logits)
-    kw = dict(dtype=torch.float32, device=logits.device)
-    logp = torch.empty(lead, **kw) if targets is not None else None
-    entropy, lse = torch.empty(lead, **kw), torch.empty(lead, **kw)
-    stats = torch.empty((2, rows), **kw)
+    new = logits.new_empty
+    logp = new(lead, dtype=torch.float32) if targets is not None else None
+    entropy, lse = new(lead, dtype=torch.float32), new(lead, dtype=torch.float32)
+    kept = new((2, rows), dtype=torch.float32) if stats else None
     top_p = top_i = None
     if top_k:
-        top_p = torch.empty((*lead, top_k), **kw)
-        top_i = torch.empty((*lead, top_k), dtype=torch.int64, device=logits.device)
+        top = (*lead, top_k)
+        top_p, top_i = new(top, dtype=torch.float32), new(top, dtype=torch.int64)
     with _guard(logits), _timed("token_logprobs"):
         rc = _lib.api().cpt_token_logprobs(
             dt, z.data_ptr(), rows, v, seq, ld_b, ld_s, wide, _ptr(targets), ignore_index,
             float(temperature), top_k, _ptr(logp), entropy.data_ptr(), lse.data_ptr(),
-            stats.data_ptr(), _ptr(top_p), _ptr(top_i), _stream(logits))
+            _ptr(kept), _ptr(top_p), _ptr(top_i), _stream(logits))
     check(rc, "token_logprobs")
-    return TokenLogprobs(logp, entropy, lse, top_p, top_i, stats)
+    return TokenLogprobs(logp, entropy, lse, top_p, top_i, kept)
 
 
 def token_logprobs_backward(logits, targets, lse, entropy, d_logprobs=None, d_entropy=None, *,
@@ -151,7 +152,7 @@ class TokenLogprobsFunction(torch.autograd.Function):
     def forward(ctx, logits, targets=None, temperature=1.0, top_k=0, ignore_index=-100,
                 inplace=False):
         r = token_logprobs(logits, targets, temperature=temperature, top_k=top_k,
-                           ignore_index=ignore_index)
+                           ignore_index=ignore_index, stats=True)
         ctx.meta = (temperature, ignore_index, inplace)
         ctx.save_for_backward(logits, targets, r.entropy, r.stats)
         ctx.set_materialize_grads(False)

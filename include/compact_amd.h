@@ -740,7 +740,7 @@ int cpt_grad_norm(int grad_dtype, const cpt_adamw_tensor* tensors, int64_t count
                   void* norm, void* workspace, void* stream);
 
 /* What 8-bit moments m, v (with their scales) stand for, as bf16, which holds them
- * exactly: m's written to `p`, v's to `master`. */
+ * exactly: m's written to `p`, v's to `g`. */
 int cpt_adamw_8bit_values(const cpt_adamw_tensor* tensors, int64_t count, void* stream);
 
 #ifdef __cplusplus

@@ -143,7 +143,7 @@ def test_backward(device, dtype, rows, vocab, tau, which):
     a = torch.randn(rows, generator=g) if which != "entropy" else None
     b = torch.randn(rows, generator=g) if which != "logprobs" else None
     zd = z.to(device)
-    r = cpt.token_logprobs(zd, y.to(device), temperature=tau)
+    r = cpt.token_logprobs(zd, y.to(device), temperature=tau, stats=True)
     on = [None if t is None else t.to(device) for t in (a, b)]
     got = cpt.token_logprobs_backward(zd, y.to(device), r.lse, r.entropy, *on, stats=r.stats,
                                       temperature=tau)
@@ -203,8 +203,8 @@ def test_strided_logits_and_inplace(device, dtype):
     z, y = _logits(30, 777, TYPES[dtype], seed=6)
     z, y = z.view(5, 6, 777).to(device), y.view(5, 6).to(device)
     view, labels = z[:, :-1], y[:, 1:]
-    want = cpt.token_logprobs(view.contiguous(), labels.contiguous(), top_k=3)
-    got = cpt.token_logprobs(view, labels, top_k=3)
+    want = cpt.token_logprobs(view.contiguous(), labels.contiguous(), top_k=3, stats=True)
+    got = cpt.token_logprobs(view, labels, top_k=3, stats=True)
     for a, b in zip(got, want):
         assert torch.equal(a, b)
     d = torch.randn(5, 5, device=device)
@@ -264,7 +264,7 @@ def test_empty_streams_and_graph(device):
     d = torch.randn(900, device=device)
 
     def both():
-        r = cpt.token_logprobs(z, y, top_k=9)
+        r = cpt.token_logprobs(z, y, top_k=9, stats=True)
         return (*r, cpt.token_logprobs_backward(z, y, None, r.entropy, d, d, stats=r.stats))
 
     want = both()
