@@ -2,15 +2,19 @@
 on the library's kernels: scaled embedding, residual norms between the blocks,
 FlashFFN v3 in every MLP, and the loss of a teacher's top logits.
 
-  forward(model, ids)      the student's logits (embedding, norms and adds fused)
+  forward(model, ids)      the student's logits (embedding, norms and adds fused; with
+                           `rope` the position rotation too)
   teacher_top(model, ids)  a teacher's top-K logits, their indices and log-sum-exp
   train_step(...)          forward, distill_loss, backward, optimizer
+  score(model, ids, ...)   each token's log probability, entropy and alternatives
 
 `python -m compact_amd.distill_step` times the step on a random-initialised
 student of the TinyLlama configuration of e2e.py (synthetic tokens, a
 random-initialised two-layer teacher); `--stock` runs torch's embedding, the
 model's own norms and adds, and the loss in elementary operations instead.
-Attention, the LM head and AdamW are stock in both.
+`--rope` turns queries and keys by qk_rope, `--optimizer adamw` (or `adamw8bit`,
+moments in 8 bits) steps by compact_amd.AdamW; otherwise these are stock as
+attention and the LM head are.
 """
 
 from __future__ import annotations
@@ -23,17 +27,37 @@ import torch.nn.functional as F
 
 from . import e2e
 from .lm import EmbeddingFunction, ResidualNormFunction, distill_loss
+from .optim import AdamW
+from .rope import QKRopeFunction
+from .scoring import token_logprobs
 
 
-def forward(model, ids, embed_scale: float = 1.0) -> torch.Tensor:
+def _attention(attn, x, rotary):
+    """A LlamaAttention over whole sequences with queries and keys turned by one
+    operator, at the model's own frequencies."""
+    b, s, _ = x.shape
+    q, k, v = (p(x).view(b, s, -1, attn.head_dim) for p in (attn.q_proj, attn.k_proj, attn.v_proj))
+    q, k = QKRopeFunction.apply(q, k, None, rotary.inv_freq.float(), None, None, 0.0, False,
+                                rotary.attention_scaling)
+    if attn.num_key_value_groups > 1:
+        k, v = (t.repeat_interleave(attn.num_key_value_groups, 2) for t in (k, v))
+    y = F.scaled_dot_product_attention(*(t.transpose(1, 2) for t in (q, k, v)), is_causal=True,
+                                       dropout_p=attn.attention_dropout if attn.training else 0.0,
+                                       scale=attn.scaling)
+    return attn.o_proj(y.transpose(1, 2).reshape(b, s, -1))
+
+
+def forward(model, ids, embed_scale: float = 1.0, rope: bool = False) -> torch.Tensor:
     """Logits of a LlamaForCausalLM for whole sequences `ids` [B, S]: the model's
     own weights, attention and MLPs; each block's residual add and the norm that
-    follows it are one operator."""
+    follows it are one operator, and with `rope` the rotation of queries and keys."""
     m = model.model
     emb = m.embed_tokens
     h = EmbeddingFunction.apply(ids, emb.weight, embed_scale, emb.padding_idx)
-    pos = torch.arange(ids.shape[1], device=ids.device).unsqueeze(0)
-    rope = m.rotary_emb(h, position_ids=pos)
+    angles = None
+    if not rope:
+        pos = torch.arange(ids.shape[1], device=ids.device).unsqueeze(0)
+        angles = m.rotary_emb(h, position_ids=pos)
     layers = list(m.layers)
 
     def norm(residual, y, module):
@@ -42,7 +66,10 @@ def forward(model, ids, embed_scale: float = 1.0) -> torch.Tensor:
 
     r, x = norm(h, None, layers[0].input_layernorm)
     for layer, after in zip(layers, [n.input_layernorm for n in layers[1:]] + [m.norm]):
-        a = layer.self_attn(x, position_embeddings=rope, attention_mask=None)[0]
+        if rope:
+            a = _attention(layer.self_attn, x, m.rotary_emb)
+        else:
+            a = layer.self_attn(x, position_embeddings=angles, attention_mask=None)[0]
         r, x = norm(r, a, layer.post_attention_layernorm)
         r, x = norm(r, layer.mlp(x), after)
     return model.lm_head(x)
@@ -71,21 +98,30 @@ def stock_loss(logits, top, idx, labels, temperature: float, alpha: float):
 
 
 def train_step(model, opt, ids, labels, top, idx, lse=None, *, temperature: float = 2.0,
-               alpha: float = 0.5, stock: bool = False) -> torch.Tensor:
-    """One step; labels [B, S] are the next tokens (-100: no loss there).  Returns
-    the loss."""
+               alpha: float = 0.5, stock: bool = False, rope: bool = False) -> torch.Tensor:
+    """One step of `opt`, torch's or compact_amd's AdamW; labels [B, S] are the next
+    tokens (-100: no loss there).  Returns the loss."""
     with e2e.fused_attention_only():
         if stock:
             logits = model(input_ids=ids, use_cache=False).logits
             loss = stock_loss(logits, top, idx, labels, temperature, alpha)
         else:
             # the logits are this step's own: their gradient takes their memory
-            loss = distill_loss(forward(model, ids), top, idx, labels, top_lse=lse,
+            loss = distill_loss(forward(model, ids, rope=rope), top, idx, labels, top_lse=lse,
                                 temperature=temperature, alpha=alpha, inplace=True)
         loss.backward()
     opt.step()
     opt.zero_grad(set_to_none=True)
     return loss.detach()
+
+
+@torch.no_grad()
+def score(model, ids, labels, top_k: int = 0, temperature: float = 1.0, rope: bool = False):
+    """TokenLogprobs [B, S] of the next tokens `labels` (-100: left out) under the model:
+    what an evaluation, a policy's old log probabilities or a teacher's soft labels are."""
+    with e2e.fused_attention_only():
+        logits = forward(model, ids, rope=rope)
+    return token_logprobs(logits, labels, top_k=top_k, temperature=temperature)
 
 
 def main(argv=None):
@@ -97,11 +133,20 @@ def main(argv=None):
     ap.add_argument("--k", type=int, default=64)
     ap.add_argument("--tail", action="store_true",
                     help="hold the teacher's mass outside its top k against the student's")
+    ap.add_argument("--rope", action="store_true", help="turn queries and keys by qk_rope")
+    ap.add_argument("--optimizer", choices=("torch", "adamw", "adamw8bit"), default="torch")
+    ap.add_argument("--max-norm", type=float, help="clip the gradients to this global norm")
     args = ap.parse_args(argv)
     assert not (args.stock and args.tail), "the stock loss has no tail"
+    assert not (args.stock and args.rope), "the stock step turns by the model's own operators"
+    assert args.max_norm is None or args.optimizer != "torch", "--max-norm: of adamw, adamw8bit"
     dev = torch.device("cuda", 0)
     cfg = dict(e2e.CONFIGS["c4"], layers=args.layers)
     model, opt = e2e.prepare(cfg, dev)
+    if args.optimizer != "torch":
+        opt = AdamW([p for p in model.parameters() if p.requires_grad], lr=1e-5,
+                    state="8bit" if args.optimizer == "adamw8bit" else "float32",
+                    max_norm=args.max_norm)
     teacher = e2e.build_llama(dict(cfg, layers=2), dev, seed=1).eval()
     ids = e2e.random_batch(cfg, dev)
     labels = torch.full_like(ids, -100)
@@ -114,13 +159,18 @@ def main(argv=None):
         torch.cuda.synchronize()
         t = time.perf_counter()
         loss = train_step(model, opt, ids, labels, top, idx, lse if args.tail else None,
-                          stock=args.stock)
+                          stock=args.stock, rope=args.rope)
         torch.cuda.synchronize()
         if i >= args.warmup:
             times.append((time.perf_counter() - t) * 1e3)
     print(f"{'stock' if args.stock else 'fused'} operators, {args.layers} layers, "
           f"{ids.numel()} tokens: {sorted(times)[len(times) // 2]:.2f} ms a step, peak "
           f"{torch.cuda.max_memory_allocated() / 2 ** 30:.2f} GiB, loss {float(loss):.4f}")
+    model.eval()
+    scores = score(model, ids, labels, rope=args.rope)
+    live = labels != -100
+    print(f"next tokens: {float(-scores.logprobs[live].mean()):.4f} nats, entropy "
+          f"{float(scores.entropy[live].mean()):.4f}")
 
 
 if __name__ == "__main__":
