@@ -73,7 +73,11 @@ struct Tensor : ScaleAddress<BITS8>, MasterAddress<MASTER> {
   int64_t n;
 };
 struct StepCommon {
-  const Control* control;         // null: no clipping
+  const Control* control;         // null: no clipping, or
+  const double* partial;          // the squares' sums, from which each block decides itself
+  float* norm;
+  int partials;
+  float max_norm;
   const DeviceStep* device_step;  // null: inv1, inv2, and keys of seed and step
   const float* lr_device;         // null: lr
   int64_t chunk;                  // elements a block, a multiple of 2048
@@ -100,13 +104,17 @@ __host__ __device__ __forceinline__ uint32_t tensor_key(uint32_t seed, uint32_t 
   return mix(seed * 0x37E15163u + step * 0x6A09E667u + i * 0x3C6EF373u);
 }
 
-// The tensor that a block works on: the last whose first block is not past it.
-__device__ __forceinline__ int find_tensor(const int* first, int count, int block) {
-  int n = 0;
-  for (int i = 0; i < count; i += 64) {
-    const int at = i + (threadIdx.x & 63);
-    n += __popcll(__ballot(at < count && first[min(at, count - 1)] <= block));
-  }
+// The tensor that a block works on: the last whose first block is not past it.  All
+// loads before the first wait.
+template <int MOST>
+__device__ __forceinline__ int find_tensor(const int (&first)[MOST], int count, int block) {
+  constexpr int kLoads = (MOST + 63) / 64;
+  const int lane = threadIdx.x & 63;
+  int v[kLoads], n = 0;
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) v[i] = first[min(i * 64 + lane, count - 1)];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) n += __popcll(__ballot(i * 64 + lane < count && v[i] <= block));
   return __builtin_amdgcn_readfirstlane(n - 1);
 }
 
@@ -175,6 +183,23 @@ __device__ __forceinline__ int block_scale(uint32_t bits, int top) {
   return max((int)(bits >> 23) - 127 - top, 1 - kScaleBias);
 }
 
+__device__ __forceinline__ Control decide(float norm, float max_norm) {
+  return Control{fminf(1.f, max_norm / add(norm, 1e-6f)), !(norm < INFINITY)};
+}
+// The root of n numbers' sum, in every thread of a block of THREADS.
+template <int THREADS>
+__device__ __forceinline__ float root_of_sum(const double* p, int n) {
+  __shared__ double part[THREADS / 64];
+  double s = 0;
+  for (int i = threadIdx.x; i < n; i += THREADS) s += p[i];
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  double t = 0;
+  for (int i = 0; i < THREADS / 64; ++i) t += part[i];
+  return (float)sqrt(t);
+}
+
 // m / (sqrt(v) + eps).  Beside moments of three bits the hardware's root and reciprocal,
 // good to one unit in the last place (and a root of a denormal to nothing) are exact
 // enough; the IEEE ones are 25 instructions of about 80 an element there.
@@ -191,9 +216,17 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const StepArgs<BITS8, M
   const int ti = find_tensor(A.first, A.count, blockIdx.x);
   const auto& T = A.t[ti];
   float clip = 1.f;
-  if (A.control) {
-    if (A.control->skip) return;
-    clip = A.control->clip;
+  if (A.control || A.partial) {
+    Control c;
+    if (A.partial) {
+      const float norm = root_of_sum<kThreads>(A.partial, A.partials);
+      if (blockIdx.x == 0 && threadIdx.x == 0) *A.norm = norm;
+      c = decide(norm, A.max_norm);
+    } else {
+      c = *A.control;
+    }
+    if (c.skip) return;
+    clip = c.clip;
   }
   float inv1 = A.inv1, inv2 = A.inv2;
   uint32_t key = tensor_key(A.seed, A.step, A.base + ti);
@@ -346,29 +379,17 @@ __global__ __launch_bounds__(kThreads) void grad_squares(const NormArgs A) {
   if (threadIdx.x == 0) A.partial[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-__device__ __forceinline__ void decide(float norm, float max_norm, Control* control) {
-  control->clip = fminf(1.f, max_norm / add(norm, 1e-6f));
-  control->skip = !(norm < INFINITY);
-}
 __global__ void decide_kernel(const float* norm, float max_norm, Control* control) {
-  decide(*norm, max_norm, control);
+  *control = decide(*norm, max_norm);
 }
 
 // The norm, and what the step does with it.  One block.
 __global__ __launch_bounds__(1024) void norm_kernel(const double* partial, int n, float max_norm,
                                                     float* norm, Control* control) {
-  __shared__ double part[16];
-  double s = 0;
-  for (int i = threadIdx.x; i < n; i += 1024) s += partial[i];
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
-  __syncthreads();
+  const float f = root_of_sum<1024>(partial, n);
   if (threadIdx.x == 0) {
-    double t = 0;
-    for (int i = 0; i < 16; ++i) t += part[i];
-    const float f = (float)sqrt(t);
     *norm = f;
-    if (control) decide(f, max_norm, control);
+    if (control) *control = decide(f, max_norm);
   }
 }
 
@@ -445,11 +466,19 @@ int64_t chunks(int64_t n, int64_t c) { return (n + c - 1) / c; }
 int64_t chunk_for(int64_t total, int64_t blocks, int64_t most) {
   return std::min(std::max<int64_t>(total / blocks / kPass, 1), most) * kPass;
 }
-// The step's: a pass while that is under eight blocks a CU (230 k elements: 3.9 us, 7.9
-// in blocks of four passes), four passes of large calls.
-int64_t step_chunk(int64_t total) { return chunk_for(total, 2048, 4); }
-// The norm's, four passes together: its blocks' sums are added by one block.
-int64_t norm_chunk(int64_t total) { return 4 * chunk_for(total, 8192, 1 << 30); }
+// The step's: few passes, so that a CU has many blocks (31 M elements in 320 tensors: 155
+// us with one pass a block, 174 with four); two where a pass's start shows (8-bit: 144
+// and 154) or blocks are many.
+int64_t step_chunk(int64_t total, bool bits8) {
+  return (bits8 || total >= 1 << 27 ? 2 : 1) * kPass;
+}
+// A small step's blocks add the norm's sums themselves, a launch less (0.5 M elements
+// clipped: 21 us, 17.6 without it); more blocks than the chip holds would each wait for them.
+constexpr int64_t kOwnNorm = 2048 * kPass;
+// The norm's: four passes together, few enough blocks for what adds their sums.
+int64_t norm_chunk(int64_t total) {
+  return 4 * chunk_for(total, total <= kOwnNorm ? 1024 : 8192, 1 << 30);
+}
 
 struct Sizes {
   int64_t total = 0;
@@ -495,7 +524,8 @@ int launch_squares(const cpt_adamw_tensor* t, int64_t count, int64_t chunk, floa
 }
 
 int grad_norm(int gd, const cpt_adamw_tensor* t, int64_t count, int64_t total, float grad_scale,
-              float max_norm, float* norm, Control* control, double* partial, hipStream_t st) {
+              float max_norm, float* norm, Control* control, double* partial, int64_t* partials,
+              hipStream_t st) {
   int64_t blocks = 0;
   const int64_t chunk = norm_chunk(total);
   const int rc = gd == kF32 ? launch_squares<kF32>(t, count, chunk, grad_scale, partial, &blocks, st)
@@ -503,6 +533,10 @@ int grad_norm(int gd, const cpt_adamw_tensor* t, int64_t count, int64_t total, f
                      ? launch_squares<kF16>(t, count, chunk, grad_scale, partial, &blocks, st)
                      : launch_squares<kBF16>(t, count, chunk, grad_scale, partial, &blocks, st);
   if (rc) return rc;
+  if (partials) {       // left to the step
+    *partials = blocks;
+    return kOk;
+  }
   norm_kernel<<<1, 1024, 0, st>>>(partial, (int)blocks, max_norm, norm, control);
   return ok();
 }
@@ -573,7 +607,7 @@ int cpt_grad_norm(int grad_dtype, const cpt_adamw_tensor* tensors, int64_t count
   for (int64_t i = 0; i < count; ++i)
     if (tensors[i].n && !tensors[i].g) return kErrShape;
   return grad_norm(grad_dtype, tensors, count, s.total, grad_scale, 0.f, (float*)norm, nullptr,
-                   (double*)workspace, (hipStream_t)stream);
+                   (double*)workspace, nullptr, (hipStream_t)stream);
 }
 
 int cpt_adamw(int dtype, int grad_dtype, int bits8, int has_master, const cpt_adamw_tensor* tensors,
@@ -599,17 +633,28 @@ int cpt_adamw(int dtype, int grad_dtype, int bits8, int has_master, const cpt_ad
   }
   if ((clip && !norm) || ((clip || on_device) && !workspace)) return kErrShape;
   const hipStream_t st = (hipStream_t)stream;
+  StepCommon C{};
   Control* control = nullptr;
   DeviceStep* steps = nullptr;
   if (clip) {
     control = (Control*)workspace;
+    bool one = !on_device && !norm_given && s.total > 0 && s.total <= kOwnNorm &&
+               count <= StepArgs<true, true>::kTensors;
+    for (int64_t i = 1; i < count; ++i) one = one && tensors[i].step == tensors[0].step;
     double* partial = (double*)((char*)workspace + kControlBytes + step_bytes(count));
+    int64_t partials = 0;
     if (norm_given) {
       decide_kernel<<<1, 1, 0, st>>>((const float*)norm, (float)max_norm, control);
       if (ok()) return kErrLaunch;
     } else if (const int rc = grad_norm(grad_dtype, tensors, count, s.total, (float)grad_scale,
-                                        (float)max_norm, (float*)norm, control, partial, st)) {
+                                        (float)max_norm, (float*)norm, control, partial,
+                                        one ? &partials : nullptr, st)) {
       return rc;
+    }
+    if (one) {
+      C.partial = partial, C.partials = (int)partials;
+      C.norm = (float*)norm, C.max_norm = (float)max_norm;
+      control = nullptr;
     }
   }
   if (on_device) {
@@ -624,9 +669,8 @@ int cpt_adamw(int dtype, int grad_dtype, int bits8, int has_master, const cpt_ad
       if (ok()) return kErrLaunch;
     }
   }
-  StepCommon C{};
   C.control = control, C.device_step = steps, C.lr_device = (const float*)lr_device;
-  C.chunk = step_chunk(s.total), C.seed = (uint32_t)seed;
+  C.chunk = step_chunk(s.total, bits8), C.seed = (uint32_t)seed;
   C.lr = (float)lr, C.wd = (float)weight_decay, C.b1 = (float)beta1, C.b2 = (float)beta2;
   C.c1 = (float)(1 - beta1), C.c2 = (float)(1 - beta2);
   C.eps = (float)eps, C.grad_scale = (float)grad_scale;
@@ -649,7 +693,7 @@ int cpt_adamw_8bit_values(const cpt_adamw_tensor* tensors, int64_t count, void* 
   for (int64_t i = 0; i < count;) {
     ValueArgs A;
     A.count = 0;
-    A.chunk = step_chunk(s.total);
+    A.chunk = step_chunk(s.total, true);
     int64_t grid = 0;
     for (; i < count && A.count < ValueArgs::kTensors; ++i) {
       const cpt_adamw_tensor& t = tensors[i];

@@ -48,25 +48,37 @@ struct RopeArgs {
   const float* inv_freq;
   int64_t pos_stride;
   FastDivU32 seq;
-  int tokens, d, rot, lanes, pos_wide, wdt;
+  int tokens, d, rot, lanes, width, pos_wide, wdt;   // width: columns of the table side by side
   float eps, scaling;
 };
 
-// A lane's eight pairs of a head: pair(t) for t = 0 .. 7.  VEC: eight neighbours,
-// moved 16 bytes at a time; otherwise (d or R not a multiple of 16) every
-// `lanes`-th, an element at a time.
+// A lane's eight pairs of a head, pair(t) for t = 0 .. 7.  VEC: eight neighbours, moved 16
+// bytes at a time at any alignment; where they would end past the head's (or, in
+// halves, past those that turn) they are the last eight, of which the lane before has
+// the first `skip` too.  Otherwise (fewer than eight of a kind) every `lanes`-th, an
+// element at a time.
 template <int DT, bool VEC, bool INTER>
 struct HeadLane {
   using R = Row8<DT>;
   using T = typename R::T;
-  int lane, lanes, pairs, rot, d;
+  int lane, lanes, pairs, rot, d, first, skip;
 
-  __device__ __forceinline__ bool on(int t) const {
-    return VEC ? lane * 8 < pairs : lane + t * lanes < pairs;
+  __device__ __forceinline__ HeadLane(int lane, int lanes, int rot, int d)
+      : lane(lane), lanes(lanes), pairs(d / 2), rot(rot), d(d) {
+    // in halves a lane has turning pairs or others: not both
+    const int ahead = INTER ? 0 : (rot / 2 + 7) / 8;
+    const bool turns = INTER || lane < ahead;
+    const int begin = turns ? 0 : rot / 2, end = INTER || !turns ? pairs : rot / 2;
+    const int want = begin + 8 * (turns ? lane : lane - ahead);
+    first = max(min(want, end - 8), 0);
+    skip = min(want - first, 8);
   }
-  // pairs past the end are taken as the last one(s)
+  __device__ __forceinline__ bool on(int t) const {
+    return VEC ? t >= skip : lane + t * lanes < pairs;
+  }
+  // without VEC pairs past the end are taken as the last one
   __device__ __forceinline__ int pair(int t) const {
-    return VEC ? min(lane * 8, pairs - 8) + t : min(lane + t * lanes, pairs - 1);
+    return VEC ? first + t : min(lane + t * lanes, pairs - 1);
   }
   __device__ __forceinline__ int col_a(int i) const {
     if (INTER) return 2 * i;
@@ -101,8 +113,8 @@ struct HeadLane {
   }
   __device__ __forceinline__ void st(T* row, const float a[8], const float b[8]) const {
     if constexpr (VEC) {
-      if (!on(0)) return;
-      const int i = lane * 8;
+      if (skip == 8) return;
+      const int i = first;      // shared pairs are stored by each: with the same values
       if constexpr (INTER) {
         float v[16];
 #pragma unroll
@@ -130,7 +142,7 @@ template <int DT, bool VEC, bool INTER>
 __device__ __forceinline__ void ld_weights(const HeadLane<DT, VEC, INTER>& io, const void* w,
                                            int wdt, float a[8], float b[8]) {
   if (DT != kF32 && wdt == kF32) {
-    const HeadLane<kF32, VEC, INTER> wide{io.lane, io.lanes, io.pairs, io.rot, io.d};
+    const HeadLane<kF32, VEC, INTER> wide(io.lane, io.lanes, io.rot, io.d);
     wide.ld((const float*)w, a, b);
   } else {
     io.ld((const typename Elem<DT>::T*)w, a, b);
@@ -143,25 +155,46 @@ __device__ __forceinline__ float head_sum(float v, int lanes) {
   return v;
 }
 
-// cos and sin of a tile's tokens, and where their rows start.
+// A token's row of the table, a hole after eight pairs: lanes that each read eight in a row
+// do not meet in LDS's banks.
+__host__ __device__ __forceinline__ int table_at(int pair) { return pair + (pair >> 3); }
+__host__ __device__ __forceinline__ int table_row(int d) { return table_at(d / 2) + 1; }
+
+// cos and sin of `turn` turns: reduced to an eighth of a turn in 64 bits, so that what is
+// left fits 32, then both Taylor series (1e-10 off at most there, 2 x 2^-24 in fp32).
+__device__ __forceinline__ float2 cos_sin(double turn) {
+  turn -= rint(turn);
+  const double quarter = rint(4.0 * turn);
+  const float x = 6.283185307179586f * (float)fma(-0.25, quarter, turn), y = x * x;
+  float c = fmaf(y, -1.f / 3628800, 1.f / 40320), s = fmaf(y, 1.f / 362880, -1.f / 5040);
+  c = fmaf(y, fmaf(y, fmaf(y, c, -1.f / 720), 1.f / 24), -0.5f);
+  s = fmaf(y, fmaf(y, s, 1.f / 120), -1.f / 6);
+  c = fmaf(y, c, 1.f);
+  s = fmaf(x * y, s, x);
+  const int q = (int)quarter & 3;
+  const float u = q & 1 ? s : c, v = q & 1 ? c : s;
+  return make_float2(q == 1 || q == 2 ? -u : u, q >= 2 ? -v : v);
+}
+
+// cos and sin of a tile's tokens, a column of pairs a thread, and where the tokens start.
 template <bool BWD>
 __device__ __forceinline__ void rope_table(const RopeArgs& A, const RopeSide& S, int t0, int nt,
                                            float2* table, int64_t (*base)[kRopeMaxTile]) {
-  const int pairs = A.d / 2, turning = A.rot / 2;
-  for (int i = threadIdx.x; i < nt * pairs; i += kRopeThreads) {
-    const int tok = i / pairs, p = i - tok * pairs;
-    float c = 1.f, s = 0.f;
-    if (p < turning) {
-      const uint32_t b = A.seq.div(t0 + tok), n = t0 + tok - b * A.seq.d;
-      const int64_t pos = A.positions ? ld_index(A.positions, A.pos_wide, b * A.pos_stride + n)
-                                      : (int64_t)n;
-      double turn = (double)pos * ((double)A.inv_freq[p] * 0.15915494309189533577);
-      turn -= rint(turn);
-      sincospif(2.f * (float)turn, &s, &c);
-      c *= A.scaling;
-      s *= A.scaling;
+  const int pairs = A.d / 2, turning = A.rot / 2, width = A.width, row = table_row(A.d);
+  for (int p = threadIdx.x & (width - 1); p < pairs; p += width) {
+    const double f = p < turning ? (double)A.inv_freq[p] * 0.15915494309189533577 : 0.0;
+    for (int tok = threadIdx.x / width; tok < nt; tok += kRopeThreads / width) {
+      float2 cs = make_float2(1.f, 0.f);
+      if (p < turning) {
+        const uint32_t b = A.seq.div(t0 + tok), n = t0 + tok - b * A.seq.d;
+        const int64_t pos = A.positions ? ld_index(A.positions, A.pos_wide, b * A.pos_stride + n)
+                                        : (int64_t)n;
+        cs = cos_sin((double)pos * f);
+        cs.x *= A.scaling;
+        cs.y *= A.scaling;
+      }
+      table[tok * row + table_at(p)] = cs;
     }
-    table[i] = make_float2(c, s);
   }
   if (threadIdx.x < nt) {
     const uint32_t b = A.seq.div(t0 + threadIdx.x), n = t0 + threadIdx.x - b * A.seq.d;
@@ -180,8 +213,8 @@ __global__ __launch_bounds__(kRopeThreads) void rope_forward(const RopeArgs A, i
   const int k_side = blockIdx.x >= A.side[0].blocks;
   const RopeSide& S = A.side[k_side];
   const int block = blockIdx.x - (k_side ? A.side[0].blocks : 0);
-  const int group = threadIdx.x / A.lanes, groups = kRopeThreads / A.lanes, pairs = A.d / 2;
-  const HeadLane<DT, VEC, INTER> io{(int)threadIdx.x & (A.lanes - 1), A.lanes, pairs, A.rot, A.d};
+  const int group = threadIdx.x / A.lanes, groups = kRopeThreads / A.lanes, row = table_row(A.d);
+  const HeadLane<DT, VEC, INTER> io((int)threadIdx.x & (A.lanes - 1), A.lanes, A.rot, A.d);
   float wa[8], wb[8];
   if (NORM) ld_weights(io, S.w, A.wdt, wa, wb);
   const int t0 = block * S.tile, nt = min(S.tile, A.tokens - t0);
@@ -202,7 +235,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_forward(const RopeArgs A, i
     }
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
-      const float2 cs = table[tok * pairs + io.pair(t)];
+      const float2 cs = table[tok * row + table_at(io.pair(t))];
       const float s = inverse ? -cs.y : cs.y;
       const float u = a[t] * cs.x - b[t] * s;
       b[t] = b[t] * cs.x + a[t] * s;
@@ -220,8 +253,8 @@ __global__ __launch_bounds__(kRopeThreads) void rope_norm_backward(const RopeArg
   const int k_side = blockIdx.x >= A.side[0].blocks;
   const RopeSide& S = A.side[k_side];
   const int block = blockIdx.x - (k_side ? A.side[0].blocks : 0);
-  const int group = threadIdx.x / A.lanes, groups = kRopeThreads / A.lanes, pairs = A.d / 2;
-  const HeadLane<DT, VEC, INTER> io{(int)threadIdx.x & (A.lanes - 1), A.lanes, pairs, A.rot, A.d};
+  const int group = threadIdx.x / A.lanes, groups = kRopeThreads / A.lanes, row = table_row(A.d);
+  const HeadLane<DT, VEC, INTER> io((int)threadIdx.x & (A.lanes - 1), A.lanes, A.rot, A.d);
   float wa[8], wb[8], da[8], db[8];
   ld_weights(io, S.w, A.wdt, wa, wb);
 #pragma unroll
@@ -240,7 +273,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_norm_backward(const RopeArg
       float ss = 0.f, sd = 0.f;
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
-        const float2 cs = table[tok * pairs + io.pair(t)];
+        const float2 cs = table[tok * row + table_at(io.pair(t))];
         const float u = ga[t] * cs.x + gb[t] * cs.y;
         gb[t] = gb[t] * cs.x - ga[t] * cs.y;
         ga[t] = u;
@@ -324,20 +357,27 @@ int pow2_at_least(int n) {
   return l;
 }
 
-// Lanes a head, and whether it moves 16 bytes at a time.
-bool rope_vec(int64_t d, int64_t rot, bool inter) {
-  return d % 16 == 0 && (inter || rot % 16 == 0);
+// Eights of a head's pairs: in halves those that turn and the others apart.
+int rope_eights(int64_t d, int64_t rot, bool inter) {
+  return (int)(inter ? (d / 2 + 7) / 8 : (rot / 2 + 7) / 8 + ((d - rot) / 2 + 7) / 8);
 }
-int rope_lanes(int64_t d) { return pow2_at_least((int)((d / 2 + 7) / 8)); }
+// Whether a head moves 16 bytes at a time: eight pairs of a kind at least, and a lane each.
+bool rope_vec(int64_t d, int64_t rot, bool inter) {
+  return (inter ? d >= 16 : rot >= 16 && (d == rot || d - rot >= 16)) &&
+         rope_eights(d, rot, inter) <= 64;
+}
+int rope_lanes(int64_t d, int64_t rot, bool inter) {
+  return pow2_at_least(rope_vec(d, rot, inter) ? rope_eights(d, rot, inter) : (int)((d / 2 + 7) / 8));
+}
 
 // Tokens a tile: as many as give every group of the block a head, and up to four times
 // that where there are tokens for 1024 blocks all the same, as far as the table holds.
 // (3009 tokens of 3 heads x 80: 10 a tile; with 3, two thirds of the block had none.)
 int rope_tile(int64_t tokens, int64_t heads, int64_t d) {
-  const int64_t groups = kRopeThreads / rope_lanes(d);
+  const int64_t groups = kRopeThreads / pow2_at_least((int)((d / 2 + 7) / 8));
   const int64_t once = std::max<int64_t>(1, groups / heads);
   const int64_t rounds = std::min<int64_t>(4, std::max<int64_t>(1, tokens / (once * 1024)));
-  const int64_t most = std::min<int64_t>(kRopeTableBytes / (d / 2 * 8), kRopeMaxTile);
+  const int64_t most = std::min<int64_t>(kRopeTableBytes / (8 * table_row((int)d)), kRopeMaxTile);
   return (int)std::max<int64_t>(1, std::min(std::min(once * rounds, most), tokens));
 }
 
@@ -435,9 +475,11 @@ int cpt_qk_rope(int dtype, int weight_dtype, int interleaved, int inverse, const
   A.positions = positions, A.pos_wide = pos_wide, A.pos_stride = pos_batch;
   A.inv_freq = (const float*)inv_freq;
   A.seq = FastDivU32::make((uint32_t)seq);
-  A.tokens = (int)tokens, A.d = (int)d, A.rot = (int)rotary, A.lanes = rope_lanes(d);
+  A.tokens = (int)tokens, A.d = (int)d, A.rot = (int)rotary;
+  A.lanes = rope_lanes(d, rotary, interleaved);
+  A.width = std::min(kRopeThreads, pow2_at_least((int)d / 2));
   A.wdt = weight_dtype, A.eps = eps, A.scaling = scaling;
-  const size_t lds = (size_t)most * (d / 2) * 8;
+  const size_t lds = (size_t)most * table_row((int)d) * 8;
   const bool vec = rope_vec(d, rotary, interleaved), norm = w_q != nullptr;
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == kF32) return launch_forward<kF32>(A, vec, interleaved, norm, inverse, lds, st);
@@ -493,10 +535,12 @@ int cpt_qk_rope_backward(int dtype, int weight_dtype, int interleaved, const voi
   A.positions = positions, A.pos_wide = pos_wide, A.pos_stride = pos_batch;
   A.inv_freq = (const float*)inv_freq;
   A.seq = FastDivU32::make((uint32_t)seq);
-  A.tokens = (int)tokens, A.d = (int)d, A.rot = (int)rotary, A.lanes = rope_lanes(d);
+  A.tokens = (int)tokens, A.d = (int)d, A.rot = (int)rotary;
+  A.lanes = rope_lanes(d, rotary, interleaved);
+  A.width = std::min(kRopeThreads, pow2_at_least((int)d / 2));
   A.wdt = weight_dtype, A.eps = eps, A.scaling = scaling;
   // the table, and at the end four rows of sums in its place
-  const size_t lds = std::max<size_t>((size_t)most * (d / 2) * 8, (size_t)d * 16);
+  const size_t lds = std::max<size_t>((size_t)most * table_row((int)d) * 8, (size_t)d * 16);
   const bool vec = rope_vec(d, rotary, interleaved);
   const hipStream_t st = (hipStream_t)stream;
   const int err = dtype == kF32   ? launch_backward<kF32>(A, vec, interleaved, lds, st)

@@ -65,7 +65,9 @@ def _check(got, x, pos, inv, w, inter, dt, scaling=1.0):
 
 SHAPES = [(1, 1, 1, 1, 2, 2), (4, 1, 32, 4, 64, 64), (2, 33, 6, 2, 128, 128), (3, 7, 5, 3, 80, 40),
           (2, 5, 3, 1, 96, 96), (1, 9, 2, 2, 6, 4), (2, 3, 7, 1, 20, 20), (1, 130, 3, 2, 48, 16),
-          (1, 2, 2, 1, 1024, 1024), (2, 3, 2, 2, 258, 130), (1, 1500, 2, 1, 16, 16)]
+          (1, 2, 2, 1, 1024, 1024), (2, 3, 2, 2, 258, 130), (1, 1500, 2, 1, 16, 16),
+          (2, 5, 3, 1, 42, 42), (1, 4, 2, 1, 300, 150), (1, 3, 2, 1, 1024, 510), (1, 3, 2, 1, 1022, 510),
+          (2, 3, 1, 1, 18, 16), (1, 70, 1, 1, 128, 128)]
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
