@@ -30,7 +30,7 @@
 #include "row_ops.h"
 
 namespace cpt {
-namespace {
+namespace adamw {
 
 constexpr int kThreads = 256;
 constexpr int kArgBytes = 4096;       // of a kernel
@@ -489,7 +489,7 @@ int tensor_sizes(const cpt_adamw_tensor* t, int64_t count, Sizes* s) {
     if (t[i].n > 1ll << 40) return kErrTooLarge;
     s->total += t[i].n;
   }
-  return s->total > 1ll << 42 ? kErrTooLarge : kOk;
+  return s->total > 1ll << 40 ? kErrTooLarge : kOk;
 }
 
 // Workspace: a Control, a DeviceStep a tensor, partial sums.
@@ -586,15 +586,16 @@ int launch_kind(const StepCommon& C, const cpt_adamw_tensor* t, int64_t count, d
                : launch_step<PD, GD, false, false>(C, t, count, beta1, beta2, st);
 }
 
-}  // namespace
+}  // namespace adamw
 }  // namespace cpt
 
 using namespace cpt;
+using namespace cpt::adamw;
 
 extern "C" {
 
 int64_t cpt_adamw_workspace_bytes(int64_t count, int64_t elements) {
-  if (count < 0 || elements < 0 || count > 1 << 24 || elements > 1ll << 42) return -1;
+  if (count < 0 || elements < 0 || count > 1 << 24 || elements > 1ll << 40) return -1;
   return workspace_bytes(count, elements);
 }
 

@@ -23,7 +23,7 @@
 #include "row_ops.h"
 
 namespace cpt {
-namespace {
+namespace logprobs {
 
 constexpr int kMaxTop = 128;          // alternatives
 constexpr int kSlots = 4;             // of a thread: four maxima each, of some of its vectors
@@ -497,16 +497,18 @@ __global__ __launch_bounds__(kGradThreads) void logprobs_grad_kernel(const LogGr
 int check_logits(int dtype, int64_t rows, int64_t vocab, int64_t seq, const void* logits,
                  float temperature) {
   if (dtype < 0 || dtype > 2) return kErrDType;
-  if (rows < 0 || vocab <= 0 || seq <= 0 || !(temperature > 0.f) || !(temperature < INFINITY))
+  if (rows < 0 || vocab <= 0 || seq <= 0 || !(temperature > 0.f) || !(temperature < INFINITY) ||
+      !(kLog2e / temperature < INFINITY))
     return kErrShape;
   if (vocab > 1 << 24 || rows > 0x7FFFFFFF) return kErrTooLarge;
   return rows && !logits ? kErrShape : kOk;
 }
 
-}  // namespace
+}  // namespace logprobs
 }  // namespace cpt
 
 using namespace cpt;
+using namespace cpt::logprobs;
 
 extern "C" {
 

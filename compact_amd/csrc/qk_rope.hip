@@ -23,7 +23,7 @@
 #include "row_ops.h"
 
 namespace cpt {
-namespace {
+namespace qkrope {
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeTableBytes = 16384;    // cos and sin of a tile of tokens
@@ -438,10 +438,11 @@ int launch_backward(const RopeArgs& A, bool vec, bool inter, size_t lds, hipStre
   return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
-}  // namespace
+}  // namespace qkrope
 }  // namespace cpt
 
 using namespace cpt;
+using namespace cpt::qkrope;
 
 extern "C" {
 

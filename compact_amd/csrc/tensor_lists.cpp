@@ -9,7 +9,6 @@
 
 #include <cstring>
 #include <string>
-#include <unordered_set>
 #include <vector>
 
 #include "compact_amd.h"
@@ -74,8 +73,6 @@ int code(at::ScalarType t) {
   return t == at::kFloat ? 0 : t == at::kHalf ? 1 : t == at::kBFloat16 ? 2 : -1;
 }
 
-int64_t address(const at::Tensor& t) { return reinterpret_cast<int64_t>(t.data_ptr()); }
-
 void expect(const at::Tensor& t, const at::Tensor& p, at::ScalarType type, const char* name) {
   if (t.scalar_type() != type || t.device() != p.device() || t.sizes() != p.sizes() || !alike(p, t))
     refuse(std::string(name) + ": " + c10::toString(type) + " that lies as " + describe(p) +
@@ -87,6 +84,31 @@ void expect_bytes(const at::Tensor& t, const at::Tensor& p, int64_t n, const cha
     refuse(std::string(name) + ": contiguous Byte of " + std::to_string(n) + " on " +
            p.device().str() + " expected, got " + describe(t));
 }
+
+// Addresses met so far; a hash table in place of a set of the library's, which allocates
+// for each.
+class Addresses {
+ public:
+  explicit Addresses(int64_t most) {
+    size_t n = 16;
+    while (n < static_cast<size_t>(2 * most)) n *= 2;
+    table_.resize(n);
+  }
+  // Whether p is new.
+  bool add(const void* p) {
+    const size_t mask = table_.size() - 1;
+    size_t at = (reinterpret_cast<uintptr_t>(p) >> 4) * 0x9E3779B97F4A7C15ull >> 32 & mask;
+    while (table_[at]) {
+      if (table_[at] == p) return false;
+      at = (at + 1) & mask;
+    }
+    table_[at] = p;
+    return true;
+  }
+
+ private:
+  std::vector<const void*> table_;
+};
 
 constexpr int64_t kBlock = 128;   // elements of an 8-bit moment that share a scale
 
@@ -147,7 +169,7 @@ void steps(PyObject* step, std::vector<cpt_adamw_tensor>& rows, const at::Device
   const List list(step, "step");
   if (list.size() != n) refuse("step: " + std::to_string(n) + " expected");
   const bool on_device = n && THPVariable_Check(list.object(0));
-  std::unordered_set<void*> seen;
+  Addresses seen(n);
   for (int64_t i = 0; i < n; ++i) {
     if (!on_device) {
       rows[i].step = number(list.object(i));
@@ -155,17 +177,17 @@ void steps(PyObject* step, std::vector<cpt_adamw_tensor>& rows, const at::Device
     }
     if (!THPVariable_Check(list.object(i))) refuse("step: a count each expected");
     rows[i].step_device = counts(list.object(i), 1);
-    if (!seen.insert(rows[i].step_device).second)
+    if (!seen.add(rows[i].step_device))
       refuse("step: a count of its own for each parameter expected");
   }
 }
 
-// adamw_table(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales, masters, step):
-// (table, address, elements, dtype, grads' dtype, [indices of gradients that lie
-// otherwise than their parameters])
+// adamw_table(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales, masters, step,
+// written): (table, address, elements, dtype, grads' dtype, [indices of gradients that lie
+// otherwise than their parameters]).  written: the moments are, and lie apart.
 PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    if (n != 8) refuse("eight arguments expected");
+    if (n != 9) refuse("nine arguments expected");
     const List p(a[0], "params"), g(a[1], "grads"), m(a[2], "exp_avgs"), v(a[3], "exp_avg_sqs"),
         ms(a[4], "m_scales"), vs(a[5], "v_scales"), w(a[6], "masters");
     for (const List* l : {&g, &m, &v, &ms, &vs, &w})
@@ -174,8 +196,8 @@ PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
                std::to_string(l->size()));
     const int64_t count = p.size();
     std::vector<cpt_adamw_tensor> rows(count);
-    std::unordered_set<void*> seen;
-    seen.reserve(count);
+    const bool written = PyObject_IsTrue(a[8]) == 1;
+    Addresses seen(6 * count);
     const at::ScalarType type = p[0].scalar_type(), grad_type = g[0].scalar_type();
     const at::Device device = p[0].device();
     if (code(type) < 0) refuse("params: unsupported " + describe(p[0]));
@@ -198,7 +220,7 @@ PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
       r.n = pi.numel();
       total += r.n;
       r.p = pi.data_ptr();
-      if (r.n && !seen.insert(r.p).second) refuse("a parameter is there twice");
+      if (r.n && !seen.add(r.p)) refuse("params: a tensor is there twice, " + describe(pi));
       if (alike(pi, gi)) {
         r.g = gi.data_ptr();
       } else {
@@ -223,6 +245,9 @@ PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
         expect(w[i], pi, at::kFloat, w.name());
         r.master = w[i].data_ptr();
       }
+      if (written && r.n)
+        for (const void* at : {r.m, r.v, r.m_scale, r.v_scale, r.master})
+          if (at && !seen.add(at)) refuse("two of a step's tensors share memory: " + describe(pi));
     }
     steps(a[7], rows, device);
     return result(rows, total, code(type), code(grad_type), otherwise.release());

@@ -35,6 +35,11 @@ def _first(tensors):
     return dev
 
 
+def _listed(tensors):
+    """None, a list or a tuple, or what else is iterable as a list."""
+    return tensors if tensors is None or type(tensors) in (list, tuple) else list(tensors)
+
+
 def _scalar(t, dev, what):
     assert t.dtype == torch.float32 and t.numel() == 1 and t.get_device() == dev, \
         f"{what}: one float32 on the tensors' device expected"
@@ -97,6 +102,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.
     tensors than these.  A norm that is not finite leaves parameters, moments and
     counts as they were."""
     params, grads = list(params), list(grads)
+    exp_avgs, exp_avg_sqs = _listed(exp_avgs), _listed(exp_avg_sqs)
+    m_scales, v_scales, masters = _listed(m_scales), _listed(v_scales), _listed(masters)
     b1, b2 = betas
     assert (m_scales is None) == (v_scales is None), "m_scales and v_scales belong together"
     assert 0 <= b1 < 1 and 0 <= b2 < 1, f"betas={betas}"
@@ -109,7 +116,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.
     assert grads, "parameters without gradients"
     dev = _first(params)
     lists = _lib.lists()
-    args = exp_avgs, exp_avg_sqs, m_scales, v_scales, masters, step
+    args = exp_avgs, exp_avg_sqs, m_scales, v_scales, masters, step, True
     table, at, total, dt, gdt, loose = lists.adamw_table(params, grads, *args)
     if loose:
         for i in loose:
@@ -148,7 +155,7 @@ def adamw_8bit_values(exp_avgs, exp_avg_sqs, m_scales, v_scales):
     m = [t.new_empty(t.shape, dtype=torch.bfloat16) for t in exp_avgs]
     v = [t.new_empty(t.shape, dtype=torch.bfloat16) for t in exp_avgs]
     table, at, *_ = _lib.lists().adamw_table(m, v, exp_avgs, exp_avg_sqs, m_scales, v_scales, None,
-                                             1)
+                                             1, False)
     with _guard(m[0]), _timed("adamw_8bit_values"):
         rc = _lib.api().cpt_adamw_8bit_values(at, len(m), _stream(m[0]))
     check(rc, "adamw_8bit_values")
@@ -206,36 +213,38 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        # lists of one type each; the state decides by itself what kind of step it needs
         buckets = {}
         for gi, group in enumerate(self.param_groups):
             for p in group["params"]:
-                if p.grad is not None:
-                    buckets.setdefault((gi, p.device, p.dtype, p.grad.dtype), []).append(p)
+                g = p.grad
+                if g is not None:
+                    s = self._init_state(p, group)
+                    buckets.setdefault((gi, p.dtype, g.dtype, p.get_device(), "m_scale" in s,
+                                        "master" in s), []).append((p, g, s))
         norm = None
         if self.max_norm is not None and len(buckets) > 1:
-            norms = [grad_norm([p.grad for p in ps], grad_scale=grad_scale)
-                     for ps in buckets.values()]
+            norms = [grad_norm([g for _, g, _ in b], grad_scale=grad_scale)
+                     for b in buckets.values()]
             norm = torch.linalg.vector_norm(torch.stack([n.to(norms[0].device) for n in norms]))
-        for k, ((gi, dev, dt, _), ps) in enumerate(buckets.items()):
+        for k, ((gi, _, _, _, bits8, master), b) in enumerate(buckets.items()):
             group = self.param_groups[gi]
-            states = [self._init_state(p, group) for p in ps]
+            params, grads, states = zip(*b)
             if group["capturable"]:
                 steps = [s["step"] for s in states]
             else:
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("AdamW: a captured step needs capturable=True")
                 steps = [s["step"] + 1 for s in states]
-            bits8 = group["state"] == "8bit"
-            lists = {n: [s[n] for s in states]
-                     for n in (("m_scale", "v_scale") if bits8 else ())}
             got = adamw_step(
-                ps, [p.grad for p in ps], [s["exp_avg"] for s in states],
-                [s["exp_avg_sq"] for s in states], steps, lr=group["lr"], betas=group["betas"],
-                eps=group["eps"], weight_decay=group["weight_decay"],
-                m_scales=lists.get("m_scale"), v_scales=lists.get("v_scale"),
-                masters=[s["master"] for s in states] if "master" in states[0] else None,
+                params, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
+                steps, lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                weight_decay=group["weight_decay"],
+                m_scales=[s["m_scale"] for s in states] if bits8 else None,
+                v_scales=[s["v_scale"] for s in states] if bits8 else None,
+                masters=[s["master"] for s in states] if master else None,
                 grad_scale=grad_scale, max_norm=self.max_norm,
-                norm=None if norm is None else norm.to(dev), seed=self.seed + k)
+                norm=None if norm is None else norm.to(params[0].device), seed=self.seed + k)
             if not group["capturable"]:
                 for s, n in zip(states, steps):
                     s["step"] = n
@@ -245,13 +254,28 @@ class AdamW(torch.optim.Optimizer):
             self.norm = norm
         return loss
 
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_norm": self.max_norm, "seed": self.seed,
+                "norm": self.norm}
+
     def load_state_dict(self, state_dict):
-        """As torch's, with every part of the state in the type that it was saved in."""
+        """As torch's, with every part of the state in the type that it was saved in.  A state
+        of torch.optim.AdamW is taken too: its moments as float32."""
         super().load_state_dict(state_dict)
+        for group in self.param_groups:
+            for name, value in self.defaults.items():
+                group.setdefault(name, value)
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        for i, p in zip(ids, params):
+        owners = [(p, g) for g in self.param_groups for p in g["params"]]
+        for i, (p, group) in zip(ids, owners):
             saved = state_dict["state"].get(i)
-            if saved is not None:
-                self.state[p] = {n: t.detach().to(p.device, copy=True)
-                                 if isinstance(t, torch.Tensor) else t for n, t in saved.items()}
+            if saved is None:
+                continue
+            s = {n: t.detach().to(p.device, copy=True) if isinstance(t, torch.Tensor) else t
+                 for n, t in saved.items()}
+            for n in ("exp_avg", "exp_avg_sq"):
+                if n in s and s[n].is_floating_point():
+                    s[n] = s[n].float()
+            count = int(s.get("step", 0))
+            s["step"] = torch.tensor(count, device=p.device) if group["capturable"] else count
+            self.state[p] = s

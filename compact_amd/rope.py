@@ -78,6 +78,19 @@ def _distinct(t):
     return True
 
 
+def _share_heads(q, k):
+    """Whether q and k are the same memory, or views of one buffer with heads in common."""
+    if q.numel() == 0 or k.numel() == 0:
+        return False
+    if q.data_ptr() == k.data_ptr():
+        return True
+    st = q.stride()
+    if st != k.stride() or q.untyped_storage().data_ptr() != k.untyped_storage().data_ptr():
+        return False
+    off = k.storage_offset() - q.storage_offset()
+    return off % st[-2] == 0 and -k.shape[-2] < off // st[-2] < q.shape[-2]
+
+
 def qk_rope(q: torch.Tensor, k: torch.Tensor, positions, inv_freq: torch.Tensor, *, w_q=None,
             w_k=None, eps: float = 1e-6, interleaved: bool = False, scaling: float = 1.0,
             inplace: bool = False, inverse: bool = False):
@@ -102,7 +115,7 @@ def qk_rope(q: torch.Tensor, k: torch.Tensor, positions, inv_freq: torch.Tensor,
     q2, sq = _strides(q)
     k2, sk = _strides(k)
     if inplace:
-        assert q2 is q and k2 is k and _distinct(q) and _distinct(k), \
+        assert q2 is q and k2 is k and _distinct(q) and _distinct(k) and not _share_heads(q, k), \
             "inplace: heads with contiguous columns, no two elements in one place, expected"
         q_out, k_out, oq, ok = q, k, sq, sk
     else:

@@ -381,6 +381,42 @@ def test_state_dict(device, state, master):
     assert abs(float(oa.norm) - float(want)) <= U * float(want)
 
 
+def test_copies_and_torchs_state(device):
+    """A copied optimizer goes on as the first; a state of torch's AdamW is taken."""
+    kw = dict(lr=1e-2, max_norm=1.0, seed=3, state="8bit")
+    a = _model(torch.bfloat16, device)
+    _grads(a, 0)
+    opt = cpt.AdamW(a.parameters(), **kw)
+    opt.step()
+    pair = copy.deepcopy((a, opt))
+    for net, o in ((a, opt), pair):
+        _grads(net, 1)
+        o.step()
+    assert all(torch.equal(x, y) for x, y in zip(a.parameters(), pair[0].parameters()))
+    assert float(pair[1].norm) == float(opt.norm)
+    b, c = _model(torch.float32, device), _model(torch.float32, device)
+    ref = torch.optim.AdamW(b.parameters(), lr=1e-2, weight_decay=0.1)
+    for i in range(2):
+        _grads(b, i)
+        ref.step()
+    for capturable in (False, True):
+        c.load_state_dict(b.state_dict())
+        own = cpt.AdamW(c.parameters(), lr=1e-2, weight_decay=0.1, capturable=capturable)
+        saved = copy.deepcopy(ref.state_dict())
+        saved["param_groups"][0]["capturable"] = capturable
+        own.load_state_dict(saved)
+        _grads(c, 5)
+        own.step()
+        d = copy.deepcopy(b)
+        there = torch.optim.AdamW(d.parameters(), lr=1e-2, weight_decay=0.1, foreach=False)
+        there.load_state_dict(copy.deepcopy(ref.state_dict()))
+        _grads(d, 5)
+        there.step()
+        for x, y in zip(c.parameters(), d.parameters()):
+            # one step's update of lr x 5 at most, and a rounding of the parameter each
+            assert (x - y).abs().max() <= 4 * U * y.abs().max() + 24 * U * 1e-2 * 5
+
+
 def test_clipping_over_several_kinds(device):
     """One norm over parameters of two types: as each list clipped by that norm."""
     a = _model(torch.bfloat16, device)

@@ -29,11 +29,7 @@ def _logits(rows, vocab, dt, seed=0):
 
 def _order(z, k):
     """Columns of the k largest values of each row, equals by column, NaN largest."""
-    out = []
-    for row in z.double().tolist():
-        key = [(-(float("inf") if x != x else x), x == x, i) for i, x in enumerate(row)]
-        out.append([i for _, _, i in sorted(key)[:k]])
-    return torch.tensor(out)
+    return torch.sort(z.double(), dim=1, descending=True, stable=True).indices[:, :k]
 
 
 def _check(r, z, y, tau, k, live=None):
@@ -69,7 +65,8 @@ def _check(r, z, y, tau, k, live=None):
 @pytest.mark.parametrize("rows,vocab,k,tau", [
     (1, 1, 1, 1.0), (3, 5, 5, 0.7), (5, 100, 20, 1.0), (2, 511, 128, 1.3), (4, 512, 64, 1.0),
     (3, 1000, 128, 1.0), (2, 2047, 17, 1.0), (2, 4097, 1, 0.7), (7, 32000, 5, 1.0),
-    (2, 50021, 50, 1.3), (1, 131075, 128, 1.0), (600, 5003, 20, 1.0), (520, 2048, 0, 1.0)])
+    (2, 50021, 50, 1.3), (1, 131075, 128, 1.0), (600, 5003, 20, 1.0),
+    (257, 70001, 30, 0.7), (300, 9000, 128, 1.0), (520, 2048, 0, 1.0)])
 def test_forward(device, dtype, rows, vocab, k, tau):
     z, y = _logits(rows, vocab, TYPES[dtype], seed=vocab)
     r = cpt.token_logprobs(z.to(device), y.to(device), temperature=tau, top_k=k)
@@ -240,6 +237,13 @@ def test_function(device):
     ref = z.to(device).requires_grad_(True)
     cpt.token_scores(ref, y.to(device), temperature=0.8)[0].sum().backward()
     assert torch.equal(leaf.grad, ref.grad)
+    mid = leaf * 1.0
+    lp = cpt.token_scores(mid, y.to(device), inplace=True)[0].sum()
+    lp.backward(retain_graph=True)
+    with pytest.raises(RuntimeError):       # the logits are gone
+        lp.backward()
+    with pytest.raises(RuntimeError):       # a leaf's gradient would be the leaf
+        cpt.token_scores(leaf, y.to(device), inplace=True)
     leaf = z.to(device).requires_grad_(True)
     mid = leaf.exp()        # its gradient needs mid itself
     lp = cpt.token_scores(mid, y.to(device), inplace=True)[0]

@@ -245,6 +245,27 @@ def test_differentiable_once_and_casts(device):
     assert m.w_q.dtype == torch.bfloat16 and "inv_freq" not in m.state_dict()
 
 
+def test_gradients_as_attention_leaves_them(device):
+    """Expanded gradients and those with heads before tokens; float32 weights."""
+    q, k, pos, inv, wq, wk = (t.to(device) for t in
+                              _make(2, 9, 4, 2, 64, 32, torch.bfloat16, True, seed=6))
+    wq, wk = wq.float(), wk.float()
+    d = [torch.randn(t.shape, device=device).bfloat16() for t in (q, k)]
+    kw = dict(w_q=wq, w_k=wk, eps=EPS)
+    want = cpt.qk_rope_backward(*d, q, k, pos, inv, **kw)
+    assert want[2].dtype == torch.float32
+    first = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in d]
+    got = cpt.qk_rope_backward(*first, q, k, pos, inv, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    one = torch.ones((), device=device, dtype=torch.bfloat16)
+    got = cpt.qk_rope_backward(one.expand_as(q), one.expand_as(k), q, k, pos, inv, **kw)
+    want = cpt.qk_rope_backward(torch.ones_like(q), torch.ones_like(k), q, k, pos, inv, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    none = cpt.qk_rope_backward(one.expand_as(q), one.expand_as(k), None, None, pos, inv)
+    want = cpt.qk_rope(torch.ones_like(q), torch.ones_like(k), pos, inv, inverse=True)
+    assert torch.equal(none[0], want[0]) and none[2] is None
+
+
 def test_repeats_bits_streams_and_graph(device):
     """The same bits on every run, on another stream, and in a graph replayed with other
     work between."""

@@ -71,6 +71,9 @@ def test_rope_refusals(library):
            lambda: cpt.qk_rope(q[:, :, :0], k, pos, inv),
            lambda: cpt.qk_rope(q.transpose(2, 3).contiguous().transpose(2, 3), k, pos, inv, inplace=True),
            lambda: cpt.qk_rope(q[:, :, :1].expand(2, 5, 4, 16), k, pos, inv, inplace=True),
+           lambda: cpt.qk_rope(q, q, pos, inv, inplace=True),
+           lambda: cpt.qk_rope(q[:, :, :3], q[:, :, 2:], pos, inv, inplace=True),
+           lambda: cpt.qk_rope(q, k, pos[None], inv), lambda: cpt.qk_rope(q[0], k[0], pos[:1], inv),
            lambda: cpt.qk_rope_backward(q, k[:, :, :1], q, k, pos, inv, w_q=w, w_k=w),
            lambda: cpt.qk_rope_backward(q.half(), k, q, k, pos, inv, w_q=w, w_k=w),
            lambda: cpt.QKNormRope(16, rotary=18), lambda: cpt.QKNormRope(16, rotary=7)]
@@ -108,6 +111,7 @@ def test_scoring_refusals(library):
     bad = [lambda: cpt.token_logprobs(z, y[:3]), lambda: cpt.token_logprobs(z, y.float()),
            lambda: cpt.token_logprobs(z, y, temperature=0.0),
            lambda: cpt.token_logprobs(z, y, temperature=float("inf")),
+           lambda: cpt.token_logprobs(z, y, temperature=float("nan")),
            lambda: cpt.token_logprobs(z, y, top_k=51), lambda: cpt.token_logprobs(z, y, top_k=-1),
            lambda: cpt.token_logprobs(torch.zeros(4, 500), y, top_k=129),
            lambda: cpt.token_logprobs(z.double(), y), lambda: cpt.token_logprobs(z[:, :0], y),
@@ -165,6 +169,7 @@ def test_adamw_refusals(library):
            lambda: s(p, g, [m[0].t().contiguous().t(), m[1]], v, 1),
            lambda: s([p[0], p[0]], [g[0], g[0]], [m[0], m[0]], [v[0], v[0]], 1),
            lambda: s([p[1][::2], p[0]], [g[1][::2], g[0]], [m[1][::2], m[0]], [v[1][::2], v[0]], 1),
+           lambda: s(p, g, m, m, 1), lambda: s(p, g, p, v, 1), lambda: s(p, g, m, [v[0], m[1]], 1),
            lambda: s(p, g, codes, codes, 1, m_scales=scales, v_scales=scales[:1]),
            lambda: s(p, g, codes, codes, 1, m_scales=scales, v_scales=scales[::-1]),
            lambda: s(p, g, m, codes, 1, m_scales=scales, v_scales=scales),
@@ -236,7 +241,7 @@ def test_c_refusals(c_abi):
                                     top, None)
 
     assert lp(dt=5) == _lib.ERR_DTYPE
-    assert lp(v=0) == lp(t=0.0) == lp(t=float("inf")) == lp(k=51) == lp(y=None) == _lib.ERR_SHAPE
+    assert lp(t=1e-39) == lp(v=0) == lp(t=0.0) == lp(t=float("inf")) == lp(k=51) == lp(y=None) == _lib.ERR_SHAPE
     assert lp(top=None) == lp(rows=-1) == _lib.ERR_SHAPE
     assert lp(v=500, k=129) == lp(v=1 << 25) == lp(rows=1 << 31) == _lib.ERR_TOO_LARGE
     assert lp(rows=0) == _lib.OK
