@@ -118,8 +118,15 @@ __device__ __forceinline__ int find_tensor(const int (&first)[MOST], int count, 
   return __builtin_amdgcn_readfirstlane(n - 1);
 }
 
-__device__ __forceinline__ float mul(float a, float b) { return __fmul_rn(a, b); }
-__device__ __forceinline__ float add(float a, float b) { return __fadd_rn(a, b); }
+// Rounded by themselves, whatever they are inlined into.
+__device__ __forceinline__ float mul(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+__device__ __forceinline__ float add(float a, float b) {
+#pragma clang fp contract(off)
+  return a + b;
+}
 
 // Eight elements [i, i + 8) of a tensor of n: whole vectors unless they end past it.
 template <int DT>
@@ -332,20 +339,16 @@ struct NormArgs {
   NormTensor t[kTensors];
 };
 
-// Eight squares' sum in fp32, the sums in 64 bits: their order does not show.  Squares
-// near the ends of fp32's range (a gradient past 2e19, all under 1e-15) in 64 bits too.
+// In 64 bits: no gradient's square is out of range, and neither the sum's order nor its
+// rounding shows in the norm.  It costs nothing beside the reading.
 __device__ __forceinline__ double squares(const float g[8], float scale) {
-  float x[8], s = 0.f;
+  double s = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    x[j] = mul(g[j], scale);
-    s = fmaf(x[j], x[j], s);
+    const double x = mul(g[j], scale);
+    s = fma(x, x, s);
   }
-  if (s >= 1e-30f && s < INFINITY) return s;
-  double d = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) d = fma((double)x[j], (double)x[j], d);
-  return d;
+  return s;
 }
 
 template <int GD>

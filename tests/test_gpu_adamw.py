@@ -137,6 +137,9 @@ def test_float32_moments(device, dtype, gtype, master, clip):
         # clip and norm are fp32 too: three roundings more of g, six of g^2
         assert ((md[i].cpu().double() - m1).abs() <= 8 * U * size + 1e-45).all()
         assert ((vd[i].cpu().double() - v1).abs() <= 12 * U * v1 + 1e-45).all()
+        if clip is None:        # each operation rounded by itself: the same bits anywhere
+            same = _moments(g[i], m[i], v[i], scale)
+            assert torch.equal(md[i].cpu(), same[0]) and torch.equal(vd[i].cpu(), same[1])
         want, up = _param(copies[i] if master else p[i], md[i].cpu(), vd[i].cpu(), t)
         _close_param(pd[i], want, up, dt)
         if master:
