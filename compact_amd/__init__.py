@@ -3,7 +3,8 @@
 A LLaMA-style SwiGLU FFN whose backward cache is int4/int8 per-group absmax
 codes of h_gate/h_up, computed by hand-written gfx950 HIP kernels behind the C
 ABI in include/compact_amd.h (libcompact_amd.so).  The
-Python API mirrors the reference's src/flashffn.py.
+Python API mirrors the reference's src/flashffn.py.  Beside it, what a training
+step needs around the FFN: lm.py, rope.py, scoring.py and optim.py.
 """
 
 from .kernels import (  # noqa: F401

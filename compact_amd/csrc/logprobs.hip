@@ -16,6 +16,11 @@
 // reach) leaves about k threads with candidates, and only those threads' columns are
 // looked at again, dealt out over the block.  Where a bound leaves too many (constant
 // rows, rows with little but -inf, NaN), a radix selection takes its place.
+//
+// Measured on one MI355X, 15% of the rows left out: 8192 x 32000 bf16 83 us without
+// alternatives (5.4 TB/s), 93 with 20, 115 with 50 in all; 1531 x 50021 fp16, 50 of them,
+// 45; 7 x 32000, 5 of them, 10; the gradient of 8192 x 32000 bf16 180 us (5.4 TB/s, in part
+// from the Infinity Cache).
 
 #include <algorithm>
 

@@ -16,6 +16,10 @@
 // Angles are products in 64 bits reduced to a turn (a position of 10^6 times a
 // frequency rounded in 32 bits is 0.03 off), once per token and pair into LDS for
 // all heads.
+//
+// Measured on one MI355X: 8192 tokens x 36 heads x 64 bf16 13.6 us (5.5 TB/s, in part from
+// the Infinity Cache); with norms 8192 x 64 x 128 bf16 46 us; its gradient 80 us (5.0
+// TB/s) and 4.8 for the partial sums; 4 tokens 3.6 us.
 
 #include <algorithm>
 
