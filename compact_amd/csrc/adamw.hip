@@ -21,7 +21,7 @@
 //
 // Bound: HBM, 22 bytes an element with 16-bit parameters and gradients and fp32
 // moments, 28 with an fp32 copy of the parameters, 10 with 8-bit moments.  The
-// tensors' pointers are kernel arguments, up to 80 a launch: no table to upload or keep.
+// tensors' pointers are kernel arguments, up to 90 a launch: no table to upload or keep.
 //
 // Measured on one MI355X: 1.1 G bf16 parameters with an fp32 copy 5760 us (5.3 TB/s) and 420
 // for the norm; 371 M with 8-bit moments 750-780 (4.9), their values 390; 31.6 M in 320
@@ -54,7 +54,7 @@ struct DeviceStep {
 };
 
 // A tensor of a launch; what a kind of step has none of takes no room, so that one
-// launch has as many tensors as fit (84 with fp32 moments alone).
+// launch has as many tensors as fit (90 with fp32 moments alone).
 template <bool BITS8>
 struct ScaleAddress {};
 template <>

@@ -279,8 +279,7 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LogArgs A) {
   const float chosen = threadIdx.x == 0 && A.targets ? Elem<DT>::ld(row + y) : 0.f;
   const int vecs = (v + 7) / 8, whole = v / 8;
 
-  // 1. maximum, sum and weighted sum of this thread's columns: four vectors at a time, the
-  // next four on their way
+  // 1. maximum, sum and weighted sum of this thread's columns: four vectors at a time
   Stats st{-INFINITY, 0.f, 0.f, 0.f, false};
   if (whole > 0) {
     Four<DT> cur;
@@ -352,7 +351,8 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LogArgs A) {
   const float log_s = logf(s) - (st.wide ? 0.f : fmaf(m, c, -st.base) * kLn2);
   if (threadIdx.x == 0) {
     A.lse[r] = empty ? -INFINITY : fmaf(m, A.inv_t, log_s);
-    A.entropy[r] = empty ? 0.f : logf(s) - (w2 / s) * kLn2;
+    const float h = logf(s) - (w2 / s) * kLn2;
+    A.entropy[r] = empty || h < 0.f ? 0.f : h;    // no less than 0 by rounding; NaN stays
     if (A.targets)
       A.logp[r] = empty ? -INFINITY : (chosen - m) * A.inv_t - log_s;
     if (A.stats) {

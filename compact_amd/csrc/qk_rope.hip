@@ -140,6 +140,11 @@ struct HeadLane {
   }
 };
 
+// A token's row of the table, a hole after eight pairs: lanes that each read eight in a row
+// do not meet in LDS's banks.
+__host__ __device__ __forceinline__ int table_at(int pair) { return pair + (pair >> 3); }
+__host__ __device__ __forceinline__ int table_row(int d) { return table_at(d / 2) + 1; }
+
 // A head's weights as a lane has its columns: one branch, then loads alone (a load
 // under a branch of its own is waited for by itself).
 template <int DT, bool VEC, bool INTER>
@@ -153,16 +158,28 @@ __device__ __forceinline__ void ld_weights(const HeadLane<DT, VEC, INTER>& io, c
   }
 }
 
+// Pairs turned by their cos and sin, `back` or forth.  Those that do not turn are left
+// alone: with cos 1 and sin 0 an infinity would make its partner NaN.
+template <int DT, bool VEC, bool INTER>
+__device__ __forceinline__ void turn(const HeadLane<DT, VEC, INTER>& io, const float2* table,
+                                     bool back, float a[8], float b[8]) {
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    const int p = io.pair(t);
+    const float2 cs = table[table_at(p)];
+    const float s = back ? -cs.y : cs.y;
+    const float u = a[t] * cs.x - b[t] * s, v = b[t] * cs.x + a[t] * s;
+    const bool turns = io.rot == io.d || p < io.rot / 2;
+    a[t] = turns ? u : a[t];
+    b[t] = turns ? v : b[t];
+  }
+}
+
 // The sum over a head's lanes, in each of them.
 __device__ __forceinline__ float head_sum(float v, int lanes) {
   for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
   return v;
 }
-
-// A token's row of the table, a hole after eight pairs: lanes that each read eight in a row
-// do not meet in LDS's banks.
-__host__ __device__ __forceinline__ int table_at(int pair) { return pair + (pair >> 3); }
-__host__ __device__ __forceinline__ int table_row(int d) { return table_at(d / 2) + 1; }
 
 // cos and sin of `turn` turns: reduced to an eighth of a turn in 64 bits, so that what is
 // left fits 32, then both Taylor series (1e-10 off at most there, 2 x 2^-24 in fp32).
@@ -237,14 +254,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_forward(const RopeArgs A, i
 #pragma unroll
       for (int t = 0; t < 8; ++t) a[t] *= rho * wa[t], b[t] *= rho * wb[t];
     }
-#pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      const float2 cs = table[tok * row + table_at(io.pair(t))];
-      const float s = inverse ? -cs.y : cs.y;
-      const float u = a[t] * cs.x - b[t] * s;
-      b[t] = b[t] * cs.x + a[t] * s;
-      a[t] = u;
-    }
+    turn(io, table + tok * row, inverse, a, b);
     io.st((T*)S.out + base[1][tok] + h * S.os[2], a, b);
   }
 }
@@ -275,13 +285,10 @@ __global__ __launch_bounds__(kRopeThreads, VEC && DT != kF32 ? 4 : 1) void rope_
       float a[8], b[8], ga[8], gb[8];
       io.ld((const T*)S.x + base[0][tok] + h * S.xs[2], a, b);
       io.ld((const T*)S.dy + base[2][tok] + h * S.ys[2], ga, gb);
+      turn(io, table + tok * row, true, ga, gb);
       float ss = 0.f, sd = 0.f;
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
-        const float2 cs = table[tok * row + table_at(io.pair(t))];
-        const float u = ga[t] * cs.x + gb[t] * cs.y;
-        gb[t] = gb[t] * cs.x - ga[t] * cs.y;
-        ga[t] = u;
         const float xa = io.on(t) ? a[t] : 0.f, xb = io.on(t) ? b[t] : 0.f;
         ss += xa * xa + xb * xb;
         sd += ga[t] * wa[t] * xa + gb[t] * wb[t] * xb;

@@ -228,6 +228,28 @@ def test_8bit_extremes(device):
     assert pd[4 * 128:].isnan().all() and pd[:4 * 128].isfinite().all()
 
 
+def test_unaligned_codes(device):
+    """Codes, scales and parameters that start anywhere in memory."""
+    n = 700
+    g = torch.Generator().manual_seed(5)
+    p, grad = torch.randn(n, generator=g).bfloat16(), torch.randn(n, generator=g).bfloat16()
+    runs = []
+    for off in (0, 1, 3, 13):
+        def at(t):
+            whole = torch.zeros(t.numel() + 32, dtype=t.dtype, device=device)
+            whole[off:off + t.numel()] = t.to(device)
+            return whole[off:off + t.numel()]
+        c = [at(torch.zeros(n, dtype=torch.uint8)) for _ in range(2)]
+        s = [at(torch.zeros(6, dtype=torch.uint8)) for _ in range(2)]
+        x, y = at(p), at(grad)
+        for t in (1, 2):
+            cpt.adamw_step([x], [y], c[:1], c[1:], t, m_scales=s[:1], v_scales=s[1:], seed=2, **HP)
+        m, v = cpt.adamw_8bit_values(c[:1], c[1:], s[:1], s[1:])
+        runs.append([x.clone(), *(t.clone() for t in c + s), m[0], v[0]])
+    for other in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+
+
 def test_layouts(device):
     """Transposed and sliced parameters, gradients that lie otherwise, unaligned starts."""
     g = torch.Generator().manual_seed(3)

@@ -170,6 +170,21 @@ def test_inplace(device, norm):
     assert torch.equal(qkv[:, :, 8:], old[:, :, 8:])
 
 
+@pytest.mark.parametrize("d,r", [(64, 32), (10, 4)])
+@pytest.mark.parametrize("inter", [False, True])
+def test_infinities_past_the_rotated_columns(device, d, r, inter):
+    """Without norms a column that does not turn is itself, whatever the others are."""
+    q, k, pos, inv, _, _ = _make(1, 3, 2, 1, d, r, torch.float32, False)
+    q[0, 1, 0, r + 1] = float("inf")
+    q[0, 1, 1, d - 1] = float("nan")
+    q[0, 2, 0, r] = -float("inf")
+    for back in (False, True):
+        got, _ = cpt.qk_rope(*(t.to(device) for t in (q, k, pos, inv)), interleaved=inter,
+                             inverse=back)
+        assert torch.equal(got[..., r:].cpu().nan_to_num(7.0), q[..., r:].nan_to_num(7.0))
+        assert got[..., :r].isfinite().all()
+
+
 def test_zeros_nan_and_empty(device):
     """A head of zeros stays zeros; NaN and inf stay in their head; no tokens, no launch."""
     q, k, pos, inv, wq, wk = (t.to(device) for t in
