@@ -529,11 +529,13 @@ int cpt_token_logprobs(int dtype, const void* logits, int64_t rows, int64_t voca
   if (!entropy || !lse || (targets != nullptr) != (logprobs != nullptr) ||
       (k && (!top_logprobs || !top_indices)))
     return kErrShape;
-  // A row is one wavefront's where it is short: nothing to wait for (30000 x 4096 bf16, 20
-  // alternatives: 61 us, with 256 threads 129; 8192 x 32000: 108 and 98), unless so many
-  // alternatives are asked that its lanes' maxima are a weak bound.  A row for each CU
-  // or fewer: the chain of loads is shorter with more threads.
-  const int threads = vocab <= 8192 && k <= 48 ? 64 : rows <= 256 && vocab > 8192 ? 1024 : 256;
+  // A row is one wavefront's where it is short: nothing to wait for (with 20 alternatives,
+  // 16384 x 12000 bf16 83 us, with 256 threads 105; 8192 x 16000 58 and 59, without
+  // alternatives 49 and 45; 8192 x 16000 fp32 93 and 85), unless so many are asked that its
+  // lanes' maxima are a weak bound.  A row for each CU or fewer: the chain of loads is
+  // shorter with more threads.
+  const bool narrow = vocab * (dtype == kF32 ? 4 : 2) <= (k > 0 ? 32768 : 24576);
+  const int threads = rows <= 256 && vocab > 8192 ? 1024 : narrow && k <= 48 ? 64 : 256;
   int shift = 0;
   while ((vocab / 8 + ((4 * threads) << shift) - 1) / ((4 * threads) << shift) > kSlots) ++shift;
   const LogArgs A{logits, targets, (float*)logprobs, (float*)entropy, (float*)lse,

@@ -84,9 +84,16 @@ def token_logprobs(logits, targets=None, *, temperature: float = 1.0, top_k: int
     assert 0 <= top_k <= min(v, MAX_TOP), f"top_k={top_k} of {v} (at most {MAX_TOP})"
     z, rows, seq, ld_b, ld_s = _logit_rows(logits)
     new = logits.new_empty
-    logp = new(lead, dtype=torch.float32) if targets is not None else None
-    entropy, lse = new(lead, dtype=torch.float32), new(lead, dtype=torch.float32)
-    kept = new((2, rows), dtype=torch.float32) if stats else None
+    logp = kept = None
+    if stats:       # for an autograd graph, whose tensors are no views of one another
+        if targets is not None:
+            logp = new(lead, dtype=torch.float32)
+        entropy, lse = new(lead, dtype=torch.float32), new(lead, dtype=torch.float32)
+        kept = new((2, rows), dtype=torch.float32)
+    elif targets is not None:
+        logp, entropy, lse = new((3, *lead), dtype=torch.float32).unbind()
+    else:
+        entropy, lse = new((2, *lead), dtype=torch.float32).unbind()
     top_p = top_i = None
     if top_k:
         top = (*lead, top_k)

@@ -66,7 +66,8 @@ def _check(r, z, y, tau, k, live=None):
     (1, 1, 1, 1.0), (3, 5, 5, 0.7), (5, 100, 20, 1.0), (2, 511, 128, 1.3), (4, 512, 64, 1.0),
     (3, 1000, 128, 1.0), (2, 2047, 17, 1.0), (2, 4097, 1, 0.7), (7, 32000, 5, 1.0),
     (2, 50021, 50, 1.3), (1, 131075, 128, 1.0), (600, 5003, 20, 1.0),
-    (257, 70001, 30, 0.7), (300, 9000, 128, 1.0), (520, 2048, 0, 1.0)])
+    (257, 70001, 30, 0.7), (300, 9000, 128, 1.0), (300, 9000, 48, 1.0),
+    (300, 12345, 0, 1.0), (1000, 16384, 20, 1.0), (520, 2048, 0, 1.0)])
 def test_forward(device, dtype, rows, vocab, k, tau):
     z, y = _logits(rows, vocab, TYPES[dtype], seed=vocab)
     r = cpt.token_logprobs(z.to(device), y.to(device), temperature=tau, top_k=k)
