@@ -46,10 +46,10 @@ class List {
   const char* name() const { return name_; }
   PyObject* object(int64_t i) const { return items_[i]; }
   const at::Tensor& operator[](int64_t i) const {
-    if (!THPVariable_Check(items_[i])) refuse(std::string(name_) + ": tensors expected");
+    if (!THPVariable_CheckExact(items_[i]) && !THPVariable_Check(items_[i]))
+      refuse(std::string(name_) + ": tensors expected");
     const at::Tensor& t = THPVariable_Unpack(items_[i]);
-    if (t.layout() != at::kStrided || t.is_complex())
-      refuse(std::string(name_) + ": dense real tensors expected");
+    if (t.layout() != at::kStrided) refuse(std::string(name_) + ": strided tensors expected");
     return t;
   }
 
@@ -195,6 +195,7 @@ PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
         refuse(std::string(l->name()) + ": " + std::to_string(p.size()) + " tensors expected, got " +
                std::to_string(l->size()));
     const int64_t count = p.size();
+    if (count == 0 || !g || !m || !v) refuse("adamw_table: tensors expected");
     std::vector<cpt_adamw_tensor> rows(count);
     const bool written = PyObject_IsTrue(a[8]) == 1;
     Addresses seen(6 * count);
@@ -208,7 +209,7 @@ PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!otherwise) throw python_error();
     int64_t total = 0;
     for (int64_t i = 0; i < count; ++i) {
-      const at::Tensor &pi = p[i], &gi = g[i];
+      const at::Tensor &pi = p[i], &gi = g[i], &mi = m[i], &vi = v[i];
       cpt_adamw_tensor& r = rows[i];
       if (pi.scalar_type() != type || pi.device() != device)
         refuse("params: " + describe(p[0]) + " and " + describe(pi));
@@ -229,21 +230,23 @@ PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
       }
       if (ms) {
         const int64_t blocks = (r.n + kBlock - 1) / kBlock;
-        expect_bytes(m[i], pi, r.n, m.name());
-        expect_bytes(v[i], pi, r.n, v.name());
-        expect_bytes(ms[i], pi, blocks, ms.name());
-        expect_bytes(vs[i], pi, blocks, vs.name());
-        r.m_scale = ms[i].data_ptr();
-        r.v_scale = vs[i].data_ptr();
+        const at::Tensor &msi = ms[i], &vsi = vs[i];
+        expect_bytes(mi, pi, r.n, m.name());
+        expect_bytes(vi, pi, r.n, v.name());
+        expect_bytes(msi, pi, blocks, ms.name());
+        expect_bytes(vsi, pi, blocks, vs.name());
+        r.m_scale = msi.data_ptr();
+        r.v_scale = vsi.data_ptr();
       } else {
-        expect(m[i], pi, at::kFloat, m.name());
-        expect(v[i], pi, at::kFloat, v.name());
+        expect(mi, pi, at::kFloat, m.name());
+        expect(vi, pi, at::kFloat, v.name());
       }
-      r.m = m[i].data_ptr();
-      r.v = v[i].data_ptr();
+      r.m = mi.data_ptr();
+      r.v = vi.data_ptr();
       if (w) {
-        expect(w[i], pi, at::kFloat, w.name());
-        r.master = w[i].data_ptr();
+        const at::Tensor& wi = w[i];
+        expect(wi, pi, at::kFloat, w.name());
+        r.master = wi.data_ptr();
       }
       if (written && r.n)
         for (const void* at : {r.m, r.v, r.m_scale, r.v_scale, r.master})
@@ -260,6 +263,7 @@ PyObject* grads_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     if (n != 1) refuse("one argument expected");
     const List g(a[0], "grads");
+    if (g.size() == 0) refuse("grads_table: tensors expected");
     std::vector<cpt_adamw_tensor> rows(g.size());
     const at::ScalarType type = g[0].scalar_type();
     const at::Device device = g[0].device();

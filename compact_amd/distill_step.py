@@ -55,7 +55,10 @@ def forward(model, ids, embed_scale: float = 1.0, rope: bool = False) -> torch.T
     emb = m.embed_tokens
     h = EmbeddingFunction.apply(ids, emb.weight, embed_scale, emb.padding_idx)
     angles = None
-    if not rope:
+    if rope:
+        kind = getattr(m.rotary_emb, "rope_type", "default")
+        assert kind not in ("dynamic", "longrope"), f"{kind}: frequencies that go by the length"
+    else:
         pos = torch.arange(ids.shape[1], device=ids.device).unsqueeze(0)
         angles = m.rotary_emb(h, position_ids=pos)
     layers = list(m.layers)

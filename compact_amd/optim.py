@@ -168,7 +168,8 @@ class AdamW(torch.optim.Optimizer):
     state: "float32" or "8bit" moments.  master: keep an fp32 copy of 16-bit
     parameters and step that.  max_norm clips all gradients by their global norm; the
     last step's norm is in `norm` (on the device), and a step whose norm is not finite
-    changes nothing.  seed: of the 8-bit moments' rounding.  capturable: step counts
+    changes nothing (but the step count, which is only known to the device where
+    capturable).  seed: of the 8-bit moments' rounding.  capturable: step counts
     on the device, so that a step can be captured into a graph (give lr as a float32
     tensor there to change it); the step before has to be an eager one, which makes the
     state."""
