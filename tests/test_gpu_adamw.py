@@ -517,3 +517,27 @@ def test_streams_and_repeated_bits(device):
         runs.append([*args[0], *args[2], *args[3], norm])
     for other in runs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+
+
+def test_elements_past_32_bits(device):
+    """The end of a tensor of over 2^32 elements, by its own numbers and the dither of its
+    place (of which 32 bits count), and its norm."""
+    n, tail = (1 << 32) + 128 * 5 + 77, 128 * 3 + 77
+    g = torch.zeros(n, dtype=torch.bfloat16, device=device)
+    part = (1e-2 * torch.randn(tail, generator=torch.Generator().manual_seed(3))).bfloat16()
+    g[-tail:] = part.to(device)
+    p = torch.ones(n, dtype=torch.bfloat16, device=device)
+    c = [torch.zeros(n, dtype=torch.uint8, device=device) for _ in range(2)]
+    s = [torch.zeros(-(-n // 128), dtype=torch.uint8, device=device) for _ in range(2)]
+    norm = cpt.adamw_step([p], [g], c[:1], c[1:], 1, m_scales=s[:1], v_scales=s[1:], seed=4,
+                          max_norm=1e6, **HP)
+    want = part.double().norm()
+    assert abs(float(norm) - want) <= U * want
+    m1, v1 = _moments(part, torch.zeros(tail), torch.zeros(tail))
+    up = _param(torch.ones(tail), m1, v1, 1)
+    _close_param(p[-tail:], *up, torch.bfloat16)
+    # elements from 2^32 + 256 on: their low 32 bits
+    for j, (x, u) in enumerate(zip((m1, v1), _dither(256 + tail, 4, 1, 0))):
+        code, scale = _encode(x, u[256:], 4 + j)
+        assert torch.equal(c[j][-tail:].cpu(), code) and torch.equal(s[j][-4:].cpu(), scale)
+    assert not c[0][:-tail].any()

@@ -288,3 +288,22 @@ def test_empty_streams_and_graph(device):
         again = both()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, again))
+
+
+def test_offsets_past_32_bits(device):
+    """Rows that start past 2^31 elements, in both directions."""
+    n, v = 67200, 32000
+    z = torch.zeros(n, v, dtype=torch.bfloat16, device=device)
+    last, y3 = _logits(3, v, torch.bfloat16, seed=9)
+    z[-3:] = last.to(device)
+    y = torch.full((n,), -100, device=device)
+    y[-3:] = y3.to(device)
+    r = cpt.token_logprobs(z, y, top_k=5, stats=True)
+    tail = cpt.TokenLogprobs(*[t[-3:] for t in r[:5]], None)
+    _check(tail, last, y3, 1.0, 5)
+    assert (r.top_indices[:-3] == -1).all() and (r.logprobs[:-3] == 0).all()
+    d = torch.randn(n, device=device)
+    grad = cpt.token_logprobs_backward(z, y, None, r.entropy, d, d, stats=r.stats)
+    want = cpt.token_logprobs_backward(z[-3:], y[-3:], None, r.entropy[-3:], d[-3:], d[-3:],
+                                       stats=r.stats[:, -3:].contiguous())
+    assert torch.equal(grad[-3:], want) and not grad[:-3].any()

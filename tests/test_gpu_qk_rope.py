@@ -308,3 +308,30 @@ def test_repeats_bits_streams_and_graph(device):
         again = both()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, again))
+
+
+def test_offsets_past_32_bits(device):
+    """Tokens that start past 2^31 elements: as a call of their own."""
+    s, h, d = 131100, 128, 128
+    q = torch.zeros(1, s, h, d, dtype=torch.bfloat16, device=device)
+    k = torch.randn(1, s, 1, d, device=device).bfloat16()
+    _, _, _, inv, wq, wk = (t.to(device) for t in _make(1, 1, 1, 1, d, d, torch.bfloat16, True))
+    g = torch.Generator(device).manual_seed(1)
+    q[:, -3:] = torch.randn(1, 3, h, d, device=device, generator=g).bfloat16()
+    pos = torch.arange(s, device=device)
+    kw = dict(w_q=wq, w_k=wk, eps=EPS)
+    big, _ = cpt.qk_rope(q, k, None, inv, **kw)
+    small, _ = cpt.qk_rope(q[:, -3:], k[:, -3:], pos[-3:], inv, **kw)
+    assert torch.equal(big[:, -3:], small) and (big[:, :7] == 0).all()
+    dq, *_ = cpt.qk_rope_backward(q, k, q, k, pos, inv, **kw)
+    small, *_ = cpt.qk_rope_backward(q[:, -3:], k[:, -3:], q[:, -3:], k[:, -3:], pos[-3:], inv, **kw)
+    assert torch.equal(dq[:, -3:], small)
+
+
+def test_inference_mode(device):
+    with torch.inference_mode():
+        q, k, pos, inv, _, _ = (t if t is None else t.to(device) for t in
+                                _make(4, 1, 4, 2, 64, 64, torch.float16, False))
+        want = cpt.qk_rope(q, k, pos, inv)
+        got = cpt.qk_rope(q, k, pos, inv, inplace=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(k, want[1])
