@@ -265,9 +265,11 @@ __global__ __launch_bounds__(kRopeThreads, VEC && DT != kF32 ? 4 : 1) void rope_
   extern __shared__ float2 table[];
   __shared__ int64_t base[3][kRopeMaxTile];
   using T = typename Elem<DT>::T;
-  const int k_side = blockIdx.x >= A.side[0].blocks;
+  // the keys first: with few heads their blocks are few and long (8192 tokens of 8 heads x
+  // 256 and one: 38 us, 35 so)
+  const int k_side = blockIdx.x < A.side[1].blocks;
   const RopeSide& S = A.side[k_side];
-  const int block = blockIdx.x - (k_side ? A.side[0].blocks : 0);
+  const int block = blockIdx.x - (k_side ? 0 : A.side[1].blocks);
   const int group = threadIdx.x / A.lanes, groups = kRopeThreads / A.lanes, row = table_row(A.d);
   const HeadLane<DT, VEC, INTER> io((int)threadIdx.x & (A.lanes - 1), A.lanes, A.rot, A.d);
   float wa[8], wb[8], da[8], db[8];
