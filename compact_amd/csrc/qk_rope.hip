@@ -175,10 +175,33 @@ __device__ __forceinline__ void turn(const HeadLane<DT, VEC, INTER>& io, const f
   }
 }
 
-// The sum over a head's lanes, in each of them.
-__device__ __forceinline__ float head_sum(float v, int lanes) {
-  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+// A thread's place: heads lie side by side in a wavefront, the lanes past the last whole
+// head idle (lane -1 of a group that no head goes to).
+struct Place {
+  int lane, group, groups;
+  __device__ __forceinline__ explicit Place(int lanes) {
+    const int in_wave = threadIdx.x & 63, per_wave = 64 / lanes, g = in_wave / lanes;
+    lane = in_wave - g * lanes;
+    groups = per_wave * (kRopeThreads / 64);
+    group = g < per_wave ? (int)(threadIdx.x >> 6) * per_wave + g : 1 << 30;
+  }
+};
+
+// The sum over a head's lanes, in each of them: by exchanges where they are a power of
+// two, otherwise folded into the first and read from there.
+__device__ __forceinline__ float head_sum(float v, int lane, int lanes) {
+  if ((lanes & (lanes - 1)) == 0) {
+    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+  }
+  int left = lanes;
+  while (left > 1) {
+    const int half = (left + 1) >> 1;
+    const float u = __shfl_down(v, half);
+    v += lane + half < left ? u : 0.f;
+    left = half;
+  }
+  return __shfl(v, (int)(threadIdx.x & 63) - lane);
 }
 
 // cos and sin of `turn` turns: reduced to an eighth of a turn in 64 bits, so that what is
@@ -234,15 +257,16 @@ __global__ __launch_bounds__(kRopeThreads) void rope_forward(const RopeArgs A, i
   const int k_side = blockIdx.x >= A.side[0].blocks;
   const RopeSide& S = A.side[k_side];
   const int block = blockIdx.x - (k_side ? A.side[0].blocks : 0);
-  const int group = threadIdx.x / A.lanes, groups = kRopeThreads / A.lanes, row = table_row(A.d);
-  const HeadLane<DT, VEC, INTER> io((int)threadIdx.x & (A.lanes - 1), A.lanes, A.rot, A.d);
+  const Place at(A.lanes);
+  const int row = table_row(A.d);
+  const HeadLane<DT, VEC, INTER> io(at.lane, A.lanes, A.rot, A.d);
   float wa[8], wb[8];
   if (NORM) ld_weights(io, S.w, A.wdt, wa, wb);
   const int t0 = block * S.tile, nt = min(S.tile, A.tokens - t0);
   rope_table<false>(A, S, t0, nt, table, base);
   __syncthreads();
   const int items = nt * S.heads.d;
-  for (int it = group; it < items; it += groups) {
+  for (int it = at.group; it < items; it += at.groups) {
     const uint32_t tok = S.heads.div(it), h = it - tok * S.heads.d;
     float a[8], b[8];
     io.ld((const T*)S.x + base[0][tok] + h * S.xs[2], a, b);
@@ -250,7 +274,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_forward(const RopeArgs A, i
       float ss = 0.f;
 #pragma unroll
       for (int t = 0; t < 8; ++t) ss += io.on(t) ? a[t] * a[t] + b[t] * b[t] : 0.f;
-      const float rho = rsqrtf(head_sum(ss, A.lanes) / A.d + A.eps);
+      const float rho = rsqrtf(head_sum(ss, at.lane, A.lanes) / A.d + A.eps);
 #pragma unroll
       for (int t = 0; t < 8; ++t) a[t] *= rho * wa[t], b[t] *= rho * wb[t];
     }
@@ -270,8 +294,9 @@ __global__ __launch_bounds__(kRopeThreads, VEC && DT != kF32 ? 4 : 1) void rope_
   const int k_side = blockIdx.x < A.side[1].blocks;
   const RopeSide& S = A.side[k_side];
   const int block = blockIdx.x - (k_side ? 0 : A.side[1].blocks);
-  const int group = threadIdx.x / A.lanes, groups = kRopeThreads / A.lanes, row = table_row(A.d);
-  const HeadLane<DT, VEC, INTER> io((int)threadIdx.x & (A.lanes - 1), A.lanes, A.rot, A.d);
+  const Place at(A.lanes);
+  const int row = table_row(A.d);
+  const HeadLane<DT, VEC, INTER> io(at.lane, A.lanes, A.rot, A.d);
   float wa[8], wb[8], da[8], db[8];
   ld_weights(io, S.w, A.wdt, wa, wb);
 #pragma unroll
@@ -282,7 +307,7 @@ __global__ __launch_bounds__(kRopeThreads, VEC && DT != kF32 ? 4 : 1) void rope_
     rope_table<true>(A, S, (int)t0, nt, table, base);
     __syncthreads();
     const int items = nt * S.heads.d;
-    for (int it = group; it < items; it += groups) {
+    for (int it = at.group; it < items; it += at.groups) {
       const uint32_t tok = S.heads.div(it), h = it - tok * S.heads.d;
       float a[8], b[8], ga[8], gb[8];
       io.ld((const T*)S.x + base[0][tok] + h * S.xs[2], a, b);
@@ -295,8 +320,8 @@ __global__ __launch_bounds__(kRopeThreads, VEC && DT != kF32 ? 4 : 1) void rope_
         ss += xa * xa + xb * xb;
         sd += ga[t] * wa[t] * xa + gb[t] * wb[t] * xb;
       }
-      ss = head_sum(ss, A.lanes);
-      sd = head_sum(sd, A.lanes);
+      ss = head_sum(ss, at.lane, A.lanes);
+      sd = head_sum(sd, at.lane, A.lanes);
       const float rho = rsqrtf(ss * inv_d + A.eps);
       const float m = rho * rho * (sd * inv_d);
 #pragma unroll
@@ -310,16 +335,20 @@ __global__ __launch_bounds__(kRopeThreads, VEC && DT != kF32 ? 4 : 1) void rope_
     }
     __syncthreads();
   }
-  // the groups' sums: within a wavefront by exchange, then one row a wavefront in LDS
-  for (int o = A.lanes; o < 64; o <<= 1)
+  // the groups' sums, in their order: within a wavefront by exchange where lanes are a power
+  // of two, then one row a wavefront, otherwise a group, in LDS
+  float* sums = reinterpret_cast<float*>(table);
+  const bool even = (A.lanes & (A.lanes - 1)) == 0;
+  if (even)
+    for (int o = A.lanes; o < 64; o <<= 1)
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      da[t] += __shfl_xor(da[t], o);
-      db[t] += __shfl_xor(db[t], o);
-    }
-  float* sums = reinterpret_cast<float*>(table);    // [4, d]
-  if ((threadIdx.x & 63) < A.lanes) {
-    float* mine = sums + (threadIdx.x >> 6) * A.d;
+      for (int t = 0; t < 8; ++t) {
+        da[t] += __shfl_xor(da[t], o);
+        db[t] += __shfl_xor(db[t], o);
+      }
+  const int rows = even ? kRopeThreads / 64 : at.groups;
+  if (even ? (threadIdx.x & 63) < A.lanes : at.group < at.groups) {
+    float* mine = sums + (even ? (int)threadIdx.x >> 6 : at.group) * A.d;
 #pragma unroll
     for (int t = 0; t < 8; ++t)
       if (io.on(t)) {
@@ -328,9 +357,12 @@ __global__ __launch_bounds__(kRopeThreads, VEC && DT != kF32 ? 4 : 1) void rope_
       }
   }
   __syncthreads();
-  for (int j = threadIdx.x; j < A.d; j += kRopeThreads)
-    S.partial[(int64_t)block * A.d + j] =
-        (sums[j] + sums[A.d + j]) + (sums[2 * A.d + j] + sums[3 * A.d + j]);
+  for (int j = threadIdx.x; j < A.d; j += kRopeThreads) {
+    float s = 0.f;
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) s += sums[r * A.d + j];
+    S.partial[(int64_t)block * A.d + j] = s;
+  }
 }
 
 // dw[j] = the blocks' partial sums, 16 columns a block, 64 threads each.
@@ -380,8 +412,13 @@ bool rope_vec(int64_t d, int64_t rot, bool inter) {
   return (inter ? d >= 16 : rot >= 16 && (d == rot || d - rot >= 16)) &&
          rope_eights(d, rot, inter) <= 64;
 }
+// Where the eights leave lanes of a power of two idle and more heads fit a wavefront
+// without, they are the lanes (8192 x 40 x 80 bf16, gradient: 43 us, 49 with 8 lanes for 5;
+// 4000 x 24 x 300 fp16 forward 24.5 and 29).
 int rope_lanes(int64_t d, int64_t rot, bool inter) {
-  return pow2_at_least(rope_vec(d, rot, inter) ? rope_eights(d, rot, inter) : (int)((d / 2 + 7) / 8));
+  if (!rope_vec(d, rot, inter)) return pow2_at_least((int)((d / 2 + 7) / 8));
+  const int eights = rope_eights(d, rot, inter), even = pow2_at_least(eights);
+  return 64 / eights > 64 / even ? eights : even;
 }
 
 // Tokens a tile: as many as give every group of the block a head, and up to four times that
@@ -390,8 +427,9 @@ int rope_lanes(int64_t d, int64_t rot, bool inter) {
 // chip holds 1024, where there are more than 1024 of both sides.  (3009 tokens of 12 and
 // 3 heads x 80 fp32: gradient 20 us, 22.5 by the forward's rule, 28 where a block had no
 // regard to its groups.)
-int rope_tile(int64_t tokens, int64_t heads, int64_t all_heads, int64_t d, bool backward) {
-  const int64_t groups = kRopeThreads / pow2_at_least((int)((d / 2 + 7) / 8));
+int rope_tile(int64_t tokens, int64_t heads, int64_t all_heads, int64_t d, int lanes,
+              bool backward) {
+  const int64_t groups = 64 / lanes * (kRopeThreads / 64);
   const int64_t once = std::max<int64_t>(1, groups / heads);
   const int64_t full = backward ? (tokens * all_heads + groups * 1024 - 1) / (groups * 1024)
                                 : tokens / (once * 1024);
@@ -488,7 +526,8 @@ int cpt_qk_rope(int dtype, int weight_dtype, int interleaved, int inverse, const
   const int64_t heads[2] = {heads_q, heads_k};
   int most = 1;
   for (int i = 0; i < 2; ++i) {
-    A.side[i].tile = rope_tile(tokens, std::max<int64_t>(heads[i], 1), heads_q + heads_k, d, false);
+    A.side[i].tile = rope_tile(tokens, std::max<int64_t>(heads[i], 1), heads_q + heads_k, d, rope_lanes(d, rotary, interleaved),
+                               false);
     A.side[i].blocks = heads[i] ? (int)rope_blocks(tokens, A.side[i].tile) : 0;
     if (heads[i]) most = std::max(most, A.side[i].tile);
   }
@@ -512,9 +551,10 @@ int64_t cpt_qk_rope_backward_workspace_bytes(int64_t tokens, int64_t heads_q, in
   if (tokens < 0 || heads_q < 0 || heads_k < 0 || d < 2 || d > 1024 || tokens >= 1ll << 30)
     return -1;
   if (tokens == 0 || heads_q == 0 || heads_k == 0) return 0;
+  // a token a tile at the least
   const int64_t all = heads_q + heads_k;
-  return (rope_blocks_bounded(tokens, rope_tile(tokens, heads_q, all, d, true), heads_q, all) +
-          rope_blocks_bounded(tokens, rope_tile(tokens, heads_k, all, d, true), heads_k, all)) *
+  return (rope_blocks_bounded(tokens, 1, heads_q, all) +
+          rope_blocks_bounded(tokens, 1, heads_k, all)) *
          d * 4;
 }
 
@@ -546,7 +586,8 @@ int cpt_qk_rope_backward(int dtype, int weight_dtype, int interleaved, const voi
   int most = 1;
   for (int i = 0; i < 2; ++i) {
     RopeSide& s = A.side[i];
-    s.tile = rope_tile(tokens, heads[i], heads_q + heads_k, d, true);
+    s.tile = rope_tile(tokens, heads[i], heads_q + heads_k, d, rope_lanes(d, rotary, interleaved),
+                       true);
     s.blocks = (int)rope_blocks_bounded(tokens, s.tile, heads[i], heads_q + heads_k);
     s.partial = ws;
     ws += (int64_t)s.blocks * d;
@@ -559,8 +600,10 @@ int cpt_qk_rope_backward(int dtype, int weight_dtype, int interleaved, const voi
   A.lanes = rope_lanes(d, rotary, interleaved);
   A.width = std::min(kRopeThreads, pow2_at_least((int)d / 2));
   A.wdt = weight_dtype, A.eps = eps, A.scaling = scaling;
-  // the table, and at the end four rows of sums in its place
-  const size_t lds = std::max<size_t>((size_t)most * table_row((int)d) * 8, (size_t)d * 16);
+  // the table, and at the end the sums of the wavefronts, or groups, in its place
+  const bool even = (A.lanes & (A.lanes - 1)) == 0;
+  const size_t rows = even ? 4 : 64 / A.lanes * 4;
+  const size_t lds = std::max<size_t>((size_t)most * table_row((int)d) * 8, rows * d * 4);
   const bool vec = rope_vec(d, rotary, interleaved);
   const hipStream_t st = (hipStream_t)stream;
   const int err = dtype == kF32   ? launch_backward<kF32>(A, vec, interleaved, lds, st)
