@@ -190,6 +190,7 @@ class AdamW(torch.optim.Optimizer):
         s = self.state[p]
         if s:
             return s
+        _require_device(p)
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: the state has to be there before a step is captured")
         dev = p.device

@@ -54,6 +54,16 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+def test_optimizer_refuses_cpu_parameters():
+    p = torch.nn.Parameter(torch.zeros(4))
+    p.grad = torch.ones(4)
+    for kw in ({}, {"capturable": True}, {"state": "8bit", "max_norm": 1.0}):
+        opt = cpt.AdamW([p], **kw)
+        with pytest.raises(RuntimeError, match="HIP device only"):
+            opt.step()
+        assert not opt.state[p] and torch.equal(p.detach(), torch.zeros(4))
+
+
 def test_rope_refusals(library):
     q, k, inv = torch.zeros(2, 5, 4, 16), torch.zeros(2, 5, 2, 16), torch.ones(8)
     w, pos = torch.ones(16), torch.zeros(2, 5, dtype=torch.int64)
