@@ -215,23 +215,35 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        # lists of one type each; the state decides by itself what kind of step it needs
-        buckets = {}
-        for gi, group in enumerate(self.param_groups):
-            for p in group["params"]:
-                g = p.grad
-                if g is not None:
-                    s = self._init_state(p, group)
-                    buckets.setdefault((gi, p.dtype, g.dtype, p.get_device(), "m_scale" in s,
-                                        "master" in s), []).append((p, g, s))
+        # lists of one kind each: the types, the device, and what the state holds (each kind of
+        # state has another number of parts)
+        buckets = []
+        for group in self.param_groups:
+            params = group["params"]
+            grads = [p.grad for p in params]
+            if any([g is None for g in grads]):
+                params = [p for p, g in zip(params, grads) if g is not None]
+                grads = [g for g in grads if g is not None]
+            if not params:
+                continue
+            states = [self.state[p] for p in params]
+            if not all(states):
+                states = [self._init_state(p, group) for p in params]
+            same = _lib.lists().one_kind
+            if same(params) and same(grads) and len({len(s) for s in states}) == 1:
+                buckets.append((group, params, grads, states))
+                continue
+            kinds = [(p.dtype, g.dtype, p.get_device(), len(s))
+                     for p, g, s in zip(params, grads, states)]
+            for kind in dict.fromkeys(kinds):
+                at = [i for i, other in enumerate(kinds) if other == kind]
+                buckets.append((group, *([x[i] for i in at] for x in (params, grads, states))))
         norm = None
         if self.max_norm is not None and len(buckets) > 1:
-            norms = [grad_norm([g for _, g, _ in b], grad_scale=grad_scale)
-                     for b in buckets.values()]
+            norms = [grad_norm(grads, grad_scale=grad_scale) for _, _, grads, _ in buckets]
             norm = torch.linalg.vector_norm(torch.stack([n.to(norms[0].device) for n in norms]))
-        for k, ((gi, _, _, _, bits8, master), b) in enumerate(buckets.items()):
-            group = self.param_groups[gi]
-            params, grads, states = zip(*b)
+        for k, (group, params, grads, states) in enumerate(buckets):
+            bits8, master = "m_scale" in states[0], "master" in states[0]
             if group["capturable"]:
                 steps = [s["step"] for s in states]
             else:
