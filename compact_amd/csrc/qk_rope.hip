@@ -163,15 +163,18 @@ __device__ __forceinline__ void ld_weights(const HeadLane<DT, VEC, INTER>& io, c
 template <int DT, bool VEC, bool INTER>
 __device__ __forceinline__ void turn(const HeadLane<DT, VEC, INTER>& io, const float2* table,
                                      bool back, float a[8], float b[8]) {
+  // in halves a lane's eight are of a kind
+  if (VEC && !INTER && io.first >= io.rot / 2) return;
+  const float sign = back ? -1.f : 1.f;
+  const bool all = (VEC && !INTER) || io.rot == io.d;
 #pragma unroll
   for (int t = 0; t < 8; ++t) {
     const int p = io.pair(t);
     const float2 cs = table[table_at(p)];
-    const float s = back ? -cs.y : cs.y;
+    const float s = sign * cs.y;
     const float u = a[t] * cs.x - b[t] * s, v = b[t] * cs.x + a[t] * s;
-    const bool turns = io.rot == io.d || p < io.rot / 2;
-    a[t] = turns ? u : a[t];
-    b[t] = turns ? v : b[t];
+    a[t] = all || p < io.rot / 2 ? u : a[t];
+    b[t] = all || p < io.rot / 2 ? v : b[t];
   }
 }
 
