@@ -189,4 +189,6 @@ def token_scores(logits, targets=None, *, temperature: float = 1.0, top_k: int =
     """token_logprobs' (logprobs, entropy, lse, top_logprobs, top_indices), the first two
     differentiable in the logits.  `inplace` lets the gradient take the logits' memory
     (they must not be read after the backward)."""
-    return TokenLogprobsFunction.apply(logits, targets, temperature, top_k, ignore_index, inplace)
+    # without gradients nothing is taken: a leaf is then as good as any
+    return TokenLogprobsFunction.apply(logits, targets, temperature, top_k, ignore_index,
+                                       inplace and torch.is_grad_enabled())

@@ -245,6 +245,8 @@ def test_function(device):
         lp.backward()
     with pytest.raises(RuntimeError):       # a leaf's gradient would be the leaf
         cpt.token_scores(leaf, y.to(device), inplace=True)
+    with torch.no_grad():                   # no gradient: nothing to refuse
+        cpt.token_scores(leaf, y.to(device), inplace=True)
     leaf = z.to(device).requires_grad_(True)
     mid = leaf.exp()        # its gradient needs mid itself
     lp = cpt.token_scores(mid, y.to(device), inplace=True)[0]
