@@ -274,7 +274,13 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, with every part of the state in the type that it was saved in.  A state
-        of torch.optim.AdamW is taken too: its moments as float32."""
+        of torch.optim.AdamW is taken too: its moments as float32.  One whose options ask for
+        another formula (maximize, amsgrad, decay within the gradient) is refused."""
+        for g in state_dict["param_groups"]:
+            for name in ("maximize", "amsgrad"):
+                assert not g.get(name), f"AdamW: a state with {name}={g[name]} cannot go on here"
+            assert g.get("decoupled_weight_decay", True) or g["weight_decay"] == 0, \
+                "AdamW: a state with decay within the gradient cannot go on here"
         super().load_state_dict(state_dict)
         for group in self.param_groups:
             for name, value in self.defaults.items():
