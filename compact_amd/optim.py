@@ -188,22 +188,24 @@ class AdamW(torch.optim.Optimizer):
 
     def _init_state(self, p, group):
         s = self.state[p]
-        if s:
+        master = group["master"] and p.dtype != torch.float32
+        if s and (not master or "master" in s):
             return s
         _require_device(p)
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: the state has to be there before a step is captured")
         dev = p.device
-        s["step"] = torch.zeros((), dtype=torch.int64, device=dev) if group["capturable"] else 0
-        if group["state"] == "8bit":
-            n, blocks = p.numel(), -(-p.numel() // BLOCK)
-            for name, size in (("exp_avg", n), ("exp_avg_sq", n), ("m_scale", blocks),
-                               ("v_scale", blocks)):
-                s[name] = torch.zeros(size, dtype=torch.uint8, device=dev)
-        else:
-            s["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
-            s["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
-        if group["master"] and p.dtype != torch.float32:
+        if not s:
+            s["step"] = torch.zeros((), dtype=torch.int64, device=dev) if group["capturable"] else 0
+            if group["state"] == "8bit":
+                n, blocks = p.numel(), -(-p.numel() // BLOCK)
+                for name, size in (("exp_avg", n), ("exp_avg_sq", n), ("m_scale", blocks),
+                                   ("v_scale", blocks)):
+                    s[name] = torch.zeros(size, dtype=torch.uint8, device=dev)
+            else:
+                s["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
+                s["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
+        if master:
             s["master"] = p.detach().to(torch.float32, copy=True)
         return s
 
@@ -227,7 +229,7 @@ class AdamW(torch.optim.Optimizer):
             if not params:
                 continue
             states = [self.state[p] for p in params]
-            if not all(states):
+            if not all(states) or (group["master"] and not all(["master" in s for s in states])):
                 states = [self._init_state(p, group) for p in params]
             same = _lib.lists().one_kind
             if same(params) and same(grads) and len({len(s) for s in states}) == 1:
@@ -274,7 +276,8 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, with every part of the state in the type that it was saved in.  A state
-        of torch.optim.AdamW is taken too: its moments as float32.  One whose options ask for
+        of torch.optim.AdamW is taken too: its moments as float32; the fp32 copy that `master`
+        asks for is then made of the parameters by the next step.  One whose options ask for
         another formula (maximize, amsgrad, decay within the gradient) is refused."""
         for g in state_dict["param_groups"]:
             for name in ("maximize", "amsgrad"):

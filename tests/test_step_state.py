@@ -68,3 +68,34 @@ def test_states_of_another_formula_are_refused(library, kw):
     # without decay Adam is AdamW
     own.load_state_dict(_torch_state(ps, opt=torch.optim.Adam))
     assert own.state[ps[0]]["step"] == 1
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_loaded_state_gets_its_fp32_copy(library, dtype):
+    """master=True and a state without the copies: the step makes them of the parameters as
+    they then are, and steps them."""
+    ps = _params(dtype, dtype)
+    own = cpt.AdamW(ps, master=True)
+    own.load_state_dict(_torch_state(ps))
+    with torch.no_grad():       # the model's weights may be loaded after the optimizer's state
+        ps[0].mul_(3)
+    own.step()
+    (call,) = library.steps()
+    assert call[3] == 1
+    for p in ps:
+        s = own.state[p]
+        assert s["step"] == 2 and s["exp_avg"].dtype == torch.float32
+        assert s["master"].dtype == torch.float32 and torch.equal(s["master"], p.detach().float())
+    kept = [own.state[p]["master"] for p in ps]
+    own.step()
+    assert all(own.state[p]["master"] is m for p, m in zip(ps, kept))
+
+
+def test_a_captured_step_needs_the_fp32_copy(library, monkeypatch):
+    ps = _params(torch.bfloat16)
+    own = cpt.AdamW(ps, master=True, capturable=True)
+    own.load_state_dict(_torch_state(ps))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before a step is captured"):
+        own.step()
+    assert "master" not in own.state[ps[0]] and not library.steps()
