@@ -217,8 +217,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        # lists of one kind each: the types, the device, and what the state holds (each kind of
-        # state has another number of parts)
+        # lists of one kind each: the types, the device, and what the state holds
         buckets = []
         for group in self.param_groups:
             params = group["params"]
@@ -232,11 +231,12 @@ class AdamW(torch.optim.Optimizer):
             if not all(states) or (group["master"] and not all(["master" in s for s in states])):
                 states = [self._init_state(p, group) for p in params]
             same = _lib.lists().one_kind
-            if same(params) and same(grads) and len({len(s) for s in states}) == 1:
+            held = [("m_scale" in s, "master" in s) for s in states]
+            if same(params) and same(grads) and len(set(held)) == 1:
                 buckets.append((group, params, grads, states))
                 continue
-            kinds = [(p.dtype, g.dtype, p.get_device(), len(s))
-                     for p, g, s in zip(params, grads, states)]
+            kinds = [(p.dtype, g.dtype, p.get_device(), h)
+                     for p, g, h in zip(params, grads, held)]
             for kind in dict.fromkeys(kinds):
                 at = [i for i, other in enumerate(kinds) if other == kind]
                 buckets.append((group, *([x[i] for i in at] for x in (params, grads, states))))

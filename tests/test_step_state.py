@@ -99,3 +99,24 @@ def test_a_captured_step_needs_the_fp32_copy(library, monkeypatch):
     with pytest.raises(RuntimeError, match="before a step is captured"):
         own.step()
     assert "master" not in own.state[ps[0]] and not library.steps()
+
+
+def test_kinds_of_state_go_by_their_parts(library):
+    """A state with a part of the caller's own beside one with as many parts, one of them an
+    fp32 copy: two lists, each in its form."""
+    ps = _params(torch.bfloat16, torch.bfloat16)
+    own = cpt.AdamW([{"params": ps[:1]}])
+    own.step()
+    own.state[ps[0]]["note"] = "kept"
+    own.param_groups[0]["params"].append(ps[1])
+    own.state[ps[1]].update(own.state[ps[0]], master=ps[1].detach().float(), step=3)
+    for n in ("exp_avg", "exp_avg_sq"):
+        own.state[ps[1]][n] = torch.zeros(5)
+    del own.state[ps[1]]["note"]
+    assert len(own.state[ps[0]]) == len(own.state[ps[1]]) == 4
+    for order in (1, -1):
+        library.calls.clear()
+        own.param_groups[0]["params"] = ps[::order]
+        own.step()
+        assert [a[3] for a in library.steps()] == [0, 1][::order]
+    assert own.state[ps[0]]["note"] == "kept" and own.state[ps[1]]["step"] == 5
