@@ -276,18 +276,23 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, with every part of the state in the type that it was saved in.  A state
-        of torch.optim.AdamW is taken too: its moments as float32; the fp32 copy that `master`
-        asks for is then made of the parameters by the next step.  One whose options ask for
+        of torch.optim.AdamW is taken too: its moments as float32
+        (and the group's `state` with them); the fp32 copy that `master` asks for is then made
+        of the parameters by the next step.  One whose options ask for
         another formula (maximize, amsgrad, decay within the gradient) is refused."""
         for g in state_dict["param_groups"]:
             for name in ("maximize", "amsgrad"):
                 assert not g.get(name), f"AdamW: a state with {name}={g[name]} cannot go on here"
             assert g.get("decoupled_weight_decay", True) or g["weight_decay"] == 0, \
                 "AdamW: a state with decay within the gradient cannot go on here"
+        before = self.param_groups
         super().load_state_dict(state_dict)
-        for group in self.param_groups:
-            for name, value in self.defaults.items():
+        # what a state of torch's does not say stays as each group has it
+        for group, old, saved in zip(self.param_groups, before, state_dict["param_groups"]):
+            for name, value in old.items():
                 group.setdefault(name, value)
+            if "state" not in saved and any(i in state_dict["state"] for i in saved["params"]):
+                group["state"] = "float32"      # as the moments that came
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         owners = [(p, g) for g in self.param_groups for p in g["params"]]
         for i, (p, group) in zip(ids, owners):

@@ -120,3 +120,28 @@ def test_kinds_of_state_go_by_their_parts(library):
         own.step()
         assert [a[3] for a in library.steps()] == [0, 1][::order]
     assert own.state[ps[0]]["note"] == "kept" and own.state[ps[1]]["step"] == 5
+
+
+def test_loading_keeps_each_groups_own_options(library):
+    """torch's state says nothing of `state` and `master`: they stay what the groups, not the
+    optimizer's defaults, say; moments that came are float32, and so is the group's state."""
+    ps = _params(torch.bfloat16, torch.bfloat16, torch.bfloat16)
+    groups = [{"params": ps[:1], "master": True}, {"params": ps[1:2], "state": "8bit"},
+              {"params": ps[2:]}]
+    saved = _torch_state(ps)
+    of = saved["param_groups"][0]
+    saved["param_groups"] = [{**of, "params": [i]} for i in range(3)]
+    del saved["state"][1]           # of a parameter that was not stepped
+    own = cpt.AdamW(groups, state="8bit")
+    own.load_state_dict(saved)
+    assert [(g["state"], g["master"]) for g in own.param_groups] == \
+        [("float32", True), ("8bit", False), ("float32", False)]
+    own.step()
+    assert [tuple(own.state[p]) for p in ps] == \
+        [("step", "exp_avg", "exp_avg_sq", "master"),
+         ("step", "exp_avg", "exp_avg_sq", "m_scale", "v_scale"), ("step", "exp_avg", "exp_avg_sq")]
+    # its own state says all of it
+    again = cpt.AdamW([{"params": [p]} for p in ps])
+    again.load_state_dict(own.state_dict())
+    assert [(g["state"], g["master"]) for g in again.param_groups] == \
+        [(g["state"], g["master"]) for g in own.param_groups]
