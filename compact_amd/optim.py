@@ -243,7 +243,9 @@ class AdamW(torch.optim.Optimizer):
         norm = None
         if self.max_norm is not None and len(buckets) > 1:
             norms = [grad_norm(grads, grad_scale=grad_scale) for _, _, grads, _ in buckets]
-            norm = torch.linalg.vector_norm(torch.stack([n.to(norms[0].device) for n in norms]))
+            # squares in 64 bits, as each list's own: those of norms past 1e19 are inf in fp32
+            norm = torch.linalg.vector_norm(torch.stack([n.to(norms[0].device) for n in norms]),
+                                            dtype=torch.float64).float()
         for k, (group, params, grads, states) in enumerate(buckets):
             bits8, master = "m_scale" in states[0], "master" in states[0]
             if group["capturable"]:

@@ -1,0 +1,72 @@
+"""The optimizer over several lists, states and options, on the device.  Tolerances as
+test_gpu_adamw.py derives them."""
+
+import copy
+
+import pytest
+import torch
+
+import compact_amd as cpt
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+def _two(device, dtypes=(torch.float32, torch.float32), sizes=(300, 5000), seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.nn.Parameter(torch.randn(n, generator=g).to(device, t))
+            for n, t in zip(sizes, dtypes)]
+
+
+def _draw(ps, i, size=1.0):
+    g = torch.Generator().manual_seed(50 + i)
+    return [(size * torch.randn(p.shape, generator=g)).to(p.device, p.dtype) for p in ps]
+
+
+@pytest.mark.parametrize("size", [1e-25, 1e-2, 1e20, 1e30])
+def test_the_norm_does_not_go_by_the_groups(device, size):
+    """One group and two: the same norm to a rounding of each list's, and a step of the same
+    clipped gradients (the clip to 3 roundings, the update to 12 more)."""
+    one, two = _two(device), _two(device)
+    opts = [cpt.AdamW(one, lr=1e-2, max_norm=1.0),
+            cpt.AdamW([{"params": [p]} for p in two], lr=1e-2, max_norm=1.0)]
+    before = [p.detach().clone() for p in one]
+    for ps, opt in zip((one, two), opts):
+        for p, g in zip(ps, _draw(ps, 0, size)):
+            p.grad = g
+        opt.step()
+    want = torch.cat([p.grad.double() for p in one]).norm()
+    for opt in opts:
+        assert abs(float(opt.norm) - float(want)) <= 3 * U * float(want)
+    for a, b, old in zip(one, two, before):
+        # every update is at most lr, decay lr x 1e-2 |p|
+        assert ((a - b).abs() <= 2 * U * old.abs() + 24 * U * 1e-2).all()
+        if size > 1e-20:        # below, eps outweighs the gradient's root
+            assert (a != old).all()
+
+
+def test_captured_step_over_two_lists(device):
+    """A graph of a clipped step over two types, replayed with eager work between: as eager."""
+    types = (torch.float32, torch.bfloat16)
+    nets = [_two(device, types) for _ in range(2)]
+    opts = [cpt.AdamW(n, lr=1e-2, max_norm=0.5, capturable=True, state="8bit") for n in nets]
+    for net, opt in zip(nets, opts):
+        for p, g in zip(net, _draw(net, 0)):
+            p.grad = g
+        opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opts[0].step()
+    for i in range(1, 5):
+        for p, q, g in zip(*nets, _draw(nets[0], i, 10.0 ** (i - 2))):
+            p.grad.copy_(g)
+            q.grad = g.clone()
+        graph.replay()
+        opts[1].step()
+        torch.cuda.synchronize()
+        assert torch.equal(opts[0].norm, opts[1].norm)
+        for p, q in zip(*nets):
+            assert torch.equal(p, q)
+            for n, t in opts[0].state[p].items():
+                assert torch.equal(t, opts[1].state[q][n]), n

@@ -145,3 +145,16 @@ def test_loading_keeps_each_groups_own_options(library):
     again.load_state_dict(own.state_dict())
     assert [(g["state"], g["master"]) for g in again.param_groups] == \
         [(g["state"], g["master"]) for g in own.param_groups]
+
+
+@pytest.mark.parametrize("size", [1e-30, 1.0, 1e19, 6e37])
+def test_norms_of_several_lists_join_in_64_bits(library, monkeypatch, size):
+    """3 and 4 times any size make 5 times it, to a rounding of each and of the sum."""
+    ps = _params(torch.float32, torch.bfloat16)
+    parts = iter([3 * size, 4 * size])
+    monkeypatch.setattr(optim, "grad_norm", lambda g, grad_scale: torch.tensor(next(parts)))
+    own = cpt.AdamW(ps, max_norm=1.0)
+    own.step()
+    assert own.norm.dtype == torch.float32
+    assert abs(float(own.norm) - 5 * size) <= 2 * 2.0 ** -24 * 5 * size
+    assert [a[14] for a in library.steps()] == [1, 1]     # the norm is given to each
