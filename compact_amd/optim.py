@@ -97,10 +97,10 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.
     increases: what a captured graph needs.  lr: a number, or a float32 scalar on the
     device.
 
-    max_norm clips by the global norm of grad_scale * grads, which is returned (float32
-    scalar on the device; else None); `norm` gives it where it is known, as for more
-    tensors than these.  A norm that is not finite leaves parameters, moments and
-    counts as they were."""
+    max_norm clips by the global norm of grad_scale * grads (inf: measures it alone),
+    which is returned (float32 scalar on the device; else None); `norm` gives it where it
+    is known, as for more tensors than these.  A norm that is not finite leaves
+    parameters, moments and counts as they were."""
     params, grads = list(params), list(grads)
     exp_avgs, exp_avg_sqs = _listed(exp_avgs), _listed(exp_avg_sqs)
     m_scales, v_scales, masters = _listed(m_scales), _listed(v_scales), _listed(masters)
@@ -108,7 +108,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.
     assert (m_scales is None) == (v_scales is None), "m_scales and v_scales belong together"
     assert 0 <= b1 < 1 and 0 <= b2 < 1, f"betas={betas}"
     assert eps >= 0 and weight_decay >= 0, f"eps={eps}, weight_decay={weight_decay}"
-    assert max_norm is None or 0 < max_norm < float("inf"), f"max_norm={max_norm}"
+    assert max_norm is None or max_norm > 0, f"max_norm={max_norm}"
     assert norm is None or max_norm is not None, "norm goes with max_norm"
     if not params:
         assert not grads, "gradients without parameters"
@@ -166,11 +166,11 @@ class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's step by adamw_step.
 
     state: "float32" or "8bit" moments.  master: keep an fp32 copy of 16-bit
-    parameters and step that.  max_norm clips all gradients by their global norm; the
-    last step's norm is in `norm` (on the device), and a step whose norm is not finite
-    changes nothing (but the step count, which is only known to the device where
-    capturable).  seed: of the 8-bit moments' rounding.  capturable: step counts
-    on the device, so that a step can be captured into a graph (give lr as a float32
+    parameters and step that.  max_norm clips all gradients by their global norm (inf:
+    measures it alone); the last step's norm is in `norm` (on the device), and a step
+    whose norm is not finite changes nothing (but the step count, which is only known to
+    the device where capturable).  seed: of the 8-bit moments' rounding.  capturable: step
+    counts on the device, so that a step can be captured into a graph (give lr as a float32
     tensor there to change it); the step before has to be an eager one, which makes the
     state."""
 

@@ -70,3 +70,23 @@ def test_captured_step_over_two_lists(device):
             assert torch.equal(p, q)
             for n, t in opts[0].state[p].items():
                 assert torch.equal(t, opts[1].state[q][n]), n
+
+
+@pytest.mark.parametrize("lists", [1, 2])
+def test_an_infinite_max_norm_measures(device, lists):
+    """The norm, and the bits of a step without clipping; one that is not finite still
+    leaves the step out."""
+    a, b = _two(device), _two(device)
+    groups = [{"params": [p]} for p in a] if lists == 2 else a
+    opt, ref = cpt.AdamW(groups, max_norm=float("inf")), cpt.AdamW(b)
+    for i in range(2):
+        for x, y, g in zip(a, b, _draw(a, i, 7.0)):
+            x.grad, y.grad = g, g.clone()
+        opt.step()
+        ref.step()
+    want = torch.cat([p.grad.double() for p in a]).norm()
+    assert abs(float(opt.norm) - float(want)) <= 3 * U * float(want)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    a[0].grad[3] = float("inf")
+    opt.step()
+    assert float(opt.norm) == float("inf") and all(torch.equal(x, y) for x, y in zip(a, b))

@@ -158,3 +158,17 @@ def test_norms_of_several_lists_join_in_64_bits(library, monkeypatch, size):
     assert own.norm.dtype == torch.float32
     assert abs(float(own.norm) - 5 * size) <= 2 * 2.0 ** -24 * 5 * size
     assert [a[14] for a in library.steps()] == [1, 1]     # the norm is given to each
+
+
+def test_an_infinite_max_norm_is_taken(library):
+    """As torch's clip_grad_norm_ takes it: the norm is measured, nothing is clipped."""
+    ps = _params(torch.float32)
+    own = cpt.AdamW(ps, max_norm=float("inf"))
+    own.step()
+    assert library.steps()[0][13] == float("inf") and own.norm is not None
+    for bad in (0.0, -1.0, float("nan")):
+        with pytest.raises(AssertionError):
+            cpt.AdamW(ps, max_norm=bad)
+        with pytest.raises(AssertionError):
+            cpt.adamw_step(ps, [p.grad for p in ps], [torch.zeros(5)], [torch.zeros(5)], 1,
+                           max_norm=bad)
