@@ -162,6 +162,19 @@ def adamw_8bit_values(exp_avgs, exp_avg_sqs, m_scales, v_scales):
     return m, v
 
 
+def _check_options(g):
+    """A group's options: in range, and no other formula asked for."""
+    lr, betas, eps, decay, state = (g[n] for n in ("lr", "betas", "eps", "weight_decay", "state"))
+    assert state in ("float32", "8bit"), f"state={state!r}: 'float32' or '8bit' expected"
+    assert isinstance(lr, torch.Tensor) or lr >= 0, f"lr={lr}"
+    assert 0 <= betas[0] < 1 and 0 <= betas[1] < 1, f"betas={betas}"
+    assert eps >= 0 and decay >= 0, f"eps={eps}, weight_decay={decay}"
+    for name in ("maximize", "amsgrad"):
+        assert not g.get(name), f"AdamW: {name}={g[name]} is not what its step does"
+    assert g.get("decoupled_weight_decay", True) or decay == 0, \
+        "AdamW: decay within the gradient is not what its step does"
+
+
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's step by adamw_step.
 
@@ -177,14 +190,17 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state: str = "float32", master: bool = False,
                  max_norm: float | None = None, seed: int = 0, capturable: bool = False):
-        assert state in ("float32", "8bit"), f"state={state!r}: 'float32' or '8bit' expected"
-        assert isinstance(lr, torch.Tensor) or lr >= 0, f"lr={lr}"
-        assert 0 <= betas[0] < 1 and 0 <= betas[1] < 1, f"betas={betas}"
-        assert eps >= 0 and weight_decay >= 0, f"eps={eps}, weight_decay={weight_decay}"
         assert max_norm is None or max_norm > 0, f"max_norm={max_norm}"
         self.max_norm, self.seed, self.norm = max_norm, seed, None
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
-                                      state=state, master=master, capturable=capturable))
+        defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state=state,
+                        master=master, capturable=capturable)
+        _check_options(defaults)
+        super().__init__(params, defaults)
+
+    def add_param_group(self, param_group):
+        if isinstance(param_group, dict):
+            _check_options({**self.defaults, **param_group})
+        super().add_param_group(param_group)
 
     def _init_state(self, p, group):
         s = self.state[p]
@@ -283,10 +299,7 @@ class AdamW(torch.optim.Optimizer):
         of the parameters by the next step.  One whose options ask for
         another formula (maximize, amsgrad, decay within the gradient) is refused."""
         for g in state_dict["param_groups"]:
-            for name in ("maximize", "amsgrad"):
-                assert not g.get(name), f"AdamW: a state with {name}={g[name]} cannot go on here"
-            assert g.get("decoupled_weight_decay", True) or g["weight_decay"] == 0, \
-                "AdamW: a state with decay within the gradient cannot go on here"
+            _check_options({**self.defaults, **g})
         before = self.param_groups
         super().load_state_dict(state_dict)
         # what a state of torch's does not say stays as each group has it

@@ -172,3 +172,21 @@ def test_an_infinite_max_norm_is_taken(library):
         with pytest.raises(AssertionError):
             cpt.adamw_step(ps, [p.grad for p in ps], [torch.zeros(5)], [torch.zeros(5)], 1,
                            max_norm=bad)
+
+
+@pytest.mark.parametrize("bad", [{"state": "4bit"}, {"state": "8Bit"}, {"lr": -1.0},
+                                 {"betas": (0.9, 1.0)}, {"eps": -1e-8}, {"weight_decay": -0.1},
+                                 {"maximize": True}, {"amsgrad": True}])
+def test_a_groups_options_are_checked(library, bad):
+    ps = _params(torch.float32, torch.float32)
+    with pytest.raises(AssertionError):
+        cpt.AdamW([{"params": ps[:1]}, {"params": ps[1:], **bad}])
+    own = cpt.AdamW(ps[:1])
+    with pytest.raises(AssertionError):
+        own.add_param_group({"params": ps[1:], **bad})
+    assert len(own.param_groups) == 1
+    own.add_param_group({"params": ps[1:], "state": "8bit", "maximize": False})
+    own.step()
+    assert [a[2] for a in library.steps()] == [0, 1]
+    with pytest.raises(TypeError):
+        own.add_param_group(ps)
