@@ -225,6 +225,17 @@ class AdamW(torch.optim.Optimizer):
             s["master"] = p.detach().to(torch.float32, copy=True)
         return s
 
+    @staticmethod
+    def _move_counts(params, states, capturable):
+        """Step counts, to the device or from it: of a group whose `capturable` was changed."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: the counts have to be on the device before a step is "
+                               "captured")
+        for p, s in zip(params, states):
+            n = int(s["step"])
+            s["step"] = torch.tensor(n, device=p.device) if capturable else n
+        return [s["step"] for s in states]
+
     @torch.no_grad()
     def step(self, closure=None, *, grad_scale: float = 1.0):
         """One step over the parameters that have gradients; grad_scale multiplies these
@@ -264,12 +275,14 @@ class AdamW(torch.optim.Optimizer):
                                             dtype=torch.float64).float()
         for k, (group, params, grads, states) in enumerate(buckets):
             bits8, master = "m_scale" in states[0], "master" in states[0]
-            if group["capturable"]:
-                steps = [s["step"] for s in states]
-            else:
-                if torch.cuda.is_current_stream_capturing():
-                    raise RuntimeError("AdamW: a captured step needs capturable=True")
-                steps = [s["step"] + 1 for s in states]
+            capturable, steps = group["capturable"], [s["step"] for s in states]
+            if not capturable and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: a captured step needs capturable=True")
+            kinds = set(map(type, steps))
+            if (int in kinds) if capturable else (kinds != {int}):
+                steps = self._move_counts(params, states, capturable)
+            if not capturable:
+                steps = [n + 1 for n in steps]
             got = adamw_step(
                 params, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
                 steps, lr=group["lr"], betas=group["betas"], eps=group["eps"],
@@ -279,7 +292,7 @@ class AdamW(torch.optim.Optimizer):
                 masters=[s["master"] for s in states] if master else None,
                 grad_scale=grad_scale, max_norm=self.max_norm,
                 norm=None if norm is None else norm.to(params[0].device), seed=self.seed + k)
-            if not group["capturable"]:
+            if not capturable:
                 for s, n in zip(states, steps):
                     s["step"] = n
             if norm is None:

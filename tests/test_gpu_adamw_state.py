@@ -90,3 +90,45 @@ def test_an_infinite_max_norm_measures(device, lists):
     a[0].grad[3] = float("inf")
     opt.step()
     assert float(opt.norm) == float("inf") and all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_capturable_may_be_changed(device):
+    """Steps with host counts, then captured ones, then host counts again: as with host
+    counts throughout (1 / (1 - b^t) of two pow()s: the update to 4 roundings)."""
+    a, b = _two(device), _two(device)
+    opt, ref = cpt.AdamW(a, lr=1e-2), cpt.AdamW(b, lr=1e-2)
+
+    def grads(i):
+        for x, y, g in zip(a, b, _draw(a, i)):
+            if x.grad is None:
+                x.grad = g.clone()
+            x.grad.copy_(g)
+            y.grad = g
+
+    for i in range(2):
+        grads(i)
+        opt.step()
+        ref.step()
+    opt.param_groups[0]["capturable"] = True
+    grads(2)
+    opt.step()
+    ref.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for i in range(3, 6):
+        grads(i)
+        graph.replay()
+        ref.step()
+        torch.cuda.synchronize()
+    opt.param_groups[0]["capturable"] = False
+    grads(6)
+    opt.step()
+    ref.step()
+    for x, y in zip(a, b):
+        s, t = opt.state[x], ref.state[y]
+        assert s["step"] == t["step"] == 7
+        assert torch.equal(s["exp_avg"], t["exp_avg"])
+        assert torch.equal(s["exp_avg_sq"], t["exp_avg_sq"])
+        # seven updates of 5 lr at most, a rounding of the parameter each
+        assert ((x - y).abs() <= 7 * (2 * U * y.abs() + 4 * U * 5e-2)).all()

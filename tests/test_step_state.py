@@ -190,3 +190,32 @@ def test_a_groups_options_are_checked(library, bad):
     assert [a[2] for a in library.steps()] == [0, 1]
     with pytest.raises(TypeError):
         own.add_param_group(ps)
+
+
+def test_capturable_may_be_changed(library, monkeypatch):
+    """Counts move to the device and back with the group's option, whose steps go on from
+    them; while a step is captured they cannot."""
+    ps = _params(torch.float32, torch.float32)
+    own = cpt.AdamW(ps)
+    for _ in range(5):
+        own.step()
+    own.param_groups[0]["capturable"] = True
+    own.step()
+    counts = [own.state[p]["step"] for p in ps]
+    # the library, which is not there, would add one
+    assert all(c.dtype == torch.int64 and int(c) == 5 for c in counts)
+    assert counts[0].data_ptr() != counts[1].data_ptr()
+    own.step()
+    assert all(own.state[p]["step"] is c for p, c in zip(ps, counts))
+    own.param_groups[0]["capturable"] = False
+    own.step()
+    assert [own.state[p]["step"] for p in ps] == [6, 6]
+    own.param_groups[0]["capturable"] = True
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    n = len(library.steps())
+    with pytest.raises(RuntimeError, match="before a step is captured"):
+        own.step()
+    own.param_groups[0]["capturable"] = False
+    with pytest.raises(RuntimeError, match="capturable=True"):
+        own.step()
+    assert len(library.steps()) == n and own.state[ps[0]]["step"] == 6
