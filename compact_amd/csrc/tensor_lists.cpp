@@ -196,6 +196,8 @@ PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
                std::to_string(l->size()));
     const int64_t count = p.size();
     if (count == 0 || !g || !m || !v) refuse("adamw_table: tensors expected");
+    if (static_cast<bool>(ms) != static_cast<bool>(vs))
+      refuse("m_scales and v_scales belong together");
     std::vector<cpt_adamw_tensor> rows(count);
     const bool written = PyObject_IsTrue(a[8]) == 1;
     Addresses seen(6 * count);

@@ -151,6 +151,7 @@ def adamw_8bit_values(exp_avgs, exp_avg_sqs, m_scales, v_scales):
     exp_avgs = list(exp_avgs)
     if not exp_avgs:
         return [], []
+    assert m_scales is not None and v_scales is not None, "both moments' scales expected"
     _first(exp_avgs)
     m = [t.new_empty(t.shape, dtype=torch.bfloat16) for t in exp_avgs]
     v = [t.new_empty(t.shape, dtype=torch.bfloat16) for t in exp_avgs]

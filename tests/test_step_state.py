@@ -219,3 +219,21 @@ def test_capturable_may_be_changed(library, monkeypatch):
     with pytest.raises(RuntimeError, match="capturable=True"):
         own.step()
     assert len(library.steps()) == n and own.state[ps[0]]["step"] == 6
+
+
+def test_moments_without_both_scales_are_refused(library):
+    """Each of the two left out, in the wrapper and in the helper that reads the lists."""
+    codes = [torch.zeros(20, dtype=torch.uint8)]
+    scales = [torch.zeros(1, dtype=torch.uint8)]
+    wide = [torch.zeros(20)]
+    for a, b in ((scales, None), (None, scales), (None, None)):
+        for m in (codes, wide):
+            with pytest.raises(AssertionError):
+                cpt.adamw_8bit_values(m, m, a, b)
+    out = [[torch.zeros(20, dtype=torch.bfloat16)] for _ in range(2)]
+    for a, b in ((scales, None), (None, scales)):
+        with pytest.raises(AssertionError):
+            _lib.lists().adamw_table(*out, codes, codes, a, b, None, 1, False)
+    assert not library.calls
+    cpt.adamw_8bit_values(codes, codes, scales, scales)
+    assert [n for n, _ in library.calls] == ["cpt_adamw_8bit_values"]
