@@ -114,6 +114,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.
         assert not grads, "gradients without parameters"
         return norm
     assert grads, "parameters without gradients"
+    if not isinstance(step, (int, torch.Tensor)):
+        step = _listed(step)
     dev = _first(params)
     lists = _lib.lists()
     args = exp_avgs, exp_avg_sqs, m_scales, v_scales, masters, step, True
@@ -131,7 +133,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.
         if not given:
             norm = p0.new_empty((), dtype=torch.float32)
         norm_at = _scalar(norm, dev, "norm")
-    if max_norm is not None or not isinstance(step if isinstance(step, int) else step[0], int):
+    # counts on the device: a tensor of them, or one each
+    if max_norm is not None or isinstance(step, torch.Tensor) or \
+            (type(step) in (list, tuple) and isinstance(step[0], torch.Tensor)):
         ws = _workspace(p0, count, total)
     with _guard(p0), _timed("adamw_step"):
         rc = _lib.api().cpt_adamw(dt, gdt, int(m_scales is not None), int(masters is not None), at,

@@ -237,3 +237,24 @@ def test_moments_without_both_scales_are_refused(library):
     assert not library.calls
     cpt.adamw_8bit_values(codes, codes, scales, scales)
     assert [n for n, _ in library.calls] == ["cpt_adamw_8bit_values"]
+
+
+@pytest.mark.parametrize("max_norm", [None, 1.0])
+def test_steps_of_any_sequence(library, max_norm):
+    """Numbers and counts as a list, a tuple or what gives them one by one; one parameter's
+    count as a scalar."""
+    def call(step, n=2):
+        p, g, m, v = ([torch.ones(5) for _ in range(n)] for _ in range(4))
+        cpt.adamw_step(p, g, m, v, step, max_norm=max_norm)
+        workspace = library.steps()[-1][17]
+        return workspace is not None
+
+    for step in ([3, 4], (3, 4), (i for i in (3, 4)), range(3, 5), 3):
+        assert call(step) is (max_norm is not None)
+    counts = torch.zeros(2, dtype=torch.int64)
+    for step in (counts, list(counts.clone().split(1)), iter(counts.clone().split(1))):
+        assert call(step)
+    assert call(torch.tensor(0), 1) and call([torch.tensor(0)], 1)
+    for bad in ((i for i in (3,)), iter([3, 0]), torch.tensor(0), []):
+        with pytest.raises(AssertionError):
+            call(bad)
