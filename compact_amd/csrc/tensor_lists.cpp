@@ -7,6 +7,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
+#include <algorithm>
 #include <cstring>
 #include <string>
 #include <vector>
@@ -105,9 +106,74 @@ class Addresses {
     table_[at] = p;
     return true;
   }
+  bool has(const void* p) const {
+    const size_t mask = table_.size() - 1;
+    size_t at = (reinterpret_cast<uintptr_t>(p) >> 4) * 0x9E3779B97F4A7C15ull >> 32 & mask;
+    while (table_[at] && table_[at] != p) at = (at + 1) & mask;
+    return table_[at];
+  }
 
  private:
   std::vector<const void*> table_;
+};
+
+// The memory of a step's tensors.  What is written lies apart from all else, or its elements
+// depend on which thread comes first; a gradient may be its parameter or moment itself, whose
+// elements are each read before they are written.
+class Memory {
+ public:
+  explicit Memory(int64_t most) : storages_(most) {}
+
+  // Tensor i of a list, dense.
+  void write(int list, const at::Tensor& t, int64_t i) {
+    if (t.numel() == 0) return;
+    shared_ |= !storages_.add(t.storage().data());
+    lists_[list].push_back(range(t, i));
+  }
+  // Once all that is written is known.
+  void read(const at::Tensor& t, int64_t i) {
+    if (t.numel() != 0 && storages_.has(t.storage().data())) read_.push_back(range(t, i));
+  }
+  void check(const List& p) {
+    if (!shared_ && read_.empty()) return;      // each in a storage of its own
+    // lists cut from a buffer each lie in order, one behind the other
+    for (auto& l : lists_) order(l);
+    std::sort(lists_, lists_ + kLists, [](const Ranges& a, const Ranges& b) {
+      return !a.empty() && (b.empty() || before(a[0], b[0]));
+    });
+    Ranges all;
+    for (const auto& l : lists_) all.insert(all.end(), l.begin(), l.end());
+    order(all);
+    for (size_t i = 1; i < all.size(); ++i)
+      if (all[i].at < all[i - 1].end)
+        refuse("two of a step's tensors share memory: " + describe(p[all[i].tensor]));
+    for (const Range& r : read_) {
+      auto w = std::upper_bound(all.begin(), all.end(), r, before);
+      if (w != all.begin()) --w;
+      for (; w != all.end() && w->at < r.end; ++w)
+        if (w->end > r.at && (w->at != r.at || w->end != r.end || w->tensor != r.tensor))
+          refuse("grads: a step writes to the memory of that for " + describe(p[r.tensor]));
+    }
+  }
+
+ private:
+  static constexpr int kLists = 6;
+  struct Range {
+    uintptr_t at, end;
+    int64_t tensor;
+  };
+  using Ranges = std::vector<Range>;
+  static bool before(const Range& a, const Range& b) { return a.at < b.at; }
+  static void order(Ranges& r) {
+    if (!std::is_sorted(r.begin(), r.end(), before)) std::sort(r.begin(), r.end(), before);
+  }
+  static Range range(const at::Tensor& t, int64_t i) {
+    const auto at = reinterpret_cast<uintptr_t>(t.data_ptr());
+    return Range{at, at + t.numel() * t.element_size(), i};
+  }
+  Addresses storages_;
+  Ranges lists_[kLists], read_;
+  bool shared_ = false;
 };
 
 constexpr int64_t kBlock = 128;   // elements of an 8-bit moment that share a scale
@@ -200,7 +266,7 @@ PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
       refuse("m_scales and v_scales belong together");
     std::vector<cpt_adamw_tensor> rows(count);
     const bool written = PyObject_IsTrue(a[8]) == 1;
-    Addresses seen(6 * count);
+    Memory memory(6 * count);
     const at::ScalarType type = p[0].scalar_type(), grad_type = g[0].scalar_type();
     const at::Device device = p[0].device();
     if (code(type) < 0) refuse("params: unsupported " + describe(p[0]));
@@ -223,7 +289,7 @@ PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
       r.n = pi.numel();
       total += r.n;
       r.p = pi.data_ptr();
-      if (r.n && !seen.add(r.p)) refuse("params: a tensor is there twice, " + describe(pi));
+      memory.write(0, pi, i);
       if (alike(pi, gi)) {
         r.g = gi.data_ptr();
       } else {
@@ -239,6 +305,7 @@ PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
         expect_bytes(vsi, pi, blocks, vs.name());
         r.m_scale = msi.data_ptr();
         r.v_scale = vsi.data_ptr();
+        if (written) memory.write(3, msi, i), memory.write(4, vsi, i);
       } else {
         expect(mi, pi, at::kFloat, m.name());
         expect(vi, pi, at::kFloat, v.name());
@@ -249,11 +316,13 @@ PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor& wi = w[i];
         expect(wi, pi, at::kFloat, w.name());
         r.master = wi.data_ptr();
+        memory.write(5, wi, i);
       }
-      if (written && r.n)
-        for (const void* at : {r.m, r.v, r.m_scale, r.v_scale, r.master})
-          if (at && !seen.add(at)) refuse("two of a step's tensors share memory: " + describe(pi));
+      if (written) memory.write(1, mi, i), memory.write(2, vi, i);
     }
+    for (int64_t i = 0; i < count; ++i)
+      if (rows[i].g) memory.read(g[i], i);
+    memory.check(p);
     steps(a[7], rows, device);
     return result(rows, total, code(type), code(grad_type), otherwise.release());
   });

@@ -90,7 +90,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.
     the moments are 8-bit codes (uint8 [numel], in the order of the parameter's memory)
     rounded by `seed`.  masters: float32 parameters that are stepped in the place of
     16-bit ones, which become their rounding.  Zeros are a valid start for all moments,
-    codes and scales.
+    codes and scales.  What is written lies apart from all else; a gradient may be its
+    parameter or moment itself.
 
     step: this step's number, from 1 (for all, or a list), or int64 counts of the steps
     done on the device (one tensor of len(params), or one each), which the call

@@ -258,3 +258,63 @@ def test_steps_of_any_sequence(library, max_norm):
     for bad in ((i for i in (3,)), iter([3, 0]), torch.tensor(0), []):
         with pytest.raises(AssertionError):
             call(bad)
+
+
+def _cut(buf, *starts, n=40):
+    return [buf[a:a + n] for a in starts]
+
+
+def test_a_steps_tensors_lie_apart(library):
+    """Views of one buffer that meet anywhere are refused: of one list, of two, of codes and
+    scales, of a gradient and what is written; those side by side in any order are taken."""
+    def flat(dt=torch.float32, n=400):
+        return torch.zeros(n, dtype=dt)
+
+    def call(p, g, m, v, **kw):
+        cpt.adamw_step(p, g, m, v, 1, **kw)
+
+    def two(dt=torch.float32):
+        return _cut(flat(dt), 0, 40)
+
+    one = flat()
+    x, y = flat(), flat()
+    call(_cut(one, 0, 40), _cut(one, 80, 120), _cut(one, 160, 200), _cut(one, 240, 280))
+    call(_cut(x, 0, 80), two(), _cut(x, 40, 120), _cut(x, 200, 160))     # in turn, backwards
+    call(_cut(x, 40, 0), _cut(x, 80, 120), two(), two())
+    m = two()
+    call(two(), m, m, two())                      # a gradient that is its moment
+    p = two()
+    call(p, p, two(), two())
+    call([flat(n=0), flat()], [flat(n=0), flat()], [x[5:5], flat()], [x[3:3], x])
+    grid = flat(n=1600).view(40, 40)              # columns and rows of one matrix apart
+    call([grid[:10].t()], [torch.zeros(40, 10)], [grid[10:20].t()], [grid[20:30].t()])
+    codes, scales = torch.zeros(100, dtype=torch.uint8), torch.zeros(8, dtype=torch.uint8)
+    call(two(), two(), _cut(codes, 0, 50), _cut(torch.zeros_like(codes), 0, 50),
+         m_scales=list(scales[:2].split(1)), v_scales=list(scales[2:4].split(1)))
+    call(two(), two(), _cut(codes, 0, 50), _cut(codes.clone(), 0, 50),      # between two codes
+         m_scales=[codes[49:50], scales[:1]], v_scales=list(scales[1:3].split(1)))
+    half = two(torch.bfloat16)
+    call(half, two(torch.bfloat16), two(), two(), masters=_cut(x, 0, 40))
+    taken = len(library.steps())
+    assert taken == 10
+    bad = [lambda: call(_cut(one, 0, 39), two(), two(), two()),
+           lambda: call(_cut(one, 39, 0), two(), two(), two()),
+           lambda: call(two(), two(), _cut(one, 0, 80), _cut(one, 200, 119)),
+           lambda: call(two(), two(), _cut(one, 0, 80), _cut(one, 40, 81)),
+           lambda: call(_cut(one, 0, 40), two(), two(), _cut(one, 100, 1)),
+           lambda: call([one], [flat()], [flat()], [one]),
+           lambda: call([one, one[7:9]], [flat(), flat(n=2)], [flat(), flat(n=2)],
+                        [flat(), flat(n=2)]),
+           lambda: call(two(), two(), _cut(codes, 0, 50), _cut(codes.clone(), 0, 50),
+                        m_scales=list(scales[:2].split(1)), v_scales=list(scales[1:3].split(1))),
+           lambda: call(two(), two(), _cut(codes, 0, 50), _cut(codes.clone(), 0, 50),
+                        m_scales=[codes[89:90], scales[:1]], v_scales=list(scales[1:3].split(1))),
+           lambda: call(half, two(torch.bfloat16), _cut(x, 0, 80), two(), masters=_cut(x, 119, 40)),
+           lambda: call(_cut(one, 0, 40), _cut(one, 100, 79), two(), two()),
+           lambda: call(_cut(one, 0, 40), _cut(one, 40, 100), two(), two()),
+           lambda: call(half, [t[:20].view(torch.bfloat16) for t in m], m, two())]
+    for i, f in enumerate(bad):
+        with pytest.raises(AssertionError, match="memory"):
+            f()
+            pytest.fail(f"call {i} was taken")
+    assert len(library.steps()) == taken
