@@ -78,17 +78,33 @@ def _distinct(t):
     return True
 
 
-def _share_heads(q, k):
-    """Whether q and k are the same memory, or views of one buffer with heads in common."""
+def _meet(q, k):
+    """Whether q and k have elements in one place: whether differences of their indices can
+    make up for the distance between them.  Along nested axes, the largest stride first,
+    few can; views that would take long to tell apart count as meeting."""
     if q.numel() == 0 or k.numel() == 0:
         return False
-    if q.data_ptr() == k.data_ptr():
-        return True
-    st = q.stride()
-    if st != k.stride() or q.untyped_storage().data_ptr() != k.untyped_storage().data_ptr():
+    off = (k.data_ptr() - q.data_ptr()) // q.element_size()
+    sq, sk = q.stride(), k.stride()
+    if sq == sk:
+        axes = sorted([(st, 1 - n, m - 1) for st, m, n in zip(sq, q.shape, k.shape)])
+    else:
+        axes = sorted([(st, 0, n - 1) for st, n in zip(sq, q.shape)] +
+                      [(st, 1 - n, 0) for st, n in zip(sk, k.shape)])
+    least = sum([st * first for st, first, _ in axes])
+    most = sum([st * last for st, _, last in axes])
+    if not least <= off <= most:
         return False
-    off = k.storage_offset() - q.storage_offset()
-    return off % st[-2] == 0 and -k.shape[-2] < off // st[-2] < q.shape[-2]
+    left = {off}
+    for st, first, last in reversed(axes):
+        # what the smaller strides reach
+        least, most = least - st * first, most - st * last
+        if first < last:
+            left = {t - st * n for t in left for n in range(max(first, -((most - t) // st)),
+                                                            min(last, (t - least) // st) + 1)}
+            if len(left) > 64:
+                return True
+    return 0 in left
 
 
 def qk_rope(q: torch.Tensor, k: torch.Tensor, positions, inv_freq: torch.Tensor, *, w_q=None,
@@ -105,7 +121,7 @@ def qk_rope(q: torch.Tensor, k: torch.Tensor, positions, inv_freq: torch.Tensor,
     from R on are normed alone.  positions: int32 or int64 [B, S] or [S], None: 0
     to S - 1; angles are exact at any position.  Weights share one dtype, the heads'
     or float32.  Outputs are contiguous; `inplace` writes over q and k, which must
-    be the caller's own.  `inverse` turns back, without norms: the gradient."""
+    be the caller's own and lie apart.  `inverse` turns back, without norms: the gradient."""
     _on_device(q, k, positions, inv_freq, w_q, w_k)
     dt = _dtype_code(q)
     b, s, hq, hk, d, rot, pos, wide, pos_batch, wdt = _rope_args(q, k, positions, inv_freq, w_q,
@@ -115,7 +131,7 @@ def qk_rope(q: torch.Tensor, k: torch.Tensor, positions, inv_freq: torch.Tensor,
     q2, sq = _strides(q)
     k2, sk = _strides(k)
     if inplace:
-        assert q2 is q and k2 is k and _distinct(q) and _distinct(k) and not _share_heads(q, k), \
+        assert q2 is q and k2 is k and _distinct(q) and _distinct(k) and not _meet(q, k), \
             "inplace: heads with contiguous columns, no two elements in one place, expected"
         q_out, k_out, oq, ok = q, k, sq, sk
     else:

@@ -318,3 +318,39 @@ def test_a_steps_tensors_lie_apart(library):
             f()
             pytest.fail(f"call {i} was taken")
     assert len(library.steps()) == taken
+
+
+def test_rotation_in_place_takes_heads_that_lie_apart(library):
+    """Heads of one buffer side by side along any axis, and columns in turn."""
+    x = torch.zeros(3, 8, 6, 16)
+    inv = torch.ones(4)
+    pairs = [(x[..., :8], x[..., 8:]), (x[:, :, :4], x[:, :, 4:]), (x[:, :, 4:], x[:, :, :4]),
+             (x[:, :, ::2], x[:, :, 1::2]), (x[:, :4], x[:, 4:]), (x[:1], x[1:2]),
+             (x[:, ::2], x[:, 1::2]), (x[0], x[1]),
+             (x.flatten(1, 2)[:, ::2, None], x.flatten(1, 2)[:, 1::2, None]),
+             (x[:, :, 0].unsqueeze(2), x[:, :, 1:]),
+             (x[:, :, :2].transpose(1, 2), x[:, :, 2:4].transpose(1, 2)),
+             (x[..., :8], x.view(3, 8, 12, 8)[:, :, 1::2]), (torch.zeros(1, 8, 4, 16), x[:1, :, :3]),
+             (x[:, :0], x[:, :0])]
+    for i, (q, k) in enumerate(pairs):
+        cpt.qk_rope(q, k, None, inv, inplace=True)
+        assert len(library.calls) == i + 1, i
+
+
+def test_rotation_in_place_refuses_heads_that_meet(library):
+    """Views shifted by a token, a sequence, part of a head or both of two axes."""
+    x = torch.zeros(3, 8, 6, 16)
+    inv = torch.ones(4)
+    flat = x.flatten()
+    shifted = [flat[a:a + 2 * 8 * 6 * 16].view(2, 8, 6, 16) for a in (0, 8, 16, 40, 96, 100, 768)]
+    pairs = [(x[:, :-1], x[:, 1:]), (x[:, 1:], x[:, :-1]), (x[:-1], x[1:]), (x[1:], x[:-1]),
+             (x[..., :10], x[..., 6:]), (x[:, :, :4], x[:, :, 3:]), (x[:, :, 3:], x[:, :, :4]),
+             (x[:2, 1:], x[1:, :-1]), (x[:, :-1, 2:], x[:, 1:, :4]), (x, x),
+             (x[0, :6], x[0, :6].transpose(0, 1)),
+             (x[..., :8], x.view(3, 8, 12, 8)[:, :, ::2]), (x[..., :8], x.view(3, 8, 12, 8)),
+             *((shifted[0], s) for s in shifted[1:])]
+    for i, (q, k) in enumerate(pairs):
+        with pytest.raises(AssertionError, match="one place"):
+            cpt.qk_rope(q, k, None, inv, inplace=True)
+            pytest.fail(f"pair {i} was taken")
+    assert not library.calls
