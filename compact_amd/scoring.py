@@ -158,7 +158,9 @@ class TokenLogprobsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets=None, temperature=1.0, top_k=0, ignore_index=-100,
                 inplace=False):
-        if inplace and logits.requires_grad and logits.is_leaf:
+        # a view's root is a leaf, too, if the view is of a parameter
+        root = logits if logits._base is None else logits._base
+        if inplace and logits.requires_grad and root.is_leaf and root.requires_grad:
             raise RuntimeError("TokenLogprobsFunction: a leaf's gradient cannot take its memory")
         r = token_logprobs(logits, targets, temperature=temperature, top_k=top_k,
                            ignore_index=ignore_index, stats=True)

@@ -31,3 +31,24 @@ def test_rotation_in_place_of_heads_side_by_side(device, norm, cut):
     assert not torch.equal(want, x)
     cpt.qk_rope(q, k, pos, inv, inplace=True, **kw)
     assert torch.equal(x, want)
+
+
+def test_a_score_in_place_of_a_computed_view(device):
+    """Logits that are a view of a computed tensor give up their memory: the gradient of
+    their root is that without inplace; a view of a parameter keeps its own."""
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(3, 7, 200, generator=g).to(device)
+    y = torch.randint(0, 200, (3, 6), generator=g).to(device)
+    grads = []
+    for inplace in (False, True):
+        leaf = x.clone().requires_grad_(True)
+        lp, h, *_ = cpt.token_scores((leaf * 1.0)[:, :-1], y, inplace=inplace)
+        (lp.sum() - 0.1 * h.sum()).backward()
+        assert torch.equal(leaf.detach(), x)
+        grads.append(leaf.grad)
+    assert torch.equal(*grads) and not grads[0][:, -1].any() and grads[0].any()
+    leaf = x.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="leaf"):
+        cpt.token_scores(leaf[:, :-1], y, inplace=True)
+    cpt.token_scores(leaf[:, :-1], y)[0].sum().backward()
+    assert torch.equal(leaf.detach(), x)

@@ -354,3 +354,20 @@ def test_rotation_in_place_refuses_heads_that_meet(library):
             cpt.qk_rope(q, k, None, inv, inplace=True)
             pytest.fail(f"pair {i} was taken")
     assert not library.calls
+
+
+def test_a_score_in_place_spares_leaves_and_their_views(library):
+    """The gradient may not be written over a parameter, seen whole or in part."""
+    w = torch.zeros(4, 64, requires_grad=True)
+    y = torch.zeros(4, dtype=torch.int64)
+    for z in (w, w[:, :32], w.view(4, 64), w[:, 8:][:, :9], w.unsqueeze(0)[0], w.t()[:4, :4].t()):
+        with pytest.raises(RuntimeError, match="leaf"):
+            cpt.token_scores(z, y, inplace=True)
+        assert not library.calls
+        cpt.token_scores(z, y)
+        with torch.no_grad():
+            cpt.token_scores(z, y, inplace=True)
+        library.calls.clear()
+    for z in (w * 1.0, (w * 1.0)[:, :32], w.detach()[:, :32], torch.zeros(4, 64)[:, 1:]):
+        cpt.token_scores(z, y, inplace=True)[0]
+    assert len(library.calls) == 4
