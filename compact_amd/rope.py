@@ -215,28 +215,38 @@ class QKRopeFunction(torch.autograd.Function):
 
 class QKNormRope(nn.Module):
     """(q, k) -> (q_out, k_out): heads normed with learned weights (`norm`) and turned
-    by their positions.  Frequencies are base^(-2 i / rotary), in float32 whatever the
-    module is cast to."""
+    by their positions.  Frequencies are base^(-2 i / rotary), or those given ([R / 2],
+    R = `rotary`); in float32 whatever the module is cast to."""
 
     def __init__(self, head_dim: int, rotary: int | None = None, base: float = 10000.0,
                  norm: bool = True, eps: float = 1e-6, interleaved: bool = False,
-                 scaling: float = 1.0, device=None, dtype=None):
+                 scaling: float = 1.0, device=None, dtype=None, inv_freq=None):
         super().__init__()
+        if inv_freq is not None:
+            assert inv_freq.dim() == 1 and rotary in (None, 2 * inv_freq.numel()), \
+                f"inv_freq {tuple(inv_freq.shape)} for rotary={rotary}"
+            rotary = 2 * inv_freq.numel()
         self.rotary = head_dim if rotary is None else rotary
         assert 0 < self.rotary <= head_dim and self.rotary % 2 == 0, f"rotary={rotary}"
         self.base, self.eps, self.interleaved, self.scaling = base, eps, interleaved, scaling
         kw = dict(device=device, dtype=dtype)
         self.w_q = nn.Parameter(torch.ones(head_dim, **kw)) if norm else None
         self.w_k = nn.Parameter(torch.ones(head_dim, **kw)) if norm else None
+        self._given = None if inv_freq is None else inv_freq.detach().cpu().float()
         self.register_buffer("inv_freq", self._frequencies(device), persistent=False)
 
     def _frequencies(self, device):
+        if self._given is not None:
+            return self._given.to(device, copy=True)
         i = torch.arange(0, self.rotary, 2, dtype=torch.float64, device=device)
         return (self.base ** (-i / self.rotary)).float()
 
     def _apply(self, fn, recurse=True):
+        kept = self.inv_freq
         super()._apply(fn, recurse)
-        self.inv_freq = self._frequencies(self.inv_freq.device)     # not cast, not left empty
+        # moved as they are, also where they were changed since: not cast, not left empty
+        device = self.inv_freq.device
+        self.inv_freq = self._frequencies(device) if kept.is_meta else kept.to(device)
         return self
 
     def extra_repr(self):

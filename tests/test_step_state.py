@@ -371,3 +371,36 @@ def test_a_score_in_place_spares_leaves_and_their_views(library):
     for z in (w * 1.0, (w * 1.0)[:, :32], w.detach()[:, :32], torch.zeros(4, 64)[:, 1:]):
         cpt.token_scores(z, y, inplace=True)[0]
     assert len(library.calls) == 4
+
+
+def test_a_modules_frequencies_stay(library):
+    """Given to the module or changed in it, they are kept through casts and moves; a module
+    made without memory gets them with it."""
+    own = torch.rand(8, dtype=torch.float64) / 3
+    m = cpt.QKNormRope(24, inv_freq=own, norm=False)
+    assert m.rotary == 16 and m.inv_freq.dtype == torch.float32
+    assert torch.equal(m.inv_freq, own.float())
+    for cast in (lambda t: t.half(), lambda t: t.double(), lambda t: t.to(torch.bfloat16),
+                 lambda t: t.to("cpu"), lambda t: copy.deepcopy(t), lambda t: t.to_empty(device="cpu")):
+        assert torch.equal(cast(m).inv_freq, own.float())
+    with torch.no_grad():
+        m.inv_freq.mul_(0.25)
+    assert torch.equal(m.half().inv_freq, own.float() * 0.25)
+    plain = cpt.QKNormRope(16)
+    plain.inv_freq = plain.inv_freq / 8
+    want = plain.inv_freq.clone()
+    assert torch.equal(plain.bfloat16().inv_freq, want) and plain.w_q.dtype == torch.bfloat16
+    with torch.device("meta"):
+        empty = cpt.QKNormRope(24, inv_freq=torch.rand(8, device="cpu")), cpt.QKNormRope(16)
+    assert all(t.inv_freq.is_meta for t in (e.to("meta") for e in empty))
+    for e, f in zip(empty, (empty[0]._given, cpt.QKNormRope(16).inv_freq)):
+        assert torch.equal(e.to_empty(device="cpu").inv_freq, f)
+    # what the rotation is called with
+    q, k = torch.zeros(1, 2, 3, 24), torch.zeros(1, 2, 1, 24)
+    m(q, k)
+    args = library.calls[-1][1]
+    assert args[17] == m.inv_freq.data_ptr() and args[23] == 16
+    for bad in (dict(inv_freq=torch.ones(2, 4)), dict(inv_freq=torch.ones(13)),
+                dict(inv_freq=torch.ones(4), rotary=16), dict(inv_freq=torch.ones(0))):
+        with pytest.raises(AssertionError):
+            cpt.QKNormRope(24, **bad)
