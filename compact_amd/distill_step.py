@@ -33,8 +33,8 @@ from .scoring import token_logprobs
 
 
 def _attention(attn, x, rotary):
-    """A LlamaAttention over whole sequences with queries and keys turned by one
-    operator, at the model's own frequencies."""
+    """A LlamaAttention's forward over whole sequences with queries and keys turned by
+    one operator, at the model's own frequencies."""
     b, s, _ = x.shape
     q, k, v = (p(x).view(b, s, -1, attn.head_dim) for p in (attn.q_proj, attn.k_proj, attn.v_proj))
     q, k = QKRopeFunction.apply(q, k, None, rotary.inv_freq.float(), None, None, 0.0, False,
@@ -47,18 +47,33 @@ def _attention(attn, x, rotary):
     return attn.o_proj(y.transpose(1, 2).reshape(b, s, -1))
 
 
+def _check_attention(m):
+    """What `_attention` stands in for: the class's own forward, with nothing hung on it, and
+    frequencies that do not go by the length."""
+    from transformers.models.llama.modeling_llama import LlamaAttention
+    kind = getattr(m.rotary_emb, "rope_type", "default")
+    assert kind not in ("dynamic", "longrope"), f"{kind}: frequencies that go by the length"
+    for layer in m.layers:
+        a = layer.self_attn
+        assert type(a).forward is LlamaAttention.forward and "forward" not in vars(a), \
+            f"rope: {type(a).__name__} has a forward of its own"
+        assert not (a._forward_pre_hooks or a._forward_hooks or a._backward_pre_hooks or
+                    a._backward_hooks), "rope: hooks on an attention would not run"
+
+
 def forward(model, ids, embed_scale: float = 1.0, rope: bool = False) -> torch.Tensor:
     """Logits of a LlamaForCausalLM for whole sequences `ids` [B, S]: the model's
     own weights, attention and MLPs; each block's residual add and the norm that
-    follows it are one operator, and with `rope` the rotation of queries and keys."""
+    follows it are one operator, and with `rope` the rotation of queries and keys.
+    `rope` takes the place of the attention modules' forward: one that is not
+    LlamaAttention's, or has hooks, is refused."""
     m = model.model
+    if rope:
+        _check_attention(m)
     emb = m.embed_tokens
     h = EmbeddingFunction.apply(ids, emb.weight, embed_scale, emb.padding_idx)
     angles = None
-    if rope:
-        kind = getattr(m.rotary_emb, "rope_type", "default")
-        assert kind not in ("dynamic", "longrope"), f"{kind}: frequencies that go by the length"
-    else:
+    if not rope:
         pos = torch.arange(ids.shape[1], device=ids.device).unsqueeze(0)
         angles = m.rotary_emb(h, position_ids=pos)
     layers = list(m.layers)

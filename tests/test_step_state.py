@@ -404,3 +404,44 @@ def test_a_modules_frequencies_stay(library):
                 dict(inv_freq=torch.ones(4), rotary=16), dict(inv_freq=torch.ones(0))):
         with pytest.raises(AssertionError):
             cpt.QKNormRope(24, **bad)
+
+
+def test_the_fused_forward_takes_plain_attentions_alone():
+    """With `rope` an attention's own forward does not run: one that differs, or has hooks,
+    is refused before anything is computed."""
+    from transformers.models.llama.modeling_llama import LlamaAttention
+    from compact_amd import distill_step, e2e
+
+    class Other(LlamaAttention):
+        def forward(self, *args, **kw):
+            return super().forward(*args, **kw)
+
+    class Same(LlamaAttention):
+        pass
+
+    cfg = dict(layers=2, hidden=32, inter=48, heads=2, kv_heads=1, vocab=20, seq=4)
+    model = e2e.build_llama(cfg, "cpu")
+    ids = torch.zeros(1, 4, dtype=torch.int64)
+    a = model.model.layers[1].self_attn
+
+    def call(match, kind=AssertionError):
+        with pytest.raises(kind, match=match):
+            distill_step.forward(model, ids, rope=True)
+
+    call("HIP device", RuntimeError)            # the embedding's, on the CPU
+    a.__class__ = Same
+    call("HIP device", RuntimeError)
+    a.__class__ = Other
+    call("Other has a forward")
+    a.__class__ = LlamaAttention
+    a.forward = lambda *args, **kw: None
+    call("forward of its own")
+    del a.forward
+    for add in (a.register_forward_hook, a.register_forward_pre_hook,
+                a.register_full_backward_hook, a.register_full_backward_pre_hook):
+        hook = add(lambda *args: None)
+        call("hooks")
+        hook.remove()
+    call("HIP device", RuntimeError)
+    model.model.rotary_emb.rope_type = "dynamic"
+    call("go by the length")
