@@ -1,16 +1,13 @@
 """The optimizer over several lists, states and options, on the device.  Tolerances as
 test_gpu_adamw.py derives them."""
 
-import copy
-
 import pytest
 import torch
 
 import compact_amd as cpt
+from tests.test_gpu_adamw import HP, U, _close_param, _make, _moments, _param, _to
 
 pytestmark = pytest.mark.gpu
-
-U = 2.0 ** -24
 
 
 def _two(device, dtypes=(torch.float32, torch.float32), sizes=(300, 5000), seed=0):
@@ -132,3 +129,76 @@ def test_capturable_may_be_changed(device):
         assert torch.equal(s["exp_avg_sq"], t["exp_avg_sq"])
         # seven updates of 5 lr at most, a rounding of the parameter each
         assert ((x - y).abs() <= 7 * (2 * U * y.abs() + 4 * U * 5e-2)).all()
+
+
+@pytest.mark.parametrize("bits8", [False, True])
+@pytest.mark.parametrize("on", ["numbers", "counts", "a count each"])
+def test_each_way_of_counting_makes_the_formulas_parameters(device, bits8, on):
+    """Clipped bf16 steps at counts of their own: parameters against the formula in 64 bits at
+    each tensor's step number and the lr given, from moments computed in the same fp32
+    operations."""
+    sizes = [500] * 60
+    p, g, m, v = _make(sizes, torch.bfloat16, torch.bfloat16, seed=6)
+    t = [1 + i % 7 for i in range(60)]
+    step = {"numbers": t, "counts": torch.tensor([x - 1 for x in t], device=device),
+            "a count each": [torch.tensor(x - 1, device=device) for x in t]}[on]
+    kw = {}
+    if bits8:
+        # codes and scales of any moments do: those that a step leaves
+        m, v = ([torch.zeros(500, dtype=torch.uint8) for _ in sizes] for _ in range(2))
+        scales = [[torch.zeros(4, dtype=torch.uint8, device=device) for _ in sizes]
+                  for _ in range(2)]
+        kw = dict(m_scales=scales[0], v_scales=scales[1], seed=9)
+    pd, gd, md, vd = (_to(x, device) for x in (p, g, m, v))
+    if bits8:
+        other = _to(_make(sizes, torch.bfloat16, torch.bfloat16, seed=7)[1], device)
+        cpt.adamw_step([x.clone() for x in pd], other, md, vd, 1, **HP, **kw)
+        m, v = ([x.cpu().float() for x in y] for y in cpt.adamw_8bit_values(md, vd, *scales))
+    hp = {**HP, "lr": 7e-3}
+    lr = hp["lr"] if on == "numbers" else torch.tensor(hp["lr"], device=device)
+    norm = cpt.adamw_step(pd, gd, md, vd, step, max_norm=0.5, **{**hp, "lr": lr}, **kw)
+    clip = (torch.tensor(0.5) / (norm.cpu() + 1e-6)).clamp(max=1.0)
+    assert clip < 1
+    for i in range(60):
+        m1, v1 = _moments(g[i], m[i], v[i], clip=clip)
+        if not bits8:
+            assert torch.equal(md[i].cpu(), m1) and torch.equal(vd[i].cpu(), v1)
+        want, up = _param(p[i], m1, v1, t[i], hp)
+        _close_param(pd[i], want, up, torch.bfloat16)
+
+
+@pytest.mark.parametrize("state", ["float32", "8bit"])
+def test_captured_steps_are_the_hosts(device, state):
+    """A captured step with counts and lr on the device, replayed with other gradients and
+    another lr, against eager steps with numbers: moments and codes the same bits, parameters
+    apart by 1 / (1 - b^t) of two pow()s (4 roundings of the update) and their own rounding."""
+    a, b = _two(device), _two(device)
+    lr = torch.tensor(1e-2, device=device)
+    kw = dict(state=state, max_norm=2.0)
+    opt, ref = cpt.AdamW(a, lr=lr, capturable=True, **kw), cpt.AdamW(b, lr=1e-2, **kw)
+
+    def step(i, run):
+        for x, y, g in zip(a, b, _draw(a, i)):
+            x.grad = g.clone() if x.grad is None else x.grad.copy_(g)
+            y.grad = g
+        ref.param_groups[0]["lr"] = 1e-2 / (1 + i)
+        lr.fill_(1e-2 / (1 + i))
+        run()
+        ref.step()
+        torch.cuda.synchronize()
+
+    step(0, opt.step)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for i in range(1, 6):
+        before = [p.detach().clone() for p in b]
+        step(i, graph.replay)
+        assert torch.equal(opt.norm, ref.norm)
+        for x, y, old in zip(a, b, before):
+            s, t = opt.state[x], ref.state[y]
+            assert int(s["step"]) == t["step"] == i + 1
+            assert all(torch.equal(s[n], t[n]) for n in s if n != "step")
+            assert ((x - y).abs() <= (i + 1) * (2 * U * y.abs() + 4 * U * 5e-2)).all()
+            # the updates are hundreds of these bounds
+            assert (y - old).abs().mean() > 1e-4
