@@ -68,29 +68,44 @@ def _rope_args(q, k, positions, inv_freq, w_q, w_k, eps):
     return b, s, hq, hk, d, 2 * half, positions, wide, pos_batch, _DT[wdt]
 
 
-def _distinct(t):
-    """Whether no two elements of t share memory (an order of its axes nests them)."""
+def _nest(strides, shape):
+    """Whether an order of the axes nests them: then no two elements share memory."""
     extent = 1
-    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+    for stride, size in sorted([(st, n) for st, n in zip(strides, shape) if n > 1]):
         if stride < extent:
             return False
         extent = stride * size
     return True
 
 
-def _meet(q, k):
-    """Whether q and k have elements in one place: whether differences of their indices can
-    make up for the distance between them.  Along nested axes, the largest stride first,
-    few can; views that would take long to tell apart count as meeting."""
+def _apart(q, k):
+    """Whether the elements of q and of k all have places of their own."""
     if q.numel() == 0 or k.numel() == 0:
-        return False
+        return _nest(q.stride(), q.shape) and _nest(k.stride(), k.shape)
     off = (k.data_ptr() - q.data_ptr()) // q.element_size()
     sq, sk = q.stride(), k.stride()
+    if q.is_contiguous() and k.is_contiguous():
+        return off >= q.numel() or -off >= k.numel()
+    if sq == sk and sq[-2] > 0:
+        # heads of one buffer: apart if all from the first's to the last's are
+        at, rest = divmod(off, sq[-2])
+        hq, hk = q.shape[-2], k.shape[-2]
+        if rest == 0 and (at >= hq or -at >= hk):
+            heads = max(hq, at + hk) - min(0, at)
+            if _nest(sq, (*q.shape[:-2], heads, q.shape[-1])):
+                return True
+    return _nest(sq, q.shape) and _nest(sk, k.shape) and not _meet(off, sq, q.shape, sk, k.shape)
+
+
+def _meet(off, sq, nq, sk, nk):
+    """Whether views with nested axes, `off` elements apart, have elements in one place:
+    whether differences of their indices can make up for `off`.  The largest stride first,
+    few can; views that would take long to tell apart count as meeting."""
     if sq == sk:
-        axes = sorted([(st, 1 - n, m - 1) for st, m, n in zip(sq, q.shape, k.shape)])
+        axes = sorted([(st, 1 - n, m - 1) for st, m, n in zip(sq, nq, nk)])
     else:
-        axes = sorted([(st, 0, n - 1) for st, n in zip(sq, q.shape)] +
-                      [(st, 1 - n, 0) for st, n in zip(sk, k.shape)])
+        axes = sorted([(st, 0, n - 1) for st, n in zip(sq, nq)] +
+                      [(st, 1 - n, 0) for st, n in zip(sk, nk)])
     least = sum([st * first for st, first, _ in axes])
     most = sum([st * last for st, _, last in axes])
     if not least <= off <= most:
@@ -131,7 +146,7 @@ def qk_rope(q: torch.Tensor, k: torch.Tensor, positions, inv_freq: torch.Tensor,
     q2, sq = _strides(q)
     k2, sk = _strides(k)
     if inplace:
-        assert q2 is q and k2 is k and _distinct(q) and _distinct(k) and not _meet(q, k), \
+        assert q2 is q and k2 is k and _apart(q, k), \
             "inplace: heads with contiguous columns, no two elements in one place, expected"
         q_out, k_out, oq, ok = q, k, sq, sk
     else:
