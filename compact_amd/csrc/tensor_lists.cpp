@@ -117,64 +117,53 @@ class Addresses {
   std::vector<const void*> table_;
 };
 
-// The memory of a step's tensors.  What is written lies apart from all else, or its elements
-// depend on which thread comes first; a gradient may be its parameter or moment itself, whose
-// elements are each read before they are written.
-class Memory {
- public:
-  explicit Memory(int64_t most) : storages_(most) {}
-
-  // Tensor i of a list, dense.
-  void write(int list, const at::Tensor& t, int64_t i) {
-    if (t.numel() == 0) return;
-    shared_ |= !storages_.add(t.storage().data());
-    lists_[list].push_back(range(t, i));
-  }
-  // Once all that is written is known.
-  void read(const at::Tensor& t, int64_t i) {
-    if (t.numel() != 0 && storages_.has(t.storage().data())) read_.push_back(range(t, i));
-  }
-  void check(const List& p) {
-    if (!shared_ && read_.empty()) return;      // each in a storage of its own
-    // lists cut from a buffer each lie in order, one behind the other
-    for (auto& l : lists_) order(l);
-    std::sort(lists_, lists_ + kLists, [](const Ranges& a, const Ranges& b) {
-      return !a.empty() && (b.empty() || before(a[0], b[0]));
-    });
-    Ranges all;
-    for (const auto& l : lists_) all.insert(all.end(), l.begin(), l.end());
-    order(all);
-    for (size_t i = 1; i < all.size(); ++i)
-      if (all[i].at < all[i - 1].end)
-        refuse("two of a step's tensors share memory: " + describe(p[all[i].tensor]));
-    for (const Range& r : read_) {
-      auto w = std::upper_bound(all.begin(), all.end(), r, before);
-      if (w != all.begin()) --w;
-      for (; w != all.end() && w->at < r.end; ++w)
-        if (w->end > r.at && (w->at != r.at || w->end != r.end || w->tensor != r.tensor))
-          refuse("grads: a step writes to the memory of that for " + describe(p[r.tensor]));
-    }
-  }
-
- private:
-  static constexpr int kLists = 6;
-  struct Range {
-    uintptr_t at, end;
-    int64_t tensor;
-  };
-  using Ranges = std::vector<Range>;
-  static bool before(const Range& a, const Range& b) { return a.at < b.at; }
-  static void order(Ranges& r) {
-    if (!std::is_sorted(r.begin(), r.end(), before)) std::sort(r.begin(), r.end(), before);
-  }
-  static Range range(const at::Tensor& t, int64_t i) {
-    const auto at = reinterpret_cast<uintptr_t>(t.data_ptr());
-    return Range{at, at + t.numel() * t.element_size(), i};
-  }
-  Addresses storages_;
-  Ranges lists_[kLists], read_;
-  bool shared_ = false;
+// Whether what a step writes lies apart from all else: otherwise its elements depend on which
+// thread comes first.  A gradient may be its parameter or moment itself, whose elements are
+// each read before they are written.
+struct Range {
+  uintptr_t at, end;
+  int64_t tensor;
 };
+bool before(const Range& a, const Range& b) { return a.at < b.at; }
+Range range(const at::Tensor& t, int64_t i) {
+  const auto at = reinterpret_cast<uintptr_t>(t.data_ptr());
+  return Range{at, at + t.numel() * t.element_size(), i};
+}
+void order(std::vector<Range>& r) {
+  if (!std::is_sorted(r.begin(), r.end(), before)) std::sort(r.begin(), r.end(), before);
+}
+// Of dense tensors, written[0] the parameters; gradients that will be copied have no address
+// in their row.
+void check_apart(const std::vector<const List*>& written, const List& g,
+                 const std::vector<cpt_adamw_tensor>& rows) {
+  // lists cut from a buffer each lie in order, one behind the other
+  std::vector<std::vector<Range>> lists;
+  for (const List* l : written) {
+    if (!*l) continue;
+    lists.emplace_back();
+    for (int64_t i = 0; i < l->size(); ++i)
+      if ((*l)[i].numel()) lists.back().push_back(range((*l)[i], i));
+    order(lists.back());
+  }
+  std::sort(lists.begin(), lists.end(), [](const auto& a, const auto& b) {
+    return !a.empty() && (b.empty() || before(a[0], b[0]));
+  });
+  std::vector<Range> all;
+  for (const auto& l : lists) all.insert(all.end(), l.begin(), l.end());
+  order(all);
+  for (size_t i = 1; i < all.size(); ++i)
+    if (all[i].at < all[i - 1].end)
+      refuse("two of a step's tensors share memory: " + describe((*written[0])[all[i].tensor]));
+  for (int64_t i = 0; i < g.size(); ++i) {
+    if (!rows[i].g || !g[i].numel()) continue;
+    const Range r = range(g[i], i);
+    auto w = std::upper_bound(all.begin(), all.end(), r, before);
+    if (w != all.begin()) --w;
+    for (; w != all.end() && w->at < r.end; ++w)
+      if (w->end > r.at && (w->at != r.at || w->end != r.end || w->tensor != i))
+        refuse("grads: a step writes to the memory of that for " + describe((*written[0])[i]));
+  }
+}
 
 constexpr int64_t kBlock = 128;   // elements of an 8-bit moment that share a scale
 
@@ -266,7 +255,12 @@ PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
       refuse("m_scales and v_scales belong together");
     std::vector<cpt_adamw_tensor> rows(count);
     const bool written = PyObject_IsTrue(a[8]) == 1;
-    Memory memory(6 * count);
+    // tensors in storages of their own are apart
+    Addresses storages(6 * count);
+    bool shared = false;
+    const auto write = [&](const at::Tensor& t) {
+      if (t.numel()) shared |= !storages.add(t.storage().data());
+    };
     const at::ScalarType type = p[0].scalar_type(), grad_type = g[0].scalar_type();
     const at::Device device = p[0].device();
     if (code(type) < 0) refuse("params: unsupported " + describe(p[0]));
@@ -289,7 +283,7 @@ PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
       r.n = pi.numel();
       total += r.n;
       r.p = pi.data_ptr();
-      memory.write(0, pi, i);
+      write(pi);
       if (alike(pi, gi)) {
         r.g = gi.data_ptr();
       } else {
@@ -305,7 +299,7 @@ PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
         expect_bytes(vsi, pi, blocks, vs.name());
         r.m_scale = msi.data_ptr();
         r.v_scale = vsi.data_ptr();
-        if (written) memory.write(3, msi, i), memory.write(4, vsi, i);
+        if (written) write(msi), write(vsi);
       } else {
         expect(mi, pi, at::kFloat, m.name());
         expect(vi, pi, at::kFloat, v.name());
@@ -316,13 +310,13 @@ PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor& wi = w[i];
         expect(wi, pi, at::kFloat, w.name());
         r.master = wi.data_ptr();
-        memory.write(5, wi, i);
+        write(wi);
       }
-      if (written) memory.write(1, mi, i), memory.write(2, vi, i);
+      if (written) write(mi), write(vi);
     }
-    for (int64_t i = 0; i < count; ++i)
-      if (rows[i].g) memory.read(g[i], i);
-    memory.check(p);
+    for (int64_t i = 0; i < count && !shared; ++i)
+      shared = rows[i].g && rows[i].n && storages.has(g[i].storage().data());
+    if (shared && written) check_apart({&p, &m, &v, &ms, &vs, &w}, g, rows);
     steps(a[7], rows, device);
     return result(rows, total, code(type), code(grad_type), otherwise.release());
   });
@@ -370,6 +364,31 @@ PyObject* one_kind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// state_forms(states): (whether one is empty, all states' form or -1, what their counts are or
+// -1).  A form is 1 where moments are in 8 bits and 2 where there is an fp32 copy; counts are
+// 0 numbers and 1 tensors.
+PyObject* state_forms(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    static PyObject* const scale = PyUnicode_InternFromString("m_scale");
+    static PyObject* const master = PyUnicode_InternFromString("master");
+    static PyObject* const step = PyUnicode_InternFromString("step");
+    if (n != 1 || !PyList_Check(a[0])) refuse("a list expected");
+    int form = -2, counts = -2, empty = 0;
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[0]); ++i) {
+      PyObject* s = PyList_GET_ITEM(a[0], i);
+      if (!PyDict_Check(s)) refuse("dicts of a state expected");
+      empty |= PyDict_GET_SIZE(s) == 0;
+      const int f = PyDict_Contains(s, scale) | PyDict_Contains(s, master) << 1;
+      PyObject* at = PyDict_GetItemWithError(s, step);
+      if (f < 0 || PyErr_Occurred()) throw python_error();
+      const int c = at && PyLong_Check(at) ? 0 : 1;
+      form = form == -2 || form == f ? f : -1;
+      counts = counts == -2 || counts == c ? c : -1;
+    }
+    return Py_BuildValue("(iii)", empty, form, counts);
+  });
+}
+
 // bump_versions(tensors): they were written to
 PyObject* bump_versions(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -384,7 +403,7 @@ PyObject* bump_versions(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define ENTRY(name) \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ENTRY(adamw_table), ENTRY(grads_table), ENTRY(one_kind),
-                         ENTRY(bump_versions), {nullptr, nullptr, 0, nullptr}};
+                         ENTRY(state_forms), ENTRY(bump_versions), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_lists", "lists of tensors for the C ABI", -1,
                       methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -134,9 +134,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.
         if not given:
             norm = p0.new_empty((), dtype=torch.float32)
         norm_at = _scalar(norm, dev, "norm")
-    # counts on the device: a tensor of them, or one each
-    if max_norm is not None or isinstance(step, torch.Tensor) or \
-            (type(step) in (list, tuple) and isinstance(step[0], torch.Tensor)):
+    first = step if isinstance(step, (int, torch.Tensor)) else step[0]
+    if max_norm is not None or not isinstance(first, int):
         ws = _workspace(p0, count, total)
     with _guard(p0), _timed("adamw_step"):
         rc = _lib.api().cpt_adamw(dt, gdt, int(m_scales is not None), int(masters is not None), at,
@@ -238,9 +237,10 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW: the counts have to be on the device before a step is "
                                "captured")
         for p, s in zip(params, states):
+            if isinstance(s["step"], torch.Tensor) is bool(capturable):
+                continue
             n = int(s["step"])
             s["step"] = torch.tensor(n, device=p.device) if capturable else n
-        return [s["step"] for s in states]
 
     @torch.no_grad()
     def step(self, closure=None, *, grad_scale: float = 1.0):
@@ -261,32 +261,33 @@ class AdamW(torch.optim.Optimizer):
             if not params:
                 continue
             states = [self.state[p] for p in params]
-            if not all(states) or (group["master"] and not all(["master" in s for s in states])):
-                states = [self._init_state(p, group) for p in params]
-            same = _lib.lists().one_kind
-            held = [("m_scale" in s, "master" in s) for s in states]
-            if same(params) and same(grads) and len(set(held)) == 1:
+            lists = _lib.lists()
+            empty, form, counts = lists.state_forms(states)
+            if empty or (group["master"] and form < 2):
+                for p, s in zip(params, states):
+                    if not s or (group["master"] and "master" not in s):
+                        self._init_state(p, group)
+                _, form, counts = lists.state_forms(states)
+            if counts != int(bool(group["capturable"])):
+                self._move_counts(params, states, group["capturable"])
+            if form >= 0 and lists.one_kind(params) and lists.one_kind(grads):
                 buckets.append((group, params, grads, states))
                 continue
-            kinds = [(p.dtype, g.dtype, p.get_device(), h)
-                     for p, g, h in zip(params, grads, held)]
+            kinds = [(p.dtype, g.dtype, p.get_device(), "m_scale" in s, "master" in s)
+                     for p, g, s in zip(params, grads, states)]
             for kind in dict.fromkeys(kinds):
                 at = [i for i, other in enumerate(kinds) if other == kind]
                 buckets.append((group, *([x[i] for i in at] for x in (params, grads, states))))
         norm = None
         if self.max_norm is not None and len(buckets) > 1:
             norms = [grad_norm(grads, grad_scale=grad_scale) for _, _, grads, _ in buckets]
-            # squares in 64 bits, as each list's own: those of norms past 1e19 are inf in fp32
-            norm = torch.linalg.vector_norm(torch.stack([n.to(norms[0].device) for n in norms]),
-                                            dtype=torch.float64).float()
+            # in 64 bits as each list's own: the squares of norms past 1e19 are inf in fp32
+            norm = grad_norm([n.to(norms[0].device) for n in norms])
         for k, (group, params, grads, states) in enumerate(buckets):
             bits8, master = "m_scale" in states[0], "master" in states[0]
             capturable, steps = group["capturable"], [s["step"] for s in states]
             if not capturable and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("AdamW: a captured step needs capturable=True")
-            kinds = set(map(type, steps))
-            if (int in kinds) if capturable else (kinds != {int}):
-                steps = self._move_counts(params, states, capturable)
             if not capturable:
                 steps = [n + 1 for n in steps]
             got = adamw_step(

@@ -3,6 +3,8 @@ are taken for device ones and every library call is recorded and answered with s
 
 import contextlib
 import copy
+import ctypes
+import struct
 
 import pytest
 import torch
@@ -148,15 +150,30 @@ def test_loading_keeps_each_groups_own_options(library):
 
 
 @pytest.mark.parametrize("size", [1e-30, 1.0, 1e19, 6e37])
-def test_norms_of_several_lists_join_in_64_bits(library, monkeypatch, size):
-    """3 and 4 times any size make 5 times it, to a rounding of each and of the sum."""
+def test_norms_of_several_lists_join_in_64_bits(library, size):
+    """3 and 4 times any size make 5 times it, to a rounding of each and of the sum: as joined
+    by what sums each list's squares."""
+    def grad_norm(dt, table, count, scale, out, ws, stream):
+        rows = (ctypes.c_int64 * (10 * count)).from_address(table)
+        kind, load = ((ctypes.c_float, float), None, (ctypes.c_uint16, None))[dt]
+        total = 0.0
+        for i in range(count):
+            for x in (kind * rows[10 * i + 8]).from_address(rows[10 * i + 1]):
+                x = load(x) if load else struct.unpack("f", struct.pack("I", x << 16))[0]
+                total += (x * scale) ** 2
+        ctypes.c_float.from_address(out).value = total ** 0.5
+        return 0
+
+    library.cpt_grad_norm = grad_norm
     ps = _params(torch.float32, torch.bfloat16)
-    parts = iter([3 * size, 4 * size])
-    monkeypatch.setattr(optim, "grad_norm", lambda g, grad_scale: torch.tensor(next(parts)))
+    for p, x in zip(ps, (3 * size, 4 * size)):
+        p.grad.zero_()
+        p.grad[2] = x
+    want = sum(float(p.grad.double().norm()) ** 2 for p in ps) ** 0.5
     own = cpt.AdamW(ps, max_norm=1.0)
     own.step()
     assert own.norm.dtype == torch.float32
-    assert abs(float(own.norm) - 5 * size) <= 2 * 2.0 ** -24 * 5 * size
+    assert abs(float(own.norm) - want) <= 2 * 2.0 ** -24 * want
     assert [a[14] for a in library.steps()] == [1, 1]     # the norm is given to each
 
 
