@@ -117,55 +117,61 @@ class Addresses {
   std::vector<const void*> table_;
 };
 
-// Whether what a step writes lies apart from all else: otherwise its elements depend on which
-// thread comes first.  A gradient may be its parameter or moment itself, whose elements are
-// each read before they are written.
+constexpr int64_t kBlock = 128;   // elements of an 8-bit moment that share a scale
+
+// Refuses a step whose tensors' memory meets: what is written lies apart from all else, or its
+// elements depend on which thread comes first.  A gradient may be its parameter or moment
+// itself, whose elements are each read before they are written.
 struct Range {
   uintptr_t at, end;
   int64_t tensor;
 };
 bool before(const Range& a, const Range& b) { return a.at < b.at; }
-Range range(const at::Tensor& t, int64_t i) {
-  const auto at = reinterpret_cast<uintptr_t>(t.data_ptr());
-  return Range{at, at + t.numel() * t.element_size(), i};
-}
 void order(std::vector<Range>& r) {
   if (!std::is_sorted(r.begin(), r.end(), before)) std::sort(r.begin(), r.end(), before);
 }
-// Of dense tensors, written[0] the parameters; gradients that will be copied have no address
-// in their row.
-void check_apart(const std::vector<const List*>& written, const List& g,
-                 const std::vector<cpt_adamw_tensor>& rows) {
+void check_apart(const List& p, const std::vector<cpt_adamw_tensor>& rows, int64_t size,
+                 int64_t grad_size, bool bits8, bool grads) {
   // lists cut from a buffer each lie in order, one behind the other
   std::vector<std::vector<Range>> lists;
-  for (const List* l : written) {
-    if (!*l) continue;
+  const auto list = [&](void* cpt_adamw_tensor::*address, int64_t unit, int64_t block) {
     lists.emplace_back();
-    for (int64_t i = 0; i < l->size(); ++i)
-      if ((*l)[i].numel()) lists.back().push_back(range((*l)[i], i));
+    lists.back().reserve(rows.size());
+    for (size_t i = 0; i < rows.size(); ++i) {
+      const auto at = reinterpret_cast<uintptr_t>(rows[i].*address);
+      const int64_t bytes = (rows[i].n + block - 1) / block * unit;
+      if (at && bytes) lists.back().push_back(Range{at, at + bytes, static_cast<int64_t>(i)});
+    }
     order(lists.back());
-  }
+  };
+  list(&cpt_adamw_tensor::p, size, 1);
+  list(&cpt_adamw_tensor::m, bits8 ? 1 : 4, 1);
+  list(&cpt_adamw_tensor::v, bits8 ? 1 : 4, 1);
+  list(&cpt_adamw_tensor::m_scale, 1, kBlock);
+  list(&cpt_adamw_tensor::v_scale, 1, kBlock);
+  list(&cpt_adamw_tensor::master, 4, 1);
   std::sort(lists.begin(), lists.end(), [](const auto& a, const auto& b) {
     return !a.empty() && (b.empty() || before(a[0], b[0]));
   });
   std::vector<Range> all;
+  all.reserve(rows.size() * lists.size());
   for (const auto& l : lists) all.insert(all.end(), l.begin(), l.end());
   order(all);
   for (size_t i = 1; i < all.size(); ++i)
     if (all[i].at < all[i - 1].end)
-      refuse("two of a step's tensors share memory: " + describe((*written[0])[all[i].tensor]));
-  for (int64_t i = 0; i < g.size(); ++i) {
-    if (!rows[i].g || !g[i].numel()) continue;
-    const Range r = range(g[i], i);
+      refuse("two of a step's tensors share memory: " + describe(p[all[i].tensor]));
+  for (size_t i = 0; grads && i < rows.size(); ++i) {
+    // one that will be copied has no address
+    const auto at = reinterpret_cast<uintptr_t>(rows[i].g);
+    const Range r{at, at + rows[i].n * grad_size, static_cast<int64_t>(i)};
+    if (!at || !rows[i].n) continue;
     auto w = std::upper_bound(all.begin(), all.end(), r, before);
     if (w != all.begin()) --w;
     for (; w != all.end() && w->at < r.end; ++w)
-      if (w->end > r.at && (w->at != r.at || w->end != r.end || w->tensor != i))
-        refuse("grads: a step writes to the memory of that for " + describe((*written[0])[i]));
+      if (w->end > r.at && (w->at != r.at || w->end != r.end || w->tensor != r.tensor))
+        refuse("grads: a step writes to the memory of that for " + describe(p[i]));
   }
 }
-
-constexpr int64_t kBlock = 128;   // elements of an 8-bit moment that share a scale
 
 template <class F>
 PyObject* guarded(F&& f) {
@@ -314,9 +320,11 @@ PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
       }
       if (written) write(mi), write(vi);
     }
-    for (int64_t i = 0; i < count && !shared; ++i)
-      shared = rows[i].g && rows[i].n && storages.has(g[i].storage().data());
-    if (shared && written) check_apart({&p, &m, &v, &ms, &vs, &w}, g, rows);
+    bool grads = false;
+    for (int64_t i = 0; i < count && !grads; ++i)
+      grads = rows[i].g && rows[i].n && storages.has(g[i].storage().data());
+    if (written && (shared || grads))
+      check_apart(p, rows, p[0].element_size(), g[0].element_size(), static_cast<bool>(ms), grads);
     steps(a[7], rows, device);
     return result(rows, total, code(type), code(grad_type), otherwise.release());
   });
