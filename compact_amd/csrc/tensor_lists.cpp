@@ -119,52 +119,64 @@ class Addresses {
 
 constexpr int64_t kBlock = 128;   // elements of an 8-bit moment that share a scale
 
-// Refuses a step whose tensors' memory meets: what is written lies apart from all else, or its
-// elements depend on which thread comes first.  A gradient may be its parameter or moment
-// itself, whose elements are each read before they are written.
+// One of a step's lists: where its tensors' addresses stand, and the bytes of `block` elements.
+struct Written {
+  void* cpt_adamw_tensor::*address;
+  int64_t unit, block;
+};
 struct Range {
   uintptr_t at, end;
   int64_t tensor;
 };
 bool before(const Range& a, const Range& b) { return a.at < b.at; }
-void order(std::vector<Range>& r) {
-  if (!std::is_sorted(r.begin(), r.end(), before)) std::sort(r.begin(), r.end(), before);
+Range range(const void* p, int64_t bytes, int64_t i) {
+  const auto at = reinterpret_cast<uintptr_t>(p);
+  return Range{at, at + (at ? bytes : 0), i};
 }
+// Refuses a step whose tensors' memory meets: what is written lies apart from all else, or its
+// elements depend on which thread comes first.  A gradient may be its parameter or moment
+// itself, whose elements are each read before they are written.
 void check_apart(const List& p, const std::vector<cpt_adamw_tensor>& rows, int64_t size,
                  int64_t grad_size, bool bits8, bool grads) {
-  // lists cut from a buffer each lie in order, one behind the other
-  std::vector<std::vector<Range>> lists;
-  const auto list = [&](void* cpt_adamw_tensor::*address, int64_t unit, int64_t block) {
-    lists.emplace_back();
-    lists.back().reserve(rows.size());
-    for (size_t i = 0; i < rows.size(); ++i) {
-      const auto at = reinterpret_cast<uintptr_t>(rows[i].*address);
-      const int64_t bytes = (rows[i].n + block - 1) / block * unit;
-      if (at && bytes) lists.back().push_back(Range{at, at + bytes, static_cast<int64_t>(i)});
-    }
-    order(lists.back());
+  const int64_t moment = bits8 ? 1 : 4;
+  const Written lists[] = {{&cpt_adamw_tensor::p, size, 1},
+                           {&cpt_adamw_tensor::m, moment, 1},
+                           {&cpt_adamw_tensor::v, moment, 1},
+                           {&cpt_adamw_tensor::m_scale, 1, kBlock},
+                           {&cpt_adamw_tensor::v_scale, 1, kBlock},
+                           {&cpt_adamw_tensor::master, 4, 1}};
+  const auto at = [&](const Written& l, int64_t i) {
+    return range(rows[i].*l.address, (rows[i].n + l.block - 1) / l.block * l.unit, i);
   };
-  list(&cpt_adamw_tensor::p, size, 1);
-  list(&cpt_adamw_tensor::m, bits8 ? 1 : 4, 1);
-  list(&cpt_adamw_tensor::v, bits8 ? 1 : 4, 1);
-  list(&cpt_adamw_tensor::m_scale, 1, kBlock);
-  list(&cpt_adamw_tensor::v_scale, 1, kBlock);
-  list(&cpt_adamw_tensor::master, 4, 1);
-  std::sort(lists.begin(), lists.end(), [](const auto& a, const auto& b) {
-    return !a.empty() && (b.empty() || before(a[0], b[0]));
-  });
+  const int64_t count = rows.size();
+  // lists cut from a buffer each lie in order, one list behind the other: nothing to sort
+  bool apart = !grads;
+  Range spans[6];
+  int n = 0;
+  for (const Written& l : lists) {
+    Range span{0, 0, 0};
+    for (int64_t i = 0; i < count && apart; ++i) {
+      const Range r = at(l, i);
+      if (r.at == r.end) continue;
+      apart = r.at >= span.end;
+      span = Range{span.at ? span.at : r.at, r.end, 0};
+    }
+    for (int k = 0; k < n; ++k) apart &= span.end <= spans[k].at || span.at >= spans[k].end;
+    if (span.end) spans[n++] = span;
+  }
+  if (apart) return;
   std::vector<Range> all;
-  all.reserve(rows.size() * lists.size());
-  for (const auto& l : lists) all.insert(all.end(), l.begin(), l.end());
-  order(all);
+  all.reserve(count * 6);
+  for (const Written& l : lists)
+    for (int64_t i = 0; i < count; ++i)
+      if (const Range r = at(l, i); r.at != r.end) all.push_back(r);
+  std::sort(all.begin(), all.end(), before);
   for (size_t i = 1; i < all.size(); ++i)
     if (all[i].at < all[i - 1].end)
       refuse("two of a step's tensors share memory: " + describe(p[all[i].tensor]));
-  for (size_t i = 0; grads && i < rows.size(); ++i) {
-    // one that will be copied has no address
-    const auto at = reinterpret_cast<uintptr_t>(rows[i].g);
-    const Range r{at, at + rows[i].n * grad_size, static_cast<int64_t>(i)};
-    if (!at || !rows[i].n) continue;
+  for (int64_t i = 0; grads && i < count; ++i) {
+    const Range r = range(rows[i].g, rows[i].n * grad_size, i);
+    if (r.at == r.end) continue;        // one that will be copied has no address
     auto w = std::upper_bound(all.begin(), all.end(), r, before);
     if (w != all.begin()) --w;
     for (; w != all.end() && w->at < r.end; ++w)
