@@ -21,11 +21,14 @@
 //
 // Bound: HBM, 22 bytes an element with 16-bit parameters and gradients and fp32
 // moments, 28 with an fp32 copy of the parameters, 10 with 8-bit moments.  The
-// tensors' pointers are kernel arguments, up to 90 a launch: no table to upload or keep.
+// tensors' pointers are kernel arguments, up to 90 a launch: no table to upload or keep.  A
+// launch has one step number on the host: tensors whose numbers change from one to the next
+// take one each (counts on the device do not divide a call).
 //
-// Measured on one MI355X: 1.1 G bf16 parameters with an fp32 copy 5760 us (5.3 TB/s) and 420
-// for the norm; 371 M with 8-bit moments 750-780 (4.9), their values 390; 31.6 M in 320
-// tensors 136 in four launches (5.1) and 27 for the norm; 0.2 M fp32 4.1.
+// Measured on one MI355X, a trace's mean of 12: 1.1 G bf16 parameters with an fp32 copy 5750
+// us (5.4 TB/s) and 430 for the norm; 371 M with 8-bit moments 780 (4.8; the least 741),
+// their values 394; 31.6 M in 320 tensors 136 in four launches (5.1) and 27 for the norm;
+// 0.2 M fp32 4.7.
 
 #include <algorithm>
 #include <cmath>
@@ -169,8 +172,8 @@ __device__ __forceinline__ void st_codes(void* p, int64_t i, int64_t n, const ui
 // A code's value: its bits in a float's place, times 2^(129 + s).
 template <bool SIGNED>
 __device__ __forceinline__ float decode(uint32_t code, int scale) {
-  const float y =
-      __builtin_ldexpf(__uint_as_float((SIGNED ? code & 127 : code) << 20), scale - (kScaleBias - 129));
+  const float y = __builtin_ldexpf(__uint_as_float((SIGNED ? code & 127 : code) << 20),
+                                   scale - (kScaleBias - 129));
   const float v = SIGNED ? __uint_as_float(__float_as_uint(y) | (code & 128) << 24) : y;
   return scale == 255 ? __uint_as_float(0x7FC00000u) : v;
 }
@@ -535,10 +538,10 @@ int grad_norm(int gd, const cpt_adamw_tensor* t, int64_t count, int64_t total, f
               hipStream_t st) {
   int64_t blocks = 0;
   const int64_t chunk = norm_chunk(total);
-  const int rc = gd == kF32 ? launch_squares<kF32>(t, count, chunk, grad_scale, partial, &blocks, st)
-                 : gd == kF16
-                     ? launch_squares<kF16>(t, count, chunk, grad_scale, partial, &blocks, st)
-                     : launch_squares<kBF16>(t, count, chunk, grad_scale, partial, &blocks, st);
+  const auto squares = gd == kF32   ? launch_squares<kF32>
+                       : gd == kF16 ? launch_squares<kF16>
+                                    : launch_squares<kBF16>;
+  const int rc = squares(t, count, chunk, grad_scale, partial, &blocks, st);
   if (rc) return rc;
   if (partials) {       // left to the step
     *partials = blocks;

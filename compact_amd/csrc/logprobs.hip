@@ -14,13 +14,16 @@
 // log s - w / s, a sum of terms of one sign.  Alternatives cost no more reading of
 // note: the k-th largest of the threads' maxima (a bound that at least k columns
 // reach) leaves about k threads with candidates, and only those threads' columns are
-// looked at again, dealt out over the block.  Where a bound leaves too many (constant
-// rows, rows with little but -inf, NaN), a radix selection takes its place.
+// looked at again, dealt out over the block.  Where a bound leaves too many (more than
+// 1024 candidates or maxima, in a row of one wavefront 256 or 128: constant rows, rows with
+// little but -inf) or there is none (NaN; more than 64 alternatives for each wavefront
+// whose lanes all have columns, as 65 of a row under 1024 columns), a radix selection
+// takes its place: five more readings of the row.
 //
-// Measured on one MI355X, 15% of the rows left out: 8192 x 32000 bf16 83 us without
-// alternatives (5.4 TB/s), 93 with 20, 115 with 50 in all; 1531 x 50021 fp16, 50 of them,
-// 45; 7 x 32000, 5 of them, 10; the gradient of 8192 x 32000 bf16 180 us (5.4 TB/s, in part
-// from the Infinity Cache).
+// Measured on one MI355X, 15% of the rows left out, us a pass among others: 8192 x 32000
+// bf16 83 without alternatives (5.4 TB/s), 93 with 20, 115 with 50 in all; 1531 x 50021
+// fp16, 50 of them, 45; 7 x 32000, 5 of them, 13 (the kernel 11); the gradient of 8192 x
+// 32000 bf16 181 (5.4 TB/s, in part from the Infinity Cache).
 
 #include <algorithm>
 
@@ -539,8 +542,10 @@ int cpt_token_logprobs(int dtype, const void* logits, int64_t rows, int64_t voca
   int shift = 0;
   while ((vocab / 8 + ((4 * threads) << shift) - 1) / ((4 * threads) << shift) > kSlots) ++shift;
   const LogArgs A{logits, targets, (float*)logprobs, (float*)entropy, (float*)lse,
-                  (float*)stats, (float*)top_logprobs, (int64_t*)top_indices, rows, ld_batch, ld_row,
-                  ignore_index, FastDivU32::make((uint32_t)std::min<int64_t>(seq, 0x7FFFFFFF)), (int)vocab, (int)k, target_wide, shift, 1.f / temperature};
+                  (float*)stats, (float*)top_logprobs, (int64_t*)top_indices, rows, ld_batch,
+                  ld_row, ignore_index,
+                  FastDivU32::make((uint32_t)std::min<int64_t>(seq, 0x7FFFFFFF)), (int)vocab,
+                  (int)k, target_wide, shift, 1.f / temperature};
   const hipStream_t st = (hipStream_t)stream;
   const unsigned grid = (unsigned)rows;
 #define CPT_LP(DT)                                                           \
@@ -561,17 +566,19 @@ int cpt_token_logprobs_backward(int dtype, const void* logits, int64_t rows, int
                                 int64_t seq, int64_t ld_batch, int64_t ld_row, int target_wide,
                                 const void* targets, int64_t ignore_index, float temperature,
                                 const void* lse, const void* stats, const void* entropy,
-                                const void* d_logprobs, const void* d_entropy, void* grad, int64_t gld_batch,
-                                int64_t gld_row, void* stream) {
+                                const void* d_logprobs, const void* d_entropy, void* grad,
+                                int64_t gld_batch, int64_t gld_row, void* stream) {
   if (const int rc = check_logits(dtype, rows, vocab, seq, logits, temperature)) return rc;
   if (rows == 0) return kOk;
-  if ((!lse && !stats) || !grad || (d_logprobs && !targets) || (d_entropy && !entropy)) return kErrShape;
+  if ((!lse && !stats) || !grad || (d_logprobs && !targets) || (d_entropy && !entropy))
+    return kErrShape;
   LogGradArgs A{logits, targets, (const float*)lse, (const float*)stats, (const float*)entropy,
                 (const float*)d_logprobs, (const float*)d_entropy, grad, rows, ld_batch,
                 ld_row, gld_batch, gld_row, ignore_index,
                 FastDivU32::make((uint32_t)std::min<int64_t>(seq, 0x7FFFFFFF)), {}, (int)vocab,
                 target_wide, 1.f / temperature};
-  const int64_t chunks = (vocab + kGradThreads * kGradVecs * 8 - 1) / (kGradThreads * kGradVecs * 8);
+  constexpr int kChunk = kGradThreads * kGradVecs * 8;
+  const int64_t chunks = (vocab + kChunk - 1) / kChunk;
   A.chunks = FastDivU32::make((uint32_t)chunks);
   const int64_t grid = rows * chunks;
   if (grid > 0x7FFFFFFF) return kErrTooLarge;

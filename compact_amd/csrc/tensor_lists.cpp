@@ -1,7 +1,7 @@
 // Lists of tensors as the C ABI takes them: an optimizer step has hundreds of tensors
 // in five lists, and a look at each from Python costs more than the step (320 adapter
-// factors: 550 us of checks and addresses, 15 here).  Everything that the kernels rely
-// on is checked: types, devices, sizes, layouts.
+// factors: 550 us of checks and addresses, 17 here).  Everything that the kernels rely
+// on is checked: types, devices, sizes, layouts, memory that meets.
 
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -265,8 +265,8 @@ PyObject* adamw_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
         ms(a[4], "m_scales"), vs(a[5], "v_scales"), w(a[6], "masters");
     for (const List* l : {&g, &m, &v, &ms, &vs, &w})
       if (*l && l->size() != p.size())
-        refuse(std::string(l->name()) + ": " + std::to_string(p.size()) + " tensors expected, got " +
-               std::to_string(l->size()));
+        refuse(std::string(l->name()) + ": " + std::to_string(p.size()) +
+               " tensors expected, got " + std::to_string(l->size()));
     const int64_t count = p.size();
     if (count == 0 || !g || !m || !v) refuse("adamw_table: tensors expected");
     if (static_cast<bool>(ms) != static_cast<bool>(vs))

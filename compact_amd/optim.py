@@ -93,10 +93,10 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.
     codes and scales.  What is written lies apart from all else; a gradient may be its
     parameter or moment itself.
 
-    step: this step's number, from 1 (for all, or a list), or int64 counts of the steps
-    done on the device (one tensor of len(params), or one each), which the call
-    increases: what a captured graph needs.  lr: a number, or a float32 scalar on the
-    device.
+    step: this step's number, from 1 (for all, or a list: runs of equal numbers share
+    launches), or int64 counts of the steps done on the device (one tensor of
+    len(params), or one each), which the call increases: what a captured graph needs.
+    lr: a number, or a float32 scalar on the device.
 
     max_norm clips by the global norm of grad_scale * grads (inf: measures it alone),
     which is returned (float32 scalar on the device; else None); `norm` gives it where it

@@ -134,9 +134,10 @@ def qk_rope(q: torch.Tensor, k: torch.Tensor, positions, inv_freq: torch.Tensor,
 
     A pair is columns i and R / 2 + i, or with `interleaved` 2 i and 2 i + 1; columns
     from R on are normed alone.  positions: int32 or int64 [B, S] or [S], None: 0
-    to S - 1; angles are exact at any position.  Weights share one dtype, the heads'
-    or float32.  Outputs are contiguous; `inplace` writes over q and k, which must
-    be the caller's own and lie apart.  `inverse` turns back, without norms: the gradient."""
+    to S - 1; angles are products of 53 bits (1e-7 off at 2 10^9).  Weights share one
+    dtype, the heads' or float32.  Outputs are contiguous; `inplace` writes over q and
+    k, which must be the caller's own and lie apart.  `inverse` turns back, without
+    norms: the gradient."""
     _on_device(q, k, positions, inv_freq, w_q, w_k)
     dt = _dtype_code(q)
     b, s, hq, hk, d, rot, pos, wide, pos_batch, wdt = _rope_args(q, k, positions, inv_freq, w_q,

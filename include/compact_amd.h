@@ -719,13 +719,15 @@ typedef struct {
 } cpt_adamw_tensor;
 
 /* An AdamW step over `count` tensors of one type (dtype; gradients grad_dtype: dtype
- * or fp32), in place (adamw.hip has the formulas).  `tensors` is host memory, read
- * before the call returns.  Moments are fp32, or with bits8 in 8 bits, rounded at
- * random by `seed`; with has_master the fp32 parameters are stepped and p is their
- * rounding.  Gradients are multiplied by grad_scale and, with max_norm > 0, clipped
- * to that global norm, which is written to `norm` (fp32 [1]) or, with norm_given,
- * read there; a norm that is not finite leaves everything as it was.  step_device is given for all tensors or none:
- * such counts are increased by one.  lr_device: fp32 [1] in lr's place, or NULL.
+ * or fp32), in place (adamw.hip has the formulas); what is written lies apart from
+ * all else, but a gradient may be its parameter or moment of the same type.  `tensors`
+ * is host memory, read before the call returns.  Moments are fp32, or with bits8 in 8
+ * bits, rounded at random by `seed`; with has_master the fp32 parameters are stepped
+ * and p is their rounding.  Gradients are multiplied by grad_scale and, with max_norm > 0, clipped
+ * to that global norm (inf: not clipped), which is written to `norm` (fp32 [1]) or,
+ * with norm_given, read there; a norm that is not finite leaves everything as it was.
+ * step_device is given for all tensors or none: such counts are increased by one.
+ * lr_device: fp32 [1] in lr's place, or NULL.
  * workspace, for clipping or counts on the device, 16-byte aligned:
  * cpt_adamw_workspace_bytes(count, elements of all tensors) bytes. */
 int64_t cpt_adamw_workspace_bytes(int64_t count, int64_t elements);
