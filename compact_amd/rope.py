@@ -86,7 +86,8 @@ def _apart(q, k):
     sq, sk = q.stride(), k.stride()
     if q.is_contiguous() and k.is_contiguous():
         return off >= q.numel() or -off >= k.numel()
-    if sq == sk and sq[-2] > 0:
+    same = sq == sk or all([a == b or n == 1 for a, b, n in zip(sq, sk, (*q.shape[:-2], 2, 2))])
+    if same and sq[-2] > 0:
         # heads of one buffer: apart if all from the first's to the last's are
         at, rest = divmod(off, sq[-2])
         hq, hk = q.shape[-2], k.shape[-2]
@@ -101,11 +102,16 @@ def _meet(off, sq, nq, sk, nk):
     """Whether views with nested axes, `off` elements apart, have elements in one place:
     whether differences of their indices can make up for `off`.  The largest stride first,
     few can; views that would take long to tell apart count as meeting."""
-    if sq == sk:
-        axes = sorted([(st, 1 - n, m - 1) for st, m, n in zip(sq, nq, nk)])
-    else:
-        axes = sorted([(st, 0, n - 1) for st, n in zip(sq, nq)] +
-                      [(st, 1 - n, 0) for st, n in zip(sk, nk)])
+    reach = {}              # how far indices along a stride can differ, both ways
+    for st, n in zip(sq, nq):
+        if n > 1:
+            first, last = reach.get(st, (0, 0))
+            reach[st] = first, last + n - 1
+    for st, n in zip(sk, nk):
+        if n > 1:
+            first, last = reach.get(st, (0, 0))
+            reach[st] = first - n + 1, last
+    axes = sorted([(st, *ends) for st, ends in reach.items()])
     least = sum([st * first for st, first, _ in axes])
     most = sum([st * last for st, _, last in axes])
     if not least <= off <= most:
@@ -114,11 +120,10 @@ def _meet(off, sq, nq, sk, nk):
     for st, first, last in reversed(axes):
         # what the smaller strides reach
         least, most = least - st * first, most - st * last
-        if first < last:
-            left = {t - st * n for t in left for n in range(max(first, -((most - t) // st)),
-                                                            min(last, (t - least) // st) + 1)}
-            if len(left) > 64:
-                return True
+        left = {t - st * n for t in left for n in range(max(first, -((most - t) // st)),
+                                                        min(last, (t - least) // st) + 1)}
+        if len(left) > 64:
+            return True
     return 0 in left
 
 

@@ -4,6 +4,7 @@ are taken for device ones and every library call is recorded and answered with s
 import contextlib
 import copy
 import ctypes
+import random
 import struct
 
 import pytest
@@ -462,3 +463,58 @@ def test_the_fused_forward_takes_plain_attentions_alone():
     call("HIP device", RuntimeError)
     model.model.rotary_emb.rope_type = "dynamic"
     call("go by the length")
+
+
+def test_views_that_lie_apart_are_told_from_those_that_meet():
+    """Random views of one buffer against their elements' places: none that meets is taken,
+    and of these none that is apart is refused."""
+    rng = random.Random(3)
+    buf = torch.zeros(6000)
+    where = torch.arange(6000)
+    seen = [0, 0]
+
+    def strides(shape):
+        order = list(range(len(shape)))
+        if rng.random() < 0.4:
+            rng.shuffle(order)
+        out, step = [0] * len(shape), 1
+        for axis in reversed(order):
+            out[axis] = step
+            step = step * shape[axis] + rng.choice([0, 0, 0, 1, 5, step * shape[axis]])
+        return out, step
+
+    for _ in range(3000):
+        lead, d = [rng.randint(1, 3) for _ in range(rng.choice([1, 2]))], rng.choice([2, 6, 70])
+        shapes = [[*lead, rng.randint(1, 3), d] for _ in range(2)]
+        (sq, eq), (sk, ek) = strides(shapes[0]), strides(shapes[1])
+        if rng.random() < 0.7:
+            sk, ek = sq, eq * 2
+        if max(eq, ek) > 4000:
+            continue
+        at = [rng.randrange(0, rng.choice([10, 400, 1900])) for _ in range(2)]
+        q, k = (buf.as_strided(n, s, a) for n, s, a in zip(shapes, (sq, sk), at))
+        places = [set(where.as_strided(n, s, a).flatten().tolist())
+                  for n, s, a in zip(shapes, (sq, sk), at)]
+        if any(len(p) < t.numel() for p, t in zip(places, (q, k))):
+            assert not rope._apart(q, k)
+            continue
+        apart = not places[0] & places[1]
+        if not rope._nest(sq, shapes[0]) or not rope._nest(sk, shapes[1]):
+            assert not rope._apart(q, k)
+            continue
+        seen[apart] += 1
+        assert rope._apart(q, k) is apart, (q.shape, sq, k.shape, sk, at)
+    assert min(seen) > 300
+
+
+@pytest.mark.parametrize("batch", [1, 4])
+def test_one_token_of_a_split_projection_in_place(library, batch):
+    """Heads viewed from a projection's columns: an axis of one token has a stride of its own
+    in each view, which says nothing."""
+    x = torch.zeros(batch, 1, 40 * 128)
+    q, k = x[..., :4096].view(batch, 1, 32, 128), x[..., 4096:4608].view(batch, 1, 4, 128)
+    assert q.stride() != k.stride()
+    cpt.qk_rope(q, k, None, torch.ones(64), inplace=True)
+    with pytest.raises(AssertionError, match="one place"):
+        cpt.qk_rope(q, x[..., 3968:4480].view(batch, 1, 4, 128), None, torch.ones(64), inplace=True)
+    assert len(library.calls) == 1
