@@ -237,7 +237,7 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW: the counts have to be on the device before a step is "
                                "captured")
         for p, s in zip(params, states):
-            if isinstance(s["step"], torch.Tensor) is bool(capturable):
+            if isinstance(s["step"], torch.Tensor if capturable else int):
                 continue
             n = int(s["step"])
             s["step"] = torch.tensor(n, device=p.device) if capturable else n

@@ -348,8 +348,8 @@ def test_rotation_in_place_takes_heads_that_lie_apart(library):
              (x.flatten(1, 2)[:, ::2, None], x.flatten(1, 2)[:, 1::2, None]),
              (x[:, :, 0].unsqueeze(2), x[:, :, 1:]),
              (x[:, :, :2].transpose(1, 2), x[:, :, 2:4].transpose(1, 2)),
-             (x[..., :8], x.view(3, 8, 12, 8)[:, :, 1::2]), (torch.zeros(1, 8, 4, 16), x[:1, :, :3]),
-             (x[:, :0], x[:, :0])]
+             (x[..., :8], x.view(3, 8, 12, 8)[:, :, 1::2]),
+             (torch.zeros(1, 8, 4, 16), x[:1, :, :3]), (x[:, :0], x[:, :0])]
     for i, (q, k) in enumerate(pairs):
         cpt.qk_rope(q, k, None, inv, inplace=True)
         assert len(library.calls) == i + 1, i
@@ -399,7 +399,7 @@ def test_a_modules_frequencies_stay(library):
     assert m.rotary == 16 and m.inv_freq.dtype == torch.float32
     assert torch.equal(m.inv_freq, own.float())
     for cast in (lambda t: t.half(), lambda t: t.double(), lambda t: t.to(torch.bfloat16),
-                 lambda t: t.to("cpu"), lambda t: copy.deepcopy(t), lambda t: t.to_empty(device="cpu")):
+                 lambda t: t.to("cpu"), copy.deepcopy, lambda t: t.to_empty(device="cpu")):
         assert torch.equal(cast(m).inv_freq, own.float())
     with torch.no_grad():
         m.inv_freq.mul_(0.25)
